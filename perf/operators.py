@@ -168,7 +168,7 @@ def prepare(case, seed):
                 p("x"), p("w"), p("teacher"), p("tokens"), p("loss"), rows, vocab, width, s["tokens"].shape[1],
                 temperature=case["temperature"], labels=p("labels"), label_weight=_LABEL_WEIGHT if both else 0.0,
                 distill_weight=_DISTILL_WEIGHT if both else 1.0, teacher_dtype=t0g.BF16 if case["narrow"] else t0g.F32,
-                token_dtype=t0g.I32 if case["narrow"] else t0g.I64, **head)
+                token_type=t0g.I32 if case["narrow"] else t0g.I64, **head)
         s["rt"] = _rt()
     torch.cuda.synchronize()   # the runtime's stream is its own: the inputs are there before it is used
     return s
