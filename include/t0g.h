@@ -490,6 +490,71 @@ typedef enum t0g_matmul_op {
 T0G_API int t0g_matmul_kernel_name(uint32_t op, uint32_t m, uint32_t k, uint32_t n, char *buf, size_t len,
                                    uint32_t *splits);
 
+/* ---- losses of a projection onto a vocabulary -------------------------------- *
+ * The last layer of a language model and its loss in one call, without the
+ * rows x vocab logits z = logit_scale x W^T ever being kept: they are taken in
+ * pieces of the vocabulary.  No reference counterpart: the reference's training
+ * stack keeps the logits and runs its loss kernels on them (src/t0/ce_loss_kernels.rs).
+ *
+ * t0g_linear_cross_entropy, per row t with label y:
+ *   loss = lse - z_y,  lse = log sum_v exp z_v
+ * t0g_linear_distill, per row with the teacher's logits u_k at tokens i_k, at the
+ * temperature T:
+ *   Q = softmax(u / T) over the given tokens,  P = softmax(z / T) over the vocabulary
+ *   loss = distill_weight T^2 sum_v Q_v (log Q_v - log P_v)  [+ label_weight (lse - z_y)]
+ * Gradients (dx, dw; each only if asked for) are those of
+ *   loss_scale * sum_t dloss_t loss_t.
+ *
+ * A label or token outside [0, vocab), such as the usual -100, counts as missing, as
+ * does a teacher's logit of -inf; equal tokens of a row add their probabilities.  A
+ * row with neither label nor teacher's token has loss 0, lse 0 and no gradient,
+ * whatever its hidden state holds (NaN included).
+ *
+ * Products, statistics and losses are f32 on bf16 operands.  The logits' gradient
+ * is rounded to bf16 once, as an operand of the products that give dx and dw.
+ * Results do not depend on what ran before: no atomics, sums in a fixed order.
+ * Calls are asynchronous on the device stream; the scratch (about 0.5 GB at most,
+ * plus f32 partial sums of dx) belongs to the handle and grows on a shape's first call.
+ * Under stream capture it cannot grow: the call is refused unless the same call
+ * ran before. */
+typedef enum t0g_index_type { T0G_I32 = 0, T0G_I64 = 1 } t0g_index_type;
+typedef struct t0g_linear_ce_desc {
+    uint64_t x;                     /* bf16 [rows][ldx]: hidden states                 */
+    uint64_t w;                     /* bf16, NT: [vocab][ldw], NN: [hidden][ldw]       */
+    uint64_t labels;                /* label_type [rows]                               */
+    uint64_t loss;                  /* out: f32 [rows]                                 */
+    uint64_t lse;                   /* out: f32 [rows], or 0 (distill: of z / T)       */
+    uint64_t dloss;                 /* f32 [rows]: weight of each row's loss; 0 = ones */
+    uint64_t dx;                    /* out: dx_dtype [rows][lddx], or 0                */
+    uint64_t dw;                    /* out: dw_dtype, laid out as w with lddw, or 0    */
+    uint32_t rows, vocab, hidden;
+    uint32_t ldx, ldw, lddx, lddw;  /* elements; 0 = packed                            */
+    uint32_t transpose;             /* T0G_NT or T0G_NN: how w is stored               */
+    uint32_t label_type;            /* t0g_index_type                                  */
+    uint32_t dx_dtype, dw_dtype;    /* t0g_dtype                                       */
+    uint32_t max_piece;             /* tokens per piece of the vocabulary, at most; 0 = by size */
+    float loss_scale;
+    float logit_scale;              /* > 0                                             */
+} t0g_linear_ce_desc;
+typedef struct t0g_linear_distill_desc {
+    t0g_linear_ce_desc head;        /* labels may be 0: no cross entropy part          */
+    uint64_t teacher;               /* teacher_dtype [rows][ldt]: logits, in any order */
+    uint64_t tokens;                /* token_type [rows][ldt]: their tokens            */
+    uint32_t top_k;                 /* entries per row, 1 to 1024                      */
+    uint32_t ldt;                   /* elements; 0 = packed                            */
+    uint32_t teacher_dtype;         /* t0g_dtype                                       */
+    uint32_t token_type;            /* t0g_index_type                                  */
+    float temperature;              /* > 0                                             */
+    float label_weight, distill_weight;
+    uint32_t reserved;              /* 0                                               */
+} t0g_linear_distill_desc;
+T0G_API int t0g_linear_cross_entropy(t0g_device *dev, const t0g_linear_ce_desc *desc);
+T0G_API int t0g_linear_distill(t0g_device *dev, const t0g_linear_distill_desc *desc);
+/* Bytes of the handle's scratch that a call takes (host only; checks the
+ * descriptor as the call does). */
+T0G_API int t0g_linear_cross_entropy_scratch_size(const t0g_linear_ce_desc *desc, size_t *bytes);
+T0G_API int t0g_linear_distill_scratch_size(const t0g_linear_distill_desc *desc, size_t *bytes);
+
 /* ---- GEMM autotuner and its on-disk cache ----------------------------------- *
  * GemmTuner (src/t0/auto_gemm.rs:28-417): benchmark the model's best candidate
  * configs on the GPU, keep the fastest, cache it in memory and as one JSON file

@@ -1,0 +1,366 @@
+// Losses of a projection onto a vocabulary for MI355X (gfx950): the row kernels
+// around its GEMMs.  z = x W^T is taken in pieces of the vocabulary; per row the
+// softmax statistics of a chunk of columns are m = max u and s = sum 2^(u - m),
+// u = z k in units of log 2, and chunks are joined as
+//   M = max m,  S = sum s 2^(m - M),  log2 sum 2^u = M + log2 S.
+// All statistics, losses and coefficients are f32.  The logit gradients are
+// rounded to bf16 once, because the products that take them on to dx and dW
+// multiply bf16 operands.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "t0g_kernel_args.h"
+
+namespace t0g {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+template <class T>
+using gptr = __attribute__((address_space(1))) T*;
+template <class T>
+__device__ __forceinline__ gptr<T> at(uint64_t base, uint64_t i = 0) {
+    return reinterpret_cast<gptr<T>>((uintptr_t)base) + i;
+}
+
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr uint32_t kNoToken = 0xFFFFFFFFu;
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float ninf() { return -__builtin_inff(); }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// Over the workgroup's four waves; `t` is 4 floats of LDS of this call's own.
+__device__ __forceinline__ float block_max(float v, float* t) {
+    v = wave_max(v);
+    if ((threadIdx.x & 63u) == 0) t[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return __builtin_fmaxf(__builtin_fmaxf(t[0], t[1]), __builtin_fmaxf(t[2], t[3]));
+}
+__device__ __forceinline__ float block_sum(float v, float* t) {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63u) == 0) t[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (t[0] + t[1]) + (t[2] + t[3]);
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16);
+}
+
+// A label or token as an index into the vocabulary, kNoToken outside it.
+__device__ __forceinline__ uint32_t token_at(uint64_t base, uint64_t i, bool wide, uint32_t vocab) {
+    const int64_t v = wide ? *at<const int64_t>(base, i) : (int64_t)*at<const int32_t>(base, i);
+    return v >= 0 && v < (int64_t)vocab ? (uint32_t)v : kNoToken;
+}
+
+// Row `row` of x into xz, zero for an ignored row (its hidden state may hold NaN, and
+// dW's product would multiply that with the row's zero gradient) and past `hidden`.
+__device__ __forceinline__ void copy_row(const T0gLossArgs& p, uint32_t row, bool used) {
+    if (p.flags & T0G_LOSS_X_VEC) {
+        const uint32_t n = p.hidden / 8;
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+            u32x4_t v = {0u, 0u, 0u, 0u};
+            if (used) v = *at<const u32x4_t>(p.x + (uint64_t)row * p.ldx * 2, i);
+            *at<u32x4_t>(p.xz + (uint64_t)row * p.ldxz * 2, i) = v;
+        }
+    } else {
+        for (uint32_t i = threadIdx.x; i < p.ldxz; i += kThreads) {
+            uint16_t v = 0;
+            if (used && i < p.hidden) v = *at<const uint16_t>(p.x, (uint64_t)row * p.ldx + i);
+            *at<uint16_t>(p.xz, (uint64_t)row * p.ldxz + i) = v;
+        }
+    }
+}
+
+// What a row is compared with: its label and the teacher's distribution over its
+// tokens, as entries sorted by token with equal tokens joined (their probabilities
+// add), so that each entry is one logit.  A rank sort in LDS: keys are unique
+// (token, then position), so sums of equal tokens run in the order they were given.
+__device__ __forceinline__ void prepare_row(const T0gLossArgs& p, uint32_t row) {
+    constexpr uint32_t N = T0G_LOSS_MAX_TOP + 1;
+    __shared__ uint32_t tok[N], srt[N];
+    __shared__ float q[N], sq[N];
+    __shared__ float red[3][4];
+    __shared__ uint32_t wave_heads[4];
+    const uint32_t tid = threadIdx.x;
+    const uint32_t label = p.labels ? token_at(p.labels, row, p.flags & T0G_LOSS_LABEL64, p.vocab) : kNoToken;
+    const float rate = p.loss_scale * (p.dloss ? *at<const float>(p.dloss, row) : 1.0f) * p.logit_scale;
+    const float cl = label != kNoToken ? p.label_weight * rate : 0.0f;
+    uint32_t n = 0, label_slot = kNoToken;
+    float hq = 0.0f;
+    bool taught = false;
+    if (!p.teacher) {
+        n = label != kNoToken;
+        label_slot = n ? 0u : kNoToken;
+        if (tid == 0) {
+            *at<uint32_t>(p.ent_tok, (uint64_t)row * p.slots) = label;
+            *at<float>(p.ent_q, (uint64_t)row * p.slots) = 0.0f;
+        }
+    } else {
+        const uint32_t k = p.top_k, total = k + 1;
+        float top = ninf();
+        for (uint32_t i = tid; i < k; i += kThreads) {
+            const uint64_t src = (uint64_t)row * p.ldt + i;
+            uint32_t t = token_at(p.tokens, src, p.flags & T0G_LOSS_TOKEN64, p.vocab);
+            float u = (p.flags & T0G_LOSS_TEACHER16)
+                          ? (float)__builtin_bit_cast(__bf16, *at<const uint16_t>(p.teacher, src))
+                          : *at<const float>(p.teacher, src);
+            if (u == ninf()) t = kNoToken;   // no probability: not an entry
+            tok[i] = t;
+            q[i] = u;
+            if (t != kNoToken) top = __builtin_fmaxf(top, u);
+        }
+        if (tid == 0) {
+            tok[k] = label;
+            q[k] = 0.0f;
+        }
+        top = block_max(top, red[0]);
+        float sum = 0.0f, any = 0.0f;
+        const float scale = 1.44269504f / p.tau;
+        for (uint32_t i = tid; i < k; i += kThreads) {
+            float e = 0.0f;
+            if (tok[i] != kNoToken) {
+                e = exp2_((q[i] - top) * scale);
+                any = 1.0f;
+            }
+            q[i] = e;
+            sum += e;
+        }
+        sum = block_sum(sum, red[1]);
+        any = block_max(any, red[2]);
+        taught = any > 0.0f;
+        const float inv = taught ? 1.0f / sum : 0.0f;
+        for (uint32_t i = tid; i < total; i += kThreads) {
+            const uint32_t t = tok[i];
+            uint32_t rank = 0;
+            for (uint32_t j = 0; j < total; ++j) {
+                const uint32_t o = tok[j];
+                rank += o < t || (o == t && j < i);
+            }
+            srt[rank] = t;
+            sq[rank] = q[i] * inv;
+        }
+        __syncthreads();
+        // first entries of equal tokens, numbered in order
+        float part = 0.0f;
+        for (uint32_t i0 = 0; i0 < total; i0 += kThreads) {
+            const uint32_t i = i0 + tid;
+            const bool head = i < total && srt[i] != kNoToken && (i == 0 || srt[i - 1] != srt[i]);
+            const uint64_t mask = __ballot(head);
+            const uint32_t lane = tid & 63u, wave = tid >> 6;
+            if (lane == 0) wave_heads[wave] = (uint32_t)__popcll(mask);
+            __syncthreads();
+            uint32_t slot = n + (uint32_t)__popcll(mask & ((1ull << lane) - 1));
+            for (uint32_t w = 0; w < wave; ++w) slot += wave_heads[w];
+            n += wave_heads[0] + wave_heads[1] + wave_heads[2] + wave_heads[3];
+            if (head) {
+                float v = 0.0f;
+                for (uint32_t j = i; j < total && srt[j] == srt[i]; ++j) v += sq[j];
+                *at<uint32_t>(p.ent_tok, (uint64_t)row * p.slots + slot) = srt[i];
+                *at<float>(p.ent_q, (uint64_t)row * p.slots + slot) = v;
+                if (srt[i] == label) tok[0] = slot;
+                if (!(v < 1.2e-38f)) part += v * (__builtin_amdgcn_logf(v) * kLn2);   // 0 log 0 = 0; v_log takes no denormals
+            }
+            __syncthreads();
+        }
+        if (label != kNoToken) label_slot = tok[0];
+        __syncthreads();
+        hq = block_sum(part, red[0]);
+    }
+    if (tid == 0) {
+        *at<u32x2_t>(p.row_ent, row) = u32x2_t{n, label_slot};
+        *at<f32x4_t>(p.row_sub, row) =
+            f32x4_t{cl, taught ? p.distill_weight * p.tau * rate : 0.0f, hq, taught ? 1.0f : 0.0f};
+    }
+    if (p.xz) copy_row(p, row, label != kNoToken || taught);
+    __syncthreads();
+}
+
+// Statistics of one chunk of a row of raw logits, and the raw logits of the row's
+// entries in it.
+__device__ __forceinline__ void chunk_stats(const T0gLossArgs& p, uint32_t row, uint32_t chunk) {
+    __shared__ float red[3][4];
+    const uint32_t c0 = chunk * T0G_LOSS_CHUNK, tid = threadIdx.x;
+    const uint64_t base = p.z + ((uint64_t)row * p.ldz + c0) * 4;
+    const uint32_t n = min(T0G_LOSS_CHUNK, p.cols - c0);
+    f32x4_t v[4];
+    float m = ninf();
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t c = (i * kThreads + tid) * 4;
+        v[i] = f32x4_t{ninf(), ninf(), ninf(), ninf()};
+        if (c < n) {   // rows are padded to whole quads
+            v[i] = *at<const f32x4_t>(base, c / 4);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                v[i][e] = c + e < n ? v[i][e] * p.k : ninf();
+                m = __builtin_fmaxf(m, v[i][e]);
+            }
+        }
+    }
+    m = block_max(m, red[0]);
+    float s = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            if ((i * kThreads + tid) * 4 + e >= n) continue;
+            s += exp2_(v[i][e] - m);
+            if (p.flags & T0G_LOSS_DUAL) s2 += exp2_((v[i][e] - m) * p.r);
+        }
+    s = block_sum(s, red[1]);
+    if (p.flags & T0G_LOSS_DUAL) s2 = block_sum(s2, red[2]);
+    if (tid == 0) {
+        const uint64_t i = (uint64_t)(p.chunk0 + chunk) * p.rows + row;
+        *at<f32x2_t>(p.part, i) = f32x2_t{m, s};
+        if (p.flags & T0G_LOSS_DUAL) *at<float>(p.part2, i) = s2;
+    }
+    const uint32_t entries = (*at<const u32x2_t>(p.row_ent, row))[0];
+    for (uint32_t e = tid; e < entries; e += kThreads) {
+        const uint64_t slot = (uint64_t)row * p.slots + e;
+        const uint32_t c = *at<const uint32_t>(p.ent_tok, slot) - (p.v0 + c0);   // wraps below the chunk
+        if (c < n) *at<float>(p.ent_z, slot) = *at<const float>(base, c);
+    }
+    __syncthreads();
+}
+
+// A row's chunks joined: its loss, log-sum-exp and gradient coefficients.  One wave.
+__device__ __forceinline__ void combine_row(const T0gLossArgs& p, uint32_t row) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const bool dual = p.flags & T0G_LOSS_DUAL;
+    float m = ninf();
+    for (uint32_t c = lane; c < p.chunks; c += 64)
+        m = __builtin_fmaxf(m, (*at<const f32x2_t>(p.part, (uint64_t)c * p.rows + row))[0]);
+    m = wave_max(m);
+    float s = 0.0f, s2 = 0.0f;
+    for (uint32_t c = lane; c < p.chunks; c += 64) {
+        const uint64_t i = (uint64_t)c * p.rows + row;
+        const f32x2_t v = *at<const f32x2_t>(p.part, i);
+        s += v[1] * exp2_(v[0] - m);
+        if (dual) s2 += *at<const float>(p.part2, i) * exp2_((v[0] - m) * p.r);
+    }
+    s = wave_sum(s);
+    const float l0 = m + __builtin_amdgcn_logf(s);
+    float l1 = l0;
+    if (dual) l1 = m * p.r + __builtin_amdgcn_logf(wave_sum(s2));
+    const u32x2_t ent = *at<const u32x2_t>(p.row_ent, row);
+    const f32x4_t sub = *at<const f32x4_t>(p.row_sub, row);
+    const bool taught = sub[3] != 0.0f, labelled = ent[1] != kNoToken;
+    float kd = 0.0f;
+    if (taught)
+        for (uint32_t e = lane; e < ent[0]; e += 64) {
+            const uint64_t slot = (uint64_t)row * p.slots + e;
+            const float q = *at<const float>(p.ent_q, slot);
+            if (q != 0.0f) kd += q * (l1 * kLn2 - *at<const float>(p.ent_z, slot) * (p.logit_scale / p.tau));
+        }
+    kd = wave_sum(kd);
+    if (lane != 0) return;
+    float loss = 0.0f;
+    if (labelled)
+        loss = p.label_weight *
+               (l0 * kLn2 - *at<const float>(p.ent_z, (uint64_t)row * p.slots + ent[1]) * p.logit_scale);
+    if (taught) loss += p.distill_weight * p.tau * p.tau * (sub[2] + kd);
+    const bool used = labelled || taught;
+    *at<float>(p.loss, row) = loss;
+    if (p.lse) *at<float>(p.lse, row) = used ? l1 * kLn2 : 0.0f;
+    if (p.row_par)
+        *at<f32x4_t>(p.row_par, row) = !used  ? f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}
+                                       : dual ? f32x4_t{l0, l1, sub[0], sub[1]}
+                                              : f32x4_t{l0, l1, sub[0] + sub[1], 0.0f};
+}
+
+// The dense part of a logit's gradient.
+__device__ __forceinline__ float dense_grad(const T0gLossArgs& p, const f32x4_t& par, float z) {
+    const float u = z * p.k;
+    float g = par[2] * exp2_(u - par[0]);
+    if (p.flags & T0G_LOSS_DUAL) g += par[3] * exp2_(u * p.r - par[1]);
+    return g;
+}
+
+// Logit gradients of one chunk of a row in bf16, zero past the piece, then its entries.
+__device__ __forceinline__ void chunk_grad(const T0gLossArgs& p, uint32_t row, uint32_t chunk) {
+    const uint32_t c0 = chunk * T0G_LOSS_CHUNK, tid = threadIdx.x;
+    const uint64_t zb = p.z + ((uint64_t)row * p.ldz + c0) * 4, gb = p.g + ((uint64_t)row * p.ldg + c0) * 2;
+    const uint32_t n = min(T0G_LOSS_CHUNK, p.cols - c0), ng = min(T0G_LOSS_CHUNK, p.ldg - c0);
+    const f32x4_t par = *at<const f32x4_t>(p.row_par, row);
+    const bool used = par[2] != 0.0f || par[3] != 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t c = (i * kThreads + tid) * 4;
+        if (c >= ng) continue;
+        float g[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (used && c < n) {
+            const f32x4_t z = *at<const f32x4_t>(zb, c / 4);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) g[e] = c + e < n ? dense_grad(p, par, z[e]) : 0.0f;
+        }
+        *at<u32x2_t>(gb, c / 4) = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
+    }
+    __syncthreads();   // the dense part is written before its entries are replaced
+    if (used) {
+        const u32x2_t ent = *at<const u32x2_t>(p.row_ent, row);
+        const f32x4_t sub = *at<const f32x4_t>(p.row_sub, row);
+        for (uint32_t e = tid; e < ent[0]; e += kThreads) {
+            const uint64_t slot = (uint64_t)row * p.slots + e;
+            const uint32_t c = *at<const uint32_t>(p.ent_tok, slot) - (p.v0 + c0);
+            if (c >= n) continue;
+            float g = dense_grad(p, par, *at<const float>(p.ent_z, slot)) - sub[1] * *at<const float>(p.ent_q, slot);
+            if (e == ent[1]) g -= sub[0];
+            *at<__bf16>(gb, c) = (__bf16)g;
+        }
+    }
+}
+
+__device__ __forceinline__ void sum_planes(const T0gLossSumArgs& p) {
+    const uint64_t total = (uint64_t)p.rows * p.cols;
+    const uint32_t w = p.vec ? 4 : 1;
+    for (uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) * w; i < total;
+         i += (uint64_t)gridDim.x * kThreads * w) {
+        const uint64_t o = i / p.cols * p.ldo + i % p.cols;
+        if (p.vec) {
+            f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (p.acc) v = *at<const f32x4_t>(p.acc, i / 4);
+            for (uint32_t s = 0; s < p.n; ++s) v += *at<const f32x4_t>(p.planes + (uint64_t)s * total * 4, i / 4);
+            if (p.out_bf16)
+                *at<u32x2_t>(p.out, o / 4) = u32x2_t{pack2(v[0], v[1]), pack2(v[2], v[3])};
+            else
+                *at<f32x4_t>(p.out, o / 4) = v;
+        } else {
+            float v = p.acc ? *at<const float>(p.acc, i) : 0.0f;
+            for (uint32_t s = 0; s < p.n; ++s) v += *at<const float>(p.planes, (uint64_t)s * total + i);
+            if (p.out_bf16)
+                *at<__bf16>(p.out, o) = (__bf16)v;
+            else
+                *at<float>(p.out, o) = v;
+        }
+    }
+}
+
+}  // namespace t0g
+
+extern "C" __global__ void __launch_bounds__(256) t0g_loss_prepare(T0gLossArgs p) {
+    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) t0g::prepare_row(p, row);
+}
+extern "C" __global__ void __launch_bounds__(256) t0g_loss_stats(T0gLossArgs p) {
+    for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) t0g::chunk_stats(p, row, blockIdx.x);
+}
+extern "C" __global__ void __launch_bounds__(256) t0g_loss_combine(T0gLossArgs p) {
+    for (uint32_t row = blockIdx.x * 4 + threadIdx.x / 64; row < p.rows; row += gridDim.x * 4) t0g::combine_row(p, row);
+}
+extern "C" __global__ void __launch_bounds__(256) t0g_loss_grad(T0gLossArgs p) {
+    for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) t0g::chunk_grad(p, row, blockIdx.x);
+}
+extern "C" __global__ void __launch_bounds__(256) t0g_loss_sum(T0gLossSumArgs p) { t0g::sum_planes(p); }

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <functional>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -74,6 +75,19 @@ uint32_t chain_kernarg_bytes(uint32_t chain);      // tile_ir arguments after M
 // Device time (ms) of each of `iters` t0g_gemm launches of d, after `warmup`
 // untimed ones (t0g_runtime.cpp).
 int time_gemm(t0g_device *dev, const t0g_gemm_desc *d, uint32_t warmup, uint32_t iters, std::vector<double> *ms);
+
+// What the losses (t0g_losses.cpp) use of a device handle.  The caller holds
+// device_mutex() throughout.
+std::mutex &device_mutex(t0g_device *dev);
+// Before a call's launches: the handle is usable, the losses' code object loaded and a
+// scratch of `bytes` there.  Nothing of it is done under stream capture, where a call
+// that would need it is refused.
+int losses_begin(t0g_device *dev, size_t bytes, uint64_t *scratch);
+// Launch kernel `symbol` of the losses' code object on the device stream.
+int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, void *args, size_t args_size);
+// Workspace t0g_gemm may use for d (host only), and the GEMM itself.
+int losses_gemm_workspace(const t0g_gemm_desc *d, size_t *bytes);
+int losses_gemm(t0g_device *dev, const t0g_gemm_desc *d);
 
 // One kernel's entry in a code object's AMDGPU metadata (t0g_codeobj.cpp).
 struct KernelMeta {

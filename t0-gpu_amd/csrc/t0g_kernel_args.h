@@ -154,6 +154,61 @@ typedef struct T0gConvertPairArgs {
 #define T0G_REDUCE_WAVE 4u      /* as VEC; each wave takes 512 consecutive elements per step     */
 #define T0G_CONVERT_VEC 1u      /* src 16-byte and dst 8-byte aligned, n % 4 == 0: 16-byte loads */
 
+/* The losses over a vocabulary (losses_gfx950.hip).  With u = z * k the scaled logit in
+ * units of log 2 (z: a raw product x . w, k: logit scale, temperature and log2 e), a
+ * row's statistics are the sum of 2^(u - m) and, with T0G_LOSS_DUAL, of 2^((u - m) r):
+ * the labels' softmax and the teacher's at another temperature.  A logit's gradient is
+ * c0 2^(u - l0) [+ c1 2^(u r - l1)], less a sparse part at the row's entries: its label and
+ * the teacher's tokens, sorted and each token once. */
+typedef struct T0gLossArgs {
+    uint64_t x;              /* bf16 [rows][ldx]: the hidden states                   */
+    uint64_t xz;             /* bf16 [rows][ldxz]: their copy, ignored rows zero; or 0 */
+    uint64_t labels;         /* i32|i64 [rows] or 0                                   */
+    uint64_t dloss;          /* f32 [rows] or 0 (ones)                                */
+    uint64_t teacher;        /* f32|bf16 [rows][ldt]: the teacher's logits, or 0      */
+    uint64_t tokens;         /* i32|i64 [rows][ldt]: their tokens                     */
+    uint64_t loss;           /* f32 [rows]                                            */
+    uint64_t lse;            /* f32 [rows] or 0                                       */
+    uint64_t ent_tok;        /* u32 [rows][slots]: entries' tokens, ascending         */
+    uint64_t ent_q;          /* f32 [rows][slots]: the teacher's probability          */
+    uint64_t ent_z;          /* f32 [rows][slots]: the entry's raw logit              */
+    uint64_t row_ent;        /* i32 [rows][2]: entries, and the label's (-1: none)    */
+    uint64_t row_sub;        /* f32 [rows][4]: label and teacher coefficients of the sparse
+                                part (0: none), sum of Q log Q, teacher present (1 or 0) */
+    uint64_t row_par;        /* f32 [rows][4]: l0, l1, c0, c1                         */
+    uint64_t part;           /* f32 [chunks][rows][2]: m and the sum                  */
+    uint64_t part2;          /* f32 [chunks][rows]: the second sum (DUAL)             */
+    uint64_t z;              /* f32 [rows][ldz]: a piece's raw logits                 */
+    uint64_t g;              /* bf16 [rows][ldg]: a piece's logit gradients           */
+    uint32_t rows, vocab, hidden, ldx, ldxz;
+    uint32_t top_k, ldt, slots;
+    uint32_t v0, cols;       /* the piece: its first token and width                  */
+    uint32_t ldz, ldg;
+    uint32_t chunk0;         /* the piece's first chunk                               */
+    uint32_t chunks;         /* chunks of the piece, or of the vocabulary (combine)   */
+    uint32_t flags;          /* T0G_LOSS_* bits                                       */
+    float k, r;              /* u = z k; second temperature's ratio                   */
+    float logit_scale, tau;
+    float label_weight, distill_weight;
+    float loss_scale;
+} T0gLossArgs;
+#define T0G_LOSS_LABEL64 1u    /* labels are i64                                       */
+#define T0G_LOSS_TOKEN64 2u    /* the teacher's tokens are i64                         */
+#define T0G_LOSS_TEACHER16 4u  /* the teacher's logits are bf16                        */
+#define T0G_LOSS_DUAL 8u       /* labels and a teacher of another temperature          */
+#define T0G_LOSS_X_VEC 16u     /* x rows are 16-byte aligned and hidden a multiple of 8 */
+#define T0G_LOSS_CHUNK 4096u   /* columns of one workgroup in the row kernels          */
+#define T0G_LOSS_MAX_TOP 1024u /* teacher entries of a row, at most                    */
+
+/* Sum of f32 planes of a data gradient, in order, into bf16 or f32 rows. */
+typedef struct T0gLossSumArgs {
+    uint64_t acc;            /* f32 [rows][cols] summed before, or 0                  */
+    uint64_t planes;         /* f32 [n][rows][cols]                                   */
+    uint64_t out;            /* f32 | bf16 [rows][ldo]                                */
+    uint32_t n, rows, cols, ldo;
+    uint32_t out_bf16, vec;  /* vec: cols and ldo multiples of 4, out 16-byte aligned */
+} T0gLossSumArgs;
+
 /* Epilogue chain operations: tile_ir's EpilogueOp (src/t0/tile_ir.rs:41-62),
  * applied in chain order to each fp32 result before the output conversion. */
 #define T0G_EPI_OP_BIAS_ADD 1u  /* x += bias[col]                                  */

@@ -1,0 +1,408 @@
+// Losses of a projection onto a vocabulary: argument checks, the pieces of the
+// vocabulary, the scratch and the launches.  The kernels are in
+// losses_gfx950.hip; the products are the library's own GEMMs.
+//
+// One call runs
+//   prepare   every row's entries (label, teacher's tokens), the masked copy of x
+//   pieces    z = x W_p^T, the chunks' softmax statistics, the entries' logits
+//   combine   loss, log-sum-exp and gradient coefficients of every row
+//   pieces    again, last first, for the gradients: z (the last piece's is still
+//             there), G = dL/dz in bf16, dx += G W_p, dW_p = G^T x
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "t0g.h"
+#include "t0g_internal.h"
+#include "t0g_kernel_args.h"
+
+namespace t0g {
+
+namespace {
+
+// A piece's f32 logits, and the f32 partial sums of dx, take about this much each.
+constexpr uint64_t kPieceBytes = 256ull << 20;
+// Rows of a launch's y grid, at most (the kernels step through the rest).
+constexpr uint32_t kMaxGridY = 65535;
+
+struct Range {
+    uint64_t begin, end;
+    const char *name;
+};
+
+struct Problem {
+    t0g_linear_ce_desc d;                 // leading dimensions filled in
+    const t0g_linear_distill_desc *t;     // the teacher, or nullptr
+    uint32_t ldt;
+    bool grad, dual;
+};
+
+// Bytes from the first to the last element of a [rows][cols] array with leading dimension ld.
+uint64_t extent(uint64_t rows, uint64_t cols, uint64_t ld, uint64_t size) {
+    return rows && cols ? ((rows - 1) * ld + cols) * size : 0;
+}
+
+uint32_t dtype_size(uint32_t t) { return t == T0G_BF16 ? 2 : 4; }
+uint32_t index_size(uint32_t t) { return t == T0G_I64 ? 8 : 4; }
+
+int check_ld(const char *name, uint32_t *ld, uint32_t cols) {
+    if (*ld == 0) *ld = cols;
+    if (*ld < cols) return fail(T0G_ERR_INVALID_ARG, "%s=%u < %u", name, *ld, cols);
+    return T0G_OK;
+}
+
+int check_problem(const t0g_linear_ce_desc *desc, const t0g_linear_distill_desc *t, Problem *p) {
+    p->d = *desc;
+    p->t = t;
+    t0g_linear_ce_desc &d = p->d;
+    if (d.transpose > T0G_NN) return fail(T0G_ERR_INVALID_ARG, "transpose %u: the weight is NT or NN", d.transpose);
+    if (d.label_type > T0G_I64) return fail(T0G_ERR_INVALID_ARG, "bad label_type %u", d.label_type);
+    if (d.dx_dtype > T0G_BF16 || d.dw_dtype > T0G_BF16)
+        return fail(T0G_ERR_INVALID_ARG, "bad gradient type (dx %u, dw %u)", d.dx_dtype, d.dw_dtype);
+    if (d.vocab == 0 || d.hidden == 0 || d.vocab > 0x7FFFFFFFu || d.rows > 0x7FFFFFFFu)
+        return fail(T0G_ERR_INVALID_ARG, "bad size: %u rows, vocab %u, hidden %u", d.rows, d.vocab, d.hidden);
+    if (!isfinite(d.logit_scale) || d.logit_scale <= 0.0f)
+        return fail(T0G_ERR_INVALID_ARG, "logit_scale %g", (double)d.logit_scale);
+    const bool nt = d.transpose == T0G_NT;
+    const uint32_t wr = nt ? d.vocab : d.hidden, wc = nt ? d.hidden : d.vocab;
+    int rc;
+    if ((rc = check_ld("ldx", &d.ldx, d.hidden)) || (rc = check_ld("ldw", &d.ldw, wc)) ||
+        (rc = check_ld("lddx", &d.lddx, d.hidden)) || (rc = check_ld("lddw", &d.lddw, wc)))
+        return rc;
+    if (!d.w || (d.rows && (!d.x || !d.loss))) return fail(T0G_ERR_INVALID_ARG, "NULL operand");
+    if (d.rows && !t && !d.labels) return fail(T0G_ERR_INVALID_ARG, "cross entropy without labels");
+    p->ldt = 0;
+    if (t) {
+        if (t->reserved) return fail(T0G_ERR_INVALID_ARG, "reserved must be 0");
+        if (t->top_k == 0 || t->top_k > T0G_LOSS_MAX_TOP)
+            return fail(T0G_ERR_INVALID_ARG, "top_k %u (1 to %u)", t->top_k, T0G_LOSS_MAX_TOP);
+        if (t->teacher_dtype > T0G_BF16 || t->token_type > T0G_I64)
+            return fail(T0G_ERR_INVALID_ARG, "bad teacher_dtype %u or token_type %u", t->teacher_dtype, t->token_type);
+        if (!isfinite(t->temperature) || t->temperature <= 0.0f)
+            return fail(T0G_ERR_INVALID_ARG, "temperature %g", (double)t->temperature);
+        p->ldt = t->ldt;
+        if ((rc = check_ld("ldt", &p->ldt, t->top_k))) return rc;
+        if (d.rows && (!t->teacher || !t->tokens)) return fail(T0G_ERR_INVALID_ARG, "NULL teacher");
+    }
+    // every array on its element's alignment, and no output over another array
+    std::vector<Range> in, out;
+    auto add = [&](std::vector<Range> &v, const char *name, uint64_t a, uint64_t rows, uint64_t cols, uint64_t ld,
+                   uint32_t size) {
+        if (!a) return (int)T0G_OK;
+        if (a % size) return fail(T0G_ERR_INVALID_ARG, "%s is not aligned to its elements of %u bytes", name, size);
+        v.push_back(Range{a, a + extent(rows, cols, ld, size), name});
+        return (int)T0G_OK;
+    };
+    if ((rc = add(in, "x", d.x, d.rows, d.hidden, d.ldx, 2)) || (rc = add(in, "w", d.w, wr, wc, d.ldw, 2)) ||
+        (rc = add(in, "labels", d.labels, 1, d.rows, d.rows, index_size(d.label_type))) ||
+        (rc = add(in, "dloss", d.dloss, 1, d.rows, d.rows, 4)) ||
+        (rc = add(out, "loss", d.loss, 1, d.rows, d.rows, 4)) || (rc = add(out, "lse", d.lse, 1, d.rows, d.rows, 4)) ||
+        (rc = add(out, "dx", d.dx, d.rows, d.hidden, d.lddx, dtype_size(d.dx_dtype))) ||
+        (rc = add(out, "dw", d.dw, wr, wc, d.lddw, dtype_size(d.dw_dtype))))
+        return rc;
+    if (t && ((rc = add(in, "teacher", t->teacher, d.rows, t->top_k, p->ldt, dtype_size(t->teacher_dtype))) ||
+              (rc = add(in, "tokens", t->tokens, d.rows, t->top_k, p->ldt, index_size(t->token_type)))))
+        return rc;
+    for (size_t i = 0; i < out.size(); ++i) {
+        auto meets = [&](const Range &r) { return out[i].begin < r.end && r.begin < out[i].end; };
+        for (const Range &r : in)
+            if (meets(r)) return fail(T0G_ERR_INVALID_ARG, "%s overlaps %s", out[i].name, r.name);
+        for (size_t j = 0; j < i; ++j)
+            if (meets(out[j])) return fail(T0G_ERR_INVALID_ARG, "%s overlaps %s", out[i].name, out[j].name);
+    }
+    p->grad = d.dx || d.dw;
+    p->dual = t && d.labels && t->temperature != 1.0f;
+    return T0G_OK;
+}
+
+struct Piece {
+    uint32_t v0, cols, chunk0, chunks;
+};
+
+// The pieces, and where everything is in the scratch.
+struct Plan {
+    std::vector<Piece> pieces;
+    uint32_t chunks = 0, slots = 0, ldxz = 0;
+    uint32_t group = 0;          // planes of dx summed at a time (0: the one product writes dx)
+    uint64_t xz = 0, ent_tok = 0, ent_q = 0, ent_z = 0, row_ent = 0, row_sub = 0, row_par = 0, part = 0, part2 = 0;
+    uint64_t z = 0, g = 0, planes = 0, acc = 0, gemm_ws = 0;
+    uint64_t gemm_ws_bytes = 0, bytes = 0;
+};
+
+uint32_t round_up(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
+
+// The GEMMs of a piece; addresses in the scratch are offsets from `base`.
+t0g_gemm_desc gemm_of(uint64_t a, uint64_t b, uint64_t c, uint32_t m, uint32_t n, uint32_t k, uint32_t lda, uint32_t ldb,
+                      uint32_t ldc, uint32_t transpose, uint32_t dtype) {
+    t0g_gemm_desc g;
+    memset(&g, 0, sizeof g);
+    g.a = a;
+    g.b = b;
+    g.c = c;
+    g.m = m;
+    g.n = n;
+    g.k = k;
+    g.lda = lda;
+    g.ldb = ldb;
+    g.ldc = ldc;
+    g.transpose = transpose;
+    g.out_dtype = dtype;
+    return g;
+}
+
+uint64_t weight_piece(const Problem &p, uint64_t w, uint32_t v0, uint32_t ld, uint32_t size) {
+    return w + (p.d.transpose == T0G_NT ? (uint64_t)v0 * ld : v0) * size;
+}
+
+t0g_gemm_desc logits_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
+    const t0g_linear_ce_desc &d = p.d;
+    return gemm_of(p.grad ? base + pl.xz : d.x, weight_piece(p, d.w, pc.v0, d.ldw, 2), base + pl.z, d.rows, pc.cols,
+                   d.hidden, p.grad ? pl.ldxz : d.ldx, d.ldw, round_up(pc.cols, 4), d.transpose, T0G_F32);
+}
+
+// dx of a piece: the output itself, or f32 plane `plane`.
+t0g_gemm_desc dx_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base, uint32_t plane) {
+    const t0g_linear_ce_desc &d = p.d;
+    const bool whole = pl.group == 0;
+    return gemm_of(base + pl.g, weight_piece(p, d.w, pc.v0, d.ldw, 2),
+                   whole ? d.dx : base + pl.planes + (uint64_t)plane * d.rows * d.hidden * 4, d.rows, d.hidden, pc.cols,
+                   round_up(pc.cols, 8), d.ldw, whole ? d.lddx : d.hidden, d.transpose == T0G_NT ? T0G_NN : T0G_NT,
+                   whole ? d.dx_dtype : (uint32_t)T0G_F32);
+}
+
+t0g_gemm_desc dw_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
+    const t0g_linear_ce_desc &d = p.d;
+    const uint64_t c = weight_piece(p, d.dw, pc.v0, d.lddw, dtype_size(d.dw_dtype));
+    const uint32_t ldg = round_up(pc.cols, 8);
+    return d.transpose == T0G_NT
+               ? gemm_of(base + pl.g, base + pl.xz, c, pc.cols, d.hidden, d.rows, ldg, pl.ldxz, d.lddw, T0G_TN, d.dw_dtype)
+               : gemm_of(base + pl.xz, base + pl.g, c, d.hidden, pc.cols, d.rows, pl.ldxz, ldg, d.lddw, T0G_TN, d.dw_dtype);
+}
+
+int make_loss_plan(const Problem &p, Plan *pl) {
+    const t0g_linear_ce_desc &d = p.d;
+    const uint64_t rows = d.rows ? d.rows : 1;
+    // A vocabulary that is not a multiple of 8 gets its last few tokens as a piece of their
+    // own where they alone would keep the products off the aligned kernels.
+    const bool aligned = (d.w & 15) == 0 && d.ldw % 8 == 0 && d.hidden % 8 == 0;
+    const uint32_t body = aligned && d.vocab > 8 && (p.grad || d.transpose == T0G_NN) ? d.vocab & ~7u : d.vocab;
+    uint64_t width = std::max<uint64_t>(256, kPieceBytes / (rows * 4) / 256 * 256);
+    if (d.max_piece) width = std::min<uint64_t>(width, d.max_piece <= 8 ? 8 : d.max_piece & ~7u);
+    for (uint32_t v0 = 0; v0 < d.vocab;) {
+        const uint32_t end = v0 < body ? body : d.vocab;
+        const uint32_t cols = (uint32_t)std::min<uint64_t>(width, end - v0);
+        const uint32_t chunks = (cols + T0G_LOSS_CHUNK - 1) / T0G_LOSS_CHUNK;
+        pl->pieces.push_back(Piece{v0, cols, pl->chunks, chunks});
+        pl->chunks += chunks;
+        v0 += cols;
+    }
+    pl->slots = 1 + (p.t ? p.t->top_k : 0);
+    pl->ldxz = round_up(d.hidden, 8);
+    const uint64_t plane = rows * d.hidden * 4;
+    if (d.dx && pl->pieces.size() > 1)
+        pl->group = (uint32_t)std::min<uint64_t>(pl->pieces.size(), std::max<uint64_t>(1, kPieceBytes / plane));
+
+    uint64_t at = 0;
+    auto take = [&](uint64_t bytes) {
+        const uint64_t a = at;
+        at += (bytes + 255) & ~255ull;
+        return a;
+    };
+    uint32_t widest = 0;
+    for (const Piece &pc : pl->pieces) widest = std::max(widest, pc.cols);
+    if (p.grad) pl->xz = take(rows * pl->ldxz * 2);
+    pl->ent_tok = take(rows * pl->slots * 4);
+    pl->ent_q = take(rows * pl->slots * 4);
+    pl->ent_z = take(rows * pl->slots * 4);
+    pl->row_ent = take(rows * 8);
+    pl->row_sub = take(rows * 16);
+    if (p.grad) pl->row_par = take(rows * 16);
+    pl->part = take(rows * pl->chunks * 8);
+    if (p.dual) pl->part2 = take(rows * pl->chunks * 4);
+    pl->z = take(rows * round_up(widest, 4) * 4);
+    if (p.grad) pl->g = take(rows * round_up(widest, 8) * 2);
+    if (pl->group) {
+        pl->planes = take(pl->group * plane);
+        if (pl->group < pl->pieces.size()) pl->acc = take(plane);
+    }
+    // one split-K workspace for all products, which run one after another
+    for (const Piece &pc : pl->pieces) {
+        t0g_gemm_desc g[3];
+        int n = 0, rc;
+        g[n++] = logits_gemm(p, *pl, pc, 0);
+        if (d.dx) g[n++] = dx_gemm(p, *pl, pc, 0, 0);
+        if (d.dw) g[n++] = dw_gemm(p, *pl, pc, 0);
+        for (int i = 0; i < n; ++i) {
+            size_t bytes = 0;
+            if ((rc = losses_gemm_workspace(&g[i], &bytes))) return rc;
+            pl->gemm_ws_bytes = std::max<uint64_t>(pl->gemm_ws_bytes, bytes);
+        }
+    }
+    pl->gemm_ws = take(pl->gemm_ws_bytes);
+    pl->bytes = at;
+    return T0G_OK;
+}
+
+int run_gemm(t0g_device *dev, t0g_gemm_desc g, const Plan &pl, uint64_t base) {
+    g.workspace = base + pl.gemm_ws;
+    g.workspace_bytes = pl.gemm_ws_bytes;
+    return losses_gemm(dev, &g);
+}
+
+int run_loss(t0g_device *dev, const Problem &p) {
+    const t0g_linear_ce_desc &d = p.d;
+    Plan pl;
+    int rc = make_loss_plan(p, &pl);
+    if (rc) return rc;
+    uint64_t base = 0;
+    if ((rc = losses_begin(dev, pl.bytes, &base))) return rc;
+    if (d.rows == 0) {
+        for (const Piece &pc : pl.pieces)   // a product over no rows: zeros
+            if (d.dw && (rc = run_gemm(dev, dw_gemm(p, pl, pc, base), pl, base))) return rc;
+        return ok();
+    }
+    T0gLossArgs a;
+    memset(&a, 0, sizeof a);
+    a.x = d.x;
+    a.xz = p.grad ? base + pl.xz : 0;
+    a.labels = d.labels;
+    a.dloss = d.dloss;
+    a.loss = d.loss;
+    a.lse = d.lse;
+    a.ent_tok = base + pl.ent_tok;
+    a.ent_q = base + pl.ent_q;
+    a.ent_z = base + pl.ent_z;
+    a.row_ent = base + pl.row_ent;
+    a.row_sub = base + pl.row_sub;
+    a.row_par = p.grad ? base + pl.row_par : 0;
+    a.part = base + pl.part;
+    a.part2 = p.dual ? base + pl.part2 : 0;
+    a.z = base + pl.z;
+    a.g = p.grad ? base + pl.g : 0;
+    a.rows = d.rows;
+    a.vocab = d.vocab;
+    a.hidden = d.hidden;
+    a.ldx = d.ldx;
+    a.ldxz = pl.ldxz;
+    a.slots = pl.slots;
+    a.logit_scale = d.logit_scale;
+    a.loss_scale = d.loss_scale;
+    a.tau = 1.0f;
+    a.label_weight = 1.0f;
+    if (d.label_type == T0G_I64) a.flags |= T0G_LOSS_LABEL64;
+    if ((d.x & 15) == 0 && d.ldx % 8 == 0 && d.hidden % 8 == 0) a.flags |= T0G_LOSS_X_VEC;
+    if (p.t) {
+        a.teacher = p.t->teacher;
+        a.tokens = p.t->tokens;
+        a.top_k = p.t->top_k;
+        a.ldt = p.ldt;
+        a.tau = p.t->temperature;
+        a.label_weight = p.t->label_weight;
+        a.distill_weight = p.t->distill_weight;
+        if (p.t->token_type == T0G_I64) a.flags |= T0G_LOSS_TOKEN64;
+        if (p.t->teacher_dtype == T0G_BF16) a.flags |= T0G_LOSS_TEACHER16;
+    }
+    if (p.dual) a.flags |= T0G_LOSS_DUAL;
+    // with both softmaxes the first is the labels', else the only one
+    const double k = (double)d.logit_scale * 1.4426950408889634;
+    a.k = (float)(p.dual || !p.t ? k : k / p.t->temperature);
+    a.r = p.dual ? 1.0f / p.t->temperature : 1.0f;
+
+    auto row_kernel = [&](const char *symbol, uint32_t rows_per_group) {
+        const uint32_t groups = (uint32_t)(((uint64_t)d.rows + rows_per_group - 1) / rows_per_group);
+        return losses_launch(dev, symbol, std::min<uint32_t>(groups, 1u << 20), 1, &a, sizeof a);
+    };
+    auto piece_kernel = [&](const char *symbol, const Piece &pc) {
+        a.v0 = pc.v0;
+        a.cols = pc.cols;
+        a.ldz = round_up(pc.cols, 4);
+        a.ldg = round_up(pc.cols, 8);
+        a.chunk0 = pc.chunk0;
+        a.chunks = pc.chunks;
+        return losses_launch(dev, symbol, pc.chunks, std::min(d.rows, kMaxGridY), &a, sizeof a);
+    };
+    if ((rc = row_kernel("t0g_loss_prepare", 1))) return rc;
+    for (const Piece &pc : pl.pieces)
+        if ((rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base)) || (rc = piece_kernel("t0g_loss_stats", pc)))
+            return rc;
+    a.chunks = pl.chunks;
+    if ((rc = row_kernel("t0g_loss_combine", 4))) return rc;
+    if (!p.grad) return ok();
+
+    T0gLossSumArgs s;
+    memset(&s, 0, sizeof s);
+    s.planes = base + pl.planes;
+    s.rows = d.rows;
+    s.cols = d.hidden;
+    uint32_t planes = 0;
+    const size_t n = pl.pieces.size();
+    for (size_t i = n; i-- > 0;) {
+        const Piece &pc = pl.pieces[i];
+        if (i + 1 < n && (rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base))) return rc;
+        if ((rc = piece_kernel("t0g_loss_grad", pc))) return rc;
+        if (d.dw && (rc = run_gemm(dev, dw_gemm(p, pl, pc, base), pl, base))) return rc;
+        if (!d.dx) continue;
+        if ((rc = run_gemm(dev, dx_gemm(p, pl, pc, base, planes), pl, base))) return rc;
+        if (pl.group == 0) continue;
+        if (++planes < pl.group && i > 0) continue;
+        // the planes so far, onto those before
+        const bool last = i == 0;
+        s.n = planes;
+        s.out = last ? d.dx : base + pl.acc;
+        s.ldo = last ? d.lddx : d.hidden;
+        s.out_bf16 = last && d.dx_dtype == T0G_BF16;
+        s.vec = d.hidden % 4 == 0 && s.ldo % 4 == 0 && s.out % 16 == 0;
+        const uint64_t items = (uint64_t)d.rows * d.hidden / (s.vec ? 4 : 1);
+        const uint32_t groups = (uint32_t)std::min<uint64_t>((items + 255) / 256, 1u << 16);
+        if ((rc = losses_launch(dev, "t0g_loss_sum", groups, 1, &s, sizeof s))) return rc;
+        s.acc = base + pl.acc;
+        planes = 0;
+    }
+    return ok();
+}
+
+int loss_call(t0g_device *dev, const t0g_linear_ce_desc *d, const t0g_linear_distill_desc *t) {
+    if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
+    if (!d) return fail(T0G_ERR_INVALID_ARG, "desc is NULL");
+    Problem p;
+    int rc = check_problem(d, t, &p);
+    if (rc) return rc;
+    std::lock_guard<std::mutex> lk(device_mutex(dev));
+    return run_loss(dev, p);
+}
+
+int loss_scratch(const t0g_linear_ce_desc *d, const t0g_linear_distill_desc *t, size_t *bytes) {
+    if (!d || !bytes) return fail(T0G_ERR_INVALID_ARG, "NULL argument");
+    *bytes = 0;
+    Problem p;
+    Plan pl;
+    int rc = check_problem(d, t, &p);
+    if (rc || (rc = make_loss_plan(p, &pl))) return rc;
+    *bytes = pl.bytes;
+    return ok();
+}
+
+}  // namespace
+}  // namespace t0g
+
+extern "C" {
+
+int t0g_linear_cross_entropy(t0g_device *dev, const t0g_linear_ce_desc *desc) {
+    return t0g::loss_call(dev, desc, nullptr);
+}
+
+int t0g_linear_distill(t0g_device *dev, const t0g_linear_distill_desc *desc) {
+    return t0g::loss_call(dev, desc ? &desc->head : nullptr, desc);
+}
+
+int t0g_linear_cross_entropy_scratch_size(const t0g_linear_ce_desc *desc, size_t *bytes) {
+    return t0g::loss_scratch(desc, nullptr, bytes);
+}
+
+int t0g_linear_distill_scratch_size(const t0g_linear_distill_desc *desc, size_t *bytes) {
+    return t0g::loss_scratch(desc ? &desc->head : nullptr, desc, bytes);
+}
+
+}  // extern "C"

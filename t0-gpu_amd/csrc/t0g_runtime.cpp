@@ -50,6 +50,16 @@ __asm__(".section .rodata.t0g_hsaco_tl,\"a\",@progbits\n"
         ".byte 0\n"
         ".previous\n");
 extern "C" const unsigned char t0g_hsaco_tl_begin[];
+// The losses' kernels (T0G_HSACO_LOSS_FILE), loaded on a device by its first loss.
+__asm__(".section .rodata.t0g_hsaco_loss,\"a\",@progbits\n"
+        ".p2align 12\n"
+        ".hidden t0g_hsaco_loss_begin\n"
+        ".globl t0g_hsaco_loss_begin\n"
+        "t0g_hsaco_loss_begin:\n"
+        ".incbin \"" T0G_HSACO_LOSS_FILE "\"\n"
+        ".byte 0\n"
+        ".previous\n");
+extern "C" const unsigned char t0g_hsaco_loss_begin[];
 
 namespace t0g {
 
@@ -77,6 +87,10 @@ struct t0g_device {
     hipEvent_t order_event = nullptr;   // orders launches across t0g_device_set_stream
     hipModule_t module = nullptr;
     hipModule_t module_tl = nullptr;   // the timeline build of the same kernels (loaded on first use)
+    hipModule_t module_loss = nullptr;   // the losses' kernels (loaded on first use)
+    std::unordered_map<std::string, hipFunction_t> fns_loss;
+    uint64_t loss = 0;         // scratch of the losses
+    size_t loss_bytes = 0;
     std::mutex mu;
     bool poisoned = false;
     std::string poison_reason;
@@ -893,6 +907,7 @@ int t0g_device_close(t0g_device *dev) {
     if (!dev->poisoned) (void)hipStreamSynchronize(dev->stream);
     if (dev->ws) (void)hipFree((void *)dev->ws);
     if (dev->conv) (void)hipFree((void *)dev->conv);
+    if (dev->loss) (void)hipFree((void *)dev->loss);
     if (dev->sk_sync) (void)hipFree((void *)dev->sk_sync);
     for (int i = 0; i < t0g_device::kSides; ++i) {
         if (dev->side[i]) {
@@ -910,6 +925,7 @@ int t0g_device_close(t0g_device *dev) {
     for (hipModule_t m : dev->extra_modules) (void)hipModuleUnload(m);
     if (dev->module) (void)hipModuleUnload(dev->module);
     if (dev->module_tl) (void)hipModuleUnload(dev->module_tl);
+    if (dev->module_loss) (void)hipModuleUnload(dev->module_loss);
     if (dev->order_event) (void)hipEventDestroy(dev->order_event);
     if (dev->own_stream) (void)hipStreamDestroy(dev->own_stream);
     delete dev;
@@ -1730,6 +1746,70 @@ int t0g_gemm_group(t0g_device *dev, const t0g_gemm_desc *descs, uint32_t n) {
 
 namespace t0g {
 
+// Whether the device stream is being captured into a graph: a call must not allocate then.
+static bool capturing(t0g_device *dev) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    return T0G_HIP(hipStreamIsCapturing(dev->stream, &st)) != hipSuccess || st != hipStreamCaptureStatusNone;
+}
+
+// ---- for the losses (t0g_losses.cpp), with dev->mu held ---------------------------
+std::mutex &device_mutex(t0g_device *dev) { return dev->mu; }
+
+int losses_begin(t0g_device *dev, size_t bytes, uint64_t *scratch) {
+    int rc = check_usable(dev);
+    if (rc) return rc;
+    if (!dev->module_loss || !dev->sk_sync || dev->loss_bytes < bytes) {
+        if (capturing(dev))
+            return fail(T0G_ERR_INVALID_ARG,
+                        "a loss under stream capture needs %zu bytes of scratch and the handle holds %zu: run the same "
+                        "call once before the capture",
+                        bytes, dev->loss_bytes);
+        hipError_t e;
+        if (!dev->module_loss && (e = T0G_HIP(module_load(&dev->module_loss, t0g_hsaco_loss_begin))) != hipSuccess) {
+            dev->module_loss = nullptr;
+            return hip_fail(e, "hipModuleLoadData(losses code object)");
+        }
+        if ((rc = ensure_sk_sync(dev))) return rc;
+        if (dev->loss_bytes < bytes) {
+            if (dev->loss) {
+                e = T0G_HIP(hipFree((void *)dev->loss));   // waits for work using it
+                dev->loss = 0;
+                dev->loss_bytes = 0;
+                if (e != hipSuccess) return poison(dev, hip_fail(e, "hipFree(loss scratch)"));
+            }
+            void *p = nullptr;
+            if ((e = T0G_HIP(dev_malloc(&p, bytes))) != hipSuccess) return hip_fail(e, "hipMalloc(loss scratch)");
+            dev->loss = (uint64_t)p;
+            dev->loss_bytes = bytes;
+        }
+    }
+    *scratch = dev->loss;
+    return T0G_OK;
+}
+
+int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, void *args, size_t args_size) {
+    auto it = dev->fns_loss.find(symbol);
+    if (it == dev->fns_loss.end()) {
+        hipFunction_t f = nullptr;
+        hipError_t e = T0G_HIP(hipModuleGetFunction(&f, dev->module_loss, symbol));
+        if (e != hipSuccess) return hip_fail(e, symbol);
+        it = dev->fns_loss.emplace(symbol, f).first;
+    }
+    return launch(dev, it->second, grid_x, grid_y, 1, 256, args, args_size);
+}
+
+int losses_gemm_workspace(const t0g_gemm_desc *d, size_t *bytes) {
+    t0g_gemm_config cfg;
+    GemmPlan p;
+    GemmOperands o;
+    int rc = resolve_desc(d, &cfg, &p, &o, true);
+    if (rc || (rc = check_grid(p))) return rc;
+    *bytes = plan_workspace(p, d->m, d->n, kNumCUs);
+    return T0G_OK;
+}
+
+int losses_gemm(t0g_device *dev, const t0g_gemm_desc *d) { return gemm_locked(dev, d); }
+
 // Device time of `iters` back-to-back t0g_gemm launches of d (after `warmup`
 // untimed ones): one HIP event between consecutive launches on the device
 // stream, so each duration covers one whole GEMM (partials and reduce).
@@ -1814,12 +1894,6 @@ static int convert_pair_locked(t0g_device *dev, uint64_t src0, uint64_t dst0, ui
     if (rc) return rc;
     T0gConvertPairArgs a = {convert_args(src0, dst0, n0), convert_args(src1, dst1, n1)};
     return launch(dev, f, a.a.grid_blocks + a.b.grid_blocks, 1, 1, 256, &a, sizeof a);
-}
-
-// Whether the device stream is being captured into a graph: a call must not allocate then.
-static bool capturing(t0g_device *dev) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    return T0G_HIP(hipStreamIsCapturing(dev->stream, &st)) != hipSuccess || st != hipStreamCaptureStatusNone;
 }
 
 // The plan of a GEMM with f32 output whose A (and, with b_f32, B) is f32, rounded to

@@ -40,6 +40,7 @@ NT, NN, TN, TT = 0, 1, 2, 3
 LAYOUTS = {"NT": NT, "NN": NN, "TN": TN, "TT": TT}
 EPI_STORE_F32, EPI_BIAS_ADD, EPI_BIAS_ADD_RELU = 0, 1, 2
 F32, BF16 = 0, 1
+I32, I64 = 0, 1
 (MATMUL_FORWARD, MATMUL_BACKWARD_DATA, MATMUL_BACKWARD_WEIGHT, MATMUL_FORWARD_CACHED, MATMUL_BACKWARD_DATA_CACHED,
  MATMUL_WT_BF16) = range(6)
 STREAM_K = 0x80000000   # GemmConfig.split_k value selecting the stream-K schedule
@@ -145,6 +146,22 @@ class GemmDesc(ctypes.Structure):
         ("clamp_min", ctypes.c_float),
         ("clamp_max", ctypes.c_float),
     ]
+
+
+class LinearCeDesc(ctypes.Structure):
+    _fields_ = (
+        [(f, ctypes.c_uint64) for f in ("x", "w", "labels", "loss", "lse", "dloss", "dx", "dw")] +
+        [(f, ctypes.c_uint32) for f in ("rows", "vocab", "hidden", "ldx", "ldw", "lddx", "lddw", "transpose",
+                                        "label_type", "dx_dtype", "dw_dtype", "max_piece")] +
+        [("loss_scale", ctypes.c_float), ("logit_scale", ctypes.c_float)])
+
+
+class LinearDistillDesc(ctypes.Structure):
+    _fields_ = (
+        [("head", LinearCeDesc), ("teacher", ctypes.c_uint64), ("tokens", ctypes.c_uint64)] +
+        [(f, ctypes.c_uint32) for f in ("top_k", "ldt", "teacher_dtype", "token_type")] +
+        [("temperature", ctypes.c_float), ("label_weight", ctypes.c_float), ("distill_weight", ctypes.c_float),
+         ("reserved", ctypes.c_uint32)])
 
 
 class KernelMeta(ctypes.Structure):
@@ -276,6 +293,12 @@ _sig("t0g_gemm_group", ctypes.c_int, _p, ctypes.POINTER(GemmDesc), _u32)
 _sig("t0g_gemm_noalloc", ctypes.c_int, _p, ctypes.POINTER(GemmDesc))
 _sig("t0g_gemm_kernel_name", ctypes.c_int, ctypes.POINTER(GemmDesc), ctypes.c_char_p, ctypes.c_size_t)
 _sig("t0g_gemm_compile", ctypes.c_int, ctypes.POINTER(GemmDesc), ctypes.POINTER(CompiledKernel))
+_sig("t0g_linear_cross_entropy", ctypes.c_int, _p, ctypes.POINTER(LinearCeDesc))
+_sig("t0g_linear_distill", ctypes.c_int, _p, ctypes.POINTER(LinearDistillDesc))
+_sig("t0g_linear_cross_entropy_scratch_size", ctypes.c_int, ctypes.POINTER(LinearCeDesc),
+     ctypes.POINTER(ctypes.c_size_t))
+_sig("t0g_linear_distill_scratch_size", ctypes.c_int, ctypes.POINTER(LinearDistillDesc),
+     ctypes.POINTER(ctypes.c_size_t))
 _sig("t0g_f32_to_bf16", ctypes.c_int, _p, _u64, _u64, ctypes.c_size_t)
 _sig("t0g_matmul_f32", ctypes.c_int, _p, _u64, _u64, _u64, _u32, _u32, _u32)
 _sig("t0g_matmul_backward_data_f32", ctypes.c_int, _p, _u64, _u64, _u64, _u32, _u32, _u32)
@@ -495,6 +518,44 @@ def gemm_desc(a, b, c, m, n, k, transpose=NT, out_dtype=F32, lda=0, ldb=0, ldc=0
     d.epi_scale = epi_scale
     d.clamp_min, d.clamp_max = clamp
     return d
+
+
+def linear_ce_desc(x, w, labels, loss, rows, vocab, hidden, transpose=NT, lse=0, dx=0, dw=0, dloss=0, loss_scale=1.0,
+                   logit_scale=1.0, label_type=I64, dx_dtype=BF16, dw_dtype=BF16, ldx=0, ldw=0, lddx=0, lddw=0,
+                   max_piece=0):
+    """Cross entropy of x W^T: device addresses of x [rows][hidden] and w (NT [vocab][hidden], NN
+    [hidden][vocab]) in bf16, labels, and the outputs (lse, dx, dw: 0 = not wanted)."""
+    d = LinearCeDesc()
+    d.x, d.w, d.labels, d.loss, d.lse, d.dloss, d.dx, d.dw = x, w, labels, loss, lse, dloss, dx, dw
+    d.rows, d.vocab, d.hidden = rows, vocab, hidden
+    d.ldx, d.ldw, d.lddx, d.lddw = ldx, ldw, lddx, lddw
+    d.transpose = LAYOUTS[transpose] if isinstance(transpose, str) else transpose
+    d.label_type, d.dx_dtype, d.dw_dtype = label_type, dx_dtype, dw_dtype
+    d.max_piece = max_piece
+    d.loss_scale, d.logit_scale = loss_scale, logit_scale
+    return d
+
+
+def linear_distill_desc(x, w, teacher, tokens, loss, rows, vocab, hidden, top_k, temperature=1.0, labels=0,
+                        label_weight=0.0, distill_weight=1.0, teacher_dtype=F32, token_type=I64, ldt=0, **head):
+    """Divergence from a teacher's top_k logits (teacher, tokens: [rows][ldt]), plus label_weight times the
+    cross entropy of labels if there are any; head: as linear_ce_desc."""
+    d = LinearDistillDesc()
+    d.head = linear_ce_desc(x, w, labels, loss, rows, vocab, hidden, **head)
+    d.teacher, d.tokens = teacher, tokens
+    d.top_k, d.ldt = top_k, ldt
+    d.teacher_dtype, d.token_type = teacher_dtype, token_type
+    d.temperature, d.label_weight, d.distill_weight = temperature, label_weight, distill_weight
+    return d
+
+
+def linear_loss_scratch_size(desc):
+    """Bytes of the handle's scratch that a loss takes (either descriptor)."""
+    n = ctypes.c_size_t()
+    ce = isinstance(desc, LinearCeDesc)
+    f = _lib.t0g_linear_cross_entropy_scratch_size if ce else _lib.t0g_linear_distill_scratch_size
+    _check(f(ctypes.byref(desc), ctypes.byref(n)))
+    return n.value
 
 
 def gemm_workspace_size(desc):
@@ -786,6 +847,15 @@ class GpuRuntime:
     def gemm(self, a, b, c, m, n, k, **kw):
         """Enqueue C = op(A) op(B) on the device stream (asynchronous)."""
         self.gemm_desc(gemm_desc(a, b, c, m, n, k, **kw))
+
+    # losses of a projection onto a vocabulary
+    def linear_cross_entropy(self, desc):
+        """Enqueue a linear_ce_desc on the device stream (asynchronous)."""
+        _check(_lib.t0g_linear_cross_entropy(self.handle, ctypes.byref(desc)))
+
+    def linear_distill(self, desc):
+        """Enqueue a linear_distill_desc on the device stream (asynchronous)."""
+        _check(_lib.t0g_linear_distill(self.handle, ctypes.byref(desc)))
 
     # Ignis bf16_matmul caller path (src/ignis/ops/bf16_matmul.rs) on f32 device tensors
     def f32_to_bf16(self, src, dst, n):

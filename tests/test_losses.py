@@ -1,0 +1,92 @@
+"""Host side of the losses of a projection onto a vocabulary: what a call refuses, with the
+status and before anything runs, and the scratch that it asks for.  No GPU needed."""
+import pytest
+
+import t0g
+
+X, W, Y, LOSS, DX, DW = (0x10000000 * i for i in range(1, 7))
+TEACHER, TOKENS = 0x70000000, 0x80000000
+
+
+def ce(**kw):
+    d = t0g.linear_ce_desc(X, W, Y, LOSS, 16, 1000, 64)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def distill(head=None, **kw):
+    d = t0g.linear_distill_desc(X, W, TEACHER, TOKENS, LOSS, 16, 1000, 64, 8)
+    for k, v in (head or {}).items():
+        setattr(d.head, k, v)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def refused(d, *words):
+    with pytest.raises(t0g.T0gError) as e:
+        t0g.linear_loss_scratch_size(d)
+    assert e.value.code == t0g.ERR_INVALID_ARG
+    for w in words:
+        assert w in str(e.value)
+
+
+@pytest.mark.parametrize("change,word", [
+    ({"transpose": t0g.TN}, "transpose"), ({"transpose": 9}, "transpose"), ({"label_type": 2}, "label_type"),
+    ({"dx_dtype": 2}, "type"), ({"dw_dtype": 7}, "type"), ({"vocab": 0}, "size"), ({"hidden": 0}, "size"),
+    ({"vocab": 1 << 31}, "size"), ({"rows": 1 << 31}, "size"),
+    ({"logit_scale": 0.0}, "logit_scale"), ({"logit_scale": -1.0}, "logit_scale"),
+    ({"logit_scale": float("nan")}, "logit_scale"), ({"logit_scale": float("inf")}, "logit_scale"),
+    ({"ldx": 63}, "ldx"), ({"ldw": 63}, "ldw"), ({"lddx": 1}, "lddx"), ({"lddw": 63}, "lddw"),
+    ({"x": 0}, "NULL"), ({"w": 0}, "NULL"), ({"loss": 0}, "NULL"), ({"labels": 0}, "labels"),
+    ({"x": X + 1}, "aligned"), ({"w": W + 1}, "aligned"), ({"labels": Y + 4}, "aligned"), ({"loss": LOSS + 2}, "aligned"),
+    ({"lse": DX + 2}, "aligned"), ({"dloss": DX + 1}, "aligned"), ({"dx": DX + 1}, "aligned"),
+    ({"dw": DW + 2, "dw_dtype": t0g.F32}, "aligned"),
+    ({"dx": X}, "overlaps"), ({"dx": X + 16 * 64 * 2 - 2}, "overlaps"), ({"dw": W}, "overlaps"), ({"lse": LOSS}, "overlaps"),
+    ({"dx": DX, "dw": DX + 2}, "overlaps"), ({"loss": Y}, "overlaps"), ({"lse": W + 64}, "overlaps"),
+])
+def test_cross_entropy_refusals(change, word):
+    refused(ce(**change), word)
+    refused(distill(head={"labels": Y, **change}) if "labels" not in change else ce(**change), word)
+
+
+def test_neighbours_do_not_overlap():
+    assert t0g.linear_loss_scratch_size(ce(dx=X + 16 * 64 * 2, lse=LOSS + 64)) > 0
+
+
+def test_nn_leading_dimension_is_the_vocabulary():
+    refused(ce(transpose=t0g.NN, ldw=999), "ldw")
+    assert t0g.linear_loss_scratch_size(ce(transpose=t0g.NN, ldw=1000)) > 0
+
+
+@pytest.mark.parametrize("change,word", [
+    ({"top_k": 0}, "top_k"), ({"top_k": 1025}, "top_k"), ({"ldt": 7}, "ldt"), ({"teacher_dtype": 2}, "teacher_dtype"),
+    ({"token_type": 3}, "token_type"), ({"temperature": 0.0}, "temperature"), ({"temperature": -2.0}, "temperature"),
+    ({"temperature": float("inf")}, "temperature"), ({"teacher": 0}, "NULL"), ({"tokens": 0}, "NULL"),
+    ({"teacher": TEACHER + 2}, "aligned"), ({"tokens": TOKENS + 4}, "aligned"), ({"reserved": 1}, "reserved"),
+    ({"teacher": LOSS}, "overlaps"), ({"tokens": LOSS}, "overlaps"),
+])
+def test_distill_refusals(change, word):
+    refused(distill(**change), word)
+
+
+def test_labels_are_optional_beside_a_teacher():
+    assert t0g.linear_loss_scratch_size(distill()) > 0
+
+
+def test_null_arguments():
+    import ctypes
+    n = ctypes.c_size_t()
+    assert t0g._lib.t0g_linear_cross_entropy_scratch_size(None, ctypes.byref(n)) == t0g.ERR_INVALID_ARG
+    assert t0g._lib.t0g_linear_distill_scratch_size(None, ctypes.byref(n)) == t0g.ERR_INVALID_ARG
+    assert t0g._lib.t0g_linear_cross_entropy_scratch_size(ctypes.byref(ce()), None) == t0g.ERR_INVALID_ARG
+    assert t0g._lib.t0g_linear_cross_entropy(None, ctypes.byref(ce())) == t0g.ERR_INVALID_ARG
+    assert t0g._lib.t0g_linear_distill(None, ctypes.byref(distill())) == t0g.ERR_INVALID_ARG
+
+
+def test_scratch_stays_far_below_the_logits():
+    """8192 x 131072 logits take 4 GiB in f32; their pieces do not."""
+    d = t0g.linear_ce_desc(0x100000000, 0x200000000, 0x10000000, 0x20000000, 8192, 131072, 4096, dx=0x300000000,
+                           dw=0x400000000)
+    assert t0g.linear_loss_scratch_size(d) < 1.25 * 2 ** 30

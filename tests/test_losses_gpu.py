@@ -1,0 +1,434 @@
+"""Losses of a projection onto a vocabulary (t0g_linear_cross_entropy, t0g_linear_distill)
+against their definitions in 64 bits, at sizes, layouts, masks and values where they can go
+wrong; gradients also against differences of the loss.
+
+Tolerances, with u = 2^-24 (f32) and the sums of magnitudes |x||W| and |G||W| taken in 64 bits:
+  logits     f32 sums of `hidden` exact products: at most e_z = (hidden + 2) u max |x||W| c
+  statistics sums of at most 2^17 terms in f32 by lanes, chunks and joins: 2^10 u relative at the very
+             most; exp2, log2 and the products around them: 16 u (1 + |lse| + |z|)
+  loss       the sum of the errors of its terms, each weighted as in the loss
+  dx, dW     G is rounded to bf16 (2^-8 |G|, half a unit of its 8 bits), its own error is that of the probabilities
+             (2 e_z + statistics) |P|, the products are summed in f32 and rounded once to the output type
+"""
+import sys
+
+import pytest
+import torch
+
+import t0g
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _log(msg):
+    print(msg, flush=True)
+    sys.stdout.flush()
+
+
+@pytest.fixture(scope="module")
+def rt():
+    r = t0g.GpuRuntime.new(0)
+    yield r
+    r.close()
+
+
+class Case:
+    """One problem: inputs on the host, the call's buffers on the device (each in a filled allocation of its
+    own, so that a write outside shows), and the definition in 64 bits."""
+
+    def __init__(self, rows, vocab, hidden, layout="NT", seed=0, pad=0, offset=0, xpad=None, amp=2.0, c=1.0, scale=0.125,
+                 dtype="bf16", int32=False, weights=True, want="xw"):
+        self.rows, self.vocab, self.hidden, self.layout = rows, vocab, hidden, layout
+        self.c, self.scale, self.int32, self.want = c, scale, int32, want
+        self.out_type = torch.bfloat16 if dtype == "bf16" else torch.float32
+        self.pad, self.offset, self.xpad = pad, offset, pad if xpad is None else xpad
+        g = self.g = torch.Generator().manual_seed(seed)
+        self.x = torch.randn(rows, hidden, generator=g).bfloat16()
+        self.w = (torch.randn(vocab, hidden, generator=g) * amp * hidden ** -0.5).bfloat16()
+        self.labels = torch.randint(0, vocab, (rows,), generator=g)
+        self.dloss = (0.25 + torch.rand(rows, generator=g)) if weights else None
+        self.teacher = None
+
+    def teach(self, top, tau=1.0, a=0.0, b=1.0, half=False, ldt=0, repeat=False):
+        g = self.g
+        if repeat or top > self.vocab:
+            self.tokens = torch.randint(0, self.vocab, (self.rows, top), generator=g)
+        else:
+            self.tokens = torch.stack([torch.randperm(self.vocab, generator=g)[:top] for _ in range(max(1, self.rows))])
+            self.tokens = self.tokens[:self.rows]
+        self.teacher = 2 * torch.randn(self.rows, top, generator=g)
+        if half:
+            self.teacher = self.teacher.bfloat16()
+        self.top, self.tau, self.a, self.b, self.ldt = top, tau, a, b, ldt or top
+        if not a:
+            self.labels = None
+        return self
+
+    # ---- the call
+    def device(self, t, ld=None, fill=-7.0):
+        """t in a larger buffer of its own, rows ld apart, `offset` elements from an aligned address."""
+        rows, cols = (1, t.shape[0]) if t.dim() == 1 else t.shape
+        ld = ld or cols
+        buf = torch.full((self.offset + rows * ld + 64,), fill, dtype=t.dtype, device="cuda")
+        view = buf[self.offset:self.offset + rows * ld].view(rows, ld)[:, :cols]
+        view.copy_(t.view(rows, cols))
+        return buf, (view[0] if t.dim() == 1 else view)
+
+    def run(self, rt, max_piece=0, stream=None):
+        ints = torch.int32 if self.int32 else torch.int64
+        itype = t0g.I32 if self.int32 else t0g.I64
+        w = self.w if self.layout == "NT" else self.w.t().contiguous()
+        nan = float("nan")
+        bx, x = self.device(self.x, self.hidden + self.xpad, nan)
+        bw, wd = self.device(w, w.shape[1] + self.pad, nan)
+        keep = [bx, bw]
+
+        def addr(t):
+            if t is None:
+                return 0
+            keep.append(t.to("cuda"))
+            return keep[-1].data_ptr()
+
+        dt = self.out_type
+        self.bufs = {"loss": self.device(torch.zeros(self.rows)), "lse": self.device(torch.zeros(self.rows))}
+        if "x" in self.want:
+            self.bufs["dx"] = self.device(torch.zeros(self.rows, self.hidden, dtype=dt), self.hidden + self.pad)
+        if "w" in self.want:
+            self.bufs["dw"] = self.device(torch.zeros(w.shape, dtype=dt), w.shape[1] + self.pad)
+        for b, v in self.bufs.values():
+            v.fill_(-7.0)
+
+        def out(name):
+            return self.bufs[name][1].data_ptr() if name in self.bufs and self.bufs[name][1].numel() else 0
+
+        kind = t0g.BF16 if dt == torch.bfloat16 else t0g.F32
+        head = dict(transpose=self.layout, lse=out("lse"), dx=out("dx"), dw=out("dw"), dloss=addr(self.dloss),
+                    loss_scale=self.scale, logit_scale=self.c, label_type=itype, dx_dtype=kind, dw_dtype=kind,
+                    ldx=self.hidden + self.xpad, ldw=w.shape[1] + self.pad, lddx=self.hidden + self.pad,
+                    lddw=w.shape[1] + self.pad, max_piece=max_piece)
+        xa = x.data_ptr() if self.rows else 0
+        labels = addr(self.labels.to(ints)) if self.labels is not None else 0
+        if self.teacher is None:
+            d = t0g.linear_ce_desc(xa, wd.data_ptr(), labels, out("loss"), self.rows, self.vocab, self.hidden, **head)
+            call = rt.linear_cross_entropy
+        else:
+            tokens, teacher = self.tokens.to(ints), self.teacher
+            if self.ldt > self.top:   # what lies between the rows must not be read as entries
+                tokens = torch.cat([tokens, torch.zeros(self.rows, self.ldt - self.top, dtype=ints)], 1)
+                teacher = torch.cat([teacher, torch.full((self.rows, self.ldt - self.top), nan, dtype=teacher.dtype)], 1)
+            d = t0g.linear_distill_desc(xa, wd.data_ptr(), addr(teacher), addr(tokens), out("loss"), self.rows, self.vocab,
+                                        self.hidden, self.top, temperature=self.tau, labels=labels, label_weight=self.a,
+                                        distill_weight=self.b, ldt=self.ldt, token_type=itype,
+                                        teacher_dtype=t0g.BF16 if teacher.dtype == torch.bfloat16 else t0g.F32, **head)
+            call = rt.linear_distill
+        torch.cuda.synchronize()
+        self.desc, self.call, self.keep = d, call, keep
+        call(d)
+        rt.wait_idle()
+        return {k: v.cpu() for k, (b, v) in self.bufs.items()}
+
+    def untouched(self):
+        for name, (b, v) in self.bufs.items():
+            mask = torch.ones_like(b, dtype=torch.bool)
+            rows, cols = (1, v.shape[0]) if v.dim() == 1 else v.shape
+            ld = cols if v.dim() == 1 else v.stride(0)
+            mask[self.offset:self.offset + rows * ld].view(rows, ld)[:, :cols] = False
+            assert bool((b[mask] == -7.0).all()), f"{name}: written outside"
+
+    # ---- the definition
+    def define(self):
+        x, w = self.x.double(), self.w.double()
+        rows, vocab = self.rows, self.vocab
+        usable = torch.zeros(rows, dtype=torch.bool)
+        a = 1.0 if self.teacher is None else self.a
+        y = self.labels
+        labelled = (y >= 0) & (y < vocab) if y is not None else usable.clone()
+        q = torch.zeros(rows, vocab, dtype=torch.float64)
+        taught = usable.clone()
+        if self.teacher is not None:
+            for t in range(rows):
+                ok = (self.tokens[t] >= 0) & (self.tokens[t] < vocab) & (self.teacher[t] != float("-inf"))
+                if ok.any():
+                    taught[t] = True
+                    q[t].index_add_(0, self.tokens[t][ok], torch.softmax(self.teacher[t][ok].double() / self.tau, 0))
+        used = labelled | taught
+        x = torch.where(used[:, None], x, torch.zeros_like(x))
+        z = self.c * (x @ w.t())
+        tau = 1.0 if self.teacher is None else self.tau
+        lp, lpt = torch.log_softmax(z, 1), torch.log_softmax(z / tau, 1)
+        rate = self.scale * (self.dloss.double() if self.dloss is not None else torch.ones(rows)) * self.c
+        loss, grad = torch.zeros(rows, dtype=torch.float64), torch.zeros(rows, vocab, dtype=torch.float64)
+        size = torch.zeros_like(grad)
+        pick = torch.where(labelled, y, torch.zeros_like(y))[:, None] if y is not None else None
+        if y is not None:
+            loss = loss + torch.where(labelled, -a * lp.gather(1, pick)[:, 0], loss)
+            m = (labelled * a * rate)[:, None]
+            grad = grad + m * (lp.exp() - torch.zeros_like(grad).scatter_(1, pick, 1.0))
+            size = size + m.abs() * lp.exp()
+        if self.teacher is not None:
+            kl = torch.where(q > 0, q * (torch.log(q.clamp(min=1e-300)) - lpt), torch.zeros_like(q)).sum(1)
+            loss = loss + torch.where(taught, self.b * tau * tau * kl, torch.zeros_like(kl))
+            m = (taught * self.b * tau * rate)[:, None]
+            grad = grad + m * (lpt.exp() - q)
+            size = size + m.abs() * (lpt.exp() + 16 * U / 2 ** -8 * q)
+        lse = torch.where(used, torch.logsumexp(z / tau, 1), torch.zeros(rows, dtype=torch.float64))
+        ez = (self.hidden + 2) * U * self.c * (x.abs() @ w.abs().t()).amax(1) if rows else torch.zeros(0)
+        zmax = z.abs().amax(1) if rows else torch.zeros(0)
+        stat = 2.0 ** 10 * U + 16 * U * (1 + lse.abs() + zmax / min(tau, 1.0))
+        weight = abs(a) + (abs(self.b) * tau * max(1.0, tau) if self.teacher is not None else 0.0)
+        dp = 2 * ez / min(1.0, tau) + 2 * stat           # relative error of a probability
+        gerr = 2.0 ** -8 * grad.abs() + dp[:, None] * size * 1.01
+        acc = (vocab + 8) * U
+        out = {"loss": (loss, weight * (2 * ez / min(1.0, tau) + 2 * stat + 16 * U * (1 + loss.abs()))),
+               "lse": (lse, ez / tau + stat)}
+
+        def product(left, right, lerr):
+            v = left @ right
+            mag = left.abs() @ right.abs()
+            e = lerr @ right.abs() * 1.01 + (max(self.rows, acc / U) + 8) * U * mag + 1e-30
+            return v, e + ((v.abs() + e) * 2.0 ** -8 if self.out_type == torch.bfloat16 else v.abs() * U)
+
+        if "x" in self.want:
+            out["dx"] = product(grad, w, gerr)
+        if "w" in self.want:
+            v, e = product(grad.t(), x, gerr.t())
+            out["dw"] = (v, e) if self.layout == "NT" else (v.t(), e.t())
+        return out
+
+    def check(self, rt, label="", **kw):
+        got, want = self.run(rt, **kw), self.define()
+        torch.cuda.synchronize()
+        self.untouched()
+        for k, (v, tol) in want.items():
+            d = (got[k].double() - v).abs()
+            worst = float((d / tol.clamp(min=1e-38)).max()) if d.numel() else 0.0
+            _log(f"[loss] {label} {self.rows}x{self.vocab}x{self.hidden} {self.layout} {k}: {worst:.3f} of the bound")
+            assert bool((d <= tol).all()), f"{label} {k}: {worst:.3f} times the bound"
+        return got
+
+
+SIZES = [
+    (1, 1, 1), (1, 2, 8), (2, 300, 64), (3, 257, 33), (5, 1000, 200), (64, 1000, 256), (130, 4100, 72), (65, 4097, 64),
+    (257, 520, 136), (300, 777, 96), (9, 9001, 40),
+]
+
+
+@pytest.mark.parametrize("layout", ["NT", "NN"])
+@pytest.mark.parametrize("rows,vocab,hidden", SIZES)
+def test_cross_entropy(rt, rows, vocab, hidden, layout):
+    Case(rows, vocab, hidden, layout, seed=rows + vocab).check(rt, "ce")
+
+
+@pytest.mark.parametrize("layout", ["NT", "NN"])
+@pytest.mark.parametrize("rows,vocab,hidden,pad,offset,xpad", [
+    (33, 515, 64, 8, 0, 8), (33, 515, 64, 3, 0, 0), (33, 512, 64, 0, 1, 0), (20, 700, 50, 6, 2, 14), (7, 264, 96, 0, 8, 5)])
+def test_strides_and_alignment(rt, rows, vocab, hidden, pad, offset, xpad, layout):
+    Case(rows, vocab, hidden, layout, seed=3, pad=pad, offset=offset, xpad=xpad).check(rt, "strides")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("want", ["", "x", "w", "xw"])
+def test_outputs_asked_for(rt, want, dtype):
+    Case(70, 900, 128, want=want, dtype=dtype, weights=False, scale=1.0, int32=True).check(rt, f"want {want or 'loss'}")
+
+
+@pytest.mark.parametrize("rows,vocab,max_piece", [(40, 1003, 1), (40, 1003, 8), (40, 1000, 130), (300, 2051, 512), (3, 9000, 4104)])
+@pytest.mark.parametrize("layout", ["NT", "NN"])
+def test_pieces_of_the_vocabulary(rt, rows, vocab, max_piece, layout):
+    """Pieces change neither loss nor gradient beyond the order of f32 sums; labels at a piece's first and last token."""
+    c = Case(rows, vocab, 72, layout, seed=5)
+    piece = max(8, max_piece & ~7)
+    edges = [e for v0 in range(0, vocab, piece) for e in (v0, min(v0 + piece, vocab) - 1)]
+    for t in range(rows):
+        c.labels[t] = edges[(7 * t) % len(edges)]
+    c.check(rt, f"pieces of {max_piece}", max_piece=max_piece)
+
+
+def test_partial_sums_of_dx_in_groups(rt):
+    """More planes of dx than are summed at a time (a plane of 40 MiB, groups of six)."""
+    rows, hidden = 10240, 1024
+    c = Case(rows, 136, hidden, seed=6, want="x", dtype="f32")
+    c.check(rt, "groups", max_piece=8)
+
+
+def test_missing_labels(rt):
+    """Rows without a label: loss, lse and gradient 0, and a NaN or infinity there reaches nothing."""
+    c = Case(48, 600, 64, seed=7)
+    c.labels[::3] = -100
+    c.labels[1::7] = 600
+    c.labels[2::11] = 2 ** 40 + 5   # beyond 32 bits: its low word is a valid token
+    c.x[0], c.x[3], c.x[2] = float("nan"), float("inf"), float("-inf")
+    c.x[1] = 3.0e38
+    got = c.check(rt, "missing")
+    assert float(got["dx"][0].abs().max()) == 0.0 and float(got["loss"][0]) == 0.0
+    c = Case(33, 300, 40, seed=8)
+    c.labels[:] = -1
+    c.x[:] = float("nan")
+    got = c.check(rt, "none left")
+    for k in ("loss", "lse", "dx", "dw"):
+        assert float(got[k].abs().max()) == 0.0
+
+
+def test_no_rows(rt):
+    c = Case(0, 300, 64, seed=9)
+    got = c.run(rt)
+    assert got["dw"].shape == (300, 64) and float(got["dw"].abs().max()) == 0.0
+    c.untouched()
+
+
+@pytest.mark.parametrize("amp", [0.0, 60.0, 2000.0])
+def test_extreme_logits(rt, amp):
+    """Equal logits; a softmax with one token left; logits far beyond what exp takes."""
+    c = Case(40, 5000, 64, seed=10, amp=amp)
+    c.labels[:20] = (c.x[:20].double() @ c.w.double().t()).argmax(1)
+    c.check(rt, f"amplitude {amp}")
+
+
+def test_a_nan_in_a_row_stays_there(rt):
+    c = Case(16, 500, 64, seed=11)
+    c.x[5, 3] = float("nan")
+    got = c.run(rt)
+    rows = [t for t in range(16) if t != 5]
+    assert bool(torch.isnan(got["loss"][5])) and bool(torch.isnan(got["dx"][5].float()).all())
+    assert bool(torch.isfinite(got["loss"][rows]).all()) and bool(torch.isfinite(got["dx"][rows].float()).all())
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,top,tau,a,b,layout", [
+    (1, 1, 8, 1, 1.0, 0.0, 1.0, "NT"), (1, 300, 64, 7, 2.0, 0.3, 0.7, "NT"), (5, 257, 33, 64, 1.0, 0.0, 2.0, "NN"),
+    (64, 1000, 128, 50, 4.0, 0.5, 0.5, "NT"), (130, 4100, 72, 65, 0.5, 0.25, 1.0, "NT"),
+    (33, 9000, 64, 256, 2.0, 1.0, 1.0, "NN"), (17, 1500, 64, 1024, 1.0, 0.5, 0.5, "NT"), (300, 520, 96, 3, 3.0, 0.0, 1.0, "NT")])
+def test_distill(rt, rows, vocab, hidden, top, tau, a, b, layout):
+    Case(rows, vocab, hidden, layout, seed=rows + top).teach(top, tau, a, b).check(rt, f"distill {top} at {tau}")
+
+
+@pytest.mark.parametrize("half,int32,ldt", [(True, True, 0), (False, True, 12), (True, False, 9)])
+def test_teacher_types_and_strides(rt, half, int32, ldt):
+    Case(50, 700, 64, seed=12, int32=int32).teach(9, 2.0, 0.5, 0.5, half=half, ldt=ldt).check(rt, "teacher types")
+
+
+def test_teacher_entries_missing_and_equal(rt):
+    c = Case(60, 640, 64, seed=13).teach(40, 2.0, 0.25, 0.75, repeat=True)
+    c.tokens[::2, 5:9] = -1
+    c.tokens[1::2, 3] = 640
+    c.tokens[4, 2] = 2 ** 33 + 1
+    c.teacher[::2, 5:9] = float("nan")        # a missing entry's logit is not looked at
+    c.teacher[3, 10:20] = float("-inf")       # no probability
+    c.teacher[7, :] = float("-inf")           # a row without a teacher
+    c.tokens[8, :] = -1
+    c.tokens[9, :] = 77                       # one token, forty times
+    c.tokens[10, 1:] = -5                     # one entry left
+    c.labels[8] = -100                        # neither label nor teacher
+    c.x[8] = float("nan")
+    c.labels[9], c.labels[11] = 77, c.tokens[11, 0]   # the label is one of the teacher's tokens
+    c.check(rt, "entries")
+    c = Case(20, 300, 40, seed=14).teach(4)
+    c.tokens[:] = -1
+    got = c.check(rt, "no teacher left")
+    assert float(got["dw"].abs().max()) == 0.0
+
+
+def test_distill_pieces(rt):
+    c = Case(70, 2053, 64, seed=15).teach(90, 2.0, 0.5, 0.5)
+    c.check(rt, "distill pieces", max_piece=256)
+
+
+@pytest.mark.parametrize("teach", [False, True])
+def test_gradient_against_differences(rt, teach):
+    """Along a direction of +-h the loss's central difference; h and the operands are such that x +- h and
+    W +- h are bf16 numbers.  The difference's own error is h^2/6 of the third derivative, at most
+    |dz|^3 per row for a log-sum-exp, and the f32 losses' (checked above) over 2h."""
+    rows, vocab, hidden, h = 24, 200, 16, 2.0 ** -6
+    g = torch.Generator().manual_seed(16)
+    c = Case(rows, vocab, hidden, seed=16, dtype="f32", scale=1.0, weights=False)
+    c.x = (torch.randint(-31, 32, (rows, hidden), generator=g) / 32.0).bfloat16()
+    c.w = (torch.randint(-31, 32, (vocab, hidden), generator=g) / 32.0).bfloat16()
+    tau, k = 1.0, 1.0
+    if teach:
+        tau = 2.0
+        c.teach(12, tau, 0.5, 0.5)
+        k = 0.5 + 0.5 * tau * tau / tau ** 3
+    got = c.run(rt)
+    tol_loss = c.define()["loss"][1]
+    x, w = c.x.clone(), c.w.clone()
+    for name in ("x", "w"):
+        base = x if name == "x" else w
+        step = torch.where(torch.rand(base.shape, generator=g) < 0.5, -h, h)
+        grad = got["d" + name].double()
+        losses = []
+        for sign in (1, -1):
+            moved = (base.double() + sign * step.double()).bfloat16()
+            assert bool((moved.double() == base.double() + sign * step.double()).all())
+            c.x, c.w = (moved, w) if name == "x" else (x, moved)
+            losses.append(c.run(rt)["loss"].double())
+        c.x, c.w = x, w
+        dz = (step.double() @ w.double().t() if name == "x" else x.double() @ step.double().t()).abs().amax(1)
+        third = k * (2 * dz) ** 3 / 6   # dz is the whole step: h is in it
+        diff = (losses[0] - losses[1]) / 2
+        if name == "x":
+            along = (grad * step.double()).sum(1)
+            tol = third + tol_loss + 2.0 ** -8 * (grad.abs() * h).sum(1) + 2.0 ** -8 * h * hidden * 2
+            assert bool(((along - diff).abs() <= tol).all())
+        else:
+            along = (grad * step.double()).sum()
+            tol = third.sum() + tol_loss.sum() + 2.0 ** -8 * h * 2 * rows * hidden
+            assert abs(float(along - diff.sum())) <= float(tol)
+
+
+def test_same_bits_again_and_on_another_stream(rt):
+    c = Case(200, 3000, 128, seed=17).teach(30, 2.0, 0.5, 0.5)
+    first = c.run(rt, max_piece=1024)
+    again = c.run(rt, max_piece=1024)
+    side = torch.cuda.Stream()
+    rt.set_stream(side.cuda_stream)
+    try:
+        other = c.run(rt, max_piece=1024)
+    finally:
+        rt.set_stream(0)
+    for k in first:
+        assert torch.equal(first[k], again[k]) and torch.equal(first[k], other[k]), k
+
+
+def test_graph_replays(rt):
+    """Captured after one eager call; replays match it bit for bit, with eager work in between."""
+    c = Case(96, 2000, 64, seed=18).teach(20, 2.0, 0.5, 0.5)
+    want = c.run(rt, max_piece=800)
+    side = torch.cuda.Stream()
+    rt.set_stream(side.cuda_stream)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            c.call(c.desc)
+        other = Case(30, 500, 64, seed=19)
+        for _ in range(3):
+            for _, v in c.bufs.values():
+                v.fill_(-7.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for k, (_, v) in c.bufs.items():
+                assert torch.equal(v.cpu(), want[k]), k
+            other.check(rt, "between replays")
+    finally:
+        rt.set_stream(0)
+
+
+def test_capture_without_scratch_is_refused():
+    with t0g.GpuRuntime.new(0) as fresh:
+        c = Case(40, 400, 64, seed=20)
+        with t0g.GpuRuntime.new(0) as warm:
+            want = c.run(warm)
+        side = torch.cuda.Stream()
+        fresh.set_stream(side.cuda_stream)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            with pytest.raises(t0g.T0gError) as e:
+                fresh.linear_cross_entropy(c.desc)
+        assert e.value.code == t0g.ERR_INVALID_ARG and "capture" in str(e.value)
+        fresh.linear_cross_entropy(c.desc)   # the handle is as usable as before
+        fresh.wait_idle()
+        for k, (_, v) in c.bufs.items():
+            assert torch.equal(v.cpu(), want[k]), k
+        fresh.set_stream(0)
