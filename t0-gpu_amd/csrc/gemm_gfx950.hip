@@ -1233,7 +1233,8 @@ __device__ __forceinline__ void gemm_tile_fast(const T0gGemmArgs& p, const T0gGe
     const uint32_t kend = min(p.k, kbeg + p.k_per_split);
     const int nst = kend > kbeg ? (int)((kend - kbeg + BK - 1) / BK) : 0;
 
-    const uint32_t a_bytes = (A_K ? (p.m - 1) * p.lda + p.k : (p.k - 1) * p.lda + p.m) * 2;
+    // a K-contiguous A may end inside a 16-byte piece that its rows are zero padded to
+    const uint32_t a_bytes = (A_K ? (p.m - 1) * p.lda + ((p.k + 7) & ~7u) : (p.k - 1) * p.lda + p.m) * 2;
     const uint32_t b_bytes = (B_K ? (p.n - 1) * p.ldb + p.k : (p.k - 1) * p.ldb + p.n) * 2;
 
     const uint32_t lane = tid & 63u, wave = tid >> 6;
@@ -1476,6 +1477,8 @@ __device__ __forceinline__ void splitk_reduce(const T0gReduceArgs& p) {
 }
 
 }  // namespace t0g
+
+#ifndef T0G_TILES_ONLY   // the losses' code object (losses_gfx950.hip) takes the tile bodies above only
 
 // f32 -> bf16 with the rounding of the reference's operand conversion
 // (src/ignis/ops/bf16_matmul.rs:372-375): (bits + 0x7FFF + ((bits >> 16) & 1)) >> 16,
@@ -1760,3 +1763,5 @@ extern "C" __global__ void __launch_bounds__(256) t0g_splitk_reduce_f32(T0gReduc
 extern "C" __global__ void __launch_bounds__(256) t0g_splitk_reduce_bf16(T0gReduceArgs p) {
     t0g::splitk_reduce<true>(p);
 }
+
+#endif   // T0G_TILES_ONLY

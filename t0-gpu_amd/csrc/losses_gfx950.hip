@@ -6,16 +6,12 @@
 // All statistics, losses and coefficients are f32.  The logit gradients are
 // rounded to bf16 once, because the products that take them on to dx and dW
 // multiply bf16 operands.
-#include <hip/hip_runtime.h>
-#include <stdint.h>
-
-#include "t0g_kernel_args.h"
+#define T0G_TILES_ONLY
+#include "gemm_gfx950.hip"
 
 namespace t0g {
 
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 template <class T>
 using gptr = __attribute__((address_space(1))) T*;
@@ -59,6 +55,12 @@ __device__ __forceinline__ float block_sum(float v, float* t) {
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16);
 }
+
+}  // namespace t0g
+
+#include "losses_tile.h"
+
+namespace t0g {
 
 // A label or token as an index into the vocabulary, kNoToken outside it.
 __device__ __forceinline__ uint32_t token_at(uint64_t base, uint64_t i, bool wide, uint32_t vocab) {
@@ -180,6 +182,20 @@ __device__ __forceinline__ void prepare_row(const T0gLossArgs& p, uint32_t row) 
         __syncthreads();
         hq = block_sum(part, red[0]);
     }
+    if (p.ent_off) {   // entries before each block of columns
+        __syncthreads();   // the row's tokens are written
+        for (uint32_t b = tid; b < p.off_ld; b += kThreads) {
+            uint32_t lo = 0, hi = n;   // first entry at or past the block's first token
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (*at<const uint32_t>(p.ent_tok, (uint64_t)row * p.slots + mid) < b * T0G_LOSS_BLOCK)
+                    lo = mid + 1;
+                else
+                    hi = mid;
+            }
+            *at<uint16_t>(p.ent_off, (uint64_t)row * p.off_ld + b) = (uint16_t)lo;
+        }
+    }
     if (tid == 0) {
         *at<u32x2_t>(p.row_ent, row) = u32x2_t{n, label_slot};
         *at<f32x4_t>(p.row_sub, row) =
@@ -237,49 +253,79 @@ __device__ __forceinline__ void chunk_stats(const T0gLossArgs& p, uint32_t row, 
     __syncthreads();
 }
 
-// A row's chunks joined: its loss, log-sum-exp and gradient coefficients.  One wave.
-__device__ __forceinline__ void combine_row(const T0gLossArgs& p, uint32_t row) {
-    const uint32_t lane = threadIdx.x & 63u;
-    const bool dual = p.flags & T0G_LOSS_DUAL;
-    float m = ninf();
-    for (uint32_t c = lane; c < p.chunks; c += 64)
-        m = __builtin_fmaxf(m, (*at<const f32x2_t>(p.part, (uint64_t)c * p.rows + row))[0]);
-    m = wave_max(m);
-    float s = 0.0f, s2 = 0.0f;
-    for (uint32_t c = lane; c < p.chunks; c += 64) {
-        const uint64_t i = (uint64_t)c * p.rows + row;
-        const f32x2_t v = *at<const f32x2_t>(p.part, i);
-        s += v[1] * exp2_(v[0] - m);
-        if (dual) s2 += *at<const float>(p.part2, i) * exp2_((v[0] - m) * p.r);
-    }
-    s = wave_sum(s);
-    const float l0 = m + __builtin_amdgcn_logf(s);
+// Rows' chunks joined: their losses, log-sum-exps and gradient coefficients.  A workgroup
+// takes 2^row_shift rows, so that a chunk's statistics of neighbouring rows are read as
+// one line, with 256 >> row_shift threads on each.
+__device__ __forceinline__ void combine_rows(const T0gLossArgs& p, uint32_t row0) {
+    __shared__ float t0[kThreads], t1[kThreads];
+    const uint32_t tid = threadIdx.x, per = kThreads >> p.row_shift;
+    const uint32_t row = row0 + (tid & ((1u << p.row_shift) - 1)), part = tid >> p.row_shift;
+    const bool live = row < p.rows, dual = p.flags & T0G_LOSS_DUAL;
+    // threads of one row are 2^row_shift apart
+    auto join = [&](float* t, float v, bool max) {
+        __syncthreads();
+        t[tid] = v;
+        for (uint32_t o = kThreads / 2; o >> p.row_shift; o >>= 1) {
+            __syncthreads();
+            if (tid < o) t[tid] = max ? __builtin_fmaxf(t[tid], t[tid + o]) : t[tid] + t[tid + o];
+        }
+        __syncthreads();
+        return t[tid & ((1u << p.row_shift) - 1)];
+    };
+    // each thread's own chunks first, in one pass
+    float m = ninf(), s = 0.0f, s2 = 0.0f;
+    if (live)
+        for (uint32_t c = part; c < p.chunks; c += per) {
+            const uint64_t i = (uint64_t)c * p.rows + row;
+            const f32x2_t v = *at<const f32x2_t>(p.part, i);
+            const float top = __builtin_fmaxf(m, v[0]);
+            const float old = m == top ? 1.0f : exp2_(m - top), now = v[0] == top ? 1.0f : exp2_(v[0] - top);
+            s = s * old + v[1] * now;
+            if (dual) {
+                const float old2 = m == top ? 1.0f : exp2_((m - top) * p.r);
+                const float now2 = v[0] == top ? 1.0f : exp2_((v[0] - top) * p.r);
+                s2 = s2 * old2 + *at<const float>(p.part2, i) * now2;
+            }
+            m = top;
+        }
+    const float top = join(t0, m, true);
+    const float scale = m == top ? 1.0f : exp2_(m - top);
+    s = join(t0, s * scale, false);
+    const float l0 = top + __builtin_amdgcn_logf(s);
     float l1 = l0;
-    if (dual) l1 = m * p.r + __builtin_amdgcn_logf(wave_sum(s2));
-    const u32x2_t ent = *at<const u32x2_t>(p.row_ent, row);
-    const f32x4_t sub = *at<const f32x4_t>(p.row_sub, row);
+    if (dual) l1 = top * p.r + __builtin_amdgcn_logf(join(t1, s2 * (m == top ? 1.0f : exp2_((m - top) * p.r)), false));
+    u32x2_t ent = {0u, kNoToken};
+    f32x4_t sub = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (live) {
+        ent = *at<const u32x2_t>(p.row_ent, row);
+        sub = *at<const f32x4_t>(p.row_sub, row);
+    }
     const bool taught = sub[3] != 0.0f, labelled = ent[1] != kNoToken;
     float kd = 0.0f;
-    if (taught)
-        for (uint32_t e = lane; e < ent[0]; e += 64) {
-            const uint64_t slot = (uint64_t)row * p.slots + e;
-            const float q = *at<const float>(p.ent_q, slot);
-            if (q != 0.0f) kd += q * (l1 * kLn2 - *at<const float>(p.ent_z, slot) * (p.logit_scale / p.tau));
-        }
-    kd = wave_sum(kd);
-    if (lane != 0) return;
-    float loss = 0.0f;
-    if (labelled)
-        loss = p.label_weight *
-               (l0 * kLn2 - *at<const float>(p.ent_z, (uint64_t)row * p.slots + ent[1]) * p.logit_scale);
-    if (taught) loss += p.distill_weight * p.tau * p.tau * (sub[2] + kd);
-    const bool used = labelled || taught;
-    *at<float>(p.loss, row) = loss;
-    if (p.lse) *at<float>(p.lse, row) = used ? l1 * kLn2 : 0.0f;
-    if (p.row_par)
-        *at<f32x4_t>(p.row_par, row) = !used  ? f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}
-                                       : dual ? f32x4_t{l0, l1, sub[0], sub[1]}
-                                              : f32x4_t{l0, l1, sub[0] + sub[1], 0.0f};
+    if (p.teacher) {
+        if (taught)
+            for (uint32_t e = part; e < ent[0]; e += per) {
+                const uint64_t slot = (uint64_t)row * p.slots + e;
+                const float q = *at<const float>(p.ent_q, slot);
+                if (q != 0.0f) kd += q * (l1 * kLn2 - *at<const float>(p.ent_z, slot) * (p.logit_scale / p.tau));
+            }
+        kd = join(t1, kd, false);
+    }
+    if (part == 0 && live) {
+        float loss = 0.0f;
+        if (labelled)
+            loss = p.label_weight *
+                   (l0 * kLn2 - *at<const float>(p.ent_z, (uint64_t)row * p.slots + ent[1]) * p.logit_scale);
+        if (taught) loss += p.distill_weight * p.tau * p.tau * (sub[2] + kd);
+        const bool used = labelled || taught;
+        *at<float>(p.loss, row) = loss;
+        if (p.lse) *at<float>(p.lse, row) = used ? l1 * kLn2 : 0.0f;
+        if (p.row_par)
+            *at<f32x4_t>(p.row_par, row) = !used  ? f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}
+                                           : dual ? f32x4_t{l0, l1, sub[0], sub[1]}
+                                                  : f32x4_t{l0, l1, sub[0] + sub[1], 0.0f};
+    }
+    __syncthreads();
 }
 
 // The dense part of a logit's gradient.
@@ -288,6 +334,21 @@ __device__ __forceinline__ float dense_grad(const T0gLossArgs& p, const f32x4_t&
     float g = par[2] * exp2_(u - par[0]);
     if (p.flags & T0G_LOSS_DUAL) g += par[3] * exp2_(u * p.r - par[1]);
     return g;
+}
+
+// The gradients of a row's entries in columns [c0, c0 + n) of the piece, over the dense part.
+__device__ __forceinline__ void entry_grads(const T0gLossArgs& p, uint32_t row, uint32_t c0, uint32_t n,
+                                            const f32x4_t& par, uint32_t first, uint32_t step) {
+    const u32x2_t ent = *at<const u32x2_t>(p.row_ent, row);
+    const f32x4_t sub = *at<const f32x4_t>(p.row_sub, row);
+    for (uint32_t e = first; e < ent[0]; e += step) {
+        const uint64_t slot = (uint64_t)row * p.slots + e;
+        const uint32_t c = *at<const uint32_t>(p.ent_tok, slot) - (p.v0 + c0);   // wraps below the range
+        if (c >= n) continue;
+        float g = dense_grad(p, par, *at<const float>(p.ent_z, slot)) - sub[1] * *at<const float>(p.ent_q, slot);
+        if (e == ent[1]) g -= sub[0];
+        *at<__bf16>(p.g, (uint64_t)row * p.ldg + c0 + c) = (__bf16)g;
+    }
 }
 
 // Logit gradients of one chunk of a row in bf16, zero past the piece, then its entries.
@@ -310,18 +371,43 @@ __device__ __forceinline__ void chunk_grad(const T0gLossArgs& p, uint32_t row, u
         *at<u32x2_t>(gb, c / 4) = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
     }
     __syncthreads();   // the dense part is written before its entries are replaced
-    if (used) {
-        const u32x2_t ent = *at<const u32x2_t>(p.row_ent, row);
-        const f32x4_t sub = *at<const f32x4_t>(p.row_sub, row);
-        for (uint32_t e = tid; e < ent[0]; e += kThreads) {
-            const uint64_t slot = (uint64_t)row * p.slots + e;
-            const uint32_t c = *at<const uint32_t>(p.ent_tok, slot) - (p.v0 + c0);
-            if (c >= n) continue;
-            float g = dense_grad(p, par, *at<const float>(p.ent_z, slot)) - sub[1] * *at<const float>(p.ent_q, slot);
-            if (e == ent[1]) g -= sub[0];
-            *at<__bf16>(gb, c) = (__bf16)g;
+    if (used) entry_grads(p, row, c0, n, par, tid, kThreads);
+}
+
+// The same from the kept exponentials, in place: e 2^(m - l0) is the probability, and
+// with a second temperature e^r 2^(m r - l1).
+__device__ __forceinline__ void kept_grad(const T0gLossArgs& p, uint32_t row, uint32_t chunk) {
+    constexpr uint32_t kCols = 8 * kThreads;
+    const uint32_t c0 = chunk * kCols, tid = threadIdx.x, c = c0 + 8 * tid;
+    const f32x4_t par = *at<const f32x4_t>(p.row_par, row);
+    const bool used = par[2] != 0.0f || par[3] != 0.0f;
+    if (c < p.ldg) {
+        u32x4_t w = {0u, 0u, 0u, 0u};
+        if (used && c < p.cols) {
+            const float m = (*at<const f32x2_t>(p.part, (uint64_t)(p.chunk0 + c / T0G_LOSS_BLOCK) * p.rows + row))[0];
+            const float f0 = par[2] * exp2_(m - par[0]);
+            const u32x4_t e = *at<const u32x4_t>(p.g, ((uint64_t)row * p.ldg + c) / 8);
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = __builtin_bit_cast(float, (e[i] & 0xFFFFu) << 14);
+                v[2 * i + 1] = __builtin_bit_cast(float, (e[i] & 0xFFFF0000u) >> 2);
+            }
+            if (p.flags & T0G_LOSS_DUAL) {
+                const float f1 = par[3] * exp2_(m * p.r - par[1]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = f0 * v[i] + f1 * exp2_(__builtin_amdgcn_logf(v[i]) * p.r);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= f0;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack2(v[2 * i], v[2 * i + 1]);
         }
+        *at<u32x4_t>(p.g, ((uint64_t)row * p.ldg + c) / 8) = w;
     }
+    __syncthreads();   // the dense part is written before its entries are replaced
+    if (used && c0 < p.cols) entry_grads(p, row, c0, min(kCols, p.cols - c0), par, tid, kThreads);
 }
 
 __device__ __forceinline__ void sum_planes(const T0gLossSumArgs& p) {
@@ -358,9 +444,30 @@ extern "C" __global__ void __launch_bounds__(256) t0g_loss_stats(T0gLossArgs p) 
     for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) t0g::chunk_stats(p, row, blockIdx.x);
 }
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_combine(T0gLossArgs p) {
-    for (uint32_t row = blockIdx.x * 4 + threadIdx.x / 64; row < p.rows; row += gridDim.x * 4) t0g::combine_row(p, row);
+    for (uint32_t row = blockIdx.x << p.row_shift; row < p.rows; row += gridDim.x << p.row_shift) t0g::combine_rows(p, row);
 }
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_grad(T0gLossArgs p) {
     for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) t0g::chunk_grad(p, row, blockIdx.x);
 }
+extern "C" __global__ void __launch_bounds__(256) t0g_loss_grad_kept(T0gLossArgs p) {
+    for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) t0g::kept_grad(p, row, blockIdx.x);
+}
+// one wave a row
+extern "C" __global__ void __launch_bounds__(256) t0g_loss_grad_entries(T0gLossArgs p) {
+    for (uint32_t row = blockIdx.x * 4 + threadIdx.x / 64; row < p.rows; row += gridDim.x * 4) {
+        const t0g::f32x4_t par = *t0g::at<const t0g::f32x4_t>(p.row_par, row);
+        if (par[2] != 0.0f || par[3] != 0.0f) t0g::entry_grads(p, row, 0, p.cols, par, threadIdx.x & 63u, 64);
+    }
+}
+#define T0G_LOSS_GEMM(NAME, BK, KIND)                                                                             \
+    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))                  \
+        NAME(T0gLossGemmArgs a) {                                                                                 \
+        t0g::loss_tile<BK, t0g::LossTile::KIND>(a);                                                               \
+    }
+T0G_LOSS_GEMM(t0g_loss_logits_nt, true, Stats)
+T0G_LOSS_GEMM(t0g_loss_logits_nn, false, Stats)
+T0G_LOSS_GEMM(t0g_loss_logits_nt_kept, true, Keep)
+T0G_LOSS_GEMM(t0g_loss_logits_nn_kept, false, Keep)
+T0G_LOSS_GEMM(t0g_loss_again_nt, true, Grad)
+T0G_LOSS_GEMM(t0g_loss_again_nn, false, Grad)
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_sum(T0gLossSumArgs p) { t0g::sum_planes(p); }

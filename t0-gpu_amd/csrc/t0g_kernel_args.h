@@ -180,13 +180,16 @@ typedef struct T0gLossArgs {
     uint64_t part2;          /* f32 [chunks][rows]: the second sum (DUAL)             */
     uint64_t z;              /* f32 [rows][ldz]: a piece's raw logits                 */
     uint64_t g;              /* bf16 [rows][ldg]: a piece's logit gradients           */
+    uint64_t ent_off;        /* u16 [rows][off_ld] (T0gLossGemmArgs), or 0            */
     uint32_t rows, vocab, hidden, ldx, ldxz;
     uint32_t top_k, ldt, slots;
+    uint32_t off_ld;
     uint32_t v0, cols;       /* the piece: its first token and width                  */
     uint32_t ldz, ldg;
     uint32_t chunk0;         /* the piece's first chunk                               */
     uint32_t chunks;         /* chunks of the piece, or of the vocabulary (combine)   */
     uint32_t flags;          /* T0G_LOSS_* bits                                       */
+    uint32_t row_shift;      /* combine: 2^row_shift rows a workgroup, 0 to 4          */
     float k, r;              /* u = z k; second temperature's ratio                   */
     float logit_scale, tau;
     float label_weight, distill_weight;
@@ -199,6 +202,25 @@ typedef struct T0gLossArgs {
 #define T0G_LOSS_X_VEC 16u     /* x rows are 16-byte aligned and hidden a multiple of 8 */
 #define T0G_LOSS_CHUNK 4096u   /* columns of one workgroup in the row kernels          */
 #define T0G_LOSS_MAX_TOP 1024u /* teacher entries of a row, at most                    */
+
+/* The 256x256 GEMM of a piece's logits with the softmax in its epilogue: statistics per
+ * row and block of T0G_LOSS_BLOCK columns, and the entries' raw logits (t0g_loss_logits*;
+ * g.c: the exponentials 2^(u - m) in 16 bits, or none), or the logits' gradients
+ * (t0g_loss_again*; g.c: bf16).  g.c has whole tiles: rows and columns padded to 256. */
+typedef struct T0gLossGemmArgs {
+    T0gGemmArgs g;
+    uint64_t part;           /* f32 [blocks][rows][2] of this piece                   */
+    uint64_t part2;          /* f32 [blocks][rows] (DUAL)                             */
+    uint64_t ent_tok;        /* u32 [rows][slots]                                     */
+    uint64_t ent_z;          /* f32 [rows][slots]                                     */
+    uint64_t ent_off;        /* u16 [rows][off_ld]: entries before each block of the
+                                vocabulary; 0: one slot, the label's                  */
+    uint64_t row_par;        /* f32 [rows][4]                                         */
+    uint32_t v0, slots, off_ld;
+    uint32_t flags;          /* T0G_LOSS_DUAL                                         */
+    float k, r;
+} T0gLossGemmArgs;
+#define T0G_LOSS_BLOCK 128u    /* columns of one wave of the 256x256 tile              */
 
 /* Sum of f32 planes of a data gradient, in order, into bf16 or f32 rows. */
 typedef struct T0gLossSumArgs {

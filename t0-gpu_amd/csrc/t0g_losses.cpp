@@ -6,8 +6,14 @@
 //   prepare   every row's entries (label, teacher's tokens), the masked copy of x
 //   pieces    z = x W_p^T, the chunks' softmax statistics, the entries' logits
 //   combine   loss, log-sum-exp and gradient coefficients of every row
-//   pieces    again, last first, for the gradients: z (the last piece's is still
-//             there), G = dL/dz in bf16, dx += G W_p, dW_p = G^T x
+//   pieces    again, last first, for the gradients: G = dL/dz in bf16, dx += G W_p,
+//             dW_p = G^T x
+// in one of two forms:
+//   fused     the statistics are taken in the logits GEMM's epilogue (losses_tile.h), which
+//             for the last piece also leaves its exponentials, 16 bits each, where G goes;
+//             the other pieces' logits are computed again with G in the epilogue
+//   by rows   a piece's f32 logits go to the scratch and row kernels read them: products
+//             of few rows, and operands that the 256x256 tile does not take
 #include <math.h>
 #include <string.h>
 
@@ -22,8 +28,14 @@ namespace t0g {
 
 namespace {
 
-// A piece's f32 logits, and the f32 partial sums of dx, take about this much each.
+// A piece's f32 logits take this much (by rows), its logit gradients that much (fused: a
+// step of 8192 rows and 131072 tokens then keeps within 1.25 GiB of scratch), and f32
+// partial sums of dx are added up when they take more than kPlaneBytes.
 constexpr uint64_t kPieceBytes = 256ull << 20;
+constexpr uint64_t kFusedPieceBytes = 880ull << 20;
+constexpr uint64_t kPlaneBytes = 128ull << 20;
+// Rows from which the fused form is taken.
+constexpr uint32_t kFusedRows = 256;
 // Rows of a launch's y grid, at most (the kernels step through the rest).
 constexpr uint32_t kMaxGridY = 65535;
 
@@ -124,9 +136,11 @@ struct Piece {
 // The pieces, and where everything is in the scratch.
 struct Plan {
     std::vector<Piece> pieces;
-    uint32_t chunks = 0, slots = 0, ldxz = 0;
+    bool fused = false;
+    uint32_t chunks = 0, slots = 0, ldxz = 0, off_ld = 0;
     uint32_t group = 0;          // planes of dx summed at a time (0: the one product writes dx)
-    uint64_t xz = 0, ent_tok = 0, ent_q = 0, ent_z = 0, row_ent = 0, row_sub = 0, row_par = 0, part = 0, part2 = 0;
+    uint64_t xz = 0, ent_tok = 0, ent_q = 0, ent_z = 0, row_ent = 0, row_sub = 0, row_par = 0, part = 0, part2 = 0,
+             ent_off = 0;
     uint64_t z = 0, g = 0, planes = 0, acc = 0, gemm_ws = 0;
     uint64_t gemm_ws_bytes = 0, bytes = 0;
 };
@@ -152,6 +166,9 @@ t0g_gemm_desc gemm_of(uint64_t a, uint64_t b, uint64_t c, uint32_t m, uint32_t n
     return g;
 }
 
+// G's leading dimension; the fused form stores whole tiles.
+uint32_t ld_of_g(const Plan &pl, const Piece &pc) { return round_up(pc.cols, pl.fused ? 256 : 8); }
+
 uint64_t weight_piece(const Problem &p, uint64_t w, uint32_t v0, uint32_t ld, uint32_t size) {
     return w + (p.d.transpose == T0G_NT ? (uint64_t)v0 * ld : v0) * size;
 }
@@ -168,32 +185,58 @@ t0g_gemm_desc dx_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_
     const bool whole = pl.group == 0;
     return gemm_of(base + pl.g, weight_piece(p, d.w, pc.v0, d.ldw, 2),
                    whole ? d.dx : base + pl.planes + (uint64_t)plane * d.rows * d.hidden * 4, d.rows, d.hidden, pc.cols,
-                   round_up(pc.cols, 8), d.ldw, whole ? d.lddx : d.hidden, d.transpose == T0G_NT ? T0G_NN : T0G_NT,
+                   ld_of_g(pl, pc), d.ldw, whole ? d.lddx : d.hidden, d.transpose == T0G_NT ? T0G_NN : T0G_NT,
                    whole ? d.dx_dtype : (uint32_t)T0G_F32);
 }
 
-t0g_gemm_desc dw_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
+// dW of columns [c0, c0 + cols) of a piece.
+t0g_gemm_desc dw_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base, uint32_t c0, uint32_t cols) {
     const t0g_linear_ce_desc &d = p.d;
-    const uint64_t c = weight_piece(p, d.dw, pc.v0, d.lddw, dtype_size(d.dw_dtype));
-    const uint32_t ldg = round_up(pc.cols, 8);
+    const uint64_t c = weight_piece(p, d.dw, pc.v0 + c0, d.lddw, dtype_size(d.dw_dtype)), g = base + pl.g + c0 * 2ull;
+    const uint32_t ldg = ld_of_g(pl, pc);
     return d.transpose == T0G_NT
-               ? gemm_of(base + pl.g, base + pl.xz, c, pc.cols, d.hidden, d.rows, ldg, pl.ldxz, d.lddw, T0G_TN, d.dw_dtype)
-               : gemm_of(base + pl.xz, base + pl.g, c, d.hidden, pc.cols, d.rows, pl.ldxz, ldg, d.lddw, T0G_TN, d.dw_dtype);
+               ? gemm_of(g, base + pl.xz, c, cols, d.hidden, d.rows, ldg, pl.ldxz, d.lddw, T0G_TN, d.dw_dtype)
+               : gemm_of(base + pl.xz, g, c, d.hidden, cols, d.rows, pl.ldxz, ldg, d.lddw, T0G_TN, d.dw_dtype);
+}
+// The columns of dW's two products: all, or a multiple of 8 and the rest, which alone
+// would keep the whole off the aligned kernels.
+uint32_t dw_body(const Problem &p, const Piece &pc) {
+    return pc.cols > 8 && p.d.hidden % 8 == 0 ? pc.cols & ~7u : pc.cols;
 }
 
 int make_loss_plan(const Problem &p, Plan *pl) {
     const t0g_linear_ce_desc &d = p.d;
     const uint64_t rows = d.rows ? d.rows : 1;
-    // A vocabulary that is not a multiple of 8 gets its last few tokens as a piece of their
-    // own where they alone would keep the products off the aligned kernels.
-    const bool aligned = (d.w & 15) == 0 && d.ldw % 8 == 0 && d.hidden % 8 == 0;
-    const uint32_t body = aligned && d.vocab > 8 && (p.grad || d.transpose == T0G_NN) ? d.vocab & ~7u : d.vocab;
-    uint64_t width = std::max<uint64_t>(256, kPieceBytes / (rows * 4) / 256 * 256);
-    if (d.max_piece) width = std::min<uint64_t>(width, d.max_piece <= 8 ? 8 : d.max_piece & ~7u);
+    const bool aligned = (d.w & 15) == 0 && d.ldw % 8 == 0 && d.hidden % 8 == 0, nt = d.transpose == T0G_NT;
+    const uint32_t ldx = p.grad ? round_up(d.hidden, 8) : d.ldx;
+    // the 256x256 tile's operands: whole 16-byte pieces, 32-bit byte offsets, and of a
+    // weight [hidden][vocab] rows of 256 or more
+    pl->fused = d.rows >= kFusedRows && aligned && (p.grad || ((d.x & 15) == 0 && d.ldx % 8 == 0)) &&
+                (uint64_t)d.rows * ldx < (1ull << 30) && (d.max_piece == 0 || d.max_piece >= 256) &&
+                (nt ? (uint64_t)d.ldw * 256 < (1ull << 30)
+                    : d.vocab % 8 == 0 && d.ldw >= 256 && (uint64_t)d.hidden * d.ldw < (1ull << 30));
+    uint64_t width;
+    uint32_t body = d.vocab, chunk = T0G_LOSS_CHUNK;
+    if (pl->fused) {
+        chunk = T0G_LOSS_BLOCK;
+        width = p.grad ? kFusedPieceBytes / 2 / round_up(d.rows, 256) : d.vocab;
+        if (nt) width = std::min<uint64_t>(width, ((1ull << 30) - 1) / d.ldw);
+        if (d.max_piece) width = std::min<uint64_t>(width, d.max_piece);
+        width = std::max<uint64_t>(256, width / 256 * 256);
+    } else {
+        // A vocabulary that is not a multiple of 8 gets its last few tokens as a piece of
+        // their own where they alone would keep the products off the aligned kernels.
+        if (aligned && d.vocab > 8 && (p.grad || !nt)) body = d.vocab & ~7u;
+        width = std::max<uint64_t>(256, kPieceBytes / (rows * 4) / 256 * 256);
+        if (d.max_piece) width = std::min<uint64_t>(width, d.max_piece <= 8 ? 8 : d.max_piece & ~7u);
+    }
+    // fused: the last piece's exponentials are kept, so the first is the short one
+    const uint64_t whole = ((uint64_t)d.vocab + 255) / 256 * 256;
+    const uint64_t head = pl->fused && whole > width ? whole - (whole - 1) / width * width : width;
     for (uint32_t v0 = 0; v0 < d.vocab;) {
         const uint32_t end = v0 < body ? body : d.vocab;
-        const uint32_t cols = (uint32_t)std::min<uint64_t>(width, end - v0);
-        const uint32_t chunks = (cols + T0G_LOSS_CHUNK - 1) / T0G_LOSS_CHUNK;
+        const uint32_t cols = (uint32_t)std::min<uint64_t>(v0 == 0 ? head : width, end - v0);
+        const uint32_t chunks = (cols + chunk - 1) / chunk;
         pl->pieces.push_back(Piece{v0, cols, pl->chunks, chunks});
         pl->chunks += chunks;
         v0 += cols;
@@ -202,7 +245,7 @@ int make_loss_plan(const Problem &p, Plan *pl) {
     pl->ldxz = round_up(d.hidden, 8);
     const uint64_t plane = rows * d.hidden * 4;
     if (d.dx && pl->pieces.size() > 1)
-        pl->group = (uint32_t)std::min<uint64_t>(pl->pieces.size(), std::max<uint64_t>(1, kPieceBytes / plane));
+        pl->group = (uint32_t)std::min<uint64_t>(pl->pieces.size(), std::max<uint64_t>(1, kPlaneBytes / plane));
 
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
@@ -221,19 +264,31 @@ int make_loss_plan(const Problem &p, Plan *pl) {
     if (p.grad) pl->row_par = take(rows * 16);
     pl->part = take(rows * pl->chunks * 8);
     if (p.dual) pl->part2 = take(rows * pl->chunks * 4);
-    pl->z = take(rows * round_up(widest, 4) * 4);
-    if (p.grad) pl->g = take(rows * round_up(widest, 8) * 2);
+    if (pl->fused) {
+        if (p.t) {
+            pl->off_ld = pl->chunks + 1;
+            pl->ent_off = take(rows * pl->off_ld * 2);
+        }
+        if (p.grad) pl->g = take((uint64_t)round_up(d.rows, 256) * round_up(widest, 256) * 2);
+    } else {
+        pl->z = take(rows * round_up(widest, 4) * 4);
+        if (p.grad) pl->g = take(rows * round_up(widest, 8) * 2);
+    }
     if (pl->group) {
         pl->planes = take(pl->group * plane);
         if (pl->group < pl->pieces.size()) pl->acc = take(plane);
     }
     // one split-K workspace for all products, which run one after another
     for (const Piece &pc : pl->pieces) {
-        t0g_gemm_desc g[3];
+        t0g_gemm_desc g[4];
         int n = 0, rc;
-        g[n++] = logits_gemm(p, *pl, pc, 0);
+        if (!pl->fused) g[n++] = logits_gemm(p, *pl, pc, 0);
         if (d.dx) g[n++] = dx_gemm(p, *pl, pc, 0, 0);
-        if (d.dw) g[n++] = dw_gemm(p, *pl, pc, 0);
+        if (d.dw) {
+            const uint32_t body = dw_body(p, pc);
+            g[n++] = dw_gemm(p, *pl, pc, 0, 0, body);
+            if (body < pc.cols) g[n++] = dw_gemm(p, *pl, pc, 0, body, pc.cols - body);
+        }
         for (int i = 0; i < n; ++i) {
             size_t bytes = 0;
             if ((rc = losses_gemm_workspace(&g[i], &bytes))) return rc;
@@ -251,6 +306,56 @@ int run_gemm(t0g_device *dev, t0g_gemm_desc g, const Plan &pl, uint64_t base) {
     return losses_gemm(dev, &g);
 }
 
+int run_dw(t0g_device *dev, const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
+    const uint32_t body = dw_body(p, pc);
+    int rc = run_gemm(dev, dw_gemm(p, pl, pc, base, 0, body), pl, base);
+    if (rc || body == pc.cols) return rc;
+    return run_gemm(dev, dw_gemm(p, pl, pc, base, body, pc.cols - body), pl, base);
+}
+
+// One of the 256x256 kernels on a piece: statistics, statistics with the exponentials kept, or G.
+enum class Tile { Stats, Keep, Grad };
+int run_tile(t0g_device *dev, Tile kind, const Problem &p, const Plan &pl, const Piece &pc, const T0gLossArgs &a,
+             uint64_t base) {
+    const t0g_linear_ce_desc &d = p.d;
+    T0gLossGemmArgs t;
+    memset(&t, 0, sizeof t);
+    t.g.a = p.grad ? base + pl.xz : d.x;
+    t.g.b = weight_piece(p, d.w, pc.v0, d.ldw, 2);
+    t.g.c = p.grad ? base + pl.g : 0;
+    t.g.m = d.rows;
+    t.g.n = pc.cols;
+    t.g.k = d.hidden;
+    t.g.lda = p.grad ? pl.ldxz : d.ldx;
+    t.g.ldb = d.ldw;
+    t.g.ldc = ld_of_g(pl, pc);
+    t.g.tiles_m = round_up(d.rows, 256) / 256;
+    t.g.tiles_n = round_up(pc.cols, 256) / 256;
+    t.g.group_m = 8;
+    t.g.flags = T0G_FLAG_XCD_REMAP;
+    // the 256x256 GEMM kernels' rule for touching the lines of later stages
+    const uint64_t wgs = (uint64_t)t.g.tiles_m * t.g.tiles_n;
+    if (2.0 * d.hidden * ((double)d.rows + pc.cols) >= 96e6 &&
+        (wgs <= 2 * kNumCUs || (t.g.tiles_m & (t.g.tiles_m - 1)) == 0))
+        t.g.flags |= T0G_FLAG_PREFETCH;
+    t.part = a.part + (uint64_t)pc.chunk0 * d.rows * 8;
+    t.part2 = a.part2 ? a.part2 + (uint64_t)pc.chunk0 * d.rows * 4 : 0;
+    t.ent_tok = a.ent_tok;
+    t.ent_z = a.ent_z;
+    t.ent_off = a.ent_off;
+    t.row_par = a.row_par;
+    t.v0 = pc.v0;
+    t.slots = pl.slots;
+    t.off_ld = pl.off_ld;
+    t.flags = a.flags;
+    t.k = a.k;
+    t.r = a.r;
+    static const char *symbols[3][2] = {{"t0g_loss_logits_nt", "t0g_loss_logits_nn"},
+                                        {"t0g_loss_logits_nt_kept", "t0g_loss_logits_nn_kept"},
+                                        {"t0g_loss_again_nt", "t0g_loss_again_nn"}};
+    return losses_launch(dev, symbols[(int)kind][d.transpose == T0G_NN], (uint32_t)wgs, 1, &t, sizeof t);
+}
+
 int run_loss(t0g_device *dev, const Problem &p) {
     const t0g_linear_ce_desc &d = p.d;
     Plan pl;
@@ -260,7 +365,7 @@ int run_loss(t0g_device *dev, const Problem &p) {
     if ((rc = losses_begin(dev, pl.bytes, &base))) return rc;
     if (d.rows == 0) {
         for (const Piece &pc : pl.pieces)   // a product over no rows: zeros
-            if (d.dw && (rc = run_gemm(dev, dw_gemm(p, pl, pc, base), pl, base))) return rc;
+            if (d.dw && (rc = run_dw(dev, p, pl, pc, base))) return rc;
         return ok();
     }
     T0gLossArgs a;
@@ -281,6 +386,8 @@ int run_loss(t0g_device *dev, const Problem &p) {
     a.part2 = p.dual ? base + pl.part2 : 0;
     a.z = base + pl.z;
     a.g = p.grad ? base + pl.g : 0;
+    a.ent_off = pl.off_ld ? base + pl.ent_off : 0;
+    a.off_ld = pl.off_ld;
     a.rows = d.rows;
     a.vocab = d.vocab;
     a.hidden = d.hidden;
@@ -314,21 +421,32 @@ int run_loss(t0g_device *dev, const Problem &p) {
         const uint32_t groups = (uint32_t)(((uint64_t)d.rows + rows_per_group - 1) / rows_per_group);
         return losses_launch(dev, symbol, std::min<uint32_t>(groups, 1u << 20), 1, &a, sizeof a);
     };
-    auto piece_kernel = [&](const char *symbol, const Piece &pc) {
+    auto at_piece = [&](const Piece &pc) {
         a.v0 = pc.v0;
         a.cols = pc.cols;
         a.ldz = round_up(pc.cols, 4);
-        a.ldg = round_up(pc.cols, 8);
+        a.ldg = ld_of_g(pl, pc);
         a.chunk0 = pc.chunk0;
         a.chunks = pc.chunks;
-        return losses_launch(dev, symbol, pc.chunks, std::min(d.rows, kMaxGridY), &a, sizeof a);
     };
+    auto piece_kernel = [&](const char *symbol, uint32_t groups) {
+        return losses_launch(dev, symbol, groups, std::min(d.rows, kMaxGridY), &a, sizeof a);
+    };
+    const size_t n = pl.pieces.size();
     if ((rc = row_kernel("t0g_loss_prepare", 1))) return rc;
-    for (const Piece &pc : pl.pieces)
-        if ((rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base)) || (rc = piece_kernel("t0g_loss_stats", pc)))
-            return rc;
+    for (size_t i = 0; i < n; ++i) {
+        const Piece &pc = pl.pieces[i];
+        at_piece(pc);
+        if (pl.fused)
+            rc = run_tile(dev, p.grad && i + 1 == n ? Tile::Keep : Tile::Stats, p, pl, pc, a, base);
+        else if (!(rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base)))
+            rc = piece_kernel("t0g_loss_stats", pc.chunks);
+        if (rc) return rc;
+    }
     a.chunks = pl.chunks;
-    if ((rc = row_kernel("t0g_loss_combine", 4))) return rc;
+    // 16 rows read a chunk's statistics as one line; fewer where that leaves CUs idle
+    while (a.row_shift < 4 && d.rows >> (a.row_shift + 1) >= 2 * kNumCUs) ++a.row_shift;
+    if ((rc = row_kernel("t0g_loss_combine", 1u << a.row_shift))) return rc;
     if (!p.grad) return ok();
 
     T0gLossSumArgs s;
@@ -337,12 +455,18 @@ int run_loss(t0g_device *dev, const Problem &p) {
     s.rows = d.rows;
     s.cols = d.hidden;
     uint32_t planes = 0;
-    const size_t n = pl.pieces.size();
     for (size_t i = n; i-- > 0;) {
         const Piece &pc = pl.pieces[i];
-        if (i + 1 < n && (rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base))) return rc;
-        if ((rc = piece_kernel("t0g_loss_grad", pc))) return rc;
-        if (d.dw && (rc = run_gemm(dev, dw_gemm(p, pl, pc, base), pl, base))) return rc;
+        at_piece(pc);
+        if (pl.fused && i + 1 == n) {
+            rc = piece_kernel("t0g_loss_grad_kept", (a.ldg + 2047) / 2048);
+        } else if (pl.fused) {
+            if (!(rc = run_tile(dev, Tile::Grad, p, pl, pc, a, base))) rc = row_kernel("t0g_loss_grad_entries", 4);
+        } else {
+            if (i + 1 == n || !(rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base)))
+                rc = piece_kernel("t0g_loss_grad", pc.chunks);
+        }
+        if (rc || (d.dw && (rc = run_dw(dev, p, pl, pc, base)))) return rc;
         if (!d.dx) continue;
         if ((rc = run_gemm(dev, dx_gemm(p, pl, pc, base, planes), pl, base))) return rc;
         if (pl.group == 0) continue;

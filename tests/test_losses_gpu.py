@@ -13,8 +13,9 @@ Tolerances, with u = 2^-24 (f32) and the sums of magnitudes |x||W| and |G||W| ta
 import sys
 
 import pytest
-import torch
+import torch   # on the host only: the device's buffers and streams are the library's runtime's
 
+import hip_rt
 import t0g
 
 pytestmark = pytest.mark.gpu
@@ -35,7 +36,7 @@ def rt():
 
 class Case:
     """One problem: inputs on the host, the call's buffers on the device (each in a filled allocation of its
-    own, so that a write outside shows), and the definition in 64 bits."""
+    own, so that a write outside shows and what lies between rows is not read), and the definition in 64 bits."""
 
     def __init__(self, rows, vocab, hidden, layout="NT", seed=0, pad=0, offset=0, xpad=None, amp=2.0, c=1.0, scale=0.125,
                  dtype="bf16", int32=False, weights=True, want="xw"):
@@ -66,70 +67,92 @@ class Case:
         return self
 
     # ---- the call
-    def device(self, t, ld=None, fill=-7.0):
-        """t in a larger buffer of its own, rows ld apart, `offset` elements from an aligned address."""
+    def place(self, rt, t, ld=None, fill=-7.0):
+        """t in a larger device buffer of its own, rows ld apart, `offset` elements from an aligned address:
+        the buffer's address and host image, and t's place in the image."""
         rows, cols = (1, t.shape[0]) if t.dim() == 1 else t.shape
         ld = ld or cols
-        buf = torch.full((self.offset + rows * ld + 64,), fill, dtype=t.dtype, device="cuda")
-        view = buf[self.offset:self.offset + rows * ld].view(rows, ld)[:, :cols]
+        image = torch.full((self.offset + rows * ld + 64,), fill, dtype=t.dtype)
+        view = image[self.offset:self.offset + rows * ld].view(rows, ld)[:, :cols]
         view.copy_(t.view(rows, cols))
-        return buf, (view[0] if t.dim() == 1 else view)
+        addr = rt.upload(self.raw(image))
+        self.held.append(addr)
+        return addr, image, (view[0] if t.dim() == 1 else view)
 
-    def run(self, rt, max_piece=0, stream=None):
+    @staticmethod
+    def raw(image):
+        return (image.view(torch.int16) if image.dtype == torch.bfloat16 else image).numpy()
+
+    def run(self, rt, max_piece=0, keep=False):
         ints = torch.int32 if self.int32 else torch.int64
         itype = t0g.I32 if self.int32 else t0g.I64
         w = self.w if self.layout == "NT" else self.w.t().contiguous()
         nan = float("nan")
-        bx, x = self.device(self.x, self.hidden + self.xpad, nan)
-        bw, wd = self.device(w, w.shape[1] + self.pad, nan)
-        keep = [bx, bw]
+        self.held = []
 
-        def addr(t):
-            if t is None:
+        def inp(t, ld=None):
+            if t is None or t.numel() == 0:
                 return 0
-            keep.append(t.to("cuda"))
-            return keep[-1].data_ptr()
+            addr, image, _ = self.place(rt, t, ld, nan if t.dtype.is_floating_point else 0)
+            return addr + self.offset * image.element_size()
 
+        x, wd = inp(self.x, self.hidden + self.xpad), inp(w, w.shape[1] + self.pad)
         dt = self.out_type
-        self.bufs = {"loss": self.device(torch.zeros(self.rows)), "lse": self.device(torch.zeros(self.rows))}
+        self.bufs = {"loss": self.place(rt, torch.full((self.rows,), -7.0)), "lse": self.place(rt, torch.full((self.rows,), -7.0))}
         if "x" in self.want:
-            self.bufs["dx"] = self.device(torch.zeros(self.rows, self.hidden, dtype=dt), self.hidden + self.pad)
+            self.bufs["dx"] = self.place(rt, torch.full((self.rows, self.hidden), -7.0, dtype=dt), self.hidden + self.pad)
         if "w" in self.want:
-            self.bufs["dw"] = self.device(torch.zeros(w.shape, dtype=dt), w.shape[1] + self.pad)
-        for b, v in self.bufs.values():
-            v.fill_(-7.0)
+            self.bufs["dw"] = self.place(rt, torch.full(w.shape, -7.0, dtype=dt), w.shape[1] + self.pad)
 
         def out(name):
-            return self.bufs[name][1].data_ptr() if name in self.bufs and self.bufs[name][1].numel() else 0
+            if name not in self.bufs or not self.bufs[name][2].numel():
+                return 0
+            return self.bufs[name][0] + self.offset * self.bufs[name][1].element_size()
 
         kind = t0g.BF16 if dt == torch.bfloat16 else t0g.F32
-        head = dict(transpose=self.layout, lse=out("lse"), dx=out("dx"), dw=out("dw"), dloss=addr(self.dloss),
+        head = dict(transpose=self.layout, lse=out("lse"), dx=out("dx"), dw=out("dw"), dloss=inp(self.dloss),
                     loss_scale=self.scale, logit_scale=self.c, label_type=itype, dx_dtype=kind, dw_dtype=kind,
                     ldx=self.hidden + self.xpad, ldw=w.shape[1] + self.pad, lddx=self.hidden + self.pad,
                     lddw=w.shape[1] + self.pad, max_piece=max_piece)
-        xa = x.data_ptr() if self.rows else 0
-        labels = addr(self.labels.to(ints)) if self.labels is not None else 0
+        labels = inp(self.labels.to(ints)) if self.labels is not None else 0
         if self.teacher is None:
-            d = t0g.linear_ce_desc(xa, wd.data_ptr(), labels, out("loss"), self.rows, self.vocab, self.hidden, **head)
+            d = t0g.linear_ce_desc(x, wd, labels, out("loss"), self.rows, self.vocab, self.hidden, **head)
             call = rt.linear_cross_entropy
         else:
-            tokens, teacher = self.tokens.to(ints), self.teacher
-            if self.ldt > self.top:   # what lies between the rows must not be read as entries
-                tokens = torch.cat([tokens, torch.zeros(self.rows, self.ldt - self.top, dtype=ints)], 1)
-                teacher = torch.cat([teacher, torch.full((self.rows, self.ldt - self.top), nan, dtype=teacher.dtype)], 1)
-            d = t0g.linear_distill_desc(xa, wd.data_ptr(), addr(teacher), addr(tokens), out("loss"), self.rows, self.vocab,
-                                        self.hidden, self.top, temperature=self.tau, labels=labels, label_weight=self.a,
-                                        distill_weight=self.b, ldt=self.ldt, token_type=itype,
-                                        teacher_dtype=t0g.BF16 if teacher.dtype == torch.bfloat16 else t0g.F32, **head)
+            # what lies between the rows must not be read as entries
+            d = t0g.linear_distill_desc(x, wd, inp(self.teacher, self.ldt), inp(self.tokens.to(ints), self.ldt), out("loss"),
+                                        self.rows, self.vocab, self.hidden, self.top, temperature=self.tau, labels=labels,
+                                        label_weight=self.a, distill_weight=self.b, ldt=self.ldt, token_type=itype,
+                                        teacher_dtype=t0g.BF16 if self.teacher.dtype == torch.bfloat16 else t0g.F32, **head)
             call = rt.linear_distill
-        torch.cuda.synchronize()
-        self.desc, self.call, self.keep = d, call, keep
+        self.desc, self.call = d, call
         call(d)
-        rt.wait_idle()
-        return {k: v.cpu() for k, (b, v) in self.bufs.items()}
+        got = self.read(rt)
+        if not keep:
+            self.free(rt)
+        return got
+
+    def read(self, rt):
+        """The outputs, after all queued work; the whole buffers go into the images."""
+        got = {}
+        for k, (addr, image, view) in self.bufs.items():
+            raw = self.raw(image)
+            raw[:] = rt.read(addr, raw.shape, raw.dtype)
+            got[k] = view.clone()
+        return got
+
+    def refill(self, rt):
+        for addr, image, view in self.bufs.values():
+            image.fill_(-7.0)
+            rt.write(addr, self.raw(image))
+
+    def free(self, rt):
+        for addr in self.held:
+            rt.free(addr)
+        self.held = []
 
     def untouched(self):
-        for name, (b, v) in self.bufs.items():
+        for name, (_, b, v) in self.bufs.items():
             mask = torch.ones_like(b, dtype=torch.bool)
             rows, cols = (1, v.shape[0]) if v.dim() == 1 else v.shape
             ld = cols if v.dim() == 1 else v.stride(0)
@@ -198,7 +221,6 @@ class Case:
 
     def check(self, rt, label="", **kw):
         got, want = self.run(rt, **kw), self.define()
-        torch.cuda.synchronize()
         self.untouched()
         for k, (v, tol) in want.items():
             d = (got[k].double() - v).abs()
@@ -375,43 +397,50 @@ def test_gradient_against_differences(rt, teach):
             assert abs(float(along - diff.sum())) <= float(tol)
 
 
-def test_same_bits_again_and_on_another_stream(rt):
-    c = Case(200, 3000, 128, seed=17).teach(30, 2.0, 0.5, 0.5)
-    first = c.run(rt, max_piece=1024)
-    again = c.run(rt, max_piece=1024)
-    side = torch.cuda.Stream()
-    rt.set_stream(side.cuda_stream)
+def same_again(rt, c, **kw):
+    first, again = c.run(rt, **kw), c.run(rt, **kw)
+    side = hip_rt.Stream()
+    rt.set_stream(side.ptr)
     try:
-        other = c.run(rt, max_piece=1024)
+        other = c.run(rt, **kw)
     finally:
         rt.set_stream(0)
+        rt.wait_idle()
+        side.destroy()
     for k in first:
         assert torch.equal(first[k], again[k]) and torch.equal(first[k], other[k]), k
 
 
-def test_graph_replays(rt):
+def replays(rt, c, other, **kw):
     """Captured after one eager call; replays match it bit for bit, with eager work in between."""
-    c = Case(96, 2000, 64, seed=18).teach(20, 2.0, 0.5, 0.5)
-    want = c.run(rt, max_piece=800)
-    side = torch.cuda.Stream()
-    rt.set_stream(side.cuda_stream)
+    want = c.run(rt, keep=True, **kw)
+    side = hip_rt.Stream()
+    rt.set_stream(side.ptr)
+    graph = None
     try:
-        graph = torch.cuda.CUDAGraph()
-        torch.cuda.synchronize()
-        with torch.cuda.graph(graph, stream=side):
-            c.call(c.desc)
-        other = Case(30, 500, 64, seed=19)
+        graph = hip_rt.Graph(side, lambda: c.call(c.desc))
         for _ in range(3):
-            for _, v in c.bufs.values():
-                v.fill_(-7.0)
-            torch.cuda.synchronize()
-            graph.replay()
-            torch.cuda.synchronize()
-            for k, (_, v) in c.bufs.items():
-                assert torch.equal(v.cpu(), want[k]), k
+            c.refill(rt)
+            graph.launch(side)
+            got = c.read(rt)
+            for k in want:
+                assert torch.equal(got[k], want[k]), k
             other.check(rt, "between replays")
     finally:
         rt.set_stream(0)
+        rt.wait_idle()
+        if graph:
+            graph.destroy()
+        side.destroy()
+        c.free(rt)
+
+
+def test_same_bits_again_and_on_another_stream(rt):
+    same_again(rt, Case(200, 3000, 128, seed=17).teach(30, 2.0, 0.5, 0.5), max_piece=1024)
+
+
+def test_graph_replays(rt):
+    replays(rt, Case(96, 2000, 64, seed=18).teach(20, 2.0, 0.5, 0.5), Case(30, 500, 64, seed=19), max_piece=800)
 
 
 def test_capture_without_scratch_is_refused():
@@ -419,16 +448,94 @@ def test_capture_without_scratch_is_refused():
         c = Case(40, 400, 64, seed=20)
         with t0g.GpuRuntime.new(0) as warm:
             want = c.run(warm)
-        side = torch.cuda.Stream()
-        fresh.set_stream(side.cuda_stream)
-        graph = torch.cuda.CUDAGraph()
-        torch.cuda.synchronize()
-        with torch.cuda.graph(graph, stream=side):
+        c.run(warm_up := t0g.GpuRuntime.new(0), keep=True)   # buffers and descriptor; `fresh` has no scratch yet
+        side = hip_rt.Stream()
+        fresh.set_stream(side.ptr)
+        code = []
+
+        def call():
             with pytest.raises(t0g.T0gError) as e:
                 fresh.linear_cross_entropy(c.desc)
-        assert e.value.code == t0g.ERR_INVALID_ARG and "capture" in str(e.value)
+            code.append((e.value.code, str(e.value)))
+
+        graph = hip_rt.Graph(side, call)
+        assert code[0][0] == t0g.ERR_INVALID_ARG and "capture" in code[0][1]
+        c.refill(warm_up)
         fresh.linear_cross_entropy(c.desc)   # the handle is as usable as before
         fresh.wait_idle()
-        for k, (_, v) in c.bufs.items():
-            assert torch.equal(v.cpu(), want[k]), k
+        got = c.read(warm_up)
+        for k in want:
+            assert torch.equal(got[k], want[k]), k
+        graph.destroy()
         fresh.set_stream(0)
+        side.destroy()
+        c.free(warm_up)
+        warm_up.close()
+
+
+# ---- the fused form: 256 rows and more, aligned operands ------------------------------
+
+FUSED = [(256, 256, 64), (257, 1000, 72), (300, 2049, 136), (256, 131, 64), (513, 1283, 320), (260, 8, 8), (1000, 640, 40)]
+
+
+@pytest.mark.parametrize("layout", ["NT", "NN"])
+@pytest.mark.parametrize("rows,vocab,hidden", FUSED)
+def test_fused_cross_entropy(rt, rows, vocab, hidden, layout):
+    Case(rows, vocab, hidden, layout, seed=rows + vocab).check(rt, "fused ce")
+
+
+@pytest.mark.parametrize("layout,vocab", [("NT", 2307), ("NT", 2304), ("NN", 2304)])
+@pytest.mark.parametrize("max_piece", [0, 256, 1000])
+def test_fused_pieces(rt, max_piece, layout, vocab):
+    """Pieces computed twice and the last, kept one; labels at tiles' and pieces' edges, rows without one."""
+    c = Case(300, vocab, 200, layout, seed=21, pad=8)
+    edges = [e for v0 in range(0, vocab, 128) for e in (v0, min(v0 + 128, vocab) - 1)]
+    for t in range(300):
+        c.labels[t] = edges[(5 * t) % len(edges)] if t % 4 else -100
+    c.x[4], c.x[8] = float("nan"), float("inf")
+    c.check(rt, f"fused pieces of {max_piece}", max_piece=max_piece)
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,top,tau,a,b,max_piece", [
+    (256, 300, 64, 3, 1.0, 0.0, 1.0, 0), (300, 2051, 128, 100, 2.0, 0.5, 0.5, 0), (300, 2051, 128, 100, 2.0, 0.5, 0.5, 512),
+    (270, 1100, 64, 1024, 0.5, 0.25, 1.0, 256), (512, 900, 72, 40, 4.0, 1.0, 1.0, 0), (300, 1536, 64, 64, 1.0, 0.5, 0.5, 768)])
+def test_fused_distill(rt, rows, vocab, hidden, top, tau, a, b, max_piece):
+    """Many entries of a row in one tile among them, equal tokens, missing ones, rows without any."""
+    c = Case(rows, vocab, hidden, seed=rows + top).teach(top, tau, a, b, repeat=top > 500)
+    c.tokens[::5, top // 2:] = -1
+    c.tokens[7] = -1
+    c.tokens[9] = torch.randint(0, 100, (top,), generator=c.g)
+    if a:
+        c.labels[::3] = -100
+        c.labels[1] = c.tokens[1, 0]
+    c.check(rt, f"fused distill {top} at {tau}", max_piece=max_piece)
+
+
+@pytest.mark.parametrize("amp", [0.0, 60.0, 2000.0])
+@pytest.mark.parametrize("max_piece", [0, 512])
+def test_fused_extreme_logits(rt, amp, max_piece):
+    c = Case(256, 1500, 64, seed=22, amp=amp)
+    c.labels[:128] = (c.x[:128].double() @ c.w.double().t()).argmax(1)
+    c.check(rt, f"fused amplitude {amp}", max_piece=max_piece)
+
+
+def test_fused_nan_in_a_row_stays_there(rt):
+    c = Case(300, 1500, 64, seed=23)
+    c.x[5, 3] = float("nan")
+    got = c.run(rt)
+    rows = [t for t in range(300) if t != 5]
+    assert bool(torch.isnan(got["loss"][5])) and bool(torch.isnan(got["dx"][5].float()).all())
+    assert bool(torch.isfinite(got["loss"][rows]).all()) and bool(torch.isfinite(got["dx"][rows].float()).all())
+
+
+@pytest.mark.parametrize("want,dtype", [("", "f32"), ("x", "f32"), ("w", "f32"), ("xw", "bf16")])
+def test_fused_outputs_asked_for(rt, want, dtype):
+    Case(320, 2100, 128, want=want, dtype=dtype, weights=False, scale=1.0, int32=True, c=0.5).check(rt, "fused outputs")
+
+
+def test_fused_same_bits_again_and_on_another_stream(rt):
+    same_again(rt, Case(400, 3000, 128, seed=24).teach(30, 2.0, 0.5, 0.5), max_piece=1024)
+
+
+def test_fused_graph_replays(rt):
+    replays(rt, Case(300, 2000, 64, seed=25).teach(20, 2.0, 0.5, 0.5), Case(260, 500, 64, seed=26), max_piece=768)
