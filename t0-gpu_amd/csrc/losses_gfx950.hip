@@ -374,8 +374,9 @@ __device__ __forceinline__ void chunk_grad(const T0gLossArgs& p, uint32_t row, u
     if (used) entry_grads(p, row, c0, n, par, tid, kThreads);
 }
 
-// The same from the kept exponentials, in place: e 2^(m - l0) is the probability, and
-// with a second temperature e^r 2^(m r - l1).
+// The same from the kept exponentials, in place: kept e = 2^(u - m) less a factor that
+// was put in for its rounding, so e 2^(m - l0) is the probability, and with a second
+// temperature e^r 2^(m r - l1).
 __device__ __forceinline__ void kept_grad(const T0gLossArgs& p, uint32_t row, uint32_t chunk) {
     constexpr uint32_t kCols = 8 * kThreads;
     const uint32_t c0 = chunk * kCols, tid = threadIdx.x, c = c0 + 8 * tid;
@@ -384,7 +385,8 @@ __device__ __forceinline__ void kept_grad(const T0gLossArgs& p, uint32_t row, ui
     if (c < p.ldg) {
         u32x4_t w = {0u, 0u, 0u, 0u};
         if (used && c < p.cols) {
-            const float m = (*at<const f32x2_t>(p.part, (uint64_t)(p.chunk0 + c / T0G_LOSS_BLOCK) * p.rows + row))[0];
+            const float m =
+                (*at<const f32x2_t>(p.part, (uint64_t)(p.chunk0 + c / T0G_LOSS_BLOCK) * p.rows + row))[0] + kKeepLog2;
             const float f0 = par[2] * exp2_(m - par[0]);
             const u32x4_t e = *at<const u32x4_t>(p.g, ((uint64_t)row * p.ldg + c) / 8);
             float v[8];

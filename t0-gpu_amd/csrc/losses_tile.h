@@ -13,11 +13,13 @@ template <int CTRL>
 __device__ __forceinline__ float dpp_row(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
+// (maximum, which passes NaN on, is one instruction; fmax quiets its operands first.)
+__device__ __forceinline__ float max_(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ float row16_max(float v) {
-    v = __builtin_fmaxf(v, dpp_row<0x128>(v));
-    v = __builtin_fmaxf(v, dpp_row<0x124>(v));
-    v = __builtin_fmaxf(v, dpp_row<0x122>(v));
-    return __builtin_fmaxf(v, dpp_row<0x121>(v));
+    v = max_(v, dpp_row<0x128>(v));
+    v = max_(v, dpp_row<0x124>(v));
+    v = max_(v, dpp_row<0x122>(v));
+    return max_(v, dpp_row<0x121>(v));
 }
 __device__ __forceinline__ float row16_sum(float v) {
     v += dpp_row<0x128>(v);
@@ -27,11 +29,14 @@ __device__ __forceinline__ float row16_sum(float v) {
 }
 
 // e = 2^(u - m) is in [0, 2): no sign and a top exponent bit of 0, so 16 bits hold 7 of
-// exponent and 9 of mantissa (rounded to nearest; relative error 2^-10, a quarter of
-// bf16's).  A NaN does not survive, but its row's sum is NaN and scales every e.
+// exponent and 9 of mantissa, two more than bf16's.  They are cut off, not rounded: e is
+// formed larger by the factor 1 + 2^-10 / (2 ln 2), what cutting takes off in the mean, which
+// leaves a relative error of 0.7 2^-9 at most and none on average.  The factor costs
+// nothing: its logarithm is subtracted from m.  A NaN does not survive, but its row's
+// sum is NaN and scales every e.
+constexpr float kKeepLog2 = 0.00101594f;
 __device__ __forceinline__ uint32_t pack_e(float lo, float hi) {
-    const uint32_t a = (__builtin_bit_cast(uint32_t, lo) + 0x2000u) >> 14, b = (__builtin_bit_cast(uint32_t, hi) + 0x2000u) << 2;
-    return (a & 0xFFFFu) | (b & 0xFFFF0000u);
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi) << 2, __builtin_bit_cast(uint32_t, lo) << 2, 0x07060302u);
 }
 
 // One 16-row band of a wave's sub-tiles, packed in 16 bits (w[j]: the lane's 4 rows of
@@ -70,70 +75,86 @@ __device__ __forceinline__ void store_band16(const uint64_t (&w)[SN], uint64_t c
         }
 }
 
-// Element `reg` (0..3, uniform) of sub-tile `sub` = 8 i + j (uniform) of the accumulators, whose
-// AGPRs can only be named: a binary tree of uniform branches.
-template <int LO, int HI, int SM, int SN>
-__device__ __forceinline__ float acc_pick(const f32x4_t (&acc)[SM][SN], uint32_t sub, uint32_t reg) {
-    if constexpr (HI - LO == 1) {
-        constexpr int I = LO / SN, J = LO % SN;
-        const float a = acc_read(acc[I][J][0]), b = acc_read(acc[I][J][1]), c = acc_read(acc[I][J][2]),
-                    d = acc_read(acc[I][J][3]);
-        return reg < 2 ? (reg == 0 ? a : b) : (reg == 2 ? c : d);
-    } else {
-        constexpr int MID = (LO + HI) / 2;
-        return sub < MID ? acc_pick<LO, MID>(acc, sub, reg) : acc_pick<MID, HI>(acc, sub, reg);
+// The raw logits of the entries (sorted tokens of each row) in a wave's 128 x 128 tile.
+// Lane l looks after rows l and 64 + l.  Which entries a row has there, and its first two
+// tokens, are loaded two bands of statistics ahead of their use, which covers the
+// latency.  A 16-row band with any entry goes to LDS, [4-row quad][column][row in quad],
+// from where the 16 lanes of its rows take what they need.  Taking each entry from the
+// accumulators instead, through a tree of uniform branches, cost 13 us a tile with 64
+// entries a row over 32000 tokens, as much as a quarter of the K loop at K = 2048.
+struct EntryScan {
+    uint32_t range[2];      // entries before the block and before the next (u16 each)
+    uint32_t tok[2][2];
+};
+
+__device__ __forceinline__ void scan_ranges(const T0gLossGemmArgs& a, EntryScan& e, uint32_t row0, uint32_t col0,
+                                            uint32_t lane) {
+    typedef uint32_t u32_2 __attribute__((aligned(2)));
+    const uint32_t block = min((a.v0 + col0) / T0G_LOSS_BLOCK, a.off_ld - 2);   // a wave past the vocabulary takes none
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t row = row0 + 64u * h + lane;
+        e.range[h] = 1u << 16;
+        if (a.ent_off)
+            e.range[h] = *reinterpret_cast<gptr<const u32_2>>(
+                (uintptr_t)(a.ent_off + ((uint64_t)min(row, a.g.m - 1) * a.off_ld + block) * 2));
     }
 }
 
-// The raw logits of the entries (sorted tokens of each row) in a wave's 128 x 128 tile.  A
-// lane looks at two rows; each hit is taken by the whole wave, from the lane that holds it.
-template <int SM, int SN>
-__device__ __forceinline__ void pick_entries(const T0gLossGemmArgs& a, const f32x4_t (&acc)[SM][SN], uint32_t row0,
-                                             uint32_t col0, uint32_t lane) {
+__device__ __forceinline__ void scan_tokens(const T0gLossGemmArgs& a, EntryScan& e, uint32_t row0, uint32_t lane) {
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t row = row0 + 64u * h + lane;
+        if (row >= a.g.m) e.range[h] = 0;
+        const uint64_t slot = (uint64_t)min(row, a.g.m - 1) * a.slots;
+        const uint32_t lo = e.range[h] & 0xFFFFu;
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) e.tok[h][i] = *at<const uint32_t>(a.ent_tok, slot + min(lo + i, a.slots - 1));
+    }
+}
+
+template <int I, int SM, int SN>
+__device__ __forceinline__ void pick_band(const T0gLossGemmArgs& a, const f32x4_t (&acc)[SM][SN], const EntryScan& e,
+                                          uint32_t row0, uint32_t col0, uint32_t lane, uint32_t lds) {
+    typedef __attribute__((address_space(3))) f32x4_t lds_f32x4;
+    typedef const __attribute__((address_space(3))) float lds_f32;
+    constexpr uint32_t H = I / 4;
     const uint32_t width = col0 < a.g.n ? min(a.g.n - col0, T0G_LOSS_BLOCK) : 0u, first = a.v0 + col0;
-#pragma unroll 1
-    for (uint32_t half = 0; half < 2; ++half) {
-        const uint32_t row = row0 + 64u * half + lane;
-        uint32_t lo = 0, hi = 0;
-        if (row < a.g.m) {
-            hi = 1;
-            if (a.ent_off) {
-                const uint64_t o = (uint64_t)row * a.off_ld + first / T0G_LOSS_BLOCK;
-                lo = *at<const uint16_t>(a.ent_off, o);
-                hi = *at<const uint16_t>(a.ent_off, o + 1);
-            }
-        }
-        for (;;) {
-            uint32_t c = kNoToken;
-            if (lo < hi) c = *at<const uint32_t>(a.ent_tok, (uint64_t)row * a.slots + lo) - first;
-            uint64_t hits = __ballot(c < width);
-            while (hits) {
-                const uint32_t b = (uint32_t)__builtin_ctzll(hits);
-                hits &= hits - 1;
-                const uint32_t col = (uint32_t)__builtin_amdgcn_readlane((int)c, (int)b);
-                const uint32_t slot = (uint32_t)__builtin_amdgcn_readlane((int)lo, (int)b);
-                const uint32_t rr = 64u * half + b;
-                const float z = acc_pick<0, SM * SN>(acc, (rr >> 4) * SN + (col >> 4), rr & 3u);
-                if (lane == (((rr >> 2) & 3u) << 4 | (col & 15u)))
-                    *at<float>(a.ent_z, (uint64_t)(row0 + rr) * a.slots + slot) = z;
-            }
-            ++lo;
-            if (__ballot(lo < hi) == 0) break;
+    const uint32_t lo = e.range[H] & 0xFFFFu, hi = e.range[H] >> 16;
+    const bool mine = (lane >> 4) == I % 4 && lo < hi;
+    // a row without an offset table has one slot, which may hold any token or none
+    if (__ballot(mine && (a.ent_off || e.tok[H][0] - first < width)) == 0) return;
+    const uint32_t l16 = lane & 15u, q = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < SN; ++j)
+        *reinterpret_cast<lds_f32x4*>((uintptr_t)(lds + q * (SN * 256) + (16u * j + l16) * 16u)) =
+            f32x4_t{acc_read(acc[I][j][0]), acc_read(acc[I][j][1]), acc_read(acc[I][j][2]), acc_read(acc[I][j][3])};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (mine) {
+        const uint64_t slot = (uint64_t)(row0 + 64u * H + lane) * a.slots;
+        const uint32_t base = lds + (l16 >> 2) * (SN * 256) + (l16 & 3u) * 4u;   // row 16 I + l16 of the tile
+        for (uint32_t s = lo; s < hi; ++s) {
+            const uint32_t t = s == lo ? e.tok[H][0] : s == lo + 1 ? e.tok[H][1] : *at<const uint32_t>(a.ent_tok, slot + s);
+            const uint32_t c = t - first;
+            if (c < width) *at<float>(a.ent_z, slot + s) = *reinterpret_cast<lds_f32*>((uintptr_t)(base + c * 16u));
         }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the next band overwrites it
 }
 
 // Statistics of a wave's tile, per row over its 128 columns; KEEP: the exponentials go out
 // in 16 bits.  Bound by v_exp_f32 (256 per lane, a quarter of the VALU's rate).
 template <bool KEEP, int SM, int SN>
 __device__ __forceinline__ void tile_stats(const T0gLossGemmArgs& a, const f32x4_t (&acc)[SM][SN], uint32_t row0,
-                                           uint32_t col0, uint32_t lane, uint32_t lds) {
+                                           uint32_t col0, uint32_t lane, uint32_t lds, uint32_t pick_lds) {
     asm volatile("v_mov_b32 %0, %0" : "+v"(lane));   // nothing below is hoisted above the K loop
+    EntryScan scan;
+    scan_ranges(a, scan, row0, col0, lane);
     const uint32_t l16 = lane & 15u, q = lane >> 4;
     const uint32_t width = col0 < a.g.n ? min(a.g.n - col0, T0G_LOSS_BLOCK) : 0u;
     const uint64_t out = (uint64_t)(col0 / T0G_LOSS_BLOCK) * a.g.m;
-#pragma unroll
-    for (int i = 0; i < SM; ++i) {
+    auto pick = [&](auto band) { pick_band<band.value>(a, acc, scan, row0, col0, lane, pick_lds); };
+    auto stats = [&](int i) {
         __builtin_amdgcn_sched_barrier(0);   // one band at a time
         float z[SN][4], m[4], s[4], s2[4];
 #pragma unroll
@@ -149,8 +170,8 @@ __device__ __forceinline__ void tile_stats(const T0gLossGemmArgs& a, const f32x4
         for (int r = 0; r < 4; ++r) {
             m[r] = z[0][r];
 #pragma unroll
-            for (int j = 1; j < SN; ++j) m[r] = __builtin_fmaxf(m[r], z[j][r]);
-            m[r] = row16_max(m[r]) * a.k;
+            for (int j = 1; j < SN; ++j) m[r] = max_(m[r], z[j][r]);
+            m[r] = KEEP ? __builtin_fmaf(row16_max(m[r]), a.k, -kKeepLog2) : row16_max(m[r]) * a.k;
             m[r] = width ? m[r] : 0.0f;   // no columns: every exponential below is 2^-inf
             s[r] = s2[r] = 0.0f;
         }
@@ -188,7 +209,25 @@ __device__ __forceinline__ void tile_stats(const T0gLossGemmArgs& a, const f32x4
             if (a.flags & T0G_LOSS_DUAL)
                 *at<float>(a.part2, out + row) = l16 < 2 ? (l16 == 0 ? s2[0] : s2[1]) : (l16 == 2 ? s2[2] : s2[3]);
         }
-    }
+    };
+    static_assert(SM == 8, "eight bands");
+    stats(0);
+    scan_tokens(a, scan, row0, lane);
+    stats(1);
+    stats(2);
+    pick(std::integral_constant<int, 0>{});
+    stats(3);
+    pick(std::integral_constant<int, 1>{});
+    stats(4);
+    pick(std::integral_constant<int, 2>{});
+    stats(5);
+    pick(std::integral_constant<int, 3>{});
+    stats(6);
+    pick(std::integral_constant<int, 4>{});
+    stats(7);
+    pick(std::integral_constant<int, 5>{});
+    pick(std::integral_constant<int, 6>{});
+    pick(std::integral_constant<int, 7>{});
 }
 
 // The dense part of the logits' gradients, zero past the piece's columns and rows.
@@ -256,7 +295,7 @@ __device__ __forceinline__ void loss_tile(const T0gLossGemmArgs& a) {
     const int nst = (int)((p.k + 63) / 64);
     const uint32_t a_bytes = ((p.m - 1) * p.lda + p.k) * 2;
     const uint32_t b_bytes = (B_K ? (p.n - 1) * p.ldb + p.k : (p.k - 1) * p.ldb + p.n) * 2;
-    const uint32_t lane = tid & 63u, wave = tid >> 6, wm = wave / 2, wn = wave % 2;
+    const uint32_t lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / 2, wn = wave % 2;
     OpA la;
     OpB lb;
     la.init(tid, m0, p.lda, wm * WT);
@@ -272,27 +311,26 @@ __device__ __forceinline__ void loss_tile(const T0gLossGemmArgs& a) {
         k_pipeline16<true, A_BYTES, STAGE, kVmemPerStage>(acc, la, lb, p, a_bytes, b_bytes, 0, p.k, nst, lds0);
     } else if (p.flags & T0G_FLAG_PREFETCH) {
         const uint32_t rows = p.tiles_m >= 8 ? 8u : p.tiles_m >= 4 ? 4u : 2u, cols = rows == 8 ? 4u : 8u;
-        const uint32_t w = __builtin_amdgcn_readfirstlane(wave);
         Prefetch16 pf;
-        pf.off = w < 2 ? prefetch_line<true>(m0, p.lda, cols, (n0 / BN) % cols, w & 1u, lane)
-                       : prefetch_line<B_K>(n0, p.ldb, rows, (m0 / BM) % rows, w & 1u, lane);
-        pf.base = w < 2 ? p.a : p.b;
-        pf.bytes = w < 2 ? a_bytes : b_bytes;
-        pf.kstep = 2u * (w < 2 || B_K ? 1u : p.ldb);
+        pf.off = wave < 2 ? prefetch_line<true>(m0, p.lda, cols, (n0 / BN) % cols, wave & 1u, lane)
+                          : prefetch_line<B_K>(n0, p.ldb, rows, (m0 / BM) % rows, wave & 1u, lane);
+        pf.base = wave < 2 ? p.a : p.b;
+        pf.bytes = wave < 2 ? a_bytes : b_bytes;
+        pf.kstep = 2u * (wave < 2 || B_K ? 1u : p.ldb);
         k_pipeline16<false, A_BYTES, STAGE, kVmemPerStage, true>(acc, la, lb, p, a_bytes, b_bytes, 0, p.k, nst, lds0, pf);
     } else {
         k_pipeline16<false, A_BYTES, STAGE, kVmemPerStage>(acc, la, lb, p, a_bytes, b_bytes, 0, p.k, nst, lds0);
     }
-    static_assert(2 * SN * 512 * (NT / 64) <= 2 * STAGE, "the staged bands fit");
+    constexpr uint32_t kBands = 2 * SN * 512, kPick = SN * 1024;   // LDS of a wave: two bands in 16 bits, one in f32
+    static_assert((kBands + kPick) * (NT / 64) <= 2 * STAGE, "the staged bands fit");
     mfma16_drain();
     T0G_WAIT_VMCNT(0);
     barrier_no_fence();
-    const uint32_t row0 = m0 + wm * WT, col0 = n0 + wn * WT, lds = lds_addr(smem) + wave * (2 * SN * 512);
+    const uint32_t row0 = m0 + wm * WT, col0 = n0 + wn * WT, lds = lds_addr(smem) + wave * kBands;
     if constexpr (KIND == LossTile::Grad) {
         tile_grad(a, acc, row0, col0, lane, lds);
     } else {
-        tile_stats<KIND == LossTile::Keep>(a, acc, row0, col0, lane, lds);
-        pick_entries(a, acc, row0, col0, lane);
+        tile_stats<KIND == LossTile::Keep>(a, acc, row0, col0, lane, lds, lds_addr(smem) + 4 * kBands + wave * kPick);
     }
 }
 
