@@ -487,6 +487,12 @@ __device__ __forceinline__ uint64_t operand_bytes_wide(uint32_t rows, uint32_t k
     return K_MAJOR ? ((uint64_t)(rows - 1) * ld + k) * 2 : ((uint64_t)(k - 1) * ld + rows) * 2;
 }
 
+// The same in 32 bits, its rows' last 16-byte piece whole.
+template <bool K_MAJOR>
+__device__ __forceinline__ uint32_t operand_bytes(uint32_t rows, uint32_t k, uint32_t ld) {
+    return K_MAJOR ? ((rows - 1) * ld + ((k + 7) & ~7u)) * 2 : ((k - 1) * ld + ((rows + 7) & ~7u)) * 2;
+}
+
 // 16-byte buffer load straight into LDS: lane l's data goes to LDS address
 // m0 + 16 * l.  An SALU write of M0 needs one wait state before an LDS-DMA
 // instruction reads it, hence the s_nop.  Completion is tracked by vmcnt only
@@ -1233,9 +1239,9 @@ __device__ __forceinline__ void gemm_tile_fast(const T0gGemmArgs& p, const T0gGe
     const uint32_t kend = min(p.k, kbeg + p.k_per_split);
     const int nst = kend > kbeg ? (int)((kend - kbeg + BK - 1) / BK) : 0;
 
-    // a K-contiguous A may end inside a 16-byte piece that its rows are zero padded to
-    const uint32_t a_bytes = (A_K ? (p.m - 1) * p.lda + ((p.k + 7) & ~7u) : (p.k - 1) * p.lda + p.m) * 2;
-    const uint32_t b_bytes = (B_K ? (p.n - 1) * p.ldb + p.k : (p.k - 1) * p.ldb + p.n) * 2;
+    // operands are whole 16-byte pieces (their rows padded to them)
+    const uint32_t a_bytes = operand_bytes<A_K>(p.m, p.k, p.lda);
+    const uint32_t b_bytes = operand_bytes<B_K>(p.n, p.k, p.ldb);
 
     const uint32_t lane = tid & 63u, wave = tid >> 6;
     const uint32_t wm = wave / WAVES_N, wn = wave % WAVES_N;

@@ -770,9 +770,9 @@ __device__ __forceinline__ void gemm_tile_fast16(const T0gGemmArgs& p, const T0g
         a_bytes = operand_bytes_wide<A_K>(p.m, p.k, p.lda);
         b_bytes = operand_bytes_wide<B_K>(p.n, p.k, p.ldb);
     } else {
-        // a K-contiguous A may end inside a 16-byte piece that its rows are zero padded to
-        a_bytes = (A_K ? (p.m - 1) * p.lda + ((p.k + 7) & ~7u) : (p.k - 1) * p.lda + p.m) * 2;
-        b_bytes = (B_K ? (p.n - 1) * p.ldb + p.k : (p.k - 1) * p.ldb + p.n) * 2;
+        // operands are whole 16-byte pieces (their rows padded to them)
+        a_bytes = operand_bytes<A_K>(p.m, p.k, p.lda);
+        b_bytes = operand_bytes<B_K>(p.n, p.k, p.ldb);
     }
 
     const uint32_t lane = tid & 63u, wave = tid >> 6;
@@ -1036,8 +1036,8 @@ __device__ __forceinline__ void gemm_tile_sk(const T0gGemmSkArgs& kargs) {
             tile_of_index<BM, BN>(p, st.t, m0, n0);
             const uint32_t kbeg = kb * 64u, kend = min(p.k, ke * 64u);
             const int nst = (int)(ke - kb);
-            const uint32_t a_bytes = (A_K ? (p.m - 1) * p.lda + ((p.k + 7) & ~7u) : (p.k - 1) * p.lda + p.m) * 2;
-            const uint32_t b_bytes = (B_K ? (p.n - 1) * p.ldb + p.k : (p.k - 1) * p.ldb + p.n) * 2;
+            const uint32_t a_bytes = operand_bytes<A_K>(p.m, p.k, p.lda);
+            const uint32_t b_bytes = operand_bytes<B_K>(p.n, p.k, p.ldb);
             const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem));
             OpA la;
             OpB lb;

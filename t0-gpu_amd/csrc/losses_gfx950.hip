@@ -412,6 +412,27 @@ __device__ __forceinline__ void kept_grad(const T0gLossArgs& p, uint32_t row, ui
     if (used && c0 < p.cols) entry_grads(p, row, c0, min(kCols, p.cols - c0), par, tid, kThreads);
 }
 
+// 8 elements a thread and step.
+__device__ __forceinline__ void copy_weight(const T0gLossCopyArgs& p) {
+    typedef u32x4_t u32x4_2 __attribute__((aligned(2)));
+    const uint32_t per_row = p.ldd / 8;
+    const uint64_t total = (uint64_t)p.rows * per_row;
+    for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (uint64_t)gridDim.x * kThreads) {
+        const uint64_t row = i / per_row;
+        const uint32_t c = (uint32_t)(i - row * per_row) * 8;
+        const uint64_t src = p.src + (row * p.lds + c) * 2;
+        u32x4_t v = {0u, 0u, 0u, 0u};
+        if (c + 8 <= p.cols) {
+            v = *reinterpret_cast<gptr<const u32x4_2>>((uintptr_t)src);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e)
+                if (c + e < p.cols) v[e / 2] |= (uint32_t)*at<const uint16_t>(src, e) << 16 * (e & 1u);
+        }
+        *at<u32x4_t>(p.dst, i) = v;
+    }
+}
+
 __device__ __forceinline__ void sum_planes(const T0gLossSumArgs& p) {
     const uint64_t total = (uint64_t)p.rows * p.cols;
     const uint32_t w = p.vec ? 4 : 1;
@@ -472,4 +493,5 @@ T0G_LOSS_GEMM(t0g_loss_logits_nt_kept, true, Keep)
 T0G_LOSS_GEMM(t0g_loss_logits_nn_kept, false, Keep)
 T0G_LOSS_GEMM(t0g_loss_again_nt, true, Grad)
 T0G_LOSS_GEMM(t0g_loss_again_nn, false, Grad)
+extern "C" __global__ void __launch_bounds__(256) t0g_loss_copy_weight(T0gLossCopyArgs p) { t0g::copy_weight(p); }
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_sum(T0gLossSumArgs p) { t0g::sum_planes(p); }

@@ -293,8 +293,7 @@ __device__ __forceinline__ void loss_tile(const T0gLossGemmArgs& a) {
     uint32_t m0, n0;
     tile_origin<BM, BN>(p, m0, n0);
     const int nst = (int)((p.k + 63) / 64);
-    const uint32_t a_bytes = ((p.m - 1) * p.lda + p.k) * 2;
-    const uint32_t b_bytes = (B_K ? (p.n - 1) * p.ldb + p.k : (p.k - 1) * p.ldb + p.n) * 2;
+    const uint32_t a_bytes = operand_bytes<true>(p.m, p.k, p.lda), b_bytes = operand_bytes<B_K>(p.n, p.k, p.ldb);
     const uint32_t lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / 2, wn = wave % 2;
     OpA la;
     OpB lb;

@@ -85,10 +85,10 @@ std::mutex &device_mutex(t0g_device *dev);
 int losses_begin(t0g_device *dev, size_t bytes, uint64_t *scratch);
 // Launch kernel `symbol` of the losses' code object on the device stream.
 int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, void *args, size_t args_size);
-// Workspace t0g_gemm may use for d (host only), and the GEMM itself.  An NN product's A has its
-// rows zero padded to a multiple of 8 wherever lda leaves room for that.
-int losses_gemm_workspace(const t0g_gemm_desc *d, size_t *bytes);
-int losses_gemm(t0g_device *dev, const t0g_gemm_desc *d);
+// Workspace t0g_gemm may use for d (host only), and the GEMM itself.  padded: the operands' rows
+// hold whole 16-byte pieces, zeros past the sizes, which then need not be multiples of 8.
+int losses_gemm_workspace(const t0g_gemm_desc *d, bool padded, size_t *bytes);
+int losses_gemm(t0g_device *dev, const t0g_gemm_desc *d, bool padded);
 
 // One kernel's entry in a code object's AMDGPU metadata (t0g_codeobj.cpp).
 struct KernelMeta {

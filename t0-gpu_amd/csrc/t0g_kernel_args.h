@@ -222,6 +222,13 @@ typedef struct T0gLossGemmArgs {
 } T0gLossGemmArgs;
 #define T0G_LOSS_BLOCK 128u    /* columns of one wave of the 256x256 tile              */
 
+/* A piece of an unaligned weight into rows of whole, aligned 16-byte pieces, zeros past cols. */
+typedef struct T0gLossCopyArgs {
+    uint64_t src;            /* bf16 [rows][lds], 2-byte aligned                      */
+    uint64_t dst;            /* bf16 [rows][ldd], ldd a multiple of 8                 */
+    uint32_t rows, cols, lds, ldd;
+} T0gLossCopyArgs;
+
 /* Sum of f32 planes of a data gradient, in order, into bf16 or f32 rows. */
 typedef struct T0gLossSumArgs {
     uint64_t acc;            /* f32 [rows][cols] summed before, or 0                  */

@@ -14,6 +14,8 @@
 //             the other pieces' logits are computed again with G in the epilogue
 //   by rows   a piece's f32 logits go to the scratch and row kernels read them: products
 //             of few rows, and operands that the 256x256 tile does not take
+// A weight whose rows are not whole 16-byte pieces is copied into ones that are, piece by
+// piece, when there are rows enough to make up for that.
 #include <math.h>
 #include <string.h>
 
@@ -36,6 +38,11 @@ constexpr uint64_t kFusedPieceBytes = 880ull << 20;
 constexpr uint64_t kPlaneBytes = 128ull << 20;
 // Rows from which the fused form is taken.
 constexpr uint32_t kFusedRows = 256;
+// Rows from which an unaligned weight is copied, and what a copied piece takes at most.  Without
+// and with the copy, width 1023: loss alone over 50001 tokens 200 rows 97 / 97 us, 300 rows 120 /
+// 130, 777 rows 255 / 188; with gradients over 20001 tokens 300 rows 146 / 158, 777 rows 271 / 243.
+constexpr uint32_t kCopyRows = 512;
+constexpr uint64_t kCopyBytes = 512ull << 20;
 // Rows of a launch's y grid, at most (the kernels step through the rest).
 constexpr uint32_t kMaxGridY = 65535;
 
@@ -137,10 +144,13 @@ struct Piece {
 struct Plan {
     std::vector<Piece> pieces;
     bool fused = false;
+    bool copy_w = false;         // the pieces' weights are copied
+    bool copy_x = false;         // products take xz instead of x
+    bool padded = false;         // every operand's rows are whole 16-byte pieces
     uint32_t chunks = 0, slots = 0, ldxz = 0, off_ld = 0;
     uint32_t group = 0;          // planes of dx summed at a time (0: the one product writes dx)
     uint64_t xz = 0, ent_tok = 0, ent_q = 0, ent_z = 0, row_ent = 0, row_sub = 0, row_par = 0, part = 0, part2 = 0,
-             ent_off = 0;
+             ent_off = 0, w = 0;
     uint64_t z = 0, g = 0, planes = 0, acc = 0, gemm_ws = 0;
     uint64_t gemm_ws_bytes = 0, bytes = 0;
 };
@@ -173,76 +183,82 @@ uint64_t weight_piece(const Problem &p, uint64_t w, uint32_t v0, uint32_t ld, ui
     return w + (p.d.transpose == T0G_NT ? (uint64_t)v0 * ld : v0) * size;
 }
 
+// The operands of the products: a piece of the weight and its leading dimension, and x.
+uint64_t w_of(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
+    return pl.copy_w ? base + pl.w : weight_piece(p, p.d.w, pc.v0, p.d.ldw, 2);
+}
+uint32_t ldw_of(const Problem &p, const Plan &pl, const Piece &pc) {
+    if (!pl.copy_w) return p.d.ldw;
+    return p.d.transpose == T0G_NT ? round_up(p.d.hidden, 8) : round_up(pc.cols, 256);
+}
+uint64_t x_of(const Problem &p, const Plan &pl, uint64_t base) { return pl.copy_x ? base + pl.xz : p.d.x; }
+uint32_t ldx_of(const Problem &p, const Plan &pl) { return pl.copy_x ? pl.ldxz : p.d.ldx; }
+
 t0g_gemm_desc logits_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
     const t0g_linear_ce_desc &d = p.d;
-    return gemm_of(p.grad ? base + pl.xz : d.x, weight_piece(p, d.w, pc.v0, d.ldw, 2), base + pl.z, d.rows, pc.cols,
-                   d.hidden, p.grad ? pl.ldxz : d.ldx, d.ldw, round_up(pc.cols, 4), d.transpose, T0G_F32);
+    return gemm_of(x_of(p, pl, base), w_of(p, pl, pc, base), base + pl.z, d.rows, pc.cols, d.hidden, ldx_of(p, pl),
+                   ldw_of(p, pl, pc), round_up(pc.cols, 4), d.transpose, T0G_F32);
 }
 
 // dx of a piece: the output itself, or f32 plane `plane`.
 t0g_gemm_desc dx_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base, uint32_t plane) {
     const t0g_linear_ce_desc &d = p.d;
     const bool whole = pl.group == 0;
-    return gemm_of(base + pl.g, weight_piece(p, d.w, pc.v0, d.ldw, 2),
+    return gemm_of(base + pl.g, w_of(p, pl, pc, base),
                    whole ? d.dx : base + pl.planes + (uint64_t)plane * d.rows * d.hidden * 4, d.rows, d.hidden, pc.cols,
-                   ld_of_g(pl, pc), d.ldw, whole ? d.lddx : d.hidden, d.transpose == T0G_NT ? T0G_NN : T0G_NT,
-                   whole ? d.dx_dtype : (uint32_t)T0G_F32);
+                   ld_of_g(pl, pc), ldw_of(p, pl, pc), whole ? d.lddx : d.hidden,
+                   d.transpose == T0G_NT ? T0G_NN : T0G_NT, whole ? d.dx_dtype : (uint32_t)T0G_F32);
 }
 
-// dW of columns [c0, c0 + cols) of a piece.
-t0g_gemm_desc dw_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base, uint32_t c0, uint32_t cols) {
+t0g_gemm_desc dw_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
     const t0g_linear_ce_desc &d = p.d;
-    const uint64_t c = weight_piece(p, d.dw, pc.v0 + c0, d.lddw, dtype_size(d.dw_dtype)), g = base + pl.g + c0 * 2ull;
+    const uint64_t c = weight_piece(p, d.dw, pc.v0, d.lddw, dtype_size(d.dw_dtype));
     const uint32_t ldg = ld_of_g(pl, pc);
     return d.transpose == T0G_NT
-               ? gemm_of(g, base + pl.xz, c, cols, d.hidden, d.rows, ldg, pl.ldxz, d.lddw, T0G_TN, d.dw_dtype)
-               : gemm_of(base + pl.xz, g, c, d.hidden, cols, d.rows, pl.ldxz, ldg, d.lddw, T0G_TN, d.dw_dtype);
-}
-// The columns of dW's two products: all, or a multiple of 8 and the rest, which alone
-// would keep the whole off the aligned kernels.
-uint32_t dw_body(const Problem &p, const Piece &pc) {
-    return pc.cols > 8 && p.d.hidden % 8 == 0 ? pc.cols & ~7u : pc.cols;
+               ? gemm_of(base + pl.g, base + pl.xz, c, pc.cols, d.hidden, d.rows, ldg, pl.ldxz, d.lddw, T0G_TN, d.dw_dtype)
+               : gemm_of(base + pl.xz, base + pl.g, c, d.hidden, pc.cols, d.rows, pl.ldxz, ldg, d.lddw, T0G_TN, d.dw_dtype);
 }
 
 int make_loss_plan(const Problem &p, Plan *pl) {
     const t0g_linear_ce_desc &d = p.d;
     const uint64_t rows = d.rows ? d.rows : 1;
-    const bool aligned = (d.w & 15) == 0 && d.ldw % 8 == 0 && d.hidden % 8 == 0, nt = d.transpose == T0G_NT;
-    const uint32_t ldx = p.grad ? round_up(d.hidden, 8) : d.ldx;
-    // the 256x256 tile's operands: whole 16-byte pieces, 32-bit byte offsets, and of a
-    // weight [hidden][vocab] rows of 256 or more
-    pl->fused = d.rows >= kFusedRows && aligned && (p.grad || ((d.x & 15) == 0 && d.ldx % 8 == 0)) &&
-                (uint64_t)d.rows * ldx < (1ull << 30) && (d.max_piece == 0 || d.max_piece >= 256) &&
-                (nt ? (uint64_t)d.ldw * 256 < (1ull << 30)
-                    : d.vocab % 8 == 0 && d.ldw >= 256 && (uint64_t)d.hidden * d.ldw < (1ull << 30));
-    uint64_t width;
-    uint32_t body = d.vocab, chunk = T0G_LOSS_CHUNK;
-    if (pl->fused) {
-        chunk = T0G_LOSS_BLOCK;
-        width = p.grad ? kFusedPieceBytes / 2 / round_up(d.rows, 256) : d.vocab;
-        if (nt) width = std::min<uint64_t>(width, ((1ull << 30) - 1) / d.ldw);
-        if (d.max_piece) width = std::min<uint64_t>(width, d.max_piece);
-        width = std::max<uint64_t>(256, width / 256 * 256);
-    } else {
-        // A vocabulary that is not a multiple of 8 gets its last few tokens as a piece of
-        // their own where they alone would keep the products off the aligned kernels.
-        if (aligned && d.vocab > 8 && (p.grad || !nt)) body = d.vocab & ~7u;
-        width = std::max<uint64_t>(256, kPieceBytes / (rows * 4) / 256 * 256);
-        if (d.max_piece) width = std::min<uint64_t>(width, d.max_piece <= 8 ? 8 : d.max_piece & ~7u);
+    const bool nt = d.transpose == T0G_NT;
+    const bool aligned = (d.w & 15) == 0 && d.ldw % 8 == 0 && (nt ? d.hidden : d.vocab) % 8 == 0;
+    const bool x_aligned = (d.x & 15) == 0 && d.ldx % 8 == 0 && d.hidden % 8 == 0;
+    pl->copy_w = !aligned && d.rows >= kCopyRows;
+    pl->padded = aligned || pl->copy_w;
+    pl->copy_x = p.grad || (pl->padded && !x_aligned);
+    pl->ldxz = round_up(d.hidden, 8);
+    // the 256x256 tile takes 32-bit byte offsets, and rows of 256 or more of a weight
+    // [hidden][vocab] (a copied piece has them)
+    const uint64_t ldx = pl->copy_x ? pl->ldxz : d.ldx, ldw = pl->copy_w ? pl->ldxz : d.ldw;
+    pl->fused = d.rows >= kFusedRows && pl->padded && d.rows * ldx < (1ull << 30) &&
+                (d.max_piece == 0 || d.max_piece >= 256) &&
+                (nt ? ldw * 256 < (1ull << 30) : pl->copy_w || (d.ldw >= 256 && d.hidden * ldw < (1ull << 30)));
+    const uint32_t chunk = pl->fused ? T0G_LOSS_BLOCK : T0G_LOSS_CHUNK;
+    uint64_t width = d.vocab;
+    if (!pl->fused)
+        width = kPieceBytes / (rows * 4);
+    else if (p.grad)
+        width = kFusedPieceBytes / 2 / round_up(d.rows, 256);
+    if (pl->fused && nt) width = std::min<uint64_t>(width, ((1ull << 30) - 1) / ldw);
+    if (pl->copy_w) width = std::min<uint64_t>(width, kCopyBytes / 2 / pl->ldxz);
+    width = width >= d.vocab ? round_up(d.vocab, 256) : std::max<uint64_t>(256, width / 256 * 256);
+    if (d.max_piece) {
+        const uint32_t step = pl->fused ? 256 : 8;
+        width = std::min<uint64_t>(width, std::max(step, d.max_piece / step * step));
     }
     // fused: the last piece's exponentials are kept, so the first is the short one
     const uint64_t whole = ((uint64_t)d.vocab + 255) / 256 * 256;
     const uint64_t head = pl->fused && whole > width ? whole - (whole - 1) / width * width : width;
     for (uint32_t v0 = 0; v0 < d.vocab;) {
-        const uint32_t end = v0 < body ? body : d.vocab;
-        const uint32_t cols = (uint32_t)std::min<uint64_t>(v0 == 0 ? head : width, end - v0);
+        const uint32_t cols = (uint32_t)std::min<uint64_t>(v0 == 0 ? head : width, d.vocab - v0);
         const uint32_t chunks = (cols + chunk - 1) / chunk;
         pl->pieces.push_back(Piece{v0, cols, pl->chunks, chunks});
         pl->chunks += chunks;
         v0 += cols;
     }
     pl->slots = 1 + (p.t ? p.t->top_k : 0);
-    pl->ldxz = round_up(d.hidden, 8);
     const uint64_t plane = rows * d.hidden * 4;
     if (d.dx && pl->pieces.size() > 1)
         pl->group = (uint32_t)std::min<uint64_t>(pl->pieces.size(), std::max<uint64_t>(1, kPlaneBytes / plane));
@@ -255,7 +271,11 @@ int make_loss_plan(const Problem &p, Plan *pl) {
     };
     uint32_t widest = 0;
     for (const Piece &pc : pl->pieces) widest = std::max(widest, pc.cols);
-    if (p.grad) pl->xz = take(rows * pl->ldxz * 2);
+    if (pl->copy_x) pl->xz = take(rows * pl->ldxz * 2);
+    if (pl->copy_w) {
+        const Piece wide = {0, widest, 0, 0};
+        pl->w = take((uint64_t)ldw_of(p, *pl, wide) * (nt ? widest : d.hidden) * 2);
+    }
     pl->ent_tok = take(rows * pl->slots * 4);
     pl->ent_q = take(rows * pl->slots * 4);
     pl->ent_z = take(rows * pl->slots * 4);
@@ -280,18 +300,14 @@ int make_loss_plan(const Problem &p, Plan *pl) {
     }
     // one split-K workspace for all products, which run one after another
     for (const Piece &pc : pl->pieces) {
-        t0g_gemm_desc g[4];
+        t0g_gemm_desc g[3];
         int n = 0, rc;
         if (!pl->fused) g[n++] = logits_gemm(p, *pl, pc, 0);
         if (d.dx) g[n++] = dx_gemm(p, *pl, pc, 0, 0);
-        if (d.dw) {
-            const uint32_t body = dw_body(p, pc);
-            g[n++] = dw_gemm(p, *pl, pc, 0, 0, body);
-            if (body < pc.cols) g[n++] = dw_gemm(p, *pl, pc, 0, body, pc.cols - body);
-        }
+        if (d.dw) g[n++] = dw_gemm(p, *pl, pc, 0);
         for (int i = 0; i < n; ++i) {
             size_t bytes = 0;
-            if ((rc = losses_gemm_workspace(&g[i], &bytes))) return rc;
+            if ((rc = losses_gemm_workspace(&g[i], pl->padded, &bytes))) return rc;
             pl->gemm_ws_bytes = std::max<uint64_t>(pl->gemm_ws_bytes, bytes);
         }
     }
@@ -303,14 +319,22 @@ int make_loss_plan(const Problem &p, Plan *pl) {
 int run_gemm(t0g_device *dev, t0g_gemm_desc g, const Plan &pl, uint64_t base) {
     g.workspace = base + pl.gemm_ws;
     g.workspace_bytes = pl.gemm_ws_bytes;
-    return losses_gemm(dev, &g);
+    return losses_gemm(dev, &g, pl.padded);
 }
 
-int run_dw(t0g_device *dev, const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
-    const uint32_t body = dw_body(p, pc);
-    int rc = run_gemm(dev, dw_gemm(p, pl, pc, base, 0, body), pl, base);
-    if (rc || body == pc.cols) return rc;
-    return run_gemm(dev, dw_gemm(p, pl, pc, base, body, pc.cols - body), pl, base);
+// The copy of a piece of an unaligned weight.
+int run_copy(t0g_device *dev, const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
+    const t0g_linear_ce_desc &d = p.d;
+    T0gLossCopyArgs c;
+    memset(&c, 0, sizeof c);
+    c.src = weight_piece(p, d.w, pc.v0, d.ldw, 2);
+    c.dst = base + pl.w;
+    c.rows = d.transpose == T0G_NT ? pc.cols : d.hidden;
+    c.cols = d.transpose == T0G_NT ? d.hidden : pc.cols;
+    c.lds = d.ldw;
+    c.ldd = ldw_of(p, pl, pc);
+    const uint64_t groups = ((uint64_t)c.rows * (c.ldd / 8) + 255) / 256;
+    return losses_launch(dev, "t0g_loss_copy_weight", (uint32_t)std::min<uint64_t>(groups, 1u << 20), 1, &c, sizeof c);
 }
 
 // One of the 256x256 kernels on a piece: statistics, statistics with the exponentials kept, or G.
@@ -320,14 +344,14 @@ int run_tile(t0g_device *dev, Tile kind, const Problem &p, const Plan &pl, const
     const t0g_linear_ce_desc &d = p.d;
     T0gLossGemmArgs t;
     memset(&t, 0, sizeof t);
-    t.g.a = p.grad ? base + pl.xz : d.x;
-    t.g.b = weight_piece(p, d.w, pc.v0, d.ldw, 2);
+    t.g.a = x_of(p, pl, base);
+    t.g.b = w_of(p, pl, pc, base);
     t.g.c = p.grad ? base + pl.g : 0;
     t.g.m = d.rows;
     t.g.n = pc.cols;
     t.g.k = d.hidden;
-    t.g.lda = p.grad ? pl.ldxz : d.ldx;
-    t.g.ldb = d.ldw;
+    t.g.lda = ldx_of(p, pl);
+    t.g.ldb = ldw_of(p, pl, pc);
     t.g.ldc = ld_of_g(pl, pc);
     t.g.tiles_m = round_up(d.rows, 256) / 256;
     t.g.tiles_n = round_up(pc.cols, 256) / 256;
@@ -365,13 +389,13 @@ int run_loss(t0g_device *dev, const Problem &p) {
     if ((rc = losses_begin(dev, pl.bytes, &base))) return rc;
     if (d.rows == 0) {
         for (const Piece &pc : pl.pieces)   // a product over no rows: zeros
-            if (d.dw && (rc = run_dw(dev, p, pl, pc, base))) return rc;
+            if (d.dw && (rc = run_gemm(dev, dw_gemm(p, pl, pc, base), pl, base))) return rc;
         return ok();
     }
     T0gLossArgs a;
     memset(&a, 0, sizeof a);
     a.x = d.x;
-    a.xz = p.grad ? base + pl.xz : 0;
+    a.xz = pl.copy_x ? base + pl.xz : 0;
     a.labels = d.labels;
     a.dloss = d.dloss;
     a.loss = d.loss;
@@ -437,6 +461,7 @@ int run_loss(t0g_device *dev, const Problem &p) {
     for (size_t i = 0; i < n; ++i) {
         const Piece &pc = pl.pieces[i];
         at_piece(pc);
+        if (pl.copy_w && (rc = run_copy(dev, p, pl, pc, base))) return rc;
         if (pl.fused)
             rc = run_tile(dev, p.grad && i + 1 == n ? Tile::Keep : Tile::Stats, p, pl, pc, a, base);
         else if (!(rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base)))
@@ -458,6 +483,7 @@ int run_loss(t0g_device *dev, const Problem &p) {
     for (size_t i = n; i-- > 0;) {
         const Piece &pc = pl.pieces[i];
         at_piece(pc);
+        if (pl.copy_w && i + 1 < n && (rc = run_copy(dev, p, pl, pc, base))) return rc;
         if (pl.fused && i + 1 == n) {
             rc = piece_kernel("t0g_loss_grad_kept", (a.ldg + 2047) / 2048);
         } else if (pl.fused) {
@@ -466,7 +492,7 @@ int run_loss(t0g_device *dev, const Problem &p) {
             if (i + 1 == n || !(rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base)))
                 rc = piece_kernel("t0g_loss_grad", pc.chunks);
         }
-        if (rc || (d.dw && (rc = run_dw(dev, p, pl, pc, base)))) return rc;
+        if (rc || (d.dw && (rc = run_gemm(dev, dw_gemm(p, pl, pc, base), pl, base)))) return rc;
         if (!d.dx) continue;
         if ((rc = run_gemm(dev, dx_gemm(p, pl, pc, base, planes), pl, base))) return rc;
         if (pl.group == 0) continue;

@@ -690,10 +690,10 @@ static int run_plan(t0g_device *dev, const GemmPlan &p, const GemmOperands &o, u
     return launch(dev, fr, (uint32_t)blocks, 1, 1, threads, &r, sizeof r);
 }
 
-// a_padded: an NN product whose A rows are zero padded to a multiple of 8, so that K need not
-// be one (B's rows past K read as zero).
+// padded: the operands' rows hold whole 16-byte pieces, zeros past the sizes, so that these need
+// not be multiples of 8 for the aligned kernels (the losses' operands in their scratch).
 static int resolve_desc(const t0g_gemm_desc *d, t0g_gemm_config *cfg, GemmPlan *plan, GemmOperands *o,
-                        bool allow_fused = false, bool a_padded = false) {
+                        bool allow_fused = false, bool padded = false) {
     if (!d) return fail(T0G_ERR_INVALID_ARG, "desc is NULL");
     if (d->transpose > T0G_TT) return fail(T0G_ERR_INVALID_ARG, "bad transpose %u", d->transpose);
     if (d->out_dtype > T0G_BF16) return fail(T0G_ERR_INVALID_ARG, "bad out_dtype %u", d->out_dtype);
@@ -736,9 +736,12 @@ static int resolve_desc(const t0g_gemm_desc *d, t0g_gemm_config *cfg, GemmPlan *
     if (sk > kMaxSplitK && sk != T0G_STREAM_K)
         return fail(T0G_ERR_UNSUPPORTED_CONFIG, "split_k=%u > %u", sk, kMaxSplitK);
     const TileDef *tile = plan_tile(cfg, d->m, d->k, d->n, sk);
-    const uint32_t k_pad = a_padded && t == T0G_NN && o->lda >= ((d->k + 7) & ~7u) ? (d->k + 7) & ~7u : d->k;
-    OperandPath path = operand_path(d->a, d->b, d->m, d->n, k_pad, o->lda, o->ldb, t);
-    if (path == OperandPath::Wide && k_pad != d->k) path = OperandPath::Staged;   // extents there are exact
+    OperandPath path = operand_path(d->a, d->b, d->m, d->n, d->k, o->lda, o->ldb, t);
+    if (padded && path == OperandPath::Staged) {
+        auto whole = [](uint32_t v) { return (v + 7) & ~7u; };
+        if (operand_path(d->a, d->b, whole(d->m), whole(d->n), whole(d->k), o->lda, o->ldb, t) == OperandPath::Fast)
+            path = OperandPath::Fast;   // the wide kernels take exact extents
+    }
     if (path == OperandPath::Staged) {
         if ((rc = check_extent("A", a_k_major(t) ? d->m : d->k, o->lda))) return rc;
         if ((rc = check_extent("B", b_k_major(t) ? d->n : d->k, o->ldb))) return rc;
@@ -1275,7 +1278,7 @@ static uint64_t rd_u64(const uint8_t *p) {
     return v;
 }
 
-static int gemm_locked(t0g_device *dev, const t0g_gemm_desc *d, bool allow_fused = true, bool a_padded = false);
+static int gemm_locked(t0g_device *dev, const t0g_gemm_desc *d, bool allow_fused = true, bool padded = false);
 
 // A reference-space config (an RDNA3 tile): the problem is the one the
 // reference's kernel for cfg computes from this grid and these kernargs, and
@@ -1586,11 +1589,11 @@ int t0g_gemm_compile(const t0g_gemm_desc *d, t0g_compiled_kernel *out) {
 
 // t0g_gemm with dev->mu held.  allow_fused = false: split-K with the separate
 // reduce kernel (launches that may overlap another on this device).
-static int gemm_locked(t0g_device *dev, const t0g_gemm_desc *d, bool allow_fused, bool a_padded) {
+static int gemm_locked(t0g_device *dev, const t0g_gemm_desc *d, bool allow_fused, bool padded) {
     t0g_gemm_config cfg;
     GemmPlan p;
     GemmOperands o;
-    int rc = resolve_desc(d, &cfg, &p, &o, allow_fused, a_padded);
+    int rc = resolve_desc(d, &cfg, &p, &o, allow_fused, padded);
     if (rc) return rc;
     if ((rc = check_usable(dev))) return rc;
     if (d->m == 0 || d->n == 0) return ok();
@@ -1802,17 +1805,17 @@ int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t
     return launch(dev, it->second, grid_x, grid_y, 1, 256, args, args_size);
 }
 
-int losses_gemm_workspace(const t0g_gemm_desc *d, size_t *bytes) {
+int losses_gemm_workspace(const t0g_gemm_desc *d, bool padded, size_t *bytes) {
     t0g_gemm_config cfg;
     GemmPlan p;
     GemmOperands o;
-    int rc = resolve_desc(d, &cfg, &p, &o, true, true);
+    int rc = resolve_desc(d, &cfg, &p, &o, true, padded);
     if (rc || (rc = check_grid(p))) return rc;
     *bytes = plan_workspace(p, d->m, d->n, kNumCUs);
     return T0G_OK;
 }
 
-int losses_gemm(t0g_device *dev, const t0g_gemm_desc *d) { return gemm_locked(dev, d, true, true); }
+int losses_gemm(t0g_device *dev, const t0g_gemm_desc *d, bool padded) { return gemm_locked(dev, d, true, padded); }
 
 // Device time of `iters` back-to-back t0g_gemm launches of d (after `warmup`
 // untimed ones): one HIP event between consecutive launches on the device

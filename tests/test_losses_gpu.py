@@ -473,6 +473,29 @@ def test_capture_without_scratch_is_refused():
         warm_up.close()
 
 
+@pytest.mark.parametrize("layout", ["NT", "NN"])
+@pytest.mark.parametrize("rows,vocab,hidden,pad,offset,xpad,max_piece", [
+    (96, 515, 33, 0, 0, 0, 0), (100, 1003, 65, 3, 1, 2, 0), (130, 777, 127, 1, 0, 0, 256), (100, 515, 1023, 1, 0, 1, 104),
+    (256, 515, 33, 0, 0, 0, 0), (300, 1003, 65, 3, 1, 2, 0), (260, 1285, 127, 1, 0, 0, 256), (257, 2051, 200, 5, 0, 0, 768),
+    (300, 130, 71, 0, 3, 7, 0), (512, 515, 33, 0, 0, 0, 0), (600, 1003, 65, 3, 1, 2, 0), (513, 1285, 127, 1, 0, 0, 256),
+    (520, 2051, 200, 5, 0, 0, 768), (512, 130, 71, 0, 3, 7, 0), (530, 515, 1023, 1, 0, 1, 104)])
+def test_copied_weight(rt, rows, vocab, hidden, pad, offset, xpad, max_piece, layout):
+    """Rows that are not whole 16-byte pieces; from 512 on the weight is copied (in both forms of the call)."""
+    Case(rows, vocab, hidden, layout, seed=rows + vocab, pad=pad, offset=offset, xpad=xpad).check(
+        rt, "copied", max_piece=max_piece)
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,layout,pad,offset,xpad", [
+    (5, 600, 64, "NT", 8, 0, 3), (120, 600, 64, "NT", 0, 0, 3), (300, 600, 64, "NT", 0, 1, 0), (300, 601, 63, "NN", 0, 0, 0),
+    (300, 600, 63, "NN", 0, 0, 0), (20, 600, 63, "NN", 8, 0, 1),
+    (600, 600, 64, "NT", 0, 1, 0), (600, 601, 63, "NN", 0, 0, 0), (600, 601, 63, "NT", 1, 0, 0)])
+def test_loss_alone_of_unaligned_operands(rt, rows, vocab, hidden, layout, pad, offset, xpad):
+    c = Case(rows, vocab, hidden, layout, seed=27, pad=pad, offset=offset, xpad=xpad, want="")
+    c.labels[::3] = -1
+    c.x[3] = float("nan")
+    c.check(rt, "loss alone")
+
+
 # ---- the fused form: 256 rows and more, aligned operands ------------------------------
 
 FUSED = [(256, 256, 64), (257, 1000, 72), (300, 2049, 136), (256, 131, 64), (513, 1283, 320), (260, 8, 8), (1000, 640, 40)]
