@@ -513,9 +513,10 @@ T0G_API int t0g_matmul_kernel_name(uint32_t op, uint32_t m, uint32_t k, uint32_t
  * Products, statistics and losses are f32 on bf16 operands.  The logits' gradient
  * is rounded to bf16 once, as an operand of the products that give dx and dw.
  * Results do not depend on what ran before: no atomics, sums in a fixed order.
- * Calls are asynchronous on the device stream; the scratch (a piece of G of
- * 0.9 GB at most, f32 partial sums of dx, and less) belongs to the handle and grows on a
- * shape's first call.
+ * Calls are asynchronous on the device stream; the scratch (a piece of G, 2 GiB
+ * at most or what max_piece leaves of it, f32 partial sums of dx if there are several
+ * pieces, copies of x and of an unaligned piece of w) belongs to the handle and grows on
+ * a shape's first call.
  * Under stream capture it cannot grow: the call is refused unless the same call
  * ran before. */
 typedef enum t0g_index_type { T0G_I32 = 0, T0G_I64 = 1 } t0g_index_type;

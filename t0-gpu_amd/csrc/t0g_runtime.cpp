@@ -737,10 +737,14 @@ static int resolve_desc(const t0g_gemm_desc *d, t0g_gemm_config *cfg, GemmPlan *
         return fail(T0G_ERR_UNSUPPORTED_CONFIG, "split_k=%u > %u", sk, kMaxSplitK);
     const TileDef *tile = plan_tile(cfg, d->m, d->k, d->n, sk);
     OperandPath path = operand_path(d->a, d->b, d->m, d->n, d->k, o->lda, o->ldb, t);
-    if (padded && path == OperandPath::Staged) {
+    if (padded) {
         auto whole = [](uint32_t v) { return (v + 7) & ~7u; };
-        if (operand_path(d->a, d->b, whole(d->m), whole(d->n), whole(d->k), o->lda, o->ldb, t) == OperandPath::Fast)
-            path = OperandPath::Fast;   // the wide kernels take exact extents
+        const uint64_t a = a_k_major(t) ? (uint64_t)(d->m - 1) * o->lda + whole(d->k) : (uint64_t)(d->k - 1) * o->lda + whole(d->m);
+        const uint64_t b = b_k_major(t) ? (uint64_t)(d->n - 1) * o->ldb + whole(d->k) : (uint64_t)(d->k - 1) * o->ldb + whole(d->n);
+        // exact extents up to 2^30 elements: the kernels' out-of-range offset is 2^31 bytes
+        if (d->m && d->n && d->k && a <= (1ull << 30) && b <= (1ull << 30) &&
+            operand_path(d->a, d->b, whole(d->m), whole(d->n), whole(d->k), o->lda, o->ldb, t) != OperandPath::Staged)
+            path = OperandPath::Fast;
     }
     if (path == OperandPath::Staged) {
         if ((rc = check_extent("A", a_k_major(t) ? d->m : d->k, o->lda))) return rc;

@@ -85,8 +85,12 @@ def test_null_arguments():
     assert t0g._lib.t0g_linear_distill(None, ctypes.byref(distill())) == t0g.ERR_INVALID_ARG
 
 
-def test_scratch_stays_far_below_the_logits():
-    """8192 x 131072 logits take 4 GiB in f32; their pieces do not."""
-    d = t0g.linear_ce_desc(0x100000000, 0x200000000, 0x10000000, 0x20000000, 8192, 131072, 4096, dx=0x300000000,
-                           dw=0x400000000)
-    assert t0g.linear_loss_scratch_size(d) < 1.25 * 2 ** 30
+def test_scratch_stays_below_the_logits():
+    """8192 x 131072 logits take 4 GiB in f32 and their gradient 2 in bf16, 65536 rows eight times that; a
+    piece of the vocabulary takes what it is given."""
+    def scratch(rows, **kw):
+        return t0g.linear_loss_scratch_size(t0g.linear_ce_desc(
+            0x100000000, 0x200000000, 0x10000000, 0x20000000, rows, 131072, 4096, dx=0x300000000, dw=0x400000000, **kw))
+    assert scratch(8192) < 2.5 * 2 ** 30
+    assert scratch(65536) < 6 * 2 ** 30
+    assert scratch(8192, max_piece=8192) < 0.75 * 2 ** 30
