@@ -71,20 +71,67 @@ __device__ __forceinline__ uint32_t token_at(uint64_t base, uint64_t i, bool wid
 // Row `row` of x into xz, zero for an ignored row (its hidden state may hold NaN, and
 // dW's product would multiply that with the row's zero gradient) and past `hidden`.
 __device__ __forceinline__ void copy_row(const T0gLossArgs& p, uint32_t row, bool used) {
+    const uint64_t to = p.xz + (uint64_t)row * p.ldxz * 2, again = to + (uint64_t)p.rows * p.ldxz * 2;
+    const bool pair = p.flags & T0G_LOSS_PAIR;
     if (p.flags & T0G_LOSS_X_VEC) {
         const uint32_t n = p.hidden / 8;
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
             u32x4_t v = {0u, 0u, 0u, 0u};
             if (used) v = *at<const u32x4_t>(p.x + (uint64_t)row * p.ldx * 2, i);
-            *at<u32x4_t>(p.xz + (uint64_t)row * p.ldxz * 2, i) = v;
+            *at<u32x4_t>(to, i) = v;
+            if (pair) *at<u32x4_t>(again, i) = v;
         }
     } else {
         for (uint32_t i = threadIdx.x; i < p.ldxz; i += kThreads) {
             uint16_t v = 0;
             if (used && i < p.hidden) v = *at<const uint16_t>(p.x, (uint64_t)row * p.ldx + i);
-            *at<uint16_t>(p.xz, (uint64_t)row * p.ldxz + i) = v;
+            *at<uint16_t>(to, i) = v;
+            if (pair) *at<uint16_t>(again, i) = v;
         }
     }
+}
+
+// What a row is compared with, and the coefficients of its gradient's sparse part.
+struct RowInfo {
+    uint32_t entries, label;   // the label's entry, kNoToken for none
+    float cl, ct, hq;          // of the label, of the teacher's Q; sum of Q log Q
+    bool taught;
+    __device__ __forceinline__ bool labelled() const { return label != kNoToken; }
+    __device__ __forceinline__ bool used() const { return labelled() || taught; }
+};
+__device__ __forceinline__ float row_rate(const T0gLossArgs& p, uint32_t row) {
+    return p.loss_scale * (p.dloss ? *at<const float>(p.dloss, row) : 1.0f) * p.logit_scale;
+}
+__device__ __forceinline__ uint32_t row_label(const T0gLossArgs& p, uint32_t row) {
+    return p.labels ? token_at(p.labels, row, p.flags & T0G_LOSS_LABEL64, p.vocab) : kNoToken;
+}
+__device__ __forceinline__ RowInfo row_info(const T0gLossArgs& p, uint32_t row) {
+    if (p.flags & T0G_LOSS_DIRECT) {
+        const bool has = row_label(p, row) != kNoToken;
+        return RowInfo{has ? 1u : 0u, has ? 0u : kNoToken, has ? p.label_weight * row_rate(p, row) : 0.0f, 0.0f, 0.0f, false};
+    }
+    const u32x2_t ent = *at<const u32x2_t>(p.row_ent, row);
+    const f32x4_t sub = *at<const f32x4_t>(p.row_sub, row);
+    return RowInfo{ent[0], ent[1], sub[0], sub[1], sub[2], sub[3] != 0.0f};
+}
+__device__ __forceinline__ uint32_t entry_token(const T0gLossArgs& p, uint32_t row, uint32_t e) {
+    return (p.flags & T0G_LOSS_DIRECT) ? row_label(p, row) : *at<const uint32_t>(p.ent_tok, (uint64_t)row * p.slots + e);
+}
+__device__ __forceinline__ float entry_q(const T0gLossArgs& p, uint32_t row, uint32_t e) {
+    return (p.flags & T0G_LOSS_DIRECT) ? 0.0f : *at<const float>(p.ent_q, (uint64_t)row * p.slots + e);
+}
+// l0, l1, c0, c1 of a row's gradient.
+__device__ __forceinline__ f32x4_t row_params(const T0gLossArgs& p, const RowInfo& r, float l0, float l1) {
+    if (!r.used()) return f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    return (p.flags & T0G_LOSS_DUAL) ? f32x4_t{l0, l1, r.cl, r.ct} : f32x4_t{l0, l1, r.cl + r.ct, 0.0f};
+}
+__device__ __forceinline__ void store_loss(const T0gLossArgs& p, uint32_t row, const RowInfo& r, float l0, float l1, float zl,
+                                           float kd) {
+    float loss = 0.0f;
+    if (r.labelled()) loss = p.label_weight * (l0 * kLn2 - zl * p.logit_scale);
+    if (r.taught) loss += p.distill_weight * p.tau * p.tau * (r.hq + kd);
+    *at<float>(p.loss, row) = loss;
+    if (p.lse) *at<float>(p.lse, row) = r.used() ? l1 * kLn2 : 0.0f;
 }
 
 // What a row is compared with: its label and the teacher's distribution over its
@@ -98,8 +145,8 @@ __device__ __forceinline__ void prepare_row(const T0gLossArgs& p, uint32_t row) 
     __shared__ float red[3][4];
     __shared__ uint32_t wave_heads[4];
     const uint32_t tid = threadIdx.x;
-    const uint32_t label = p.labels ? token_at(p.labels, row, p.flags & T0G_LOSS_LABEL64, p.vocab) : kNoToken;
-    const float rate = p.loss_scale * (p.dloss ? *at<const float>(p.dloss, row) : 1.0f) * p.logit_scale;
+    const uint32_t label = row_label(p, row);
+    const float rate = row_rate(p, row);
     const float cl = label != kNoToken ? p.label_weight * rate : 0.0f;
     uint32_t n = 0, label_slot = kNoToken;
     float hq = 0.0f;
@@ -205,6 +252,40 @@ __device__ __forceinline__ void prepare_row(const T0gLossArgs& p, uint32_t row) 
     __syncthreads();
 }
 
+// One chunk of a row of raw logits in registers, times k, -inf past its end.
+__device__ __forceinline__ void load_chunk(const T0gLossArgs& p, uint64_t base, uint32_t n, f32x4_t (&v)[4]) {
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t c = (i * kThreads + threadIdx.x) * 4;
+        v[i] = f32x4_t{ninf(), ninf(), ninf(), ninf()};
+        if (c < n) {   // rows are padded to whole quads
+            v[i] = *at<const f32x4_t>(base, c / 4);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) v[i][e] = c + e < n ? v[i][e] * p.k : ninf();
+        }
+    }
+}
+__device__ __forceinline__ void reduce_chunk(const T0gLossArgs& p, const f32x4_t (&v)[4], uint32_t n, float (&red)[3][4],
+                                             float& m, float& s, float& s2) {
+    m = ninf();
+    s = s2 = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) m = __builtin_fmaxf(m, v[i][e]);
+    m = block_max(m, red[0]);
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            if ((i * kThreads + threadIdx.x) * 4 + e >= n) continue;
+            s += exp2_(v[i][e] - m);
+            if (p.flags & T0G_LOSS_DUAL) s2 += exp2_((v[i][e] - m) * p.r);
+        }
+    s = block_sum(s, red[1]);
+    if (p.flags & T0G_LOSS_DUAL) s2 = block_sum(s2, red[2]);
+}
+
 // Statistics of one chunk of a row of raw logits, and the raw logits of the row's
 // entries in it.
 __device__ __forceinline__ void chunk_stats(const T0gLossArgs& p, uint32_t row, uint32_t chunk) {
@@ -213,44 +294,45 @@ __device__ __forceinline__ void chunk_stats(const T0gLossArgs& p, uint32_t row, 
     const uint64_t base = p.z + ((uint64_t)row * p.ldz + c0) * 4;
     const uint32_t n = min(T0G_LOSS_CHUNK, p.cols - c0);
     f32x4_t v[4];
-    float m = ninf();
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t c = (i * kThreads + tid) * 4;
-        v[i] = f32x4_t{ninf(), ninf(), ninf(), ninf()};
-        if (c < n) {   // rows are padded to whole quads
-            v[i] = *at<const f32x4_t>(base, c / 4);
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) {
-                v[i][e] = c + e < n ? v[i][e] * p.k : ninf();
-                m = __builtin_fmaxf(m, v[i][e]);
-            }
-        }
-    }
-    m = block_max(m, red[0]);
-    float s = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) {
-            if ((i * kThreads + tid) * 4 + e >= n) continue;
-            s += exp2_(v[i][e] - m);
-            if (p.flags & T0G_LOSS_DUAL) s2 += exp2_((v[i][e] - m) * p.r);
-        }
-    s = block_sum(s, red[1]);
-    if (p.flags & T0G_LOSS_DUAL) s2 = block_sum(s2, red[2]);
+    float m, s, s2;
+    load_chunk(p, base, n, v);
+    reduce_chunk(p, v, n, red, m, s, s2);
     if (tid == 0) {
         const uint64_t i = (uint64_t)(p.chunk0 + chunk) * p.rows + row;
         *at<f32x2_t>(p.part, i) = f32x2_t{m, s};
         if (p.flags & T0G_LOSS_DUAL) *at<float>(p.part2, i) = s2;
     }
-    const uint32_t entries = (*at<const u32x2_t>(p.row_ent, row))[0];
-    for (uint32_t e = tid; e < entries; e += kThreads) {
-        const uint64_t slot = (uint64_t)row * p.slots + e;
-        const uint32_t c = *at<const uint32_t>(p.ent_tok, slot) - (p.v0 + c0);   // wraps below the chunk
-        if (c < n) *at<float>(p.ent_z, slot) = *at<const float>(base, c);
+    const RowInfo r = row_info(p, row);
+    for (uint32_t e = tid; e < r.entries; e += kThreads) {
+        const uint32_t c = entry_token(p, row, e) - (p.v0 + c0);   // wraps below the chunk
+        if (c < n) *at<float>(p.ent_z, (uint64_t)row * p.slots + e) = *at<const float>(base, c);
     }
+    if ((p.flags & T0G_LOSS_DIRECT) && p.xz && p.v0 == 0 && chunk == 0) copy_row(p, row, r.used());
     __syncthreads();
+}
+
+// A chunk's statistics onto those before: (m, s, s2) += (cm, cs, cs2).
+__device__ __forceinline__ void join_chunk(const T0gLossArgs& p, float& m, float& s, float& s2, float cm, float cs,
+                                           float cs2) {
+    const float top = __builtin_fmaxf(m, cm);
+    s = s * (m == top ? 1.0f : exp2_(m - top)) + cs * (cm == top ? 1.0f : exp2_(cm - top));
+    if (p.flags & T0G_LOSS_DUAL)
+        s2 = s2 * (m == top ? 1.0f : exp2_((m - top) * p.r)) + cs2 * (cm == top ? 1.0f : exp2_((cm - top) * p.r));
+    m = top;
+}
+__device__ __forceinline__ void join_chunks(const T0gLossArgs& p, uint32_t row, uint32_t first, uint32_t step, float& m,
+                                            float& s, float& s2) {
+    m = ninf();
+    s = s2 = 0.0f;
+    for (uint32_t c = first; c < p.chunks; c += step) {
+        const uint64_t i = (uint64_t)c * p.rows + row;
+        const f32x2_t v = *at<const f32x2_t>(p.part, i);
+        join_chunk(p, m, s, s2, v[0], v[1], (p.flags & T0G_LOSS_DUAL) ? *at<const float>(p.part2, i) : 0.0f);
+    }
+}
+// The teacher's term of an entry of the loss.
+__device__ __forceinline__ float entry_kd(const T0gLossArgs& p, float q, float z, float l1) {
+    return q != 0.0f ? q * (l1 * kLn2 - z * (p.logit_scale / p.tau)) : 0.0f;
 }
 
 // Rows' chunks joined: their losses, log-sum-exps and gradient coefficients.  A workgroup
@@ -272,106 +354,122 @@ __device__ __forceinline__ void combine_rows(const T0gLossArgs& p, uint32_t row0
         __syncthreads();
         return t[tid & ((1u << p.row_shift) - 1)];
     };
-    // each thread's own chunks first, in one pass
     float m = ninf(), s = 0.0f, s2 = 0.0f;
-    if (live)
-        for (uint32_t c = part; c < p.chunks; c += per) {
-            const uint64_t i = (uint64_t)c * p.rows + row;
-            const f32x2_t v = *at<const f32x2_t>(p.part, i);
-            const float top = __builtin_fmaxf(m, v[0]);
-            const float old = m == top ? 1.0f : exp2_(m - top), now = v[0] == top ? 1.0f : exp2_(v[0] - top);
-            s = s * old + v[1] * now;
-            if (dual) {
-                const float old2 = m == top ? 1.0f : exp2_((m - top) * p.r);
-                const float now2 = v[0] == top ? 1.0f : exp2_((v[0] - top) * p.r);
-                s2 = s2 * old2 + *at<const float>(p.part2, i) * now2;
-            }
-            m = top;
-        }
+    if (live) join_chunks(p, row, part, per, m, s, s2);   // each thread's own chunks first, in one pass
     const float top = join(t0, m, true);
-    const float scale = m == top ? 1.0f : exp2_(m - top);
-    s = join(t0, s * scale, false);
-    const float l0 = top + __builtin_amdgcn_logf(s);
+    const float l0 = top + __builtin_amdgcn_logf(join(t0, s * (m == top ? 1.0f : exp2_(m - top)), false));
     float l1 = l0;
     if (dual) l1 = top * p.r + __builtin_amdgcn_logf(join(t1, s2 * (m == top ? 1.0f : exp2_((m - top) * p.r)), false));
-    u32x2_t ent = {0u, kNoToken};
-    f32x4_t sub = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (live) {
-        ent = *at<const u32x2_t>(p.row_ent, row);
-        sub = *at<const f32x4_t>(p.row_sub, row);
-    }
-    const bool taught = sub[3] != 0.0f, labelled = ent[1] != kNoToken;
+    RowInfo r = {0, kNoToken, 0.0f, 0.0f, 0.0f, false};
+    if (live) r = row_info(p, row);
     float kd = 0.0f;
     if (p.teacher) {
-        if (taught)
-            for (uint32_t e = part; e < ent[0]; e += per) {
-                const uint64_t slot = (uint64_t)row * p.slots + e;
-                const float q = *at<const float>(p.ent_q, slot);
-                if (q != 0.0f) kd += q * (l1 * kLn2 - *at<const float>(p.ent_z, slot) * (p.logit_scale / p.tau));
-            }
+        if (r.taught)
+            for (uint32_t e = part; e < r.entries; e += per)
+                kd += entry_kd(p, entry_q(p, row, e), *at<const float>(p.ent_z, (uint64_t)row * p.slots + e), l1);
         kd = join(t1, kd, false);
     }
     if (part == 0 && live) {
-        float loss = 0.0f;
-        if (labelled)
-            loss = p.label_weight *
-                   (l0 * kLn2 - *at<const float>(p.ent_z, (uint64_t)row * p.slots + ent[1]) * p.logit_scale);
-        if (taught) loss += p.distill_weight * p.tau * p.tau * (sub[2] + kd);
-        const bool used = labelled || taught;
-        *at<float>(p.loss, row) = loss;
-        if (p.lse) *at<float>(p.lse, row) = used ? l1 * kLn2 : 0.0f;
-        if (p.row_par)
-            *at<f32x4_t>(p.row_par, row) = !used  ? f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}
-                                           : dual ? f32x4_t{l0, l1, sub[0], sub[1]}
-                                                  : f32x4_t{l0, l1, sub[0] + sub[1], 0.0f};
+        const float zl = r.labelled() ? *at<const float>(p.ent_z, (uint64_t)row * p.slots + r.label) : 0.0f;
+        store_loss(p, row, r, l0, l1, zl, kd);
+        if (p.row_par) *at<f32x4_t>(p.row_par, row) = row_params(p, r, l0, l1);
     }
     __syncthreads();
 }
 
-// The dense part of a logit's gradient.
-__device__ __forceinline__ float dense_grad(const T0gLossArgs& p, const f32x4_t& par, float z) {
-    const float u = z * p.k;
+// The dense part of a logit's gradient, from u.
+__device__ __forceinline__ float dense_grad(const T0gLossArgs& p, const f32x4_t& par, float u) {
     float g = par[2] * exp2_(u - par[0]);
     if (p.flags & T0G_LOSS_DUAL) g += par[3] * exp2_(u * p.r - par[1]);
     return g;
 }
 
+// The gradient of a row's entry e with raw logit z.
+__device__ __forceinline__ float entry_grad(const T0gLossArgs& p, const RowInfo& r, const f32x4_t& par, uint32_t row,
+                                            uint32_t e, float z) {
+    const float g = dense_grad(p, par, z * p.k) - r.ct * entry_q(p, row, e);
+    return e == r.label ? g - r.cl : g;
+}
+
 // The gradients of a row's entries in columns [c0, c0 + n) of the piece, over the dense part.
 __device__ __forceinline__ void entry_grads(const T0gLossArgs& p, uint32_t row, uint32_t c0, uint32_t n,
                                             const f32x4_t& par, uint32_t first, uint32_t step) {
-    const u32x2_t ent = *at<const u32x2_t>(p.row_ent, row);
-    const f32x4_t sub = *at<const f32x4_t>(p.row_sub, row);
-    for (uint32_t e = first; e < ent[0]; e += step) {
-        const uint64_t slot = (uint64_t)row * p.slots + e;
-        const uint32_t c = *at<const uint32_t>(p.ent_tok, slot) - (p.v0 + c0);   // wraps below the range
+    const RowInfo r = row_info(p, row);
+    for (uint32_t e = first; e < r.entries; e += step) {
+        const uint32_t c = entry_token(p, row, e) - (p.v0 + c0);   // wraps below the range
         if (c >= n) continue;
-        float g = dense_grad(p, par, *at<const float>(p.ent_z, slot)) - sub[1] * *at<const float>(p.ent_q, slot);
-        if (e == ent[1]) g -= sub[0];
-        *at<__bf16>(p.g, (uint64_t)row * p.ldg + c0 + c) = (__bf16)g;
+        const float g = entry_grad(p, r, par, row, e, *at<const float>(p.ent_z, (uint64_t)row * p.slots + e));
+        const uint64_t o = (uint64_t)row * p.ldg + c0 + c;
+        const __bf16 h = (__bf16)g;
+        *at<__bf16>(p.g, o) = h;
+        if (p.flags & T0G_LOSS_PAIR) *at<__bf16>(p.g, o + (uint64_t)p.rows * p.ldg) = (__bf16)(g - (float)h);
     }
 }
 
-// Logit gradients of one chunk of a row in bf16, zero past the piece, then its entries.
+// One chunk of a row of raw logits, by rows: the row's statistics (its own where the
+// vocabulary is one chunk), its loss (the first chunk), and the chunk's logit gradients
+// in bf16, zero past the piece, then its entries.
 __device__ __forceinline__ void chunk_grad(const T0gLossArgs& p, uint32_t row, uint32_t chunk) {
+    __shared__ float red[4][4], own[3][4];
     const uint32_t c0 = chunk * T0G_LOSS_CHUNK, tid = threadIdx.x;
-    const uint64_t zb = p.z + ((uint64_t)row * p.ldz + c0) * 4, gb = p.g + ((uint64_t)row * p.ldg + c0) * 2;
-    const uint32_t n = min(T0G_LOSS_CHUNK, p.cols - c0), ng = min(T0G_LOSS_CHUNK, p.ldg - c0);
-    const f32x4_t par = *at<const f32x4_t>(p.row_par, row);
-    const bool used = par[2] != 0.0f || par[3] != 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t c = (i * kThreads + tid) * 4;
-        if (c >= ng) continue;
-        float g[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (used && c < n) {
-            const f32x4_t z = *at<const f32x4_t>(zb, c / 4);
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) g[e] = c + e < n ? dense_grad(p, par, z[e]) : 0.0f;
-        }
-        *at<u32x2_t>(gb, c / 4) = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
+    const uint64_t zb = p.z + ((uint64_t)row * p.ldz + c0) * 4;
+    const uint32_t n = min(T0G_LOSS_CHUNK, p.cols - c0);
+    const bool one = p.chunks == 1, dual = p.flags & T0G_LOSS_DUAL;
+    const RowInfo r = row_info(p, row);
+    f32x4_t v[4];
+    float m, s, s2;
+    load_chunk(p, zb, n, v);
+    if (one) {
+        reduce_chunk(p, v, n, own, m, s, s2);
+    } else {
+        join_chunks(p, row, tid, kThreads, m, s, s2);
+        const float top = block_max(m, red[0]);
+        s = block_sum(s * (m == top ? 1.0f : exp2_(m - top)), red[1]);
+        if (dual) s2 = block_sum(s2 * (m == top ? 1.0f : exp2_((m - top) * p.r)), red[2]);
+        m = top;
     }
-    __syncthreads();   // the dense part is written before its entries are replaced
-    if (used) entry_grads(p, row, c0, n, par, tid, kThreads);
+    const float l0 = m + __builtin_amdgcn_logf(s), l1 = dual ? m * p.r + __builtin_amdgcn_logf(s2) : l0;
+    if (one)   // the entries' logits are all here
+        for (uint32_t e = tid; e < r.entries; e += kThreads)
+            *at<float>(p.ent_z, (uint64_t)row * p.slots + e) = *at<const float>(zb, entry_token(p, row, e));
+    if (p.v0 == 0 && chunk == 0) {
+        float kd = 0.0f;
+        if (r.taught)   // each thread reads what it wrote itself
+            for (uint32_t e = tid; e < r.entries; e += kThreads)
+                kd += entry_kd(p, entry_q(p, row, e), *at<const float>(p.ent_z, (uint64_t)row * p.slots + e), l1);
+        if (p.teacher) kd = block_sum(kd, red[3]);
+        if (tid == 0) {
+            float zl = 0.0f;
+            if (r.labelled())
+                zl = one ? *at<const float>(zb, entry_token(p, row, r.label))
+                         : *at<const float>(p.ent_z, (uint64_t)row * p.slots + r.label);
+            store_loss(p, row, r, l0, l1, zl, kd);
+        }
+        if (one && (p.flags & T0G_LOSS_DIRECT) && p.xz) copy_row(p, row, r.used());
+    }
+    if (p.g) {
+        const f32x4_t par = row_params(p, r, l0, l1);
+        const bool used = par[2] != 0.0f || par[3] != 0.0f;
+        const uint32_t ng = min(T0G_LOSS_CHUNK, p.ldg - c0);
+        const uint64_t gb = p.g + ((uint64_t)row * p.ldg + c0) * 2;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t c = (i * kThreads + tid) * 4;
+            if (c >= ng) continue;
+            float g[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) g[e] = used && c + e < n ? dense_grad(p, par, v[i][e]) : 0.0f;
+            *at<u32x2_t>(gb, c / 4) = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
+            if (p.flags & T0G_LOSS_PAIR) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) g[e] -= (float)(__bf16)g[e];
+                *at<u32x2_t>(gb + (uint64_t)p.rows * p.ldg * 2, c / 4) = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
+            }
+        }
+        __syncthreads();   // the dense part is written before its entries are replaced
+        if (used) entry_grads(p, row, c0, n, par, tid, kThreads);
+    }
+    __syncthreads();
 }
 
 // The same from the kept exponentials, in place: kept e = 2^(u - m) less a factor that
@@ -434,22 +532,31 @@ __device__ __forceinline__ void copy_weight(const T0gLossCopyArgs& p) {
 }
 
 __device__ __forceinline__ void sum_planes(const T0gLossSumArgs& p) {
-    const uint64_t total = (uint64_t)p.rows * p.cols;
-    const uint32_t w = p.vec ? 4 : 1;
-    for (uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) * w; i < total;
-         i += (uint64_t)gridDim.x * kThreads * w) {
-        const uint64_t o = i / p.cols * p.ldo + i % p.cols;
+    const uint32_t w = p.vec ? 4 : 1, per_row = p.cols / w;
+    const uint64_t total = (uint64_t)p.rows * per_row, plane = (uint64_t)p.rows * p.ldp;
+    for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (uint64_t)gridDim.x * kThreads) {
+        const uint64_t row = i / per_row;
+        const uint32_t c = (uint32_t)(i - row * per_row) * w;
+        const uint64_t o = row * p.ldo + c, q = row * p.ldp + c;
         if (p.vec) {
             f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (p.acc) v = *at<const f32x4_t>(p.acc, i / 4);
-            for (uint32_t s = 0; s < p.n; ++s) v += *at<const f32x4_t>(p.planes + (uint64_t)s * total * 4, i / 4);
+            if (p.acc) v = *at<const f32x4_t>(p.acc, q / 4);
+            for (uint32_t s0 = 0; s0 < p.n; s0 += 8) {   // eight planes' loads in flight
+                f32x4_t x[8];
+#pragma unroll
+                for (uint32_t s = 0; s < 8; ++s)
+                    if (s0 + s < p.n) x[s] = *at<const f32x4_t>(p.planes + (s0 + s) * plane * 4, q / 4);
+#pragma unroll
+                for (uint32_t s = 0; s < 8; ++s)
+                    if (s0 + s < p.n) v += x[s];
+            }
             if (p.out_bf16)
                 *at<u32x2_t>(p.out, o / 4) = u32x2_t{pack2(v[0], v[1]), pack2(v[2], v[3])};
             else
                 *at<f32x4_t>(p.out, o / 4) = v;
         } else {
-            float v = p.acc ? *at<const float>(p.acc, i) : 0.0f;
-            for (uint32_t s = 0; s < p.n; ++s) v += *at<const float>(p.planes, (uint64_t)s * total + i);
+            float v = p.acc ? *at<const float>(p.acc, q) : 0.0f;
+            for (uint32_t s = 0; s < p.n; ++s) v += *at<const float>(p.planes, s * plane + q);
             if (p.out_bf16)
                 *at<__bf16>(p.out, o) = (__bf16)v;
             else

@@ -89,6 +89,10 @@ int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t
 // hold whole 16-byte pieces, zeros past the sizes, which then need not be multiples of 8.
 int losses_gemm_workspace(const t0g_gemm_desc *d, bool padded, size_t *bytes);
 int losses_gemm(t0g_device *dev, const t0g_gemm_desc *d, bool padded);
+// The GEMM with f32 output whose K slices' planes go to c, c + m ldc, ... and stay apart; and
+// how many there are (host only).
+int losses_gemm_planes(t0g_device *dev, const t0g_gemm_desc *d, bool padded);
+int losses_gemm_planes_count(const t0g_gemm_desc *d, bool padded, uint32_t *planes);
 
 // One kernel's entry in a code object's AMDGPU metadata (t0g_codeobj.cpp).
 struct KernelMeta {

@@ -187,7 +187,7 @@ typedef struct T0gLossArgs {
     uint32_t v0, cols;       /* the piece: its first token and width                  */
     uint32_t ldz, ldg;
     uint32_t chunk0;         /* the piece's first chunk                               */
-    uint32_t chunks;         /* chunks of the piece, or of the vocabulary (combine)   */
+    uint32_t chunks;         /* chunks of the vocabulary                              */
     uint32_t flags;          /* T0G_LOSS_* bits                                       */
     uint32_t row_shift;      /* combine: 2^row_shift rows a workgroup, 0 to 4          */
     float k, r;              /* u = z k; second temperature's ratio                   */
@@ -200,6 +200,9 @@ typedef struct T0gLossArgs {
 #define T0G_LOSS_TEACHER16 4u  /* the teacher's logits are bf16                        */
 #define T0G_LOSS_DUAL 8u       /* labels and a teacher of another temperature          */
 #define T0G_LOSS_X_VEC 16u     /* x rows are 16-byte aligned and hidden a multiple of 8 */
+#define T0G_LOSS_DIRECT 32u    /* labels only, read by each kernel: no entries were prepared */
+#define T0G_LOSS_PAIR 64u      /* g and xz have 2 rows rows: the second half of g is what the
+                                  first's rounding left, of xz the same copy again       */
 #define T0G_LOSS_CHUNK 4096u   /* columns of one workgroup in the row kernels          */
 #define T0G_LOSS_MAX_TOP 1024u /* teacher entries of a row, at most                    */
 
@@ -231,11 +234,12 @@ typedef struct T0gLossCopyArgs {
 
 /* Sum of f32 planes of a data gradient, in order, into bf16 or f32 rows. */
 typedef struct T0gLossSumArgs {
-    uint64_t acc;            /* f32 [rows][cols] summed before, or 0                  */
-    uint64_t planes;         /* f32 [n][rows][cols]                                   */
+    uint64_t acc;            /* f32 [rows][ldp] summed before, or 0                   */
+    uint64_t planes;         /* f32 [n][rows][ldp], ldp a multiple of 4               */
     uint64_t out;            /* f32 | bf16 [rows][ldo]                                */
-    uint32_t n, rows, cols, ldo;
+    uint32_t n, rows, cols, ldp, ldo;
     uint32_t out_bf16, vec;  /* vec: cols and ldo multiples of 4, out 16-byte aligned */
+    uint32_t reserved;
 } T0gLossSumArgs;
 
 /* Epilogue chain operations: tile_ir's EpilogueOp (src/t0/tile_ir.rs:41-62),

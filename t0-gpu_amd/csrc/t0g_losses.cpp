@@ -14,6 +14,8 @@
 //             the other pieces' logits are computed again with G in the epilogue
 //   by rows   a piece's f32 logits go to the scratch and row kernels read them: products
 //             of few rows, and operands that the 256x256 tile does not take
+// By rows, labels alone need no preparation (each kernel reads them), and a vocabulary of
+// one chunk takes its statistics, loss and G in one kernel.
 // A weight whose rows are not whole 16-byte pieces is copied into ones that are, piece by
 // piece, when there are rows enough to make up for that.
 #include <math.h>
@@ -39,6 +41,10 @@ constexpr uint64_t kFusedPieceBytes = 2048ull << 20;
 constexpr uint64_t kPlaneBytes = 128ull << 20;
 // Rows from which the fused form is taken.
 constexpr uint32_t kFusedRows = 256;
+// Rows up to which G goes into the products as two bf16, the rounded value and what the
+// rounding left: few rows' roundings do not average out (one row's dx has the label's
+// whole, up to 2^-8), and what bounds their products is the weight's bytes.
+constexpr uint32_t kPairRows = 128;
 // Rows from which an unaligned weight is copied, and what a copied piece takes at most.  Without
 // and with the copy, width 1023: loss alone over 50001 tokens 200 rows 97 / 97 us, 300 rows 120 /
 // 130, 777 rows 255 / 188; with gradients over 20001 tokens 300 rows 146 / 158, 777 rows 271 / 243.
@@ -147,9 +153,13 @@ struct Plan {
     bool fused = false;
     bool copy_w = false;         // the pieces' weights are copied
     bool copy_x = false;         // products take xz instead of x
+    bool direct = false;         // by rows, labels alone
+    bool pair = false;           // G in two bf16, rows of g and xz twice
     bool padded = false;         // every operand's rows are whole 16-byte pieces
     uint32_t chunks = 0, slots = 0, ldxz = 0, off_ld = 0;
-    uint32_t group = 0;          // planes of dx summed at a time (0: the one product writes dx)
+    uint32_t group = 0;          // products of dx summed at a time (0: the one product writes dx)
+    uint32_t splits = 1;         // pair: planes of each product and half
+    uint32_t ldp = 0;
     uint64_t xz = 0, ent_tok = 0, ent_q = 0, ent_z = 0, row_ent = 0, row_sub = 0, row_par = 0, part = 0, part2 = 0,
              ent_off = 0, w = 0;
     uint64_t z = 0, g = 0, planes = 0, acc = 0, gemm_ws = 0;
@@ -206,18 +216,18 @@ t0g_gemm_desc dx_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_
     const t0g_linear_ce_desc &d = p.d;
     const bool whole = pl.group == 0;
     return gemm_of(base + pl.g, w_of(p, pl, pc, base),
-                   whole ? d.dx : base + pl.planes + (uint64_t)plane * d.rows * d.hidden * 4, d.rows, d.hidden, pc.cols,
-                   ld_of_g(pl, pc), ldw_of(p, pl, pc), whole ? d.lddx : d.hidden,
+                   whole ? d.dx : base + pl.planes + (uint64_t)plane * d.rows * pl.ldp * 4, pl.pair ? 2 * d.rows : d.rows,
+                   d.hidden, pc.cols, ld_of_g(pl, pc), ldw_of(p, pl, pc), whole ? d.lddx : pl.ldp,
                    d.transpose == T0G_NT ? T0G_NN : T0G_NT, whole ? d.dx_dtype : (uint32_t)T0G_F32);
 }
 
 t0g_gemm_desc dw_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
     const t0g_linear_ce_desc &d = p.d;
     const uint64_t c = weight_piece(p, d.dw, pc.v0, d.lddw, dtype_size(d.dw_dtype));
-    const uint32_t ldg = ld_of_g(pl, pc);
+    const uint32_t ldg = ld_of_g(pl, pc), rows = pl.pair ? 2 * d.rows : d.rows;
     return d.transpose == T0G_NT
-               ? gemm_of(base + pl.g, base + pl.xz, c, pc.cols, d.hidden, d.rows, ldg, pl.ldxz, d.lddw, T0G_TN, d.dw_dtype)
-               : gemm_of(base + pl.xz, base + pl.g, c, d.hidden, pc.cols, d.rows, pl.ldxz, ldg, d.lddw, T0G_TN, d.dw_dtype);
+               ? gemm_of(base + pl.g, base + pl.xz, c, pc.cols, d.hidden, rows, ldg, pl.ldxz, d.lddw, T0G_TN, d.dw_dtype)
+               : gemm_of(base + pl.xz, base + pl.g, c, d.hidden, pc.cols, rows, pl.ldxz, ldg, d.lddw, T0G_TN, d.dw_dtype);
 }
 
 int make_loss_plan(const Problem &p, Plan *pl) {
@@ -228,14 +238,19 @@ int make_loss_plan(const Problem &p, Plan *pl) {
     const bool x_aligned = (d.x & 15) == 0 && d.ldx % 8 == 0 && d.hidden % 8 == 0;
     pl->copy_w = !aligned && d.rows >= kCopyRows;
     pl->padded = aligned || pl->copy_w;
-    pl->copy_x = p.grad || (pl->padded && !x_aligned);
+    // xz is dW's operand; the logits' only where x itself is not aligned like the weight, or
+    // where ignored rows must not reach the entries (fused, and with a teacher)
     pl->ldxz = round_up(d.hidden, 8);
+    pl->copy_x = pl->padded && !x_aligned;
+    if (p.grad && (d.rows >= kFusedRows || p.t)) pl->copy_x = true;
     // the 256x256 tile takes 32-bit byte offsets, and rows of 256 or more of a weight
     // [hidden][vocab] (a copied piece has them)
     const uint64_t ldx = pl->copy_x ? pl->ldxz : d.ldx, ldw = pl->copy_w ? pl->ldxz : d.ldw;
     pl->fused = d.rows >= kFusedRows && pl->padded && d.rows * ldx < (1ull << 30) &&
                 (d.max_piece == 0 || d.max_piece >= 256) &&
                 (nt ? ldw * 256 < (1ull << 30) : pl->copy_w || (d.ldw >= 256 && d.hidden * ldw < (1ull << 30)));
+    pl->direct = !pl->fused && !p.t && !pl->copy_x;
+    pl->pair = !pl->fused && p.grad && d.rows <= kPairRows;
     const uint32_t chunk = pl->fused ? T0G_LOSS_BLOCK : T0G_LOSS_CHUNK;
     uint64_t width = d.vocab;
     if (!pl->fused)
@@ -260,8 +275,11 @@ int make_loss_plan(const Problem &p, Plan *pl) {
         v0 += cols;
     }
     pl->slots = 1 + (p.t ? p.t->top_k : 0);
-    const uint64_t plane = rows * d.hidden * 4;
-    if (d.dx && pl->pieces.size() > 1)
+    pl->ldp = round_up(d.hidden, 4);
+    const uint64_t plane = rows * pl->ldp * 4;
+    if (pl->pair)
+        pl->group = d.dx ? 1 : 0;
+    else if (d.dx && pl->pieces.size() > 1)
         pl->group = (uint32_t)std::min<uint64_t>(pl->pieces.size(), std::max<uint64_t>(1, kPlaneBytes / plane));
 
     uint64_t at = 0;
@@ -272,7 +290,8 @@ int make_loss_plan(const Problem &p, Plan *pl) {
     };
     uint32_t widest = 0;
     for (const Piece &pc : pl->pieces) widest = std::max(widest, pc.cols);
-    if (pl->copy_x) pl->xz = take(rows * pl->ldxz * 2);
+    const uint64_t halves = pl->pair ? 2 : 1;
+    if (pl->copy_x || p.grad) pl->xz = take(halves * rows * pl->ldxz * 2);
     if (pl->copy_w) {
         const Piece wide = {0, widest, 0, 0};
         pl->w = take((uint64_t)ldw_of(p, *pl, wide) * (nt ? widest : d.hidden) * 2);
@@ -293,10 +312,18 @@ int make_loss_plan(const Problem &p, Plan *pl) {
         if (p.grad) pl->g = take((uint64_t)round_up(d.rows, 256) * round_up(widest, 256) * 2);
     } else {
         pl->z = take(rows * round_up(widest, 4) * 4);
-        if (p.grad) pl->g = take(rows * round_up(widest, 8) * 2);
+        if (p.grad) pl->g = take(halves * rows * round_up(widest, 8) * 2);
     }
     if (pl->group) {
-        pl->planes = take(pl->group * plane);
+        uint32_t splits = 1;
+        if (pl->pair)
+            for (const Piece &pc : pl->pieces) {
+                const t0g_gemm_desc g = dx_gemm(p, *pl, pc, 0, 0);
+                int rc = losses_gemm_planes_count(&g, pl->padded, &splits);
+                if (rc) return rc;
+                pl->splits = std::max(pl->splits, splits);
+            }
+        pl->planes = take(pl->group * halves * pl->splits * plane);
         if (pl->group < pl->pieces.size()) pl->acc = take(plane);
     }
     // one split-K workspace for all products, which run one after another
@@ -304,7 +331,7 @@ int make_loss_plan(const Problem &p, Plan *pl) {
         t0g_gemm_desc g[3];
         int n = 0, rc;
         if (!pl->fused) g[n++] = logits_gemm(p, *pl, pc, 0);
-        if (d.dx) g[n++] = dx_gemm(p, *pl, pc, 0, 0);
+        if (d.dx && !pl->pair) g[n++] = dx_gemm(p, *pl, pc, 0, 0);
         if (d.dw) g[n++] = dw_gemm(p, *pl, pc, 0);
         for (int i = 0; i < n; ++i) {
             size_t bytes = 0;
@@ -396,7 +423,7 @@ int run_loss(t0g_device *dev, const Problem &p) {
     T0gLossArgs a;
     memset(&a, 0, sizeof a);
     a.x = d.x;
-    a.xz = pl.copy_x ? base + pl.xz : 0;
+    a.xz = pl.copy_x || p.grad ? base + pl.xz : 0;
     a.labels = d.labels;
     a.dloss = d.dloss;
     a.loss = d.loss;
@@ -437,6 +464,9 @@ int run_loss(t0g_device *dev, const Problem &p) {
         if (p.t->teacher_dtype == T0G_BF16) a.flags |= T0G_LOSS_TEACHER16;
     }
     if (p.dual) a.flags |= T0G_LOSS_DUAL;
+    if (pl.direct) a.flags |= T0G_LOSS_DIRECT;
+    if (pl.pair) a.flags |= T0G_LOSS_PAIR;
+    a.chunks = pl.chunks;
     // with both softmaxes the first is the labels', else the only one
     const double k = (double)d.logit_scale * 1.4426950408889634;
     a.k = (float)(p.dual || !p.t ? k : k / p.t->temperature);
@@ -452,27 +482,30 @@ int run_loss(t0g_device *dev, const Problem &p) {
         a.ldz = round_up(pc.cols, 4);
         a.ldg = ld_of_g(pl, pc);
         a.chunk0 = pc.chunk0;
-        a.chunks = pc.chunks;
     };
     auto piece_kernel = [&](const char *symbol, uint32_t groups) {
         return losses_launch(dev, symbol, groups, std::min(d.rows, kMaxGridY), &a, sizeof a);
     };
     const size_t n = pl.pieces.size();
-    if ((rc = row_kernel("t0g_loss_prepare", 1))) return rc;
+    const bool one = !pl.fused && pl.chunks == 1;   // by rows: the last kernel takes the statistics too
+    if (!pl.direct && (rc = row_kernel("t0g_loss_prepare", 1))) return rc;
     for (size_t i = 0; i < n; ++i) {
         const Piece &pc = pl.pieces[i];
         at_piece(pc);
         if (pl.copy_w && (rc = run_copy(dev, p, pl, pc, base))) return rc;
         if (pl.fused)
             rc = run_tile(dev, p.grad && i + 1 == n ? Tile::Keep : Tile::Stats, p, pl, pc, a, base);
-        else if (!(rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base)))
+        else if (!(rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base)) && !one)
             rc = piece_kernel("t0g_loss_stats", pc.chunks);
         if (rc) return rc;
     }
-    a.chunks = pl.chunks;
-    // 16 rows read a chunk's statistics as one line; fewer where that leaves CUs idle
-    while (a.row_shift < 4 && d.rows >> (a.row_shift + 1) >= 2 * kNumCUs) ++a.row_shift;
-    if ((rc = row_kernel("t0g_loss_combine", 1u << a.row_shift))) return rc;
+    if (pl.fused || (!p.grad && !one)) {
+        // 16 rows read a chunk's statistics as one line; fewer where that leaves CUs idle
+        while (a.row_shift < 4 && d.rows >> (a.row_shift + 1) >= 2 * kNumCUs) ++a.row_shift;
+        if ((rc = row_kernel("t0g_loss_combine", 1u << a.row_shift))) return rc;
+    } else if (!p.grad) {
+        if ((rc = piece_kernel("t0g_loss_grad", 1))) return rc;
+    }
     if (!p.grad) return ok();
 
     T0gLossSumArgs s;
@@ -480,6 +513,7 @@ int run_loss(t0g_device *dev, const Problem &p) {
     s.planes = base + pl.planes;
     s.rows = d.rows;
     s.cols = d.hidden;
+    s.ldp = pl.ldp;
     uint32_t planes = 0;
     for (size_t i = n; i-- > 0;) {
         const Piece &pc = pl.pieces[i];
@@ -495,17 +529,24 @@ int run_loss(t0g_device *dev, const Problem &p) {
         }
         if (rc || (d.dw && (rc = run_gemm(dev, dw_gemm(p, pl, pc, base), pl, base)))) return rc;
         if (!d.dx) continue;
-        if ((rc = run_gemm(dev, dx_gemm(p, pl, pc, base, planes), pl, base))) return rc;
+        const t0g_gemm_desc dx = dx_gemm(p, pl, pc, base, planes);
+        uint32_t splits = 1;
+        if (pl.pair) {
+            if ((rc = losses_gemm_planes_count(&dx, pl.padded, &splits)) || (rc = losses_gemm_planes(dev, &dx, pl.padded)))
+                return rc;
+        } else if ((rc = run_gemm(dev, dx, pl, base))) {
+            return rc;
+        }
         if (pl.group == 0) continue;
         if (++planes < pl.group && i > 0) continue;
         // the planes so far, onto those before
         const bool last = i == 0;
-        s.n = planes;
+        s.n = pl.pair ? 2 * splits : planes;
         s.out = last ? d.dx : base + pl.acc;
-        s.ldo = last ? d.lddx : d.hidden;
+        s.ldo = last ? d.lddx : pl.ldp;
         s.out_bf16 = last && d.dx_dtype == T0G_BF16;
         s.vec = d.hidden % 4 == 0 && s.ldo % 4 == 0 && s.out % 16 == 0;
-        const uint64_t items = (uint64_t)d.rows * d.hidden / (s.vec ? 4 : 1);
+        const uint64_t items = (uint64_t)d.rows * (d.hidden / (s.vec ? 4 : 1));
         const uint32_t groups = (uint32_t)std::min<uint64_t>((items + 255) / 256, 1u << 16);
         if ((rc = losses_launch(dev, "t0g_loss_sum", groups, 1, &s, sizeof s))) return rc;
         s.acc = base + pl.acc;

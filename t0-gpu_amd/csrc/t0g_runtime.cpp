@@ -1821,6 +1821,37 @@ int losses_gemm_workspace(const t0g_gemm_desc *d, bool padded, size_t *bytes) {
 
 int losses_gemm(t0g_device *dev, const t0g_gemm_desc *d, bool padded) { return gemm_locked(dev, d, true, padded); }
 
+// The data-parallel plan of a product with f32 output whose planes stay apart.
+static int planes_plan(const t0g_gemm_desc *d, bool padded, GemmPlan *p, GemmOperands *o) {
+    t0g_gemm_config cfg;
+    int rc = resolve_desc(d, &cfg, p, o, false, padded);
+    if (rc || !p->stream_k) return rc ? rc : check_grid(*p);
+    t0g_gemm_config dp = cfg;
+    dp.split_k = 0;
+    t0g_gemm_desc d2 = *d;
+    d2.config = &dp;
+    d2.split_k = 1;
+    if ((rc = resolve_desc(&d2, &cfg, p, o, false, padded))) return rc;
+    return check_grid(*p);
+}
+
+int losses_gemm_planes_count(const t0g_gemm_desc *d, bool padded, uint32_t *planes) {
+    GemmPlan p;
+    GemmOperands o;
+    int rc = planes_plan(d, padded, &p, &o);
+    if (!rc) *planes = p.splits;
+    return rc;
+}
+
+int losses_gemm_planes(t0g_device *dev, const t0g_gemm_desc *d, bool padded) {
+    GemmPlan p;
+    GemmOperands o;
+    int rc = planes_plan(d, padded, &p, &o);
+    if (rc) return rc;
+    o.c_split_stride = (uint64_t)d->m * o.ldc * 4;
+    return run_plan(dev, p, o, 0);
+}
+
 // Device time of `iters` back-to-back t0g_gemm launches of d (after `warmup`
 // untimed ones): one HIP event between consecutive launches on the device
 // stream, so each duration covers one whole GEMM (partials and reduce).
