@@ -38,18 +38,26 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
-// Over the workgroup's four waves; `t` is 4 floats of LDS of this call's own.
+// Over the workgroup's W waves; `t` is W floats of LDS of this call's own.
+template <int W = 4>
 __device__ __forceinline__ float block_max(float v, float* t) {
     v = wave_max(v);
     if ((threadIdx.x & 63u) == 0) t[threadIdx.x >> 6] = v;
     __syncthreads();
-    return __builtin_fmaxf(__builtin_fmaxf(t[0], t[1]), __builtin_fmaxf(t[2], t[3]));
+    v = t[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) v = __builtin_fmaxf(v, t[w]);
+    return v;
 }
+template <int W = 4>
 __device__ __forceinline__ float block_sum(float v, float* t) {
     v = wave_sum(v);
     if ((threadIdx.x & 63u) == 0) t[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (t[0] + t[1]) + (t[2] + t[3]);
+    v = t[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) v += t[w];
+    return v;
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -75,14 +83,14 @@ __device__ __forceinline__ void copy_row(const T0gLossArgs& p, uint32_t row, boo
     const bool pair = p.flags & T0G_LOSS_PAIR;
     if (p.flags & T0G_LOSS_X_VEC) {
         const uint32_t n = p.hidden / 8;
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+        for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
             u32x4_t v = {0u, 0u, 0u, 0u};
             if (used) v = *at<const u32x4_t>(p.x + (uint64_t)row * p.ldx * 2, i);
             *at<u32x4_t>(to, i) = v;
             if (pair) *at<u32x4_t>(again, i) = v;
         }
     } else {
-        for (uint32_t i = threadIdx.x; i < p.ldxz; i += kThreads) {
+        for (uint32_t i = threadIdx.x; i < p.ldxz; i += blockDim.x) {
             uint16_t v = 0;
             if (used && i < p.hidden) v = *at<const uint16_t>(p.x, (uint64_t)row * p.ldx + i);
             *at<uint16_t>(to, i) = v;
@@ -119,6 +127,10 @@ __device__ __forceinline__ uint32_t entry_token(const T0gLossArgs& p, uint32_t r
 }
 __device__ __forceinline__ float entry_q(const T0gLossArgs& p, uint32_t row, uint32_t e) {
     return (p.flags & T0G_LOSS_DIRECT) ? 0.0f : *at<const float>(p.ent_q, (uint64_t)row * p.slots + e);
+}
+__device__ __forceinline__ float entry_z(const T0gLossArgs& p, uint32_t row, uint32_t e) {
+    return (p.flags & T0G_LOSS_Z) ? *at<const float>(p.z, (uint64_t)row * p.ldz + entry_token(p, row, e))
+                                  : *at<const float>(p.ent_z, (uint64_t)row * p.slots + e);
 }
 // l0, l1, c0, c1 of a row's gradient.
 __device__ __forceinline__ f32x4_t row_params(const T0gLossArgs& p, const RowInfo& r, float l0, float l1) {
@@ -252,38 +264,41 @@ __device__ __forceinline__ void prepare_row(const T0gLossArgs& p, uint32_t row) 
     __syncthreads();
 }
 
-// One chunk of a row of raw logits in registers, times k, -inf past its end.
-__device__ __forceinline__ void load_chunk(const T0gLossArgs& p, uint64_t base, uint32_t n, f32x4_t (&v)[4]) {
+// n consecutive raw logits of a row in registers, N quads a thread of a workgroup of W
+// waves, times k, -inf past the end; and their statistics.
+template <int N, int W>
+__device__ __forceinline__ void load_logits(const T0gLossArgs& p, uint64_t base, uint32_t n, f32x4_t (&v)[N]) {
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t c = (i * kThreads + threadIdx.x) * 4;
+    for (uint32_t i = 0; i < N; ++i) {
+        const uint32_t c = (i * (64 * W) + threadIdx.x) * 4;
         v[i] = f32x4_t{ninf(), ninf(), ninf(), ninf()};
-        if (c < n) {   // rows are padded to whole quads
-            v[i] = *at<const f32x4_t>(base, c / 4);
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) v[i][e] = c + e < n ? v[i][e] * p.k : ninf();
-        }
+        if (c < n) v[i] = *at<const f32x4_t>(base, c / 4);   // rows are padded to whole quads
     }
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) v[i][e] = (i * (64 * W) + threadIdx.x) * 4 + e < n ? v[i][e] * p.k : ninf();
 }
-__device__ __forceinline__ void reduce_chunk(const T0gLossArgs& p, const f32x4_t (&v)[4], uint32_t n, float (&red)[3][4],
-                                             float& m, float& s, float& s2) {
+template <int N, int W>
+__device__ __forceinline__ void reduce_logits(const T0gLossArgs& p, const f32x4_t (&v)[N], uint32_t n, float (&red)[3][W],
+                                              float& m, float& s, float& s2) {
     m = ninf();
     s = s2 = 0.0f;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
+    for (uint32_t i = 0; i < N; ++i)
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) m = __builtin_fmaxf(m, v[i][e]);
-    m = block_max(m, red[0]);
+    m = block_max<W>(m, red[0]);
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
+    for (uint32_t i = 0; i < N; ++i)
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) {
-            if ((i * kThreads + threadIdx.x) * 4 + e >= n) continue;
+            if ((i * (64 * W) + threadIdx.x) * 4 + e >= n) continue;
             s += exp2_(v[i][e] - m);
             if (p.flags & T0G_LOSS_DUAL) s2 += exp2_((v[i][e] - m) * p.r);
         }
-    s = block_sum(s, red[1]);
-    if (p.flags & T0G_LOSS_DUAL) s2 = block_sum(s2, red[2]);
+    s = block_sum<W>(s, red[1]);
+    if (p.flags & T0G_LOSS_DUAL) s2 = block_sum<W>(s2, red[2]);
 }
 
 // Statistics of one chunk of a row of raw logits, and the raw logits of the row's
@@ -295,19 +310,22 @@ __device__ __forceinline__ void chunk_stats(const T0gLossArgs& p, uint32_t row, 
     const uint32_t n = min(T0G_LOSS_CHUNK, p.cols - c0);
     f32x4_t v[4];
     float m, s, s2;
-    load_chunk(p, base, n, v);
-    reduce_chunk(p, v, n, red, m, s, s2);
+    load_logits<4, 4>(p, base, n, v);
+    reduce_logits<4, 4>(p, v, n, red, m, s, s2);
     if (tid == 0) {
         const uint64_t i = (uint64_t)(p.chunk0 + chunk) * p.rows + row;
         *at<f32x2_t>(p.part, i) = f32x2_t{m, s};
         if (p.flags & T0G_LOSS_DUAL) *at<float>(p.part2, i) = s2;
     }
-    const RowInfo r = row_info(p, row);
-    for (uint32_t e = tid; e < r.entries; e += kThreads) {
-        const uint32_t c = entry_token(p, row, e) - (p.v0 + c0);   // wraps below the chunk
-        if (c < n) *at<float>(p.ent_z, (uint64_t)row * p.slots + e) = *at<const float>(base, c);
+    if (!(p.flags & T0G_LOSS_Z)) {
+        const RowInfo r = row_info(p, row);
+        for (uint32_t e = tid; e < r.entries; e += kThreads) {
+            const uint32_t c = entry_token(p, row, e) - (p.v0 + c0);   // wraps below the chunk
+            if (c < n) *at<float>(p.ent_z, (uint64_t)row * p.slots + e) = *at<const float>(base, c);
+        }
+        // before the first product with G (of a single piece, the gradient kernel does it)
+        if ((p.flags & T0G_LOSS_DIRECT) && p.xz && p.v0 == 0 && chunk == 0) copy_row(p, row, r.used());
     }
-    if ((p.flags & T0G_LOSS_DIRECT) && p.xz && p.v0 == 0 && chunk == 0) copy_row(p, row, r.used());
     __syncthreads();
 }
 
@@ -366,11 +384,11 @@ __device__ __forceinline__ void combine_rows(const T0gLossArgs& p, uint32_t row0
     if (p.teacher) {
         if (r.taught)
             for (uint32_t e = part; e < r.entries; e += per)
-                kd += entry_kd(p, entry_q(p, row, e), *at<const float>(p.ent_z, (uint64_t)row * p.slots + e), l1);
+                kd += entry_kd(p, entry_q(p, row, e), entry_z(p, row, e), l1);
         kd = join(t1, kd, false);
     }
     if (part == 0 && live) {
-        const float zl = r.labelled() ? *at<const float>(p.ent_z, (uint64_t)row * p.slots + r.label) : 0.0f;
+        const float zl = r.labelled() ? entry_z(p, row, r.label) : 0.0f;
         store_loss(p, row, r, l0, l1, zl, kd);
         if (p.row_par) *at<f32x4_t>(p.row_par, row) = row_params(p, r, l0, l1);
     }
@@ -398,7 +416,7 @@ __device__ __forceinline__ void entry_grads(const T0gLossArgs& p, uint32_t row, 
     for (uint32_t e = first; e < r.entries; e += step) {
         const uint32_t c = entry_token(p, row, e) - (p.v0 + c0);   // wraps below the range
         if (c >= n) continue;
-        const float g = entry_grad(p, r, par, row, e, *at<const float>(p.ent_z, (uint64_t)row * p.slots + e));
+        const float g = entry_grad(p, r, par, row, e, entry_z(p, row, e));
         const uint64_t o = (uint64_t)row * p.ldg + c0 + c;
         const __bf16 h = (__bf16)g;
         *at<__bf16>(p.g, o) = h;
@@ -406,69 +424,83 @@ __device__ __forceinline__ void entry_grads(const T0gLossArgs& p, uint32_t row, 
     }
 }
 
-// One chunk of a row of raw logits, by rows: the row's statistics (its own where the
-// vocabulary is one chunk), its loss (the first chunk), and the chunk's logit gradients
-// in bf16, zero past the piece, then its entries.
+// The loss of a row whose statistics are known, by the whole workgroup of W waves.
+template <int W>
+__device__ __forceinline__ void finish_row(const T0gLossArgs& p, const RowInfo& r, uint32_t row, float l0, float l1,
+                                           float* red) {
+    float kd = 0.0f;
+    if (p.teacher) {
+        if (r.taught)
+            for (uint32_t e = threadIdx.x; e < r.entries; e += 64 * W)
+                kd += entry_kd(p, entry_q(p, row, e), entry_z(p, row, e), l1);
+        kd = block_sum<W>(kd, red);
+    }
+    if (threadIdx.x == 0) store_loss(p, row, r, l0, l1, r.labelled() ? entry_z(p, row, r.label) : 0.0f, kd);
+    if ((p.flags & T0G_LOSS_DIRECT) && (p.flags & T0G_LOSS_Z) && p.xz) copy_row(p, row, r.used());
+}
+
+// Logit gradients of columns [c0, c0 + n) of a row in bf16, zero up to ng, then its entries.
+template <int N, int W>
+__device__ __forceinline__ void write_grads(const T0gLossArgs& p, const RowInfo& r, uint32_t row, const f32x4_t& par,
+                                            const f32x4_t (&v)[N], uint32_t c0, uint32_t n, uint32_t ng) {
+    const bool used = par[2] != 0.0f || par[3] != 0.0f;
+    const uint64_t gb = p.g + ((uint64_t)row * p.ldg + c0) * 2;
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+        const uint32_t c = (i * (64 * W) + threadIdx.x) * 4;
+        if (c >= ng) continue;
+        float g[4];
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) g[e] = used && c + e < n ? dense_grad(p, par, v[i][e]) : 0.0f;
+        *at<u32x2_t>(gb, c / 4) = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
+        if (p.flags & T0G_LOSS_PAIR) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) g[e] -= (float)(__bf16)g[e];
+            *at<u32x2_t>(gb + (uint64_t)p.rows * p.ldg * 2, c / 4) = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
+        }
+    }
+    __syncthreads();   // the dense part is written before its entries are replaced
+    if (used) entry_grads(p, row, c0, n, par, threadIdx.x, 64 * W);
+}
+
+// One chunk of a row, by rows: the row's statistics from the chunks', its loss (the first
+// chunk), and the chunk's logit gradients.
 __device__ __forceinline__ void chunk_grad(const T0gLossArgs& p, uint32_t row, uint32_t chunk) {
-    __shared__ float red[4][4], own[3][4];
-    const uint32_t c0 = chunk * T0G_LOSS_CHUNK, tid = threadIdx.x;
-    const uint64_t zb = p.z + ((uint64_t)row * p.ldz + c0) * 4;
+    __shared__ float red[4][4];
+    const uint32_t c0 = chunk * T0G_LOSS_CHUNK;
     const uint32_t n = min(T0G_LOSS_CHUNK, p.cols - c0);
-    const bool one = p.chunks == 1, dual = p.flags & T0G_LOSS_DUAL;
+    const bool dual = p.flags & T0G_LOSS_DUAL;
     const RowInfo r = row_info(p, row);
     f32x4_t v[4];
     float m, s, s2;
-    load_chunk(p, zb, n, v);
-    if (one) {
-        reduce_chunk(p, v, n, own, m, s, s2);
-    } else {
-        join_chunks(p, row, tid, kThreads, m, s, s2);
-        const float top = block_max(m, red[0]);
-        s = block_sum(s * (m == top ? 1.0f : exp2_(m - top)), red[1]);
-        if (dual) s2 = block_sum(s2 * (m == top ? 1.0f : exp2_((m - top) * p.r)), red[2]);
-        m = top;
-    }
-    const float l0 = m + __builtin_amdgcn_logf(s), l1 = dual ? m * p.r + __builtin_amdgcn_logf(s2) : l0;
-    if (one)   // the entries' logits are all here
-        for (uint32_t e = tid; e < r.entries; e += kThreads)
-            *at<float>(p.ent_z, (uint64_t)row * p.slots + e) = *at<const float>(zb, entry_token(p, row, e));
-    if (p.v0 == 0 && chunk == 0) {
-        float kd = 0.0f;
-        if (r.taught)   // each thread reads what it wrote itself
-            for (uint32_t e = tid; e < r.entries; e += kThreads)
-                kd += entry_kd(p, entry_q(p, row, e), *at<const float>(p.ent_z, (uint64_t)row * p.slots + e), l1);
-        if (p.teacher) kd = block_sum(kd, red[3]);
-        if (tid == 0) {
-            float zl = 0.0f;
-            if (r.labelled())
-                zl = one ? *at<const float>(zb, entry_token(p, row, r.label))
-                         : *at<const float>(p.ent_z, (uint64_t)row * p.slots + r.label);
-            store_loss(p, row, r, l0, l1, zl, kd);
-        }
-        if (one && (p.flags & T0G_LOSS_DIRECT) && p.xz) copy_row(p, row, r.used());
-    }
-    if (p.g) {
-        const f32x4_t par = row_params(p, r, l0, l1);
-        const bool used = par[2] != 0.0f || par[3] != 0.0f;
-        const uint32_t ng = min(T0G_LOSS_CHUNK, p.ldg - c0);
-        const uint64_t gb = p.g + ((uint64_t)row * p.ldg + c0) * 2;
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t c = (i * kThreads + tid) * 4;
-            if (c >= ng) continue;
-            float g[4];
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) g[e] = used && c + e < n ? dense_grad(p, par, v[i][e]) : 0.0f;
-            *at<u32x2_t>(gb, c / 4) = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
-            if (p.flags & T0G_LOSS_PAIR) {
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) g[e] -= (float)(__bf16)g[e];
-                *at<u32x2_t>(gb + (uint64_t)p.rows * p.ldg * 2, c / 4) = u32x2_t{pack2(g[0], g[1]), pack2(g[2], g[3])};
-            }
-        }
-        __syncthreads();   // the dense part is written before its entries are replaced
-        if (used) entry_grads(p, row, c0, n, par, tid, kThreads);
-    }
+    load_logits<4, 4>(p, p.z + ((uint64_t)row * p.ldz + c0) * 4, n, v);
+    join_chunks(p, row, threadIdx.x, kThreads, m, s, s2);
+    const float top = block_max(m, red[0]);
+    s = block_sum(s * (m == top ? 1.0f : exp2_(m - top)), red[1]);
+    if (dual) s2 = block_sum(s2 * (m == top ? 1.0f : exp2_((m - top) * p.r)), red[2]);
+    const float l0 = top + __builtin_amdgcn_logf(s), l1 = dual ? top * p.r + __builtin_amdgcn_logf(s2) : l0;
+    if (p.v0 == 0 && chunk == 0) finish_row<4>(p, r, row, l0, l1, red[3]);
+    write_grads<4, 4>(p, r, row, row_params(p, r, l0, l1), v, c0, n, min(T0G_LOSS_CHUNK, p.ldg - c0));
+    __syncthreads();
+}
+
+// A whole row of up to 4096 N raw logits in the registers of one workgroup: statistics, loss
+// and, if wanted, logit gradients.  Chunks with their joining in a second kernel, and this, per
+// call: loss alone, 16 rows over 1000 tokens of width 256 12.1 / 8.2 us, over 8000 of 512 13.3 /
+// 10.9, with gradients 31.8 / 28.8; at 32000 tokens (8 quads) they are level, and 16 quads spill.
+template <int N>
+__device__ __forceinline__ void whole_row(const T0gLossArgs& p, uint32_t row) {
+    constexpr int W = 16;
+    __shared__ float red[3][W], last[W];
+    const RowInfo r = row_info(p, row);
+    f32x4_t v[N];
+    float m, s, s2;
+    load_logits<N, W>(p, p.z + (uint64_t)row * p.ldz * 4, p.cols, v);
+    reduce_logits<N, W>(p, v, p.cols, red, m, s, s2);
+    const float l0 = m + __builtin_amdgcn_logf(s);
+    const float l1 = (p.flags & T0G_LOSS_DUAL) ? m * p.r + __builtin_amdgcn_logf(s2) : l0;
+    finish_row<W>(p, r, row, l0, l1, last);
+    if (p.g) write_grads<N, W>(p, r, row, row_params(p, r, l0, l1), v, 0, p.cols, p.ldg);
     __syncthreads();
 }
 
@@ -579,6 +611,12 @@ extern "C" __global__ void __launch_bounds__(256) t0g_loss_combine(T0gLossArgs p
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_grad(T0gLossArgs p) {
     for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) t0g::chunk_grad(p, row, blockIdx.x);
 }
+#define T0G_LOSS_ROW(N)                                                                             \
+    extern "C" __global__ void __launch_bounds__(1024) t0g_loss_row_##N(T0gLossArgs p) {            \
+        for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) t0g::whole_row<N>(p, row);  \
+    }
+T0G_LOSS_ROW(1)
+T0G_LOSS_ROW(4)
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_grad_kept(T0gLossArgs p) {
     for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) t0g::kept_grad(p, row, blockIdx.x);
 }

@@ -84,7 +84,8 @@ std::mutex &device_mutex(t0g_device *dev);
 // that would need it is refused.
 int losses_begin(t0g_device *dev, size_t bytes, uint64_t *scratch);
 // Launch kernel `symbol` of the losses' code object on the device stream.
-int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, void *args, size_t args_size);
+int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, void *args, size_t args_size,
+                  uint32_t threads = 256);
 // Workspace t0g_gemm may use for d (host only), and the GEMM itself.  padded: the operands' rows
 // hold whole 16-byte pieces, zeros past the sizes, which then need not be multiples of 8.
 int losses_gemm_workspace(const t0g_gemm_desc *d, bool padded, size_t *bytes);

@@ -14,8 +14,8 @@
 //             the other pieces' logits are computed again with G in the epilogue
 //   by rows   a piece's f32 logits go to the scratch and row kernels read them: products
 //             of few rows, and operands that the 256x256 tile does not take
-// By rows, labels alone need no preparation (each kernel reads them), and a vocabulary of
-// one chunk takes its statistics, loss and G in one kernel.
+// By rows, labels alone need no preparation (each kernel reads them), and a vocabulary that
+// one workgroup's registers hold takes its statistics, loss and G in one kernel.
 // A weight whose rows are not whole 16-byte pieces is copied into ones that are, piece by
 // piece, when there are rows enough to make up for that.
 #include <math.h>
@@ -41,6 +41,8 @@ constexpr uint64_t kFusedPieceBytes = 2048ull << 20;
 constexpr uint64_t kPlaneBytes = 128ull << 20;
 // Rows from which the fused form is taken.
 constexpr uint32_t kFusedRows = 256;
+// Quads a thread of the whole rows' kernels holds at most (16384 logits of a row).
+constexpr uint32_t kRowQuads = 4;
 // Rows up to which G goes into the products as two bf16, the rounded value and what the
 // rounding left: few rows' roundings do not average out (one row's dx has the label's
 // whole, up to 2^-8), and what bounds their products is the weight's bytes.
@@ -466,6 +468,7 @@ int run_loss(t0g_device *dev, const Problem &p) {
     if (p.dual) a.flags |= T0G_LOSS_DUAL;
     if (pl.direct) a.flags |= T0G_LOSS_DIRECT;
     if (pl.pair) a.flags |= T0G_LOSS_PAIR;
+    if (!pl.fused && pl.pieces.size() == 1) a.flags |= T0G_LOSS_Z;
     a.chunks = pl.chunks;
     // with both softmaxes the first is the labels', else the only one
     const double k = (double)d.logit_scale * 1.4426950408889634;
@@ -487,7 +490,12 @@ int run_loss(t0g_device *dev, const Problem &p) {
         return losses_launch(dev, symbol, groups, std::min(d.rows, kMaxGridY), &a, sizeof a);
     };
     const size_t n = pl.pieces.size();
-    const bool one = !pl.fused && pl.chunks == 1;   // by rows: the last kernel takes the statistics too
+    // by rows: one kernel for all of a row that fits a workgroup's registers
+    const uint32_t quads = (d.vocab + T0G_LOSS_ROW_QUADS - 1) / T0G_LOSS_ROW_QUADS;
+    const bool one = !pl.fused && n == 1 && quads <= kRowQuads;
+    auto whole_rows = [&] {
+        return losses_launch(dev, quads <= 1 ? "t0g_loss_row_1" : "t0g_loss_row_4", std::min<uint32_t>(d.rows, 1u << 20), 1, &a, sizeof a, 1024);
+    };
     if (!pl.direct && (rc = row_kernel("t0g_loss_prepare", 1))) return rc;
     for (size_t i = 0; i < n; ++i) {
         const Piece &pc = pl.pieces[i];
@@ -504,7 +512,7 @@ int run_loss(t0g_device *dev, const Problem &p) {
         while (a.row_shift < 4 && d.rows >> (a.row_shift + 1) >= 2 * kNumCUs) ++a.row_shift;
         if ((rc = row_kernel("t0g_loss_combine", 1u << a.row_shift))) return rc;
     } else if (!p.grad) {
-        if ((rc = piece_kernel("t0g_loss_grad", 1))) return rc;
+        if ((rc = whole_rows())) return rc;
     }
     if (!p.grad) return ok();
 
@@ -523,9 +531,11 @@ int run_loss(t0g_device *dev, const Problem &p) {
             rc = piece_kernel("t0g_loss_grad_kept", (a.ldg + 2047) / 2048);
         } else if (pl.fused) {
             if (!(rc = run_tile(dev, Tile::Grad, p, pl, pc, a, base))) rc = row_kernel("t0g_loss_grad_entries", 4);
+        } else if (one) {
+            rc = whole_rows();
         } else {
             if (i + 1 == n || !(rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base)))
-                rc = piece_kernel("t0g_loss_grad", pc.chunks);
+                rc = piece_kernel("t0g_loss_grad", (pc.cols + T0G_LOSS_CHUNK - 1) / T0G_LOSS_CHUNK);
         }
         if (rc || (d.dw && (rc = run_gemm(dev, dw_gemm(p, pl, pc, base), pl, base)))) return rc;
         if (!d.dx) continue;

@@ -1798,7 +1798,8 @@ int losses_begin(t0g_device *dev, size_t bytes, uint64_t *scratch) {
     return T0G_OK;
 }
 
-int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, void *args, size_t args_size) {
+int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, void *args, size_t args_size,
+                  uint32_t threads) {
     auto it = dev->fns_loss.find(symbol);
     if (it == dev->fns_loss.end()) {
         hipFunction_t f = nullptr;
@@ -1806,7 +1807,7 @@ int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t
         if (e != hipSuccess) return hip_fail(e, symbol);
         it = dev->fns_loss.emplace(symbol, f).first;
     }
-    return launch(dev, it->second, grid_x, grid_y, 1, 256, args, args_size);
+    return launch(dev, it->second, grid_x, grid_y, 1, threads, args, args_size);
 }
 
 int losses_gemm_workspace(const t0g_gemm_desc *d, bool padded, size_t *bytes) {
