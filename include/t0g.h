@@ -556,6 +556,16 @@ T0G_API int t0g_linear_distill(t0g_device *dev, const t0g_linear_distill_desc *d
  * descriptor as the call does). */
 T0G_API int t0g_linear_cross_entropy_scratch_size(const t0g_linear_ce_desc *desc, size_t *bytes);
 T0G_API int t0g_linear_distill_scratch_size(const t0g_linear_distill_desc *desc, size_t *bytes);
+/* How the losses run: T0G_LOSS_FORM_AUTO (0, the default) by size; T0G_LOSS_FORM_ROWS (1) with
+ * a piece's f32 logits in the scratch and kernels over its rows; T0G_LOSS_FORM_FUSED (2)
+ * with the softmax in the logits GEMM's epilogue wherever the operands allow it.  The
+ * forms differ in the order of f32 sums and, with gradients of up to 128 rows, in G's
+ * rounding (by rows its remainder goes through the products too).  Process-wide, for
+ * later calls: for tests and measurements. */
+#define T0G_LOSS_FORM_AUTO 0u
+#define T0G_LOSS_FORM_ROWS 1u
+#define T0G_LOSS_FORM_FUSED 2u
+T0G_API int t0g_set_loss_form(uint32_t form);
 
 /* ---- GEMM autotuner and its on-disk cache ----------------------------------- *
  * GemmTuner (src/t0/auto_gemm.rs:28-417): benchmark the model's best candidate

@@ -484,13 +484,14 @@ __device__ __forceinline__ void chunk_grad(const T0gLossArgs& p, uint32_t row, u
     __syncthreads();
 }
 
-// A whole row of up to 4096 N raw logits in the registers of one workgroup: statistics, loss
+// A whole row of up to 256 N W raw logits in the registers of one workgroup of W waves: statistics, loss
 // and, if wanted, logit gradients.  Chunks with their joining in a second kernel, and this, per
 // call: loss alone, 16 rows over 1000 tokens of width 256 12.1 / 8.2 us, over 8000 of 512 13.3 /
-// 10.9, with gradients 31.8 / 28.8; at 32000 tokens (8 quads) they are level, and 16 quads spill.
-template <int N>
+// 10.9, with gradients 31.8 / 28.8; at 32000 tokens they were level.  Four waves serve
+// many rows better, sixteen a long row: 4096 rows over 1000 tokens with 16 and 4 waves
+// 60.8 / 25.0 us, over 8000 121 / 68; 64 rows over 16000 with gradients 36.4 / 40.1.
+template <int N, int W>
 __device__ __forceinline__ void whole_row(const T0gLossArgs& p, uint32_t row) {
-    constexpr int W = 16;
     __shared__ float red[3][W], last[W];
     const RowInfo r = row_info(p, row);
     f32x4_t v[N];
@@ -573,13 +574,13 @@ __device__ __forceinline__ void sum_planes(const T0gLossSumArgs& p) {
         if (p.vec) {
             f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
             if (p.acc) v = *at<const f32x4_t>(p.acc, q / 4);
-            for (uint32_t s0 = 0; s0 < p.n; s0 += 8) {   // eight planes' loads in flight
-                f32x4_t x[8];
+            for (uint32_t s0 = 0; s0 < p.n; s0 += 16) {   // sixteen planes' loads in flight
+                f32x4_t x[16];
 #pragma unroll
-                for (uint32_t s = 0; s < 8; ++s)
+                for (uint32_t s = 0; s < 16; ++s)
                     if (s0 + s < p.n) x[s] = *at<const f32x4_t>(p.planes + (s0 + s) * plane * 4, q / 4);
 #pragma unroll
-                for (uint32_t s = 0; s < 8; ++s)
+                for (uint32_t s = 0; s < 16; ++s)
                     if (s0 + s < p.n) v += x[s];
             }
             if (p.out_bf16)
@@ -588,7 +589,15 @@ __device__ __forceinline__ void sum_planes(const T0gLossSumArgs& p) {
                 *at<f32x4_t>(p.out, o / 4) = v;
         } else {
             float v = p.acc ? *at<const float>(p.acc, q) : 0.0f;
-            for (uint32_t s = 0; s < p.n; ++s) v += *at<const float>(p.planes, s * plane + q);
+            for (uint32_t s0 = 0; s0 < p.n; s0 += 16) {
+                float x[16];
+#pragma unroll
+                for (uint32_t s = 0; s < 16; ++s)
+                    if (s0 + s < p.n) x[s] = *at<const float>(p.planes, (s0 + s) * plane + q);
+#pragma unroll
+                for (uint32_t s = 0; s < 16; ++s)
+                    if (s0 + s < p.n) v += x[s];
+            }
             if (p.out_bf16)
                 *at<__bf16>(p.out, o) = (__bf16)v;
             else
@@ -611,12 +620,15 @@ extern "C" __global__ void __launch_bounds__(256) t0g_loss_combine(T0gLossArgs p
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_grad(T0gLossArgs p) {
     for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) t0g::chunk_grad(p, row, blockIdx.x);
 }
-#define T0G_LOSS_ROW(N)                                                                             \
-    extern "C" __global__ void __launch_bounds__(1024) t0g_loss_row_##N(T0gLossArgs p) {            \
-        for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) t0g::whole_row<N>(p, row);  \
+#define T0G_LOSS_ROW(N, W)                                                                             \
+    extern "C" __global__ void __launch_bounds__(64 * W) t0g_loss_row_##N##x##W(T0gLossArgs p) {       \
+        for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) t0g::whole_row<N, W>(p, row);  \
     }
-T0G_LOSS_ROW(1)
-T0G_LOSS_ROW(4)
+T0G_LOSS_ROW(1, 1)
+T0G_LOSS_ROW(1, 4)
+T0G_LOSS_ROW(4, 4)
+T0G_LOSS_ROW(8, 4)
+T0G_LOSS_ROW(4, 16)
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_grad_kept(T0gLossArgs p) {
     for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) t0g::kept_grad(p, row, blockIdx.x);
 }

@@ -205,7 +205,7 @@ typedef struct T0gLossArgs {
                                   first's rounding left, of xz the same copy again       */
 #define T0G_LOSS_Z 128u        /* z holds the whole vocabulary: entries' logits are read there */
 #define T0G_LOSS_CHUNK 4096u   /* columns of one workgroup in the row kernels          */
-#define T0G_LOSS_ROW_QUADS 4096u /* logits of one quad a thread of the whole rows' kernels */
+#define T0G_LOSS_ROW_MAX 16384u /* logits of a row that one workgroup holds, at most     */
 #define T0G_LOSS_MAX_TOP 1024u /* teacher entries of a row, at most                    */
 
 /* The 256x256 GEMM of a piece's logits with the softmax in its epilogue: statistics per

@@ -22,6 +22,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 #include <vector>
 
 #include "t0g.h"
@@ -39,10 +40,19 @@ namespace {
 constexpr uint64_t kPieceBytes = 256ull << 20;
 constexpr uint64_t kFusedPieceBytes = 2048ull << 20;
 constexpr uint64_t kPlaneBytes = 128ull << 20;
-// Rows from which the fused form is taken.
-constexpr uint32_t kFusedRows = 256;
-// Quads a thread of the whole rows' kernels holds at most (16384 logits of a row).
-constexpr uint32_t kRowQuads = 4;
+// The fused form is taken from kFusedRows rows (with gradients from more than kPairRows) and
+// this many logits on.  By rows and fused, us per call: loss alone of width 512, 512 rows
+// over 6000 tokens (3.1 M) 19 / 26, over 12000 (6.1 M) 28 / 26, 192 rows over 24000 (4.6 M) 27 / 25,
+// over 98304 79 / 44; width 64, 384 rows over 12000 (4.6 M) 24 / 19; with gradients, width 512,
+// 512 rows over 12000 69 / 74, 768 rows (9.2 M) 92 / 80, 2048 rows over 6000 (12 M) 102 / 96; width 2048,
+// 384 rows over 24000 (9.2 M) 192 / 184, 4096 rows over 2048 (8.4 M) level; width 64, 8192 rows over 512 (4.2 M)
+// 57 / 64.
+constexpr uint32_t kFusedRows = 128;
+constexpr uint64_t kFusedLogits = 5ull << 20, kFusedGradLogits = 8ull << 20;
+// Teacher's entries of a row in a block of T0G_LOSS_BLOCK columns, on average, up to which
+// the fused form is taken: its epilogue takes a row's entries one after another (147 of 280
+// tokens, 2985 rows of width 768: 313 us fused, 71 by rows).
+constexpr uint64_t kFusedEntries = 8;
 // Rows up to which G goes into the products as two bf16, the rounded value and what the
 // rounding left: few rows' roundings do not average out (one row's dx has the label's
 // whole, up to 2^-8), and what bounds their products is the weight's bytes.
@@ -54,6 +64,8 @@ constexpr uint32_t kCopyRows = 512;
 constexpr uint64_t kCopyBytes = 512ull << 20;
 // Rows of a launch's y grid, at most (the kernels step through the rest).
 constexpr uint32_t kMaxGridY = 65535;
+
+std::atomic<uint32_t> g_form{T0G_LOSS_FORM_AUTO};
 
 struct Range {
     uint64_t begin, end;
@@ -240,17 +252,20 @@ int make_loss_plan(const Problem &p, Plan *pl) {
     const bool x_aligned = (d.x & 15) == 0 && d.ldx % 8 == 0 && d.hidden % 8 == 0;
     pl->copy_w = !aligned && d.rows >= kCopyRows;
     pl->padded = aligned || pl->copy_w;
-    // xz is dW's operand; the logits' only where x itself is not aligned like the weight, or
-    // where ignored rows must not reach the entries (fused, and with a teacher)
     pl->ldxz = round_up(d.hidden, 8);
-    pl->copy_x = pl->padded && !x_aligned;
-    if (p.grad && (d.rows >= kFusedRows || p.t)) pl->copy_x = true;
     // the 256x256 tile takes 32-bit byte offsets, and rows of 256 or more of a weight
     // [hidden][vocab] (a copied piece has them)
-    const uint64_t ldx = pl->copy_x ? pl->ldxz : d.ldx, ldw = pl->copy_w ? pl->ldxz : d.ldw;
-    pl->fused = d.rows >= kFusedRows && pl->padded && d.rows * ldx < (1ull << 30) &&
-                (d.max_piece == 0 || d.max_piece >= 256) &&
+    const uint64_t ldx = std::max(pl->ldxz, d.ldx), ldw = pl->copy_w ? pl->ldxz : d.ldw;
+    const uint32_t form = g_form.load();
+    const bool worth = form == T0G_LOSS_FORM_FUSED ? d.rows > 0
+                       : p.grad ? d.rows > kPairRows && rows * d.vocab >= kFusedGradLogits
+                              : d.rows >= kFusedRows && rows * d.vocab >= kFusedLogits;
+    const bool sparse = !p.t || form == T0G_LOSS_FORM_FUSED || (uint64_t)p.t->top_k * T0G_LOSS_BLOCK <= kFusedEntries * d.vocab;
+    pl->fused = form != T0G_LOSS_FORM_ROWS && worth && sparse && pl->padded && d.rows * ldx < (1ull << 30) && (d.max_piece == 0 || d.max_piece >= 256) &&
                 (nt ? ldw * 256 < (1ull << 30) : pl->copy_w || (d.ldw >= 256 && d.hidden * ldw < (1ull << 30)));
+    // xz is dW's operand; the logits' too where x itself is not aligned like the weight, and
+    // wherever it is there before them
+    pl->copy_x = (pl->padded && !x_aligned) || (p.grad && (pl->fused || p.t));
     pl->direct = !pl->fused && !p.t && !pl->copy_x;
     pl->pair = !pl->fused && p.grad && d.rows <= kPairRows;
     const uint32_t chunk = pl->fused ? T0G_LOSS_BLOCK : T0G_LOSS_CHUNK;
@@ -365,6 +380,19 @@ int run_copy(t0g_device *dev, const Problem &p, const Plan &pl, const Piece &pc,
     c.ldd = ldw_of(p, pl, pc);
     const uint64_t groups = ((uint64_t)c.rows * (c.ldd / 8) + 255) / 256;
     return losses_launch(dev, "t0g_loss_copy_weight", (uint32_t)std::min<uint64_t>(groups, 1u << 20), 1, &c, sizeof c);
+}
+
+// The whole rows' kernel for a vocabulary.
+struct RowKernel {
+    const char *symbol;
+    uint32_t threads;
+};
+RowKernel row_kernel_for(uint32_t vocab) {
+    if (vocab <= 256) return {"t0g_loss_row_1x1", 64};
+    if (vocab <= 1024) return {"t0g_loss_row_1x4", 256};
+    if (vocab <= 4096) return {"t0g_loss_row_4x4", 256};
+    if (vocab <= 8192) return {"t0g_loss_row_8x4", 256};
+    return {"t0g_loss_row_4x16", 1024};
 }
 
 // One of the 256x256 kernels on a piece: statistics, statistics with the exponentials kept, or G.
@@ -491,10 +519,10 @@ int run_loss(t0g_device *dev, const Problem &p) {
     };
     const size_t n = pl.pieces.size();
     // by rows: one kernel for all of a row that fits a workgroup's registers
-    const uint32_t quads = (d.vocab + T0G_LOSS_ROW_QUADS - 1) / T0G_LOSS_ROW_QUADS;
-    const bool one = !pl.fused && n == 1 && quads <= kRowQuads;
+    const bool one = !pl.fused && n == 1 && d.vocab <= T0G_LOSS_ROW_MAX;
     auto whole_rows = [&] {
-        return losses_launch(dev, quads <= 1 ? "t0g_loss_row_1" : "t0g_loss_row_4", std::min<uint32_t>(d.rows, 1u << 20), 1, &a, sizeof a, 1024);
+        const RowKernel k = row_kernel_for(d.vocab);
+        return losses_launch(dev, k.symbol, std::min<uint32_t>(d.rows, 1u << 20), 1, &a, sizeof a, k.threads);
     };
     if (!pl.direct && (rc = row_kernel("t0g_loss_prepare", 1))) return rc;
     for (size_t i = 0; i < n; ++i) {
@@ -597,6 +625,12 @@ int t0g_linear_cross_entropy(t0g_device *dev, const t0g_linear_ce_desc *desc) {
 
 int t0g_linear_distill(t0g_device *dev, const t0g_linear_distill_desc *desc) {
     return t0g::loss_call(dev, desc ? &desc->head : nullptr, desc);
+}
+
+int t0g_set_loss_form(uint32_t form) {
+    if (form > T0G_LOSS_FORM_FUSED) return t0g::fail(T0G_ERR_INVALID_ARG, "loss form %u", form);
+    t0g::g_form.store(form);
+    return t0g::ok();
 }
 
 int t0g_linear_cross_entropy_scratch_size(const t0g_linear_ce_desc *desc, size_t *bytes) {

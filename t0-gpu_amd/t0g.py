@@ -41,6 +41,7 @@ LAYOUTS = {"NT": NT, "NN": NN, "TN": TN, "TT": TT}
 EPI_STORE_F32, EPI_BIAS_ADD, EPI_BIAS_ADD_RELU = 0, 1, 2
 F32, BF16 = 0, 1
 I32, I64 = 0, 1
+LOSS_FORM_AUTO, LOSS_FORM_ROWS, LOSS_FORM_FUSED = 0, 1, 2
 (MATMUL_FORWARD, MATMUL_BACKWARD_DATA, MATMUL_BACKWARD_WEIGHT, MATMUL_FORWARD_CACHED, MATMUL_BACKWARD_DATA_CACHED,
  MATMUL_WT_BF16) = range(6)
 STREAM_K = 0x80000000   # GemmConfig.split_k value selecting the stream-K schedule
@@ -295,6 +296,7 @@ _sig("t0g_gemm_kernel_name", ctypes.c_int, ctypes.POINTER(GemmDesc), ctypes.c_ch
 _sig("t0g_gemm_compile", ctypes.c_int, ctypes.POINTER(GemmDesc), ctypes.POINTER(CompiledKernel))
 _sig("t0g_linear_cross_entropy", ctypes.c_int, _p, ctypes.POINTER(LinearCeDesc))
 _sig("t0g_linear_distill", ctypes.c_int, _p, ctypes.POINTER(LinearDistillDesc))
+_sig("t0g_set_loss_form", ctypes.c_int, _u32)
 _sig("t0g_linear_cross_entropy_scratch_size", ctypes.c_int, ctypes.POINTER(LinearCeDesc),
      ctypes.POINTER(ctypes.c_size_t))
 _sig("t0g_linear_distill_scratch_size", ctypes.c_int, ctypes.POINTER(LinearDistillDesc),
@@ -547,6 +549,11 @@ def linear_distill_desc(x, w, teacher, tokens, loss, rows, vocab, hidden, top_k,
     d.teacher_dtype, d.token_type = teacher_dtype, token_type
     d.temperature, d.label_weight, d.distill_weight = temperature, label_weight, distill_weight
     return d
+
+
+def set_loss_form(form):
+    """How later losses run (LOSS_FORM_*), process-wide; for tests and measurements."""
+    _check(_lib.t0g_set_loss_form(form))
 
 
 def linear_loss_scratch_size(desc):

@@ -85,6 +85,12 @@ def test_null_arguments():
     assert t0g._lib.t0g_linear_distill(None, ctypes.byref(distill())) == t0g.ERR_INVALID_ARG
 
 
+def test_loss_form_refusal():
+    with pytest.raises(t0g.T0gError) as e:
+        t0g.set_loss_form(3)
+    assert e.value.code == t0g.ERR_INVALID_ARG
+
+
 def test_scratch_stays_below_the_logits():
     """8192 x 131072 logits take 4 GiB in f32 and their gradient 2 in bf16, 65536 rows eight times that; a
     piece of the vocabulary takes what it is given."""

@@ -34,6 +34,14 @@ def rt():
     r.close()
 
 
+@pytest.fixture(autouse=True, params=["rows", "fused"])
+def form(request):
+    """Every test in both forms (fused falls back to by rows where the operands do not allow it)."""
+    t0g.set_loss_form(t0g.LOSS_FORM_FUSED if request.param == "fused" else t0g.LOSS_FORM_ROWS)
+    yield request.param
+    t0g.set_loss_form(t0g.LOSS_FORM_AUTO)
+
+
 class Case:
     """One problem: inputs on the host, the call's buffers on the device (each in a filled allocation of its
     own, so that a write outside shows and what lies between rows is not read), and the definition in 64 bits."""
@@ -496,7 +504,7 @@ def test_loss_alone_of_unaligned_operands(rt, rows, vocab, hidden, layout, pad, 
     c.check(rt, "loss alone")
 
 
-# ---- the fused form: 256 rows and more, aligned operands ------------------------------
+# ---- sizes around the fused form's tile -------------------------------------------------
 
 FUSED = [(256, 256, 64), (257, 1000, 72), (300, 2049, 136), (256, 131, 64), (513, 1283, 320), (260, 8, 8), (1000, 640, 40)]
 
@@ -562,3 +570,16 @@ def test_fused_same_bits_again_and_on_another_stream(rt):
 
 def test_fused_graph_replays(rt):
     replays(rt, Case(300, 2000, 64, seed=25).teach(20, 2.0, 0.5, 0.5), Case(260, 500, 64, seed=26), max_piece=768)
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,want,top", [(160, 54000, 64, "xw", 0), (129, 66001, 40, "x", 0),
+                                                          (140, 40000, 64, "", 0), (135, 63000, 64, "xw", 60),
+                                                          (2100, 4100, 64, "xw", 300)])
+def test_chosen_by_size(rt, form, rows, vocab, hidden, want, top):
+    """Sizes at which the choice between the forms lies; a teacher with more tokens than the fused form takes."""
+    if form == "rows":
+        t0g.set_loss_form(t0g.LOSS_FORM_AUTO)
+    c = Case(rows, vocab, hidden, seed=28, want=want, amp=4.0)
+    if top:
+        c.teach(top, 2.0, 0.5, 0.5)
+    c.check(rt, "by size")
