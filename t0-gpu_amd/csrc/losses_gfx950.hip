@@ -78,19 +78,27 @@ __device__ __forceinline__ uint32_t token_at(uint64_t base, uint64_t i, bool wid
 
 // Row `row` of x into xz, zero for an ignored row (its hidden state may hold NaN, and
 // dW's product would multiply that with the row's zero gradient) and past `hidden`.
-__device__ __forceinline__ void copy_row(const T0gLossArgs& p, uint32_t row, bool used) {
+__device__ __forceinline__ void copy_row(const T0gLossArgs& p, uint32_t row, bool used, uint32_t first, uint32_t step) {
     const uint64_t to = p.xz + (uint64_t)row * p.ldxz * 2, again = to + (uint64_t)p.rows * p.ldxz * 2;
     const bool pair = p.flags & T0G_LOSS_PAIR;
     if (p.flags & T0G_LOSS_X_VEC) {
         const uint32_t n = p.hidden / 8;
-        for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-            u32x4_t v = {0u, 0u, 0u, 0u};
-            if (used) v = *at<const u32x4_t>(p.x + (uint64_t)row * p.ldx * 2, i);
-            *at<u32x4_t>(to, i) = v;
-            if (pair) *at<u32x4_t>(again, i) = v;
+        for (uint32_t i0 = first; i0 < n; i0 += 4 * step) {
+            u32x4_t v[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                v[e] = u32x4_t{0u, 0u, 0u, 0u};
+                if (used && i0 + e * step < n) v[e] = *at<const u32x4_t>(p.x + (uint64_t)row * p.ldx * 2, i0 + e * step);
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+                if (i0 + e * step < n) {
+                    *at<u32x4_t>(to, i0 + e * step) = v[e];
+                    if (pair) *at<u32x4_t>(again, i0 + e * step) = v[e];
+                }
         }
     } else {
-        for (uint32_t i = threadIdx.x; i < p.ldxz; i += blockDim.x) {
+        for (uint32_t i = first; i < p.ldxz; i += step) {
             uint16_t v = 0;
             if (used && i < p.hidden) v = *at<const uint16_t>(p.x, (uint64_t)row * p.ldx + i);
             *at<uint16_t>(to, i) = v;
@@ -148,119 +156,183 @@ __device__ __forceinline__ void store_loss(const T0gLossArgs& p, uint32_t row, c
 
 // What a row is compared with: its label and the teacher's distribution over its
 // tokens, as entries sorted by token with equal tokens joined (their probabilities
-// add), so that each entry is one logit.  A rank sort in LDS: keys are unique
-// (token, then position), so sums of equal tokens run in the order they were given.
-__device__ __forceinline__ void prepare_row(const T0gLossArgs& p, uint32_t row) {
-    constexpr uint32_t N = T0G_LOSS_MAX_TOP + 1;
-    __shared__ uint32_t tok[N], srt[N];
+// add), so that each entry is one logit.  A rank sort: keys are unique (token, then
+// position), so sums of equal tokens run in the order they were given.
+__device__ __forceinline__ float teacher_logit(const T0gLossArgs& p, uint64_t i) {
+    return (p.flags & T0G_LOSS_TEACHER16) ? (float)__builtin_bit_cast(__bf16, *at<const uint16_t>(p.teacher, i))
+                                          : *at<const float>(p.teacher, i);
+}
+__device__ __forceinline__ void store_row(const T0gLossArgs& p, uint32_t row, uint32_t n, uint32_t label_slot, float hq,
+                                          bool taught) {
+    const float rate = row_rate(p, row);
+    *at<u32x2_t>(p.row_ent, row) = u32x2_t{n, label_slot};
+    *at<f32x4_t>(p.row_sub, row) = f32x4_t{label_slot != kNoToken ? p.label_weight * rate : 0.0f,
+                                           taught ? p.distill_weight * p.tau * rate : 0.0f, hq, taught ? 1.0f : 0.0f};
+}
+// Q log Q of one token, 0 for none (v_log takes no denormals).
+__device__ __forceinline__ float q_log_q(float q) { return q < 1.2e-38f ? 0.0f : q * (__builtin_amdgcn_logf(q) * kLn2); }
+
+// Fewer than 64 entries: one wave a row, an entry a lane (2048 rows of 63 entries and 2048
+// columns of x: 14 us, 19 us in the form below; 4752 rows of 16: 7 us against 20).
+__device__ __forceinline__ void prepare_short(const T0gLossArgs& p, uint32_t row) {
+    const uint32_t lane = threadIdx.x & 63u, k = p.teacher ? p.top_k : 0u, total = k + 1;
+    const uint32_t label = row_label(p, row);
+    uint32_t t = kNoToken;
+    float u = ninf();
+    if (lane < k) {
+        const uint64_t src = (uint64_t)row * p.ldt + lane;
+        t = token_at(p.tokens, src, p.flags & T0G_LOSS_TOKEN64, p.vocab);
+        u = teacher_logit(p, src);
+        if (u == ninf()) t = kNoToken;   // no probability: not an entry
+    }
+    const bool entry = t != kNoToken;
+    const bool taught = __ballot(entry) != 0;
+    const float top = wave_max(entry ? u : ninf());
+    float q = entry ? exp2_((u - top) * (1.44269504f / p.tau)) : 0.0f;
+    const float sum = wave_sum(q);
+    if (entry) q = q * (1.0f / sum);
+    if (lane == k) t = label;
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < total; ++j) {
+        const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)t, (int)j);
+        rank += o < t || (o == t && j < lane);
+    }
+    if (lane >= total) rank = lane;
+    const uint32_t st = (uint32_t)__builtin_amdgcn_ds_permute((int)(rank * 4), (int)t);   // lane `rank` receives
+    const float sq = __builtin_bit_cast(float, __builtin_amdgcn_ds_permute((int)(rank * 4), __builtin_bit_cast(int, q)));
+    const uint32_t before = __shfl_up(st, 1);
+    const bool valid = lane < total && st != kNoToken, head = valid && (lane == 0 || before != st);
+    const uint64_t heads = __ballot(head), members = __ballot(valid);
+    const uint32_t slot = (uint32_t)__popcll(heads & ((1ull << lane) - 1));
+    // the sum of a run of equal tokens, in order
+    const uint64_t later = heads & ~((2ull << lane) - 1);
+    const uint32_t end = later ? (uint32_t)__builtin_ctzll(later) : (uint32_t)__popcll(members);
+    float v = 0.0f;
+    for (uint32_t j = 0; __ballot(head && lane + j < end) != 0; ++j) {
+        const float x = __shfl(sq, (int)((lane + j) & 63u));
+        if (head && lane + j < end) v += x;
+    }
+    if (head) {
+        *at<uint32_t>(p.ent_tok, (uint64_t)row * p.slots + slot) = st;
+        *at<float>(p.ent_q, (uint64_t)row * p.slots + slot) = v;
+    }
+    const uint32_t n = (uint32_t)__popcll(heads);
+    if (n == 0 && lane == 0) *at<uint32_t>(p.ent_tok, (uint64_t)row * p.slots) = kNoToken;
+    const float hq = wave_sum(head ? q_log_q(v) : 0.0f);
+    const uint64_t at_label = __ballot(head && st == label && label != kNoToken);
+    const uint32_t label_slot = at_label ? (uint32_t)__popcll(heads & (at_label - 1)) : kNoToken;
+    if (p.ent_off) {   // entries before each block of columns: those with a smaller token
+        // heads' tokens to lanes 0 .. n - 1, the others past them
+        const uint32_t to = head ? slot : n + (uint32_t)__popcll(~heads & ((1ull << lane) - 1));
+        const uint32_t ht = (uint32_t)__builtin_amdgcn_ds_permute((int)(to * 4), (int)(head ? st : kNoToken));
+        for (uint32_t b0 = 0; b0 < p.off_ld; b0 += 64) {
+            const uint32_t b = b0 + lane;
+            uint32_t lo = 0;   // first lane whose token is not smaller; lane 63 is no head
+#pragma unroll
+            for (uint32_t half = 32; half; half >>= 1)
+                if ((uint32_t)__shfl((int)ht, (int)(lo + half - 1)) < b * T0G_LOSS_BLOCK) lo += half;
+            if (b < p.off_ld) *at<uint16_t>(p.ent_off, (uint64_t)row * p.off_ld + b) = (uint16_t)lo;
+        }
+    }
+    if (lane == 0) store_row(p, row, n, label_slot, hq, taught);
+    if (p.xz) copy_row(p, row, label != kNoToken || taught, lane, 64);
+}
+
+// More: a workgroup a row, its entries in LDS (4096 rows of 129 entries: 46 us; 16 bytes of
+// keys a read and the runs of equal tokens found in parallel took it there from 74).
+__device__ __forceinline__ void prepare_long(const T0gLossArgs& p, uint32_t row) {
+    constexpr uint32_t N = (T0G_LOSS_MAX_TOP + 1 + 7) & ~7u;
+    __shared__ __attribute__((aligned(16))) uint32_t tok[N];
+    __shared__ uint32_t srt[N], wave_heads[4], label_at;
     __shared__ float q[N], sq[N];
     __shared__ float red[3][4];
-    __shared__ uint32_t wave_heads[4];
-    const uint32_t tid = threadIdx.x;
+    const uint32_t tid = threadIdx.x, k = p.top_k, total = k + 1;
     const uint32_t label = row_label(p, row);
-    const float rate = row_rate(p, row);
-    const float cl = label != kNoToken ? p.label_weight * rate : 0.0f;
-    uint32_t n = 0, label_slot = kNoToken;
-    float hq = 0.0f;
-    bool taught = false;
-    if (!p.teacher) {
-        n = label != kNoToken;
-        label_slot = n ? 0u : kNoToken;
-        if (tid == 0) {
-            *at<uint32_t>(p.ent_tok, (uint64_t)row * p.slots) = label;
-            *at<float>(p.ent_q, (uint64_t)row * p.slots) = 0.0f;
-        }
-    } else {
-        const uint32_t k = p.top_k, total = k + 1;
-        float top = ninf();
-        for (uint32_t i = tid; i < k; i += kThreads) {
+    float top = ninf();
+    for (uint32_t i = tid; i < ((total + 7) & ~7u); i += kThreads) {
+        uint32_t t = kNoToken;
+        if (i < k) {
             const uint64_t src = (uint64_t)row * p.ldt + i;
-            uint32_t t = token_at(p.tokens, src, p.flags & T0G_LOSS_TOKEN64, p.vocab);
-            float u = (p.flags & T0G_LOSS_TEACHER16)
-                          ? (float)__builtin_bit_cast(__bf16, *at<const uint16_t>(p.teacher, src))
-                          : *at<const float>(p.teacher, src);
+            t = token_at(p.tokens, src, p.flags & T0G_LOSS_TOKEN64, p.vocab);
+            const float u = teacher_logit(p, src);
             if (u == ninf()) t = kNoToken;   // no probability: not an entry
-            tok[i] = t;
             q[i] = u;
             if (t != kNoToken) top = __builtin_fmaxf(top, u);
+        } else if (i == k) {
+            t = label;
+            q[i] = 0.0f;
         }
-        if (tid == 0) {
-            tok[k] = label;
-            q[k] = 0.0f;
-        }
-        top = block_max(top, red[0]);
-        float sum = 0.0f, any = 0.0f;
-        const float scale = 1.44269504f / p.tau;
-        for (uint32_t i = tid; i < k; i += kThreads) {
-            float e = 0.0f;
-            if (tok[i] != kNoToken) {
-                e = exp2_((q[i] - top) * scale);
-                any = 1.0f;
-            }
-            q[i] = e;
-            sum += e;
-        }
-        sum = block_sum(sum, red[1]);
-        any = block_max(any, red[2]);
-        taught = any > 0.0f;
-        const float inv = taught ? 1.0f / sum : 0.0f;
-        for (uint32_t i = tid; i < total; i += kThreads) {
-            const uint32_t t = tok[i];
-            uint32_t rank = 0;
-            for (uint32_t j = 0; j < total; ++j) {
-                const uint32_t o = tok[j];
-                rank += o < t || (o == t && j < i);
-            }
-            srt[rank] = t;
-            sq[rank] = q[i] * inv;
-        }
-        __syncthreads();
-        // first entries of equal tokens, numbered in order
-        float part = 0.0f;
-        for (uint32_t i0 = 0; i0 < total; i0 += kThreads) {
-            const uint32_t i = i0 + tid;
-            const bool head = i < total && srt[i] != kNoToken && (i == 0 || srt[i - 1] != srt[i]);
-            const uint64_t mask = __ballot(head);
-            const uint32_t lane = tid & 63u, wave = tid >> 6;
-            if (lane == 0) wave_heads[wave] = (uint32_t)__popcll(mask);
-            __syncthreads();
-            uint32_t slot = n + (uint32_t)__popcll(mask & ((1ull << lane) - 1));
-            for (uint32_t w = 0; w < wave; ++w) slot += wave_heads[w];
-            n += wave_heads[0] + wave_heads[1] + wave_heads[2] + wave_heads[3];
-            if (head) {
-                float v = 0.0f;
-                for (uint32_t j = i; j < total && srt[j] == srt[i]; ++j) v += sq[j];
-                *at<uint32_t>(p.ent_tok, (uint64_t)row * p.slots + slot) = srt[i];
-                *at<float>(p.ent_q, (uint64_t)row * p.slots + slot) = v;
-                if (srt[i] == label) tok[0] = slot;
-                if (!(v < 1.2e-38f)) part += v * (__builtin_amdgcn_logf(v) * kLn2);   // 0 log 0 = 0; v_log takes no denormals
-            }
-            __syncthreads();
-        }
-        if (label != kNoToken) label_slot = tok[0];
-        __syncthreads();
-        hq = block_sum(part, red[0]);
+        tok[i] = t;
     }
-    if (p.ent_off) {   // entries before each block of columns
-        __syncthreads();   // the row's tokens are written
+    if (tid == 0) label_at = kNoToken;
+    top = block_max(top, red[0]);
+    float sum = 0.0f, any = 0.0f;
+    const float scale = 1.44269504f / p.tau;
+    for (uint32_t i = tid; i < k; i += kThreads) {
+        float e = 0.0f;
+        if (tok[i] != kNoToken) {
+            e = exp2_((q[i] - top) * scale);
+            any = 1.0f;
+        }
+        q[i] = e;
+        sum += e;
+    }
+    sum = block_sum(sum, red[1]);
+    any = block_max(any, red[2]);
+    const bool taught = any > 0.0f;
+    const float inv = taught ? 1.0f / sum : 0.0f;
+    for (uint32_t i = tid; i < total; i += kThreads) {
+        const uint32_t t = tok[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < total; j += 8) {   // the padding's keys are the largest
+            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(&tok[j]), b = *reinterpret_cast<const u32x4_t*>(&tok[j + 4]);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+                rank += (a[e] < t || (a[e] == t && j + e < i)) + (b[e] < t || (b[e] == t && j + 4 + e < i));
+        }
+        srt[rank] = t;
+        sq[rank] = q[i] * inv;
+    }
+    __syncthreads();
+    // first entries of equal tokens, numbered in order; their tokens take the place of the keys
+    uint32_t n = 0;
+    float part = 0.0f;
+    for (uint32_t i0 = 0; i0 < total; i0 += kThreads) {
+        const uint32_t i = i0 + tid;
+        const bool head = i < total && srt[i] != kNoToken && (i == 0 || srt[i - 1] != srt[i]);
+        const uint64_t mask = __ballot(head);
+        const uint32_t lane = tid & 63u, wave = tid >> 6;
+        if (lane == 0) wave_heads[wave] = (uint32_t)__popcll(mask);
+        __syncthreads();
+        uint32_t slot = n + (uint32_t)__popcll(mask & ((1ull << lane) - 1));
+        for (uint32_t w = 0; w < wave; ++w) slot += wave_heads[w];
+        n += wave_heads[0] + wave_heads[1] + wave_heads[2] + wave_heads[3];
+        if (head) {
+            float v = 0.0f;
+            for (uint32_t j = i; j < total && srt[j] == srt[i]; ++j) v += sq[j];
+            *at<uint32_t>(p.ent_tok, (uint64_t)row * p.slots + slot) = srt[i];
+            *at<float>(p.ent_q, (uint64_t)row * p.slots + slot) = v;
+            tok[slot] = srt[i];
+            if (srt[i] == label) label_at = slot;
+            part += q_log_q(v);
+        }
+        __syncthreads();
+    }
+    if (p.ent_off)   // entries before each block of columns
         for (uint32_t b = tid; b < p.off_ld; b += kThreads) {
             uint32_t lo = 0, hi = n;   // first entry at or past the block's first token
             while (lo < hi) {
                 const uint32_t mid = (lo + hi) / 2;
-                if (*at<const uint32_t>(p.ent_tok, (uint64_t)row * p.slots + mid) < b * T0G_LOSS_BLOCK)
+                if (tok[mid] < b * T0G_LOSS_BLOCK)
                     lo = mid + 1;
                 else
                     hi = mid;
             }
             *at<uint16_t>(p.ent_off, (uint64_t)row * p.off_ld + b) = (uint16_t)lo;
         }
-    }
-    if (tid == 0) {
-        *at<u32x2_t>(p.row_ent, row) = u32x2_t{n, label_slot};
-        *at<f32x4_t>(p.row_sub, row) =
-            f32x4_t{cl, taught ? p.distill_weight * p.tau * rate : 0.0f, hq, taught ? 1.0f : 0.0f};
-    }
-    if (p.xz) copy_row(p, row, label != kNoToken || taught);
+    const float hq = block_sum(part, red[0]);
+    if (tid == 0) store_row(p, row, n, label_at, hq, taught);
+    if (p.xz) copy_row(p, row, label != kNoToken || taught, tid, kThreads);
     __syncthreads();
 }
 
@@ -324,7 +396,7 @@ __device__ __forceinline__ void chunk_stats(const T0gLossArgs& p, uint32_t row, 
             if (c < n) *at<float>(p.ent_z, (uint64_t)row * p.slots + e) = *at<const float>(base, c);
         }
         // before the first product with G (of a single piece, the gradient kernel does it)
-        if ((p.flags & T0G_LOSS_DIRECT) && p.xz && p.v0 == 0 && chunk == 0) copy_row(p, row, r.used());
+        if ((p.flags & T0G_LOSS_DIRECT) && p.xz && p.v0 == 0 && chunk == 0) copy_row(p, row, r.used(), threadIdx.x, blockDim.x);
     }
     __syncthreads();
 }
@@ -436,7 +508,7 @@ __device__ __forceinline__ void finish_row(const T0gLossArgs& p, const RowInfo& 
         kd = block_sum<W>(kd, red);
     }
     if (threadIdx.x == 0) store_loss(p, row, r, l0, l1, r.labelled() ? entry_z(p, row, r.label) : 0.0f, kd);
-    if ((p.flags & T0G_LOSS_DIRECT) && (p.flags & T0G_LOSS_Z) && p.xz) copy_row(p, row, r.used());
+    if ((p.flags & T0G_LOSS_DIRECT) && (p.flags & T0G_LOSS_Z) && p.xz) copy_row(p, row, r.used(), threadIdx.x, blockDim.x);
 }
 
 // Logit gradients of columns [c0, c0 + n) of a row in bf16, zero up to ng, then its entries.
@@ -608,8 +680,12 @@ __device__ __forceinline__ void sum_planes(const T0gLossSumArgs& p) {
 
 }  // namespace t0g
 
+// one wave a row
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_prepare(T0gLossArgs p) {
-    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) t0g::prepare_row(p, row);
+    for (uint32_t row = blockIdx.x * 4 + threadIdx.x / 64; row < p.rows; row += gridDim.x * 4) t0g::prepare_short(p, row);
+}
+extern "C" __global__ void __launch_bounds__(256) t0g_loss_prepare_long(T0gLossArgs p) {
+    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) t0g::prepare_long(p, row);
 }
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_stats(T0gLossArgs p) {
     for (uint32_t row = blockIdx.y; row < p.rows; row += gridDim.y) t0g::chunk_stats(p, row, blockIdx.x);

@@ -524,7 +524,11 @@ int run_loss(t0g_device *dev, const Problem &p) {
         const RowKernel k = row_kernel_for(d.vocab);
         return losses_launch(dev, k.symbol, std::min<uint32_t>(d.rows, 1u << 20), 1, &a, sizeof a, k.threads);
     };
-    if (!pl.direct && (rc = row_kernel("t0g_loss_prepare", 1))) return rc;
+    if (!pl.direct) {
+        // a wave takes a row of fewer than 64 entries
+        const bool wave = pl.slots < 64;
+        if ((rc = wave ? row_kernel("t0g_loss_prepare", 4) : row_kernel("t0g_loss_prepare_long", 1))) return rc;
+    }
     for (size_t i = 0; i < n; ++i) {
         const Piece &pc = pl.pieces[i];
         at_piece(pc);
