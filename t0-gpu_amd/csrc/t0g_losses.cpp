@@ -225,14 +225,50 @@ t0g_gemm_desc logits_gemm(const Problem &p, const Plan &pl, const Piece &pc, uin
                    ldw_of(p, pl, pc), round_up(pc.cols, 4), d.transpose, T0G_F32);
 }
 
+// dx sums over a piece's tokens, a long K, with few tiles of output: K in as many slices as fill the CUs
+// once.  The GEMMs' own choice takes powers of two, which leave up to half of them idle: 20 tiles of
+// 407x1000x74752 took 131 us against 65, 1000x768x50048 103 against 68, and in 256x256 tiles
+// 1697x1208x60624 537 against 291.  128x128 tiles while three slices fit and hold 12 stages of 64
+// each (over 60 sizes 0.50 to 1.02 of the own choice's time, but for 568x304x123912 with 1.14; slices
+// of 3 to 11 stages up to 1.64), from there 256x256 tiles with slices of 50 (0.54 to 1.00;
+// 508x2888x31880 with 49 1.07), where their number is not one the own choice has (in 4 slices 2048x2048x32000
+// took 7 us more than what it takes).  Not for the pair's products, whose planes cost more the
+// more there are (64 rows, 50304 tokens: 115 us against 108).
+void slice_long_k(t0g_gemm_desc *g) {
+    static const t0g_gemm_config small = [] {
+        t0g_gemm_config c;
+        (void)t0g_config_preset("gfx950_128x128_k64", &c);
+        return c;
+    }();
+    static const t0g_gemm_config big = [] {
+        t0g_gemm_config c;
+        (void)t0g_config_preset("gfx950_256x256_k64", &c);
+        return c;
+    }();
+    auto tiles = [g](uint32_t side) { return (uint64_t)((g->m + side - 1) / side) * ((g->n + side - 1) / side); };
+    const uint32_t stages = (g->k + 63) / 64;
+    if (tiles(128) == 0) return;
+    const uint64_t s1 = std::min<uint64_t>(kNumCUs / tiles(128), 64), s2 = kNumCUs / tiles(256);
+    if (s1 >= 3 && stages >= s1 * 12) {
+        g->config = &small;
+        g->split_k = (uint32_t)s1;
+    } else if (s1 < 3 && (s2 & (s2 - 1)) != 0 && stages >= s2 * 50) {
+        g->config = &big;
+        g->split_k = (uint32_t)s2;
+    }
+}
+
 // dx of a piece: the output itself, or f32 plane `plane`.
 t0g_gemm_desc dx_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base, uint32_t plane) {
     const t0g_linear_ce_desc &d = p.d;
     const bool whole = pl.group == 0;
-    return gemm_of(base + pl.g, w_of(p, pl, pc, base),
+    t0g_gemm_desc g =
+        gemm_of(base + pl.g, w_of(p, pl, pc, base),
                    whole ? d.dx : base + pl.planes + (uint64_t)plane * d.rows * pl.ldp * 4, pl.pair ? 2 * d.rows : d.rows,
                    d.hidden, pc.cols, ld_of_g(pl, pc), ldw_of(p, pl, pc), whole ? d.lddx : pl.ldp,
                    d.transpose == T0G_NT ? T0G_NN : T0G_NT, whole ? d.dx_dtype : (uint32_t)T0G_F32);
+    if (!pl.pair) slice_long_k(&g);
+    return g;
 }
 
 t0g_gemm_desc dw_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
