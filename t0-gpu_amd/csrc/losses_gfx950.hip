@@ -678,6 +678,97 @@ __device__ __forceinline__ void sum_planes(const T0gLossSumArgs& p) {
     }
 }
 
+template <bool STREAM, class T>
+__device__ __forceinline__ void store16(uint64_t to, T v) {
+    if constexpr (STREAM)
+        __builtin_nontemporal_store(v, at<T>(to));
+    else
+        *at<T>(to) = v;
+}
+
+// dW of few rows: C = A^T B over up to 32 KS rows, which writes far more than it reads and
+// is bound by that.  A wave takes 32 x 128 of C, small tiles of which many stand at different
+// points at once (128 x 128 took 45 us on 13 rows of 29888x2832, this 37).  A lane loads 2 and 8
+// columns of 8 rows of the operands; pairs of rows make its fragments of 16x16x32 products, whose
+// columns are 2 or 8 apart, so that the products of a fragment of A with all 8 of B's give a lane
+// 8 neighbours of C's row and 16 lanes 256 contiguous bytes of bf16.  C goes past the caches where
+// its rows are whole 128-byte lines (131072x4096: 197 us against 247; 29888x2832, whose rows are
+// not, 67 against 37 us), and then leaves the weight in them for the next call.
+template <int KS, bool STREAM>
+__device__ __forceinline__ void outer(const T0gLossOuterArgs& p) {
+    constexpr int CA = 2;
+    constexpr uint32_t kTileM = 16 * CA;
+    const uint32_t lane = threadIdx.x & 63u, l16 = lane & 15u, quad = lane >> 4;
+    const uint32_t tiles_n = (p.n + 127) / 128, tiles_m = (p.m + kTileM - 1) / kTileM;
+    const uint64_t tile = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (tile >= (uint64_t)tiles_m * tiles_n) return;
+    const uint32_t inner = p.m_inner ? tiles_m : tiles_n, t0 = (uint32_t)(tile / inner), t1 = (uint32_t)(tile % inner);
+    const uint32_t m0 = (p.m_inner ? t1 : t0) * kTileM;
+    const uint32_t ma = m0 + CA * l16, nb = (p.m_inner ? t0 : t1) * 128 + 8 * l16;
+    uint32_t a[KS][8];
+    u32x4_t b[KS][8];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t row = 32 * s + 8 * quad + i;
+            a[s][i] = 0u;
+            b[s][i] = u32x4_t{0u, 0u, 0u, 0u};
+            if (row < p.rows && ma < p.m) a[s][i] = *at<const uint32_t>(p.a + ((uint64_t)row * p.lda + ma) * 2);
+            if (row < p.rows && nb < p.n) b[s][i] = *at<const u32x4_t>(p.b + ((uint64_t)row * p.ldb + nb) * 2);
+        }
+    // the low (c = 0) or high half of 8 rows' words, rows in order
+    auto column = [](auto word, int c) {
+        const uint32_t sel = c & 1 ? 0x07060302u : 0x05040100u;
+        u32x4_t v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_perm(word(2 * i + 1), word(2 * i), sel);
+        return __builtin_bit_cast(bf16x8_t, v);
+    };
+    bf16x8_t fb[KS][8];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) fb[s][c] = column([&](int i) { return b[s][i][c >> 1]; }, c);
+#pragma unroll
+    for (int c = 0; c < CA; ++c) {
+        f32x4_t acc[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const bf16x8_t fa = column([&](int i) { return a[s][i]; }, c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa, fb[s][e], acc[e], 0, 0, 0);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t m = m0 + CA * (4 * quad + j) + c;
+            if (m >= p.m) continue;
+            const uint64_t i = (uint64_t)m * p.ldc + nb;
+            if (p.vec && nb + 8 <= p.n) {
+                if (p.out_bf16) {
+                    const u32x4_t v = {pack2(acc[0][j], acc[1][j]), pack2(acc[2][j], acc[3][j]), pack2(acc[4][j], acc[5][j]),
+                                       pack2(acc[6][j], acc[7][j])};
+                    store16<STREAM>(p.c + i * 2, v);
+                } else {
+                    store16<STREAM>(p.c + i * 4, f32x4_t{acc[0][j], acc[1][j], acc[2][j], acc[3][j]});
+                    store16<STREAM>(p.c + i * 4 + 16, f32x4_t{acc[4][j], acc[5][j], acc[6][j], acc[7][j]});
+                }
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e)
+                    if (nb + e < p.n) {
+                        if (p.out_bf16)
+                            *at<__bf16>(p.c, i + e) = (__bf16)acc[e][j];
+                        else
+                            *at<float>(p.c, i + e) = acc[e][j];
+                    }
+            }
+        }
+    }
+}
+
 }  // namespace t0g
 
 // one wave a row
@@ -728,3 +819,14 @@ T0G_LOSS_GEMM(t0g_loss_again_nt, true, Grad)
 T0G_LOSS_GEMM(t0g_loss_again_nn, false, Grad)
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_copy_weight(T0gLossCopyArgs p) { t0g::copy_weight(p); }
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_sum(T0gLossSumArgs p) { t0g::sum_planes(p); }
+#define T0G_LOSS_OUTER(KS, WAVES)                                                                        \
+    extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES))) \
+        t0g_loss_outer_##KS(T0gLossOuterArgs p) {                                                        \
+        if (p.stream)                                                                                    \
+            t0g::outer<KS, true>(p);                                                                     \
+        else                                                                                             \
+            t0g::outer<KS, false>(p);                                                                    \
+    }
+T0G_LOSS_OUTER(1, 4)
+T0G_LOSS_OUTER(2, 3)
+T0G_LOSS_OUTER(4, 2)

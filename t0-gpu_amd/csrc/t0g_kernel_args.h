@@ -244,6 +244,18 @@ typedef struct T0gLossSumArgs {
     uint32_t reserved;
 } T0gLossSumArgs;
 
+/* c[m][n] = sum over up to 128 rows of a[row][m] b[row][n] (t0g_loss_outer_*) */
+typedef struct T0gLossOuterArgs {
+    uint64_t a, b;           /* bf16 [rows][lda], [rows][ldb], 16-byte aligned rows    */
+    uint64_t c;              /* f32 | bf16 [m][ldc]                                    */
+    uint32_t rows, m, n;     /* lda >= m and ldb >= n rounded up to 8                  */
+    uint32_t lda, ldb, ldc;
+    uint32_t out_bf16, vec;  /* vec: ldc a multiple of 8, c 16-byte aligned            */
+    uint32_t stream;         /* c past the caches: its rows are whole 128-byte lines   */
+    uint32_t m_inner;        /* tiles of one block of n after another, else of m       */
+    uint32_t reserved;
+} T0gLossOuterArgs;
+
 /* Epilogue chain operations: tile_ir's EpilogueOp (src/t0/tile_ir.rs:41-62),
  * applied in chain order to each fp32 result before the output conversion. */
 #define T0G_EPI_OP_BIAS_ADD 1u  /* x += bias[col]                                  */

@@ -280,6 +280,17 @@ t0g_gemm_desc dw_gemm(const Problem &p, const Plan &pl, const Piece &pc, uint64_
                : gemm_of(base + pl.xz, base + pl.g, c, d.hidden, pc.cols, rows, pl.ldxz, ldg, d.lddw, T0G_TN, d.dw_dtype);
 }
 
+// dW of few rows as t0g_loss_outer_*, which writes at up to 5.5 TB/s where the GEMMs' tiles, each loading,
+// multiplying and storing in turn, reach 3 to 4: 13 rows of 29888x2832 185 us for the whole call against
+// 135, 32x32000x1024 77 against 70, 64 rows of 50304x768 107 against 97.  Not for small outputs (29 rows
+// of 5120x192: 33.4 us against 35.8), nor for more than 32 rows where the rows of dW are the
+// hidden ones (64 rows, 4096x128000: 816 us against 954).
+constexpr uint64_t kOuterSize = 1ull << 22;
+constexpr uint64_t kCacheBytes = 256ull << 20;
+bool outer_dw(const Problem &p, const Plan &pl) {
+    return pl.pair && p.d.rows <= (p.d.transpose == T0G_NT ? 64u : 32u) && (uint64_t)p.d.vocab * p.d.hidden >= kOuterSize;
+}
+
 int make_loss_plan(const Problem &p, Plan *pl) {
     const t0g_linear_ce_desc &d = p.d;
     const uint64_t rows = d.rows ? d.rows : 1;
@@ -385,7 +396,7 @@ int make_loss_plan(const Problem &p, Plan *pl) {
         int n = 0, rc;
         if (!pl->fused) g[n++] = logits_gemm(p, *pl, pc, 0);
         if (d.dx && !pl->pair) g[n++] = dx_gemm(p, *pl, pc, 0, 0);
-        if (d.dw) g[n++] = dw_gemm(p, *pl, pc, 0);
+        if (d.dw && !outer_dw(p, *pl)) g[n++] = dw_gemm(p, *pl, pc, 0);
         for (int i = 0; i < n; ++i) {
             size_t bytes = 0;
             if ((rc = losses_gemm_workspace(&g[i], pl->padded, &bytes))) return rc;
@@ -416,6 +427,31 @@ int run_copy(t0g_device *dev, const Problem &p, const Plan &pl, const Piece &pc,
     c.ldd = ldw_of(p, pl, pc);
     const uint64_t groups = ((uint64_t)c.rows * (c.ldd / 8) + 255) / 256;
     return losses_launch(dev, "t0g_loss_copy_weight", (uint32_t)std::min<uint64_t>(groups, 1u << 20), 1, &c, sizeof c);
+}
+
+int run_dw(t0g_device *dev, const Problem &p, const Plan &pl, const Piece &pc, uint64_t base) {
+    const t0g_linear_ce_desc &d = p.d;
+    const t0g_gemm_desc g = dw_gemm(p, pl, pc, base);
+    if (!outer_dw(p, pl)) return run_gemm(dev, g, pl, base);
+    if (g.m == 0 || g.n == 0) return T0G_OK;
+    T0gLossOuterArgs o;
+    memset(&o, 0, sizeof o);
+    o.a = g.a;
+    o.b = g.b;
+    o.c = g.c;
+    o.rows = g.k;
+    o.m = g.m;
+    o.n = g.n;
+    o.lda = g.lda;
+    o.ldb = g.ldb;
+    o.ldc = g.ldc;
+    o.out_bf16 = g.out_dtype == T0G_BF16;
+    o.vec = g.ldc % 8 == 0 && g.c % 16 == 0;
+    o.stream = g.c % 128 == 0 && (uint64_t)g.ldc * dtype_size(g.out_dtype) % 128 == 0;
+    o.m_inner = d.transpose == T0G_NN;   // the columns of x, which every block of G meets
+    const uint64_t tiles = (((uint64_t)g.m + 31) / 32) * (((uint64_t)g.n + 127) / 128);
+    const char *symbol = g.k <= 32 ? "t0g_loss_outer_1" : g.k <= 64 ? "t0g_loss_outer_2" : "t0g_loss_outer_4";
+    return losses_launch(dev, symbol, (uint32_t)((tiles + 3) / 4), 1, &o, sizeof o);
 }
 
 // The whole rows' kernel for a vocabulary.
@@ -483,7 +519,7 @@ int run_loss(t0g_device *dev, const Problem &p) {
     if ((rc = losses_begin(dev, pl.bytes, &base))) return rc;
     if (d.rows == 0) {
         for (const Piece &pc : pl.pieces)   // a product over no rows: zeros
-            if (d.dw && (rc = run_gemm(dev, dw_gemm(p, pl, pc, base), pl, base))) return rc;
+            if (d.dw && (rc = run_dw(dev, p, pl, pc, base))) return rc;
         return ok();
     }
     T0gLossArgs a;
@@ -590,6 +626,9 @@ int run_loss(t0g_device *dev, const Problem &p) {
     s.rows = d.rows;
     s.cols = d.hidden;
     s.ldp = pl.ldp;
+    // few rows: dx reads the weight again while the caches may hold it, before dW is written (100 rows of
+    // 32000x1024: 96.1 us against 94.5; with the GEMM's dW and 64 rows of 128000x4096 804 against 846)
+    const bool dx_first = pl.pair && d.dx && (outer_dw(p, pl) || (uint64_t)d.vocab * d.hidden * 2 <= kCacheBytes);
     uint32_t planes = 0;
     for (size_t i = n; i-- > 0;) {
         const Piece &pc = pl.pieces[i];
@@ -605,13 +644,14 @@ int run_loss(t0g_device *dev, const Problem &p) {
             if (i + 1 == n || !(rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base)))
                 rc = piece_kernel("t0g_loss_grad", (pc.cols + T0G_LOSS_CHUNK - 1) / T0G_LOSS_CHUNK);
         }
-        if (rc || (d.dw && (rc = run_gemm(dev, dw_gemm(p, pl, pc, base), pl, base)))) return rc;
+        if (rc || (d.dw && !dx_first && (rc = run_dw(dev, p, pl, pc, base)))) return rc;
         if (!d.dx) continue;
         const t0g_gemm_desc dx = dx_gemm(p, pl, pc, base, planes);
         uint32_t splits = 1;
         if (pl.pair) {
             if ((rc = losses_gemm_planes_count(&dx, pl.padded, &splits)) || (rc = losses_gemm_planes(dev, &dx, pl.padded)))
                 return rc;
+            if (d.dw && dx_first && (rc = run_dw(dev, p, pl, pc, base))) return rc;
         } else if ((rc = run_gemm(dev, dx, pl, base))) {
             return rc;
         }

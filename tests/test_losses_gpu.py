@@ -583,3 +583,18 @@ def test_chosen_by_size(rt, form, rows, vocab, hidden, want, top):
     if top:
         c.teach(top, 2.0, 0.5, 0.5)
     c.check(rt, "by size")
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,layout,dtype,pad,max_piece", [
+    (1, 65600, 64, "NT", "bf16", 0, 0), (16, 9100, 470, "NT", "bf16", 2, 0), (17, 9100, 470, "NT", "f32", 0, 0),
+    (32, 8200, 520, "NN", "bf16", 0, 0), (31, 65537, 65, "NN", "bf16", 0, 0), (33, 40000, 112, "NT", "f32", 0, 0),
+    (64, 66001, 64, "NT", "bf16", 0, 30000), (20, 33000, 136, "NN", "f32", 8, 16000), (64, 8200, 520, "NN", "bf16", 0, 0)])
+def test_dw_of_few_rows(rt, rows, vocab, hidden, layout, dtype, pad, max_piece):
+    """Weights of at least 2^22 values with few rows, whose dW has a kernel of its own: its row counts, ragged tiles,
+    both outputs and stores, and a NaN in an ignored row."""
+    c = Case(rows, vocab, hidden, layout, seed=60 + rows, pad=pad, dtype=dtype)
+    if rows > 1:
+        c.labels[rows // 2] = -100
+        c.x[rows // 2, 5] = float("nan")
+    c.labels[0] = vocab - 1
+    c.check(rt, f"{rows} rows", max_piece=max_piece)
