@@ -156,7 +156,7 @@ __device__ __forceinline__ void store_loss(const T0gLossArgs& p, uint32_t row, c
 
 // What a row is compared with: its label and the teacher's distribution over its
 // tokens, as entries sorted by token with equal tokens joined (their probabilities
-// add), so that each entry is one logit.  A rank sort: keys are unique (token, then
+// add), so that each entry is one logit.  Sorted by ranks: keys are unique (token, then
 // position), so sums of equal tokens run in the order they were given.
 __device__ __forceinline__ float teacher_logit(const T0gLossArgs& p, uint64_t i) {
     return (p.flags & T0G_LOSS_TEACHER16) ? (float)__builtin_bit_cast(__bf16, *at<const uint16_t>(p.teacher, i))
@@ -238,18 +238,18 @@ __device__ __forceinline__ void prepare_short(const T0gLossArgs& p, uint32_t row
     if (p.xz) copy_row(p, row, label != kNoToken || taught, lane, 64);
 }
 
-// More: a workgroup a row, its entries in LDS (4096 rows of 129 entries: 46 us; 16 bytes of
-// keys a read and the runs of equal tokens found in parallel took it there from 74).
+// More: a workgroup a row, its entries in LDS, sorted 64 at a time by a wave, whose entries then
+// search the other 64s: 4096 rows of 129 entries 43 us, 8192 of 1025 309 (1248 comparing all
+// pairs, 16 bytes of keys a read; 46 for the former).
 __device__ __forceinline__ void prepare_long(const T0gLossArgs& p, uint32_t row) {
-    constexpr uint32_t N = (T0G_LOSS_MAX_TOP + 1 + 7) & ~7u;
-    __shared__ __attribute__((aligned(16))) uint32_t tok[N];
-    __shared__ uint32_t srt[N], wave_heads[4], label_at;
+    constexpr uint32_t N = (T0G_LOSS_MAX_TOP + 1 + kThreads - 1) / kThreads * kThreads;
+    __shared__ uint32_t tok[N], srt[N], wave_heads[4], label_at;
     __shared__ float q[N], sq[N];
     __shared__ float red[3][4];
-    const uint32_t tid = threadIdx.x, k = p.top_k, total = k + 1;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, k = p.top_k, total = k + 1;
     const uint32_t label = row_label(p, row);
     float top = ninf();
-    for (uint32_t i = tid; i < ((total + 7) & ~7u); i += kThreads) {
+    for (uint32_t i = tid; i < N && i - lane < total; i += kThreads) {   // a wave's whole 64
         uint32_t t = kNoToken;
         if (i < k) {
             const uint64_t src = (uint64_t)row * p.ldt + i;
@@ -263,6 +263,7 @@ __device__ __forceinline__ void prepare_long(const T0gLossArgs& p, uint32_t row)
             q[i] = 0.0f;
         }
         tok[i] = t;
+        srt[i] = kNoToken;
     }
     if (tid == 0) label_at = kNoToken;
     top = block_max(top, red[0]);
@@ -281,14 +282,37 @@ __device__ __forceinline__ void prepare_long(const T0gLossArgs& p, uint32_t row)
     any = block_max(any, red[2]);
     const bool taught = any > 0.0f;
     const float inv = taught ? 1.0f / sum : 0.0f;
-    for (uint32_t i = tid; i < total; i += kThreads) {
-        const uint32_t t = tok[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < total; j += 8) {   // the padding's keys are the largest
-            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(&tok[j]), b = *reinterpret_cast<const u32x4_t*>(&tok[j + 4]);
+    // each wave sorts its own 64s, then every entry looks up its place in the others
+    uint32_t ranks[N / kThreads];
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e)
-                rank += (a[e] < t || (a[e] == t && j + e < i)) + (b[e] < t || (b[e] == t && j + 4 + e < i));
+    for (uint32_t g = 0; g < N / kThreads; ++g) {
+        const uint32_t i = g * kThreads + tid;
+        if (i - lane >= total) break;
+        const uint32_t t = tok[i];
+        uint32_t r = 0;
+        for (uint32_t j = 0; j < 64; ++j) {
+            const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)t, (int)j);
+            r += o < t || (o == t && j < lane);
+        }
+        tok[i - lane + r] = t;
+        ranks[g] = t != kNoToken ? r : kNoToken;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t g = 0; g < N / kThreads; ++g) {
+        const uint32_t i = g * kThreads + tid;
+        if (i - lane >= total) break;
+        if (ranks[g] == kNoToken) continue;
+        const uint32_t t = tok[i - lane + ranks[g]];
+        uint32_t rank = ranks[g];
+        for (uint32_t c = 0; c < total; c += 64) {
+            if (c == i - lane) continue;
+            const uint32_t below = c < i ? t + 1 : t;   // of equal tokens those given before
+            uint32_t lo = 0;
+#pragma unroll
+            for (uint32_t half = 32; half; half >>= 1)
+                if (tok[c + lo + half - 1] < below) lo += half;
+            rank += lo + (tok[c + lo] < below);
         }
         srt[rank] = t;
         sq[rank] = q[i] * inv;
@@ -301,7 +325,6 @@ __device__ __forceinline__ void prepare_long(const T0gLossArgs& p, uint32_t row)
         const uint32_t i = i0 + tid;
         const bool head = i < total && srt[i] != kNoToken && (i == 0 || srt[i - 1] != srt[i]);
         const uint64_t mask = __ballot(head);
-        const uint32_t lane = tid & 63u, wave = tid >> 6;
         if (lane == 0) wave_heads[wave] = (uint32_t)__popcll(mask);
         __syncthreads();
         uint32_t slot = n + (uint32_t)__popcll(mask & ((1ull << lane) - 1));

@@ -598,3 +598,14 @@ def test_dw_of_few_rows(rt, rows, vocab, hidden, layout, dtype, pad, max_piece):
         c.x[rows // 2, 5] = float("nan")
     c.labels[0] = vocab - 1
     c.check(rt, f"{rows} rows", max_piece=max_piece)
+
+
+@pytest.mark.parametrize("vocab,top", [(150, 1024), (150, 64), (65, 63), (2, 300), (5000, 257), (40, 62)])
+def test_teacher_entries_repeated(rt, vocab, top):
+    """Many equal tokens in a row, over all of the sorting's parts; some missing, and the label among them."""
+    c = Case(9, vocab, 64, seed=80 + top).teach(top, 2.0, 0.5, 0.5, repeat=True)
+    c.tokens[:, ::5] = -1
+    c.tokens[1, 1:] = c.tokens[1, 1].clamp(min=0)
+    c.tokens[2] = -1
+    c.labels[3] = c.tokens[3, 1].clamp(min=0)
+    c.check(rt, f"{top} entries of {vocab} tokens")
