@@ -609,3 +609,65 @@ def test_teacher_entries_repeated(rt, vocab, top):
     c.tokens[2] = -1
     c.labels[3] = c.tokens[3, 1].clamp(min=0)
     c.check(rt, f"{top} entries of {vocab} tokens")
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_weight_past_32_bits(rt, rows):
+    """A weight of 2^31 + 146 M values (4.6 GB), zero but for its last 300 tokens: the logits elsewhere are 0, so the
+    definition needs those alone.  G's error is 2^-8 (its bf16) + 0.7 2^-9 (kept exponentials) + 2 e_z and the
+    statistics' 2^-14; dW's sums add (rows + 2) u of their magnitudes, dx's (vocab + 2) u, and the outputs are f32."""
+    vocab, hidden, live = 140000, 16384, 300
+    g = torch.Generator().manual_seed(91)
+    x = torch.randn(rows, hidden, generator=g).bfloat16()
+    w = (2.0 * hidden ** -0.5 * torch.randn(live, hidden, generator=g)).bfloat16()
+    labels = torch.randint(0, vocab, (rows,), generator=g)
+    labels[1::2] = torch.randint(vocab - live, vocab, (rows // 2,), generator=g)
+    held = []
+
+    def up(t):
+        held.append(rt.upload(t.contiguous().view(torch.int16).numpy() if t.dtype == torch.bfloat16 else t.numpy()))
+        return held[-1]
+
+    try:
+        tail = 2 * hidden * (vocab - live)
+        wa = rt.alloc_zero(2 * hidden * vocab)
+        held.append(wa)
+        rt.write(wa + tail, w.view(torch.int16).numpy())
+        sizes = {"loss": 4 * rows, "dx": 4 * rows * hidden, "dw": 4 * vocab * hidden}
+        out = {k: rt.alloc(n) for k, n in sizes.items()}
+        held += out.values()
+        _log(f"{rows} rows")
+        rt.linear_cross_entropy(t0g.linear_ce_desc(up(x), wa, up(labels), out["loss"], rows, vocab, hidden, dx=out["dx"],
+                                                   dw=out["dw"], dx_dtype=t0g.F32, dw_dtype=t0g.F32))
+        rt.wait_idle()
+        first = vocab - live
+        xd, wd = x.double(), w.double()
+        z = xd @ wd.t()
+        lse = torch.log(torch.exp(z).sum(1) + first)
+        mag = xd.abs() @ wd.abs().t()
+        ez = float((hidden + 2) * U * mag.max())
+        rel = 2.0 ** -8 + 0.7 * 2.0 ** -9 + 2 * ez + 2.0 ** -14
+        in_tail = labels >= first
+        zy = torch.where(in_tail, z[torch.arange(rows), (labels - first).clamp(min=0)], torch.zeros(rows, dtype=torch.float64))
+        loss = torch.from_numpy(rt.read(out["loss"], (rows,), "float32").copy()).double()
+        assert float((loss - (lse - zy)).abs().max()) <= 2 * ez + 2.0 ** -14 + 16 * U * 20
+        p = torch.exp(z - lse[:, None])
+        tail_labels = torch.zeros_like(p)
+        tail_labels[in_tail, (labels - first)[in_tail]] = 1.0
+        grad, size = p - tail_labels, p + tail_labels
+        dx = torch.from_numpy(rt.read(out["dx"], (rows, hidden), "float32").copy()).double()
+        bound = (rel + (vocab + 2) * U) * (size @ wd.abs())
+        assert bool(((dx - grad @ wd).abs() <= bound).all())
+        dw = torch.from_numpy(rt.read(out["dw"] + 4 * hidden * first, (live, hidden), "float32").copy()).double()
+        bound = (rel + (rows + 2) * U) * (size.t() @ xd.abs())
+        assert bool(((dw - grad.t() @ xd).abs() <= bound).all())
+        for v in (0, 65537, 131071, 131072, first - 1, int(labels[0])):
+            hit = (labels == v).double()
+            gv = torch.exp(-lse) - hit
+            got = torch.from_numpy(rt.read(out["dw"] + 4 * hidden * v, (hidden,), "float32").copy()).double()
+            if v < first:
+                assert bool(((got - gv @ xd).abs() <= (rel + (rows + 2) * U) * ((torch.exp(-lse) + hit) @ xd.abs())).all()), v
+    finally:
+        rt.wait_idle()
+        for a in held:
+            rt.free(a)
