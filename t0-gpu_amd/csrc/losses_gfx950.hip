@@ -140,11 +140,14 @@ __device__ __forceinline__ float entry_z(const T0gLossArgs& p, uint32_t row, uin
     return (p.flags & T0G_LOSS_Z) ? *at<const float>(p.z, (uint64_t)row * p.ldz + entry_token(p, row, e))
                                   : *at<const float>(p.ent_z, (uint64_t)row * p.slots + e);
 }
-// l0, l1, c0, c1 of a row's gradient.
+// l0, l1, c0, c1 of a row's gradient.  With one softmax c1 is not a coefficient but whether the row has a
+// gradient: its label's and teacher's coefficients may cancel in c0, and its entries remain.
 __device__ __forceinline__ f32x4_t row_params(const T0gLossArgs& p, const RowInfo& r, float l0, float l1) {
     if (!r.used()) return f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    return (p.flags & T0G_LOSS_DUAL) ? f32x4_t{l0, l1, r.cl, r.ct} : f32x4_t{l0, l1, r.cl + r.ct, 0.0f};
+    if (p.flags & T0G_LOSS_DUAL) return f32x4_t{l0, l1, r.cl, r.ct};
+    return f32x4_t{l0, l1, r.cl + r.ct, r.cl != 0.0f || r.ct != 0.0f ? 1.0f : 0.0f};
 }
+__device__ __forceinline__ bool has_gradient(const f32x4_t& par) { return par[2] != 0.0f || par[3] != 0.0f; }
 __device__ __forceinline__ void store_loss(const T0gLossArgs& p, uint32_t row, const RowInfo& r, float l0, float l1, float zl,
                                            float kd) {
     float loss = 0.0f;
@@ -538,7 +541,7 @@ __device__ __forceinline__ void finish_row(const T0gLossArgs& p, const RowInfo& 
 template <int N, int W>
 __device__ __forceinline__ void write_grads(const T0gLossArgs& p, const RowInfo& r, uint32_t row, const f32x4_t& par,
                                             const f32x4_t (&v)[N], uint32_t c0, uint32_t n, uint32_t ng) {
-    const bool used = par[2] != 0.0f || par[3] != 0.0f;
+    const bool used = has_gradient(par);
     const uint64_t gb = p.g + ((uint64_t)row * p.ldg + c0) * 2;
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) {
@@ -607,7 +610,7 @@ __device__ __forceinline__ void kept_grad(const T0gLossArgs& p, uint32_t row, ui
     constexpr uint32_t kCols = 8 * kThreads;
     const uint32_t c0 = chunk * kCols, tid = threadIdx.x, c = c0 + 8 * tid;
     const f32x4_t par = *at<const f32x4_t>(p.row_par, row);
-    const bool used = par[2] != 0.0f || par[3] != 0.0f;
+    const bool used = has_gradient(par);
     if (c < p.ldg) {
         u32x4_t w = {0u, 0u, 0u, 0u};
         if (used && c < p.cols) {
@@ -826,7 +829,7 @@ extern "C" __global__ void __launch_bounds__(256) t0g_loss_grad_kept(T0gLossArgs
 extern "C" __global__ void __launch_bounds__(256) t0g_loss_grad_entries(T0gLossArgs p) {
     for (uint32_t row = blockIdx.x * 4 + threadIdx.x / 64; row < p.rows; row += gridDim.x * 4) {
         const t0g::f32x4_t par = *t0g::at<const t0g::f32x4_t>(p.row_par, row);
-        if (par[2] != 0.0f || par[3] != 0.0f) t0g::entry_grads(p, row, 0, p.cols, par, threadIdx.x & 63u, 64);
+        if (t0g::has_gradient(par)) t0g::entry_grads(p, row, 0, p.cols, par, threadIdx.x & 63u, 64);
     }
 }
 #define T0G_LOSS_GEMM(NAME, BK, KIND)                                                                             \

@@ -175,7 +175,7 @@ typedef struct T0gLossArgs {
     uint64_t row_ent;        /* i32 [rows][2]: entries, and the label's (-1: none)    */
     uint64_t row_sub;        /* f32 [rows][4]: label and teacher coefficients of the sparse
                                 part (0: none), sum of Q log Q, teacher present (1 or 0) */
-    uint64_t row_par;        /* f32 [rows][4]: l0, l1, c0, c1                         */
+    uint64_t row_par;        /* f32 [rows][4]: l0, l1, c0, c1 (without DUAL: not 0 if the row has a gradient) */
     uint64_t part;           /* f32 [chunks][rows][2]: m and the sum                  */
     uint64_t part2;          /* f32 [chunks][rows]: the second sum (DUAL)             */
     uint64_t z;              /* f32 [rows][ldz]: a piece's raw logits                 */

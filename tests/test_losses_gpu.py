@@ -671,3 +671,18 @@ def test_weight_past_32_bits(rt, rows):
         rt.wait_idle()
         for a in held:
             rt.free(a)
+
+
+# ---- weights, temperatures and masks beyond the usual ones ------------------------------
+
+@pytest.mark.parametrize("rows,vocab,hidden,top,tau,a,b,max_piece", [
+    (1, 40, 16, 1, 1.0, 1.0, -1.0, 0), (5, 300, 64, 7, 1.0, 1.0, -1.0, 0), (140, 17000, 64, 9, 1.0, -0.5, 0.5, 0),
+    (40, 1003, 64, 70, 1.0, 2.0, -2.0, 256), (300, 2051, 72, 20, 1.0, 1.0, -1.0, 0), (300, 2051, 72, 90, 1.0, -1.0, 1.0, 512),
+    (300, 700, 64, 12, 2.0, 1.0, -0.5, 0)])
+def test_weights_that_cancel(rt, rows, vocab, hidden, top, tau, a, b, max_piece):
+    """Of labels and teacher with one softmax: the dense parts of the gradient cancel, G = rate a (Q - onehot) remains."""
+    c = Case(rows, vocab, hidden, seed=100 + rows + top).teach(top, tau, a, b)
+    if rows > 3:
+        c.labels[2] = -100
+        c.tokens[3] = -1
+    c.check(rt, f"weights {a} and {b}", max_piece=max_piece)
