@@ -11,7 +11,8 @@
 // in one of two forms:
 //   fused     the statistics are taken in the logits GEMM's epilogue (losses_tile.h), which
 //             for the last piece also leaves its exponentials, 16 bits each, where G goes;
-//             the other pieces' logits are computed again with G in the epilogue
+//             the other pieces' logits are computed again with G in the epilogue (so are the
+//             last's at a temperature that its exponentials cannot be taken to)
 //   by rows   a piece's f32 logits go to the scratch and row kernels read them: products
 //             of few rows, and operands that the 256x256 tile does not take
 // By rows, labels alone need no preparation (each kernel reads them), and a vocabulary that
@@ -62,6 +63,13 @@ constexpr uint32_t kPairRows = 128;
 // 130, 777 rows 255 / 188; with gradients over 20001 tokens 300 rows 146 / 158, 777 rows 271 / 243.
 constexpr uint32_t kCopyRows = 512;
 constexpr uint64_t kCopyBytes = 512ull << 20;
+// Temperatures T at which the kept exponentials of the labels' softmax give the teacher's as well, to the
+// power 1 / T.  What is below 2^-126 of its block's maximum is lost and would be 2^(-126 / T): with T up
+// to 4 all of a block's other tokens together 127 2^-31.5 < 2^-24 of the maximum's probability.  Their
+// cutting, 0.7 2^-9, grows by 1 / T: from 0.5 on it stays below G's own rounding of 2^-8.  Other
+// temperatures take a second product of the last piece (2048 rows of 32000 tokens, width 2048: 931 us
+// against 769; 300 of 50000, width 768: 223 against 183).
+constexpr float kKeepMinT = 0.5f, kKeepMaxT = 4.0f;
 // Rows of a launch's y grid, at most (the kernels step through the rest).
 constexpr uint32_t kMaxGridY = 65535;
 
@@ -165,6 +173,7 @@ struct Piece {
 struct Plan {
     std::vector<Piece> pieces;
     bool fused = false;
+    bool keep = false;           // fused, gradients: the last piece's exponentials are kept
     bool copy_w = false;         // the pieces' weights are copied
     bool copy_x = false;         // products take xz instead of x
     bool direct = false;         // by rows, labels alone
@@ -310,6 +319,7 @@ int make_loss_plan(const Problem &p, Plan *pl) {
     const bool sparse = !p.t || form == T0G_LOSS_FORM_FUSED || (uint64_t)p.t->top_k * T0G_LOSS_BLOCK <= kFusedEntries * d.vocab;
     pl->fused = form != T0G_LOSS_FORM_ROWS && worth && sparse && pl->padded && d.rows * ldx < (1ull << 30) && (d.max_piece == 0 || d.max_piece >= 256) &&
                 (nt ? ldw * 256 < (1ull << 30) : pl->copy_w || (d.ldw >= 256 && d.hidden * ldw < (1ull << 30)));
+    pl->keep = pl->fused && p.grad && !(p.dual && !(p.t->temperature >= kKeepMinT && p.t->temperature <= kKeepMaxT));
     // xz is dW's operand; the logits' too where x itself is not aligned like the weight, and
     // wherever it is there before them
     pl->copy_x = (pl->padded && !x_aligned) || (p.grad && (pl->fused || p.t));
@@ -606,7 +616,7 @@ int run_loss(t0g_device *dev, const Problem &p) {
         at_piece(pc);
         if (pl.copy_w && (rc = run_copy(dev, p, pl, pc, base))) return rc;
         if (pl.fused)
-            rc = run_tile(dev, p.grad && i + 1 == n ? Tile::Keep : Tile::Stats, p, pl, pc, a, base);
+            rc = run_tile(dev, pl.keep && i + 1 == n ? Tile::Keep : Tile::Stats, p, pl, pc, a, base);
         else if (!(rc = run_gemm(dev, logits_gemm(p, pl, pc, base), pl, base)) && !one)
             rc = piece_kernel("t0g_loss_stats", pc.chunks);
         if (rc) return rc;
@@ -634,7 +644,7 @@ int run_loss(t0g_device *dev, const Problem &p) {
         const Piece &pc = pl.pieces[i];
         at_piece(pc);
         if (pl.copy_w && i + 1 < n && (rc = run_copy(dev, p, pl, pc, base))) return rc;
-        if (pl.fused && i + 1 == n) {
+        if (pl.keep && i + 1 == n) {
             rc = piece_kernel("t0g_loss_grad_kept", (a.ldg + 2047) / 2048);
         } else if (pl.fused) {
             if (!(rc = run_tile(dev, Tile::Grad, p, pl, pc, a, base))) rc = row_kernel("t0g_loss_grad_entries", 4);

@@ -686,3 +686,13 @@ def test_weights_that_cancel(rt, rows, vocab, hidden, top, tau, a, b, max_piece)
         c.labels[2] = -100
         c.tokens[3] = -1
     c.check(rt, f"weights {a} and {b}", max_piece=max_piece)
+
+
+@pytest.mark.parametrize("max_piece", [0, 512])
+@pytest.mark.parametrize("amp,tau", [(30.0, 20.0), (60.0, 50.0), (60.0, 4.5), (60.0, 4.0), (4.0, 0.1), (4.0, 0.4)])
+def test_temperatures_on_wide_logits(rt, amp, tau, max_piece):
+    """Tokens far below the others, which the labels' softmax has lost and the teacher's at its temperature has not, and
+    a temperature that sharpens.  (1500 tokens: a dW column is the sum of few rows' gradients.)"""
+    c = Case(300, 1500, 64, seed=int(10 * tau), amp=amp).teach(20, tau, 0.5, 0.5)
+    c.labels[:100] = (c.x[:100].double() @ c.w.double().t()).argmax(1)
+    c.check(rt, f"amplitude {amp} at {tau}", max_piece=max_piece)
