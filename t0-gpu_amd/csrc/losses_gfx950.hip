@@ -387,13 +387,14 @@ __device__ __forceinline__ void reduce_logits(const T0gLossArgs& p, const f32x4_
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) m = __builtin_fmaxf(m, v[i][e]);
     m = block_max<W>(m, red[0]);
+    const float from = m == ninf() ? 0.0f : m;   // no token left of these: sums of 0, not of 2^(-inf + inf)
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i)
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) {
             if ((i * (64 * W) + threadIdx.x) * 4 + e >= n) continue;
-            s += exp2_(v[i][e] - m);
-            if (p.flags & T0G_LOSS_DUAL) s2 += exp2_((v[i][e] - m) * p.r);
+            s += exp2_(v[i][e] - from);
+            if (p.flags & T0G_LOSS_DUAL) s2 += exp2_((v[i][e] - from) * p.r);
         }
     s = block_sum<W>(s, red[1]);
     if (p.flags & T0G_LOSS_DUAL) s2 = block_sum<W>(s2, red[2]);

@@ -156,7 +156,7 @@ __device__ __forceinline__ void tile_stats(const T0gLossGemmArgs& a, const f32x4
     auto pick = [&](auto band) { pick_band<band.value>(a, acc, scan, row0, col0, lane, pick_lds); };
     auto stats = [&](int i) {
         __builtin_amdgcn_sched_barrier(0);   // one band at a time
-        float z[SN][4], m[4], s[4], s2[4];
+        float z[SN][4], m[4], from[4], s[4], s2[4];
 #pragma unroll
         for (int j = 0; j < SN; ++j)
 #pragma unroll
@@ -173,6 +173,7 @@ __device__ __forceinline__ void tile_stats(const T0gLossGemmArgs& a, const f32x4
             for (int j = 1; j < SN; ++j) m[r] = max_(m[r], z[j][r]);
             m[r] = KEEP ? __builtin_fmaf(row16_max(m[r]), a.k, -kKeepLog2) : row16_max(m[r]) * a.k;
             m[r] = width ? m[r] : 0.0f;   // no columns: every exponential below is 2^-inf
+            from[r] = m[r] == ninf() ? 0.0f : m[r];   // no token left: sums of 0, not of 2^(-inf + inf)
             s[r] = s2[r] = 0.0f;
         }
         if (a.flags & T0G_LOSS_DUAL) {
@@ -180,7 +181,7 @@ __device__ __forceinline__ void tile_stats(const T0gLossGemmArgs& a, const f32x4
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int j = 0; j < SN; ++j) s2[r] += exp2_(__builtin_fmaf(z[j][r], k2, -(m[r] * a.r)));
+                for (int j = 0; j < SN; ++j) s2[r] += exp2_(__builtin_fmaf(z[j][r], k2, -(from[r] * a.r)));
 #pragma unroll
             for (int r = 0; r < 4; ++r) s2[r] = row16_sum(s2[r]);
         }
@@ -188,7 +189,7 @@ __device__ __forceinline__ void tile_stats(const T0gLossGemmArgs& a, const f32x4
         for (int j = 0; j < SN; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                z[j][r] = exp2_(__builtin_fmaf(z[j][r], a.k, -m[r]));
+                z[j][r] = exp2_(__builtin_fmaf(z[j][r], a.k, -from[r]));
                 s[r] += z[j][r];
             }
 #pragma unroll

@@ -696,3 +696,35 @@ def test_temperatures_on_wide_logits(rt, amp, tau, max_piece):
     c = Case(300, 1500, 64, seed=int(10 * tau), amp=amp).teach(20, tau, 0.5, 0.5)
     c.labels[:100] = (c.x[:100].double() @ c.w.double().t()).argmax(1)
     c.check(rt, f"amplitude {amp} at {tau}", max_piece=max_piece)
+
+
+@pytest.mark.parametrize("value", [-float("inf"), -3.3895313892515355e38])
+@pytest.mark.parametrize("rows,vocab,taught,max_piece", [
+    (4, 2051, False, 0), (4, 2051, True, 256), (40, 20000, False, 0), (40, 20000, True, 0),
+    (300, 2051, False, 0), (300, 2051, True, 0), (300, 2051, False, 256), (300, 2051, True, 512)])
+def test_tokens_masked_by_a_bias(rt, rows, vocab, taught, max_piece, value):
+    """The first hidden value is 1 and the weight's first column a bias that is -infinity or the type's lowest
+    value for most of the vocabulary, whole blocks, chunks and pieces of it: as if those tokens were not there.  An
+    infinite weight has no dx (0 times infinity)."""
+    hidden = 64
+    c = Case(rows, vocab, hidden, seed=120 + rows, want="w" if value == -float("inf") else "xw")
+    seen = torch.cat([torch.arange(300, 500), torch.arange(1100, 1160), torch.tensor([vocab - 1])])
+    few = Case(rows, len(seen), hidden, seed=121 + rows, want=c.want)
+    c.x[:, 0], c.w[:, 0] = 1.0, 0.0
+    few.x, few.w, few.dloss = c.x, c.w[seen].clone(), c.dloss
+    if taught:
+        few.teach(12, 2.0, 0.5, 0.5)
+        c.teach(12, 2.0, 0.5, 0.5)
+        c.tokens, c.teacher = seen[few.tokens], few.teacher
+    c.labels = seen[few.labels]
+    hidden_tokens = torch.ones(vocab, dtype=torch.bool)
+    hidden_tokens[seen] = False
+    c.w[hidden_tokens, 0] = value
+    got = c.run(rt, max_piece=max_piece)
+    c.untouched()
+    assert not bool(got["dw"][hidden_tokens].double().abs().any())
+    got["dw"] = got["dw"][seen]
+    for k, (v, tol) in few.define().items():
+        worst = float(((got[k].double() - v).abs() / tol).max())
+        _log(f"[loss] masked {rows}x{vocab} {k}: {worst:.3f} of the bound")
+        assert bool(((got[k].double() - v).abs() <= tol).all()), k
