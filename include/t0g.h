@@ -518,7 +518,10 @@ T0G_API int t0g_matmul_kernel_name(uint32_t op, uint32_t m, uint32_t k, uint32_t
  * pieces, copies of x and of an unaligned piece of w) belongs to the handle and grows on
  * a shape's first call.
  * Under stream capture it cannot grow: the call is refused unless the same call
- * ran before. */
+ * ran before.  A scratch that a captured call was given stays until the handle is closed,
+ * so its graph may be replayed after larger calls; but all calls and graphs of a handle share
+ * the scratch, so a graph's replays must be ordered with the handle's other work and with its
+ * other graphs. */
 typedef enum t0g_index_type { T0G_I32 = 0, T0G_I64 = 1 } t0g_index_type;
 typedef struct t0g_linear_ce_desc {
     uint64_t x;                     /* bf16 [rows][ldx]: hidden states                 */

@@ -19,6 +19,7 @@
 #include <set>
 #include <string>
 #include <unordered_map>
+#include <unordered_set>
 #include <vector>
 
 #include "t0g.h"
@@ -106,6 +107,9 @@ struct t0g_device {
     uint64_t pool_hits = 0, pool_misses = 0;
     uint64_t ws = 0;
     size_t ws_bytes = 0;
+    // Scratch that a captured call was given: its address is in a graph, so the block stays
+    // until the handle is closed, also when a larger one takes its place.
+    std::unordered_set<uint64_t> captured;
     uint64_t conv = 0;         // bf16 operand scratch of the matmul entry points
     size_t conv_bytes = 0;
     // GpuRuntime::bf16_cache (src/ignis/gpu_context.rs:100): tensor id -> its bf16 copy.
@@ -170,6 +174,18 @@ static std::atomic<uint64_t> g_device_allocs{0};
 static hipError_t dev_malloc(void **p, size_t bytes) {
     g_device_allocs.fetch_add(1);
     return hipMalloc(p, bytes);
+}
+
+// A call is given the scratch block at addr.
+static void give_scratch(t0g_device *dev, uint64_t addr) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(dev->stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone)
+        dev->captured.insert(addr);
+}
+
+// A larger block takes the place of the one at addr.
+static hipError_t drop_scratch(t0g_device *dev, uint64_t addr) {
+    return dev->captured.count(addr) ? hipSuccess : T0G_HIP(hipFree((void *)addr));   // hipFree waits for work using it
 }
 
 static hipError_t module_load(hipModule_t *m, const void *image) {
@@ -918,7 +934,8 @@ int t0g_device_close(t0g_device *dev) {
     if (!dev->poisoned) (void)hipStreamSynchronize(dev->stream);
     if (dev->ws) (void)hipFree((void *)dev->ws);
     if (dev->conv) (void)hipFree((void *)dev->conv);
-    if (dev->loss) (void)hipFree((void *)dev->loss);
+    if (dev->loss) (void)drop_scratch(dev, dev->loss);
+    for (uint64_t a : dev->captured) (void)hipFree((void *)a);
     if (dev->sk_sync) (void)hipFree((void *)dev->sk_sync);
     for (int i = 0; i < t0g_device::kSides; ++i) {
         if (dev->side[i]) {
@@ -1783,7 +1800,7 @@ int losses_begin(t0g_device *dev, size_t bytes, uint64_t *scratch) {
         if ((rc = ensure_sk_sync(dev))) return rc;
         if (dev->loss_bytes < bytes) {
             if (dev->loss) {
-                e = T0G_HIP(hipFree((void *)dev->loss));   // waits for work using it
+                e = drop_scratch(dev, dev->loss);
                 dev->loss = 0;
                 dev->loss_bytes = 0;
                 if (e != hipSuccess) return poison(dev, hip_fail(e, "hipFree(loss scratch)"));
@@ -1794,6 +1811,7 @@ int losses_begin(t0g_device *dev, size_t bytes, uint64_t *scratch) {
             dev->loss_bytes = bytes;
         }
     }
+    give_scratch(dev, dev->loss);
     *scratch = dev->loss;
     return T0G_OK;
 }

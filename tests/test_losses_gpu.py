@@ -728,3 +728,41 @@ def test_tokens_masked_by_a_bias(rt, rows, vocab, taught, max_piece, value):
         worst = float(((got[k].double() - v).abs() / tol).max())
         _log(f"[loss] masked {rows}x{vocab} {k}: {worst:.3f} of the bound")
         assert bool(((got[k].double() - v).abs() <= tol).all()), k
+
+
+def test_a_graph_outlives_a_larger_scratch(form):
+    """A captured call's scratch stays when a larger call takes a larger one, twice: replays give the eager
+    bits, with buffers of every size taken and filled in between."""
+    size = t0g.linear_loss_scratch_size
+    with t0g.GpuRuntime.new(0) as fresh:
+        c = Case(300, 2000, 64, seed=140).teach(20, 2.0, 0.5, 0.5)
+        want = c.run(fresh, keep=True)
+        side = hip_rt.Stream()
+        fresh.set_stream(side.ptr)
+        graph, last = None, size(c.desc)
+        try:
+            graph = hip_rt.Graph(side, lambda: c.call(c.desc))
+            for rows, vocab in ((400, 6000), (500, 20000)):
+                larger = Case(rows, vocab, 72, seed=rows)
+                larger.check(fresh, "larger call after a capture")
+                assert size(larger.desc) > last + (1 << 20)
+                filled = [fresh.alloc(n) for n in (last, last, last // 2, last // 4)]
+                for addr, n in zip(filled, (last, last, last // 2, last // 4)):
+                    fresh.memset(addr, 0xFF, n)
+                last = size(larger.desc)
+                for _ in range(2):
+                    c.refill(fresh)
+                    graph.launch(side)
+                    got = c.read(fresh)
+                    for k in want:
+                        assert torch.equal(got[k], want[k]), k
+                    larger.check(fresh, "between replays")
+                for addr in filled:
+                    fresh.free(addr)
+        finally:
+            fresh.set_stream(0)
+            fresh.wait_idle()
+            if graph:
+                graph.destroy()
+            side.destroy()
+            c.free(fresh)
