@@ -241,7 +241,10 @@ T0G_API int t0g_device_close(t0g_device *dev);
 /* Run subsequent work on a caller-owned hipStream_t (NULL: back to the device's own).
  * On a change of stream the new stream first waits for the work issued on the
  * old one (the handle's split-K workspace and control block are shared by all
- * its launches, so they must not run at the same time). */
+ * its launches, so they must not run at the same time).  A call under stream capture
+ * leaves the address of the handle's scratch in the graph; such a block stays until the
+ * handle is closed, also after larger calls took larger ones, and the graph's replays must
+ * be ordered with the handle's other work and with its other graphs. */
 T0G_API int t0g_device_set_stream(t0g_device *dev, void *hip_stream);
 T0G_API int t0g_device_get_stream(t0g_device *dev, void **hip_stream);
 T0G_API int t0g_device_is_poisoned(t0g_device *dev, int *poisoned);
@@ -518,10 +521,7 @@ T0G_API int t0g_matmul_kernel_name(uint32_t op, uint32_t m, uint32_t k, uint32_t
  * pieces, copies of x and of an unaligned piece of w) belongs to the handle and grows on
  * a shape's first call.
  * Under stream capture it cannot grow: the call is refused unless the same call
- * ran before.  A scratch that a captured call was given stays until the handle is closed,
- * so its graph may be replayed after larger calls; but all calls and graphs of a handle share
- * the scratch, so a graph's replays must be ordered with the handle's other work and with its
- * other graphs. */
+ * ran before.  (Of a captured call's scratch: t0g_device_set_stream.) */
 typedef enum t0g_index_type { T0G_I32 = 0, T0G_I64 = 1 } t0g_index_type;
 typedef struct t0g_linear_ce_desc {
     uint64_t x;                     /* bf16 [rows][ldx]: hidden states                 */

@@ -478,9 +478,12 @@ static int check_extent(const char *what, uint64_t rows, uint64_t ld) {
 }
 
 static int ensure_workspace(t0g_device *dev, size_t bytes) {
-    if (dev->ws_bytes >= bytes) return T0G_OK;
+    if (dev->ws_bytes >= bytes) {
+        if (dev->ws) give_scratch(dev, dev->ws);
+        return T0G_OK;
+    }
     if (dev->ws) {
-        hipError_t e = T0G_HIP(hipFree((void *)dev->ws));   // hipFree waits for work using it
+        hipError_t e = drop_scratch(dev, dev->ws);
         dev->ws = 0;
         dev->ws_bytes = 0;
         if (e != hipSuccess) return poison(dev, hip_fail(e, "hipFree(workspace)"));
@@ -490,6 +493,7 @@ static int ensure_workspace(t0g_device *dev, size_t bytes) {
     if (e != hipSuccess) return hip_fail(e, "hipMalloc(workspace)");
     dev->ws = (uint64_t)p;
     dev->ws_bytes = bytes;
+    give_scratch(dev, dev->ws);
     return T0G_OK;
 }
 
@@ -932,20 +936,20 @@ int t0g_device_close(t0g_device *dev) {
     if (!dev) return ok();
     (void)hipSetDevice(dev->ordinal);
     if (!dev->poisoned) (void)hipStreamSynchronize(dev->stream);
-    if (dev->ws) (void)hipFree((void *)dev->ws);
-    if (dev->conv) (void)hipFree((void *)dev->conv);
+    if (dev->ws) (void)drop_scratch(dev, dev->ws);
+    if (dev->conv) (void)drop_scratch(dev, dev->conv);
     if (dev->loss) (void)drop_scratch(dev, dev->loss);
-    for (uint64_t a : dev->captured) (void)hipFree((void *)a);
     if (dev->sk_sync) (void)hipFree((void *)dev->sk_sync);
     for (int i = 0; i < t0g_device::kSides; ++i) {
         if (dev->side[i]) {
             if (!dev->poisoned) (void)hipStreamSynchronize(dev->side[i]);
             (void)hipStreamDestroy(dev->side[i]);
         }
-        if (dev->side_ws[i]) (void)hipFree((void *)dev->side_ws[i]);
+        if (dev->side_ws[i]) (void)drop_scratch(dev, dev->side_ws[i]);
         if (dev->join_ev[i]) (void)hipEventDestroy(dev->join_ev[i]);
     }
     if (dev->fork_ev) (void)hipEventDestroy(dev->fork_ev);
+    for (uint64_t a : dev->captured) (void)hipFree((void *)a);
     for (const auto &a : dev->allocations) (void)hipFree((void *)a.first);
     for (const auto &c : dev->bf16_cache) (void)hipFree((void *)c.second.addr);
     for (const auto &bucket : dev->pool)
@@ -2053,9 +2057,12 @@ static bool staged_f32_wins(uint32_t m, uint32_t n, uint32_t k, uint32_t transpo
 }
 
 static int ensure_conv(t0g_device *dev, size_t bytes) {
-    if (dev->conv_bytes >= bytes) return T0G_OK;
+    if (dev->conv_bytes >= bytes) {
+        give_scratch(dev, dev->conv);
+        return T0G_OK;
+    }
     if (dev->conv) {
-        hipError_t e = T0G_HIP(hipFree((void *)dev->conv));   // waits for work using it
+        hipError_t e = drop_scratch(dev, dev->conv);
         dev->conv = 0;
         dev->conv_bytes = 0;
         if (e != hipSuccess) return poison(dev, hip_fail(e, "hipFree(conversion scratch)"));
@@ -2065,6 +2072,7 @@ static int ensure_conv(t0g_device *dev, size_t bytes) {
     if (e != hipSuccess) return hip_fail(e, "hipMalloc(conversion scratch)");
     dev->conv = (uint64_t)p;
     dev->conv_bytes = bytes;
+    give_scratch(dev, dev->conv);
     return T0G_OK;
 }
 
