@@ -18,7 +18,8 @@
 // By rows, labels alone need no preparation (each kernel reads them), and a vocabulary that
 // one workgroup's registers hold takes its statistics, loss and G in one kernel.
 // A weight whose rows are not whole 16-byte pieces is copied into ones that are, piece by
-// piece, when there are rows enough to make up for that.
+// piece, when there are rows enough to make up for that, or when it is too large for the
+// GEMMs' unaligned kernels.
 #include <math.h>
 #include <string.h>
 
@@ -300,13 +301,14 @@ bool outer_dw(const Problem &p, const Plan &pl) {
     return pl.pair && p.d.rows <= (p.d.transpose == T0G_NT ? 64u : 32u) && (uint64_t)p.d.vocab * p.d.hidden >= kOuterSize;
 }
 
-int make_loss_plan(const Problem &p, Plan *pl) {
+// bounded: every product takes less of the weight than 2^30 values.
+int plan_pieces(const Problem &p, bool bounded, Plan *pl) {
     const t0g_linear_ce_desc &d = p.d;
     const uint64_t rows = d.rows ? d.rows : 1;
     const bool nt = d.transpose == T0G_NT;
     const bool aligned = (d.w & 15) == 0 && d.ldw % 8 == 0 && (nt ? d.hidden : d.vocab) % 8 == 0;
     const bool x_aligned = (d.x & 15) == 0 && d.ldx % 8 == 0 && d.hidden % 8 == 0;
-    pl->copy_w = !aligned && d.rows >= kCopyRows;
+    pl->copy_w = (!aligned && d.rows >= kCopyRows) || (bounded && !nt);
     pl->padded = aligned || pl->copy_w;
     pl->ldxz = round_up(d.hidden, 8);
     // the 256x256 tile takes 32-bit byte offsets, and rows of 256 or more of a weight
@@ -331,7 +333,7 @@ int make_loss_plan(const Problem &p, Plan *pl) {
         width = kPieceBytes / (rows * 4);
     else if (p.grad)
         width = kFusedPieceBytes / 2 / round_up(d.rows, 256);
-    if (pl->fused && nt) width = std::min<uint64_t>(width, ((1ull << 30) - 1) / ldw);
+    if ((pl->fused || bounded) && nt) width = std::min<uint64_t>(width, ((1ull << 30) - 1) / ldw);
     if (pl->copy_w) width = std::min<uint64_t>(width, kCopyBytes / 2 / pl->ldxz);
     width = width >= d.vocab ? round_up(d.vocab, 256) : std::max<uint64_t>(256, width / 256 * 256);
     if (d.max_piece) {
@@ -416,6 +418,20 @@ int make_loss_plan(const Problem &p, Plan *pl) {
     pl->gemm_ws = take(pl->gemm_ws_bytes);
     pl->bytes = at;
     return T0G_OK;
+}
+
+uint64_t weight_span(const t0g_linear_ce_desc &d) { return (uint64_t)(d.transpose == T0G_NT ? d.vocab : d.hidden) * d.ldw; }
+
+// The GEMMs take operands of any size in whole 16-byte pieces and below 2^31 values otherwise.  A larger
+// weight goes in pieces below that where a product would refuse the whole: narrower ones of rows of tokens,
+// copies of a few tokens' columns.
+int make_loss_plan(const Problem &p, Plan *pl) {
+    int rc = plan_pieces(p, false, pl);
+    if (rc == T0G_ERR_INVALID_ARG && weight_span(p.d) >= (1ull << 31)) {
+        *pl = Plan();
+        rc = plan_pieces(p, true, pl);
+    }
+    return rc;
 }
 
 int run_gemm(t0g_device *dev, t0g_gemm_desc g, const Plan &pl, uint64_t base) {

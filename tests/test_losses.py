@@ -100,3 +100,15 @@ def test_scratch_stays_below_the_logits():
     assert scratch(8192) < 2.5 * 2 ** 30
     assert scratch(65536) < 6 * 2 ** 30
     assert scratch(8192, max_piece=8192) < 0.75 * 2 ** 30
+
+
+@pytest.mark.parametrize("layout", ["NT", "NN"])
+@pytest.mark.parametrize("want", ["", "x", "w", "xw"])
+@pytest.mark.parametrize("rows,vocab,hidden", [
+    (1, 140001, 16384), (5, 140000, 16385), (100, 140001, 16385), (129, 140000, 16385), (300, 1000003, 4097),
+    (511, 32001, 100001), (2000, 140000, 16385), (3, 1 << 23, 1024), (1, (1 << 24) + 8, 512)])
+def test_large_weights_of_unaligned_operands(rows, vocab, hidden, want, layout):
+    """Weights of 2^31 values and more: what the unaligned products cannot take whole goes in pieces, of at most 2^30 values."""
+    d = t0g.linear_ce_desc(1 << 40, 1 << 44, 1 << 20, 1 << 21, rows, vocab, hidden, transpose=layout,
+                           dx=(1 << 46) * ("x" in want), dw=(1 << 48) * ("w" in want))
+    assert 0 < t0g.linear_loss_scratch_size(d) < 4 << 30

@@ -766,3 +766,79 @@ def test_a_graph_outlives_a_larger_scratch(form):
                 graph.destroy()
             side.destroy()
             c.free(fresh)
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,layout,want", [
+    (5, 140000, 16385, "NT", "xw"), (5, 140001, 16384, "NT", "x"), (130, 140001, 16384, "NT", ""),
+    (5, 140001, 16384, "NN", "xw"), (140, 131080, 16385, "NN", "xw"), (2, 131080, 16385, "NN", "")])
+def test_weight_past_31_bits_of_unaligned_operands(rt, rows, vocab, hidden, layout, want):
+    """Weights of 2^31 values and more of which some product's operands are not whole 16-byte pieces.  Zero but for the
+    last 200 tokens, the definition and the bounds as in test_weight_past_32_bits."""
+    live = 200
+    first = vocab - live
+    nt = layout == "NT"
+    g = torch.Generator().manual_seed(rows + vocab)
+    x = torch.randn(rows, hidden, generator=g).bfloat16()
+    w = (2.0 * hidden ** -0.5 * torch.randn(live, hidden, generator=g)).bfloat16()
+    labels = torch.randint(0, vocab, (rows,), generator=g)
+    labels[1::2] = torch.randint(first, vocab, (rows // 2,), generator=g)
+    held = []
+
+    def up(t):
+        held.append(rt.upload(t.contiguous().view(torch.int16).numpy() if t.dtype == torch.bfloat16 else t.numpy()))
+        return held[-1]
+
+    try:
+        wa = rt.alloc_zero(2 * hidden * vocab)
+        held.append(wa)
+        if nt:
+            rt.write(wa + 2 * hidden * first, w.view(torch.int16).numpy())
+        else:
+            columns = w.t().contiguous().view(torch.int16).numpy()
+            for h in range(hidden):
+                rt.write(wa + 2 * (h * vocab + first), columns[h])
+        out = {"loss": rt.alloc(4 * rows), "dx": rt.alloc(4 * rows * hidden) if "x" in want else 0,
+               "dw": rt.alloc(4 * vocab * hidden) if "w" in want else 0}
+        held += [a for a in out.values() if a]
+        _log(f"{rows}x{vocab}x{hidden} {layout} {want}")
+        rt.linear_cross_entropy(t0g.linear_ce_desc(up(x), wa, up(labels), out["loss"], rows, vocab, hidden, transpose=layout,
+                                                   dx=out["dx"], dw=out["dw"], dx_dtype=t0g.F32, dw_dtype=t0g.F32))
+        rt.wait_idle()
+        xd, wd = x.double(), w.double()
+        z = xd @ wd.t()
+        lse = torch.log(torch.exp(z).sum(1) + first)
+        ez = float((hidden + 2) * U * (xd.abs() @ wd.abs().t()).max())
+        rel = 2.0 ** -8 + 0.7 * 2.0 ** -9 + 2 * ez + 2.0 ** -14
+        in_tail = labels >= first
+        zy = torch.where(in_tail, z[torch.arange(rows), (labels - first).clamp(min=0)], torch.zeros(rows, dtype=torch.float64))
+        loss = torch.from_numpy(rt.read(out["loss"], (rows,), "float32").copy()).double()
+        assert float((loss - (lse - zy)).abs().max()) <= 2 * ez + 2.0 ** -14 + 16 * U * 20
+        p = torch.exp(z - lse[:, None])
+        tail_labels = torch.zeros_like(p)
+        tail_labels[in_tail, (labels - first)[in_tail]] = 1.0
+        grad, size = p - tail_labels, p + tail_labels
+        if "x" in want:
+            dx = torch.from_numpy(rt.read(out["dx"], (rows, hidden), "float32").copy()).double()
+            assert bool(((dx - grad @ wd).abs() <= (rel + (vocab + 2) * U) * (size @ wd.abs())).all())
+        if "w" not in want:
+            return
+        # tokens, or hidden columns, of dW at its ends, inside and where a piece or a tile may end
+        for i in (0, 1, 255, 256, 8191, 16383) + ((131071, first - 1, int(labels[0]), vocab - 2, vocab - 1) if nt else (hidden - 1,)):
+            n = hidden if nt else vocab
+            got = torch.from_numpy(rt.read(out["dw"] + 4 * n * i, (n,), "float32").copy()).double()
+            if nt:
+                hit = (labels == i).double()
+                pi = p[:, i - first] if i >= first else torch.exp(-lse)
+                want_row, mag = (pi - hit) @ xd, (pi + hit) @ xd.abs()
+            else:
+                dense = (torch.exp(-lse) * xd[:, i]).sum()
+                want_row, mag = torch.full((vocab,), float(dense), dtype=torch.float64), torch.exp(-lse) @ xd.abs()[:, i]
+                mag = torch.full((vocab,), float(mag), dtype=torch.float64)
+                want_row[first:], mag[first:] = p.t() @ xd[:, i], p.t() @ xd.abs()[:, i]
+                want_row.index_add_(0, labels, -xd[:, i])
+                mag.index_add_(0, labels, xd.abs()[:, i])
+            assert bool(((got - want_row).abs() <= (rel + (rows + 2) * U) * mag).all()), i
+    finally:
+        rt.wait_idle()
+        for a in held:
+            rt.free(a)
