@@ -513,6 +513,10 @@ T0G_API int t0g_matmul_kernel_name(uint32_t op, uint32_t m, uint32_t k, uint32_t
  * row with neither label nor teacher's token has loss 0, lse 0 and no gradient,
  * whatever its hidden state holds (NaN included).
  *
+ * Operands may have any size and 2-byte alignment, but for hidden states that span 2^31
+ * elements or more: those take a hidden size and a vocabulary that are multiples of 8
+ * (and 256 tokens at least if w is NN).
+ *
  * Products, statistics and losses are f32 on bf16 operands.  The logits' gradient
  * is rounded to bf16 once, as an operand of the products that give dx and dw.
  * Results do not depend on what ran before: no atomics, sums in a fixed order.

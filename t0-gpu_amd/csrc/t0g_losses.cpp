@@ -180,7 +180,7 @@ struct Plan {
     bool direct = false;         // by rows, labels alone
     bool pair = false;           // G in two bf16, rows of g and xz twice
     bool padded = false;         // every operand's rows are whole 16-byte pieces
-    uint32_t chunks = 0, slots = 0, ldxz = 0, off_ld = 0;
+    uint32_t chunks = 0, slots = 0, ldxz = 0, off_ld = 0, least_ldg = 8;
     uint32_t group = 0;          // products of dx summed at a time (0: the one product writes dx)
     uint32_t splits = 1;         // pair: planes of each product and half
     uint32_t ldp = 0;
@@ -212,7 +212,9 @@ t0g_gemm_desc gemm_of(uint64_t a, uint64_t b, uint64_t c, uint32_t m, uint32_t n
 }
 
 // G's leading dimension; the fused form stores whole tiles.
-uint32_t ld_of_g(const Plan &pl, const Piece &pc) { return round_up(pc.cols, pl.fused ? 256 : 8); }
+uint32_t ld_of_g(const Plan &pl, const Piece &pc) {
+    return std::max(round_up(pc.cols, pl.fused ? 256 : 8), pl.least_ldg);
+}
 
 uint64_t weight_piece(const Problem &p, uint64_t w, uint32_t v0, uint32_t ld, uint32_t size) {
     return w + (p.d.transpose == T0G_NT ? (uint64_t)v0 * ld : v0) * size;
@@ -311,6 +313,8 @@ int plan_pieces(const Problem &p, bool bounded, Plan *pl) {
     pl->copy_w = (!aligned && d.rows >= kCopyRows) || (bounded && !nt);
     pl->padded = aligned || pl->copy_w;
     pl->ldxz = round_up(d.hidden, 8);
+    // the GEMMs take operands past 2^30 values (here dW's) with leading dimensions of 256 and more
+    if (rows * pl->ldxz >= (1ull << 30)) pl->least_ldg = 256;
     // the 256x256 tile takes 32-bit byte offsets, and rows of 256 or more of a weight
     // [hidden][vocab] (a copied piece has them)
     const uint64_t ldx = std::max(pl->ldxz, d.ldx), ldw = pl->copy_w ? pl->ldxz : d.ldw;
@@ -388,7 +392,7 @@ int plan_pieces(const Problem &p, bool bounded, Plan *pl) {
         if (p.grad) pl->g = take((uint64_t)round_up(d.rows, 256) * round_up(widest, 256) * 2);
     } else {
         pl->z = take(rows * round_up(widest, 4) * 4);
-        if (p.grad) pl->g = take(halves * rows * round_up(widest, 8) * 2);
+        if (p.grad) pl->g = take(halves * rows * ld_of_g(*pl, Piece{0, widest, 0, 0}) * 2);
     }
     if (pl->group) {
         uint32_t splits = 1;
@@ -431,6 +435,10 @@ int make_loss_plan(const Problem &p, Plan *pl) {
         *pl = Plan();
         rc = plan_pieces(p, true, pl);
     }
+    const uint64_t span = (uint64_t)p.d.rows * std::max(p.d.ldx, p.d.hidden);
+    if (rc == T0G_ERR_INVALID_ARG && span >= (1ull << 31))
+        return fail(rc, "x spans %llu elements: from 2^31 on the hidden size and the vocabulary must be multiples of 8",
+                    (unsigned long long)span);
     return rc;
 }
 

@@ -109,6 +109,21 @@ def test_scratch_stays_below_the_logits():
     (511, 32001, 100001), (2000, 140000, 16385), (3, 1 << 23, 1024), (1, (1 << 24) + 8, 512)])
 def test_large_weights_of_unaligned_operands(rows, vocab, hidden, want, layout):
     """Weights of 2^31 values and more: what the unaligned products cannot take whole goes in pieces, of at most 2^30 values."""
-    d = t0g.linear_ce_desc(1 << 40, 1 << 44, 1 << 20, 1 << 21, rows, vocab, hidden, transpose=layout,
+    d = t0g.linear_ce_desc(1 << 40, 1 << 44, 1 << 30, 1 << 31, rows, vocab, hidden, transpose=layout,
                            dx=(1 << 46) * ("x" in want), dw=(1 << 48) * ("w" in want))
     assert 0 < t0g.linear_loss_scratch_size(d) < 4 << 30
+
+
+@pytest.mark.parametrize("layout", ["NT", "NN"])
+@pytest.mark.parametrize("want", ["", "x", "w", "xw"])
+def test_hidden_states_past_31_bits(want, layout):
+    """Taken with sizes that are multiples of 8, also where the last piece of the vocabulary is narrow; else refused by name."""
+    def desc(rows, vocab, hidden, **kw):
+        return t0g.linear_ce_desc(1 << 40, 1 << 44, 1 << 30, 1 << 31, rows, vocab, hidden, transpose=layout,
+                                  dx=(1 << 46) * ("x" in want), dw=(1 << 48) * ("w" in want), **kw)
+    for d in (desc(300000, 140000, 16384), desc(600000, 1000, 4096), desc(1 << 20, 264, 2056), desc(300000, 1024, 8192, ldx=8200),
+              desc(300000, 1024, 8192, ldx=8193)):
+        assert t0g.linear_loss_scratch_size(d) > 0
+    refused(desc(300000, 32000, 8193), "x spans 2457900000")
+    if layout == "NN" or "w" in want:
+        refused(desc(300000, 32001, 8192), "x spans")

@@ -842,3 +842,57 @@ def test_weight_past_31_bits_of_unaligned_operands(rt, rows, vocab, hidden, layo
         rt.wait_idle()
         for a in held:
             rt.free(a)
+
+
+def test_hidden_states_past_31_bits(rt):
+    """300000 rows of 8192 (4.9 GB), zero but for ten of them around where byte and element offsets pass 31 and 32 bits,
+    over a vocabulary narrower than a tile.  Of a zero row the logits are 0 and G = rate (1/V - onehot); bounds as in
+    test_weight_past_32_bits, and dx is rounded to bf16."""
+    rows, vocab, hidden = 300000, 232, 8192
+    g = torch.Generator().manual_seed(150)
+    live = torch.tensor([0, 1, 5, 131071, 131072, 262143, 262144, 262145, 299998, 299999])
+    x = torch.randn(len(live), hidden, generator=g).bfloat16()
+    w = (2.0 * hidden ** -0.5 * torch.randn(vocab, hidden, generator=g)).bfloat16()
+    labels = torch.randint(0, vocab, (rows,), generator=g)
+    held = []
+
+    def up(t):
+        held.append(rt.upload(t.contiguous().view(torch.int16).numpy() if t.dtype == torch.bfloat16 else t.numpy()))
+        return held[-1]
+
+    try:
+        xa = rt.alloc_zero(2 * rows * hidden)
+        held.append(xa)
+        for i, row in zip(live.tolist(), x):
+            rt.write(xa + 2 * hidden * i, row.view(torch.int16).numpy())
+        loss, dx, dw = rt.alloc(4 * rows), rt.alloc(2 * rows * hidden), rt.alloc(4 * vocab * hidden)
+        held += [loss, dx, dw]
+        _log("300000x232x8192")
+        rt.linear_cross_entropy(t0g.linear_ce_desc(xa, up(w), up(labels), loss, rows, vocab, hidden, dx=dx, dw=dw,
+                                                   dw_dtype=t0g.F32))
+        rt.wait_idle()
+        xd, wd = x.double(), w.double()
+        z = xd @ wd.t()
+        ez = float((hidden + 2) * U * (xd.abs() @ wd.abs().t()).max())
+        rel = 2.0 ** -8 + 0.7 * 2.0 ** -9 + 2 * ez + 2.0 ** -14
+        want = torch.full((rows,), float(torch.log(torch.tensor(float(vocab), dtype=torch.float64))), dtype=torch.float64)
+        want[live] = torch.logsumexp(z, 1) - z.gather(1, labels[live][:, None])[:, 0]
+        got = torch.from_numpy(rt.read(loss, (rows,), "float32").copy()).double()
+        assert float((got - want).abs().max()) <= 2 * ez + 2.0 ** -14 + 16 * U * 20
+        onehot = torch.nn.functional.one_hot(labels[live], vocab).double()
+        p = torch.softmax(z, 1)
+        grad, size = p - onehot, p + onehot
+        dwd = torch.from_numpy(rt.read(dw, (vocab, hidden), "float32").copy()).double()
+        assert bool(((dwd - grad.t() @ xd).abs() <= (rel + (rows + 2) * U) * (size.t() @ xd.abs())).all())
+        for i in live.tolist() + [2, 131073, 262146, 270000, 299997]:
+            at = (live == i).nonzero()
+            dense = p[at[0, 0]] if len(at) else torch.full((vocab,), 1.0 / vocab, dtype=torch.float64)
+            hit = torch.nn.functional.one_hot(labels[i], vocab).double()
+            v, mag = (dense - hit) @ wd, (dense + hit) @ wd.abs()
+            e = (rel + (vocab + 2) * U) * mag
+            got = torch.from_numpy(rt.read(dx + 2 * hidden * i, (hidden,), "int16").copy()).view(torch.bfloat16).double()
+            assert bool(((got - v).abs() <= e + 2.0 ** -8 * (v.abs() + e)).all()), i
+    finally:
+        rt.wait_idle()
+        for a in held:
+            rt.free(a)
