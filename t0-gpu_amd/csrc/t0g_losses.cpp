@@ -110,7 +110,7 @@ int check_problem(const t0g_linear_ce_desc *desc, const t0g_linear_distill_desc 
     if (d.label_type > T0G_I64) return fail(T0G_ERR_INVALID_ARG, "bad label_type %u", d.label_type);
     if (d.dx_dtype > T0G_BF16 || d.dw_dtype > T0G_BF16)
         return fail(T0G_ERR_INVALID_ARG, "bad gradient type (dx %u, dw %u)", d.dx_dtype, d.dw_dtype);
-    if (d.vocab == 0 || d.hidden == 0 || d.vocab > 0x7FFFFFFFu || d.rows > 0x7FFFFFFFu)
+    if (d.vocab == 0 || d.hidden == 0 || d.vocab > 0x7FFFFFFFu || d.hidden > 0x7FFFFFFFu || d.rows > 0x7FFFFFFFu)
         return fail(T0G_ERR_INVALID_ARG, "bad size: %u rows, vocab %u, hidden %u", d.rows, d.vocab, d.hidden);
     if (!isfinite(d.logit_scale) || d.logit_scale <= 0.0f)
         return fail(T0G_ERR_INVALID_ARG, "logit_scale %g", (double)d.logit_scale);

@@ -127,3 +127,11 @@ def test_hidden_states_past_31_bits(want, layout):
     refused(desc(300000, 32000, 8193), "x spans 2457900000")
     if layout == "NN" or "w" in want:
         refused(desc(300000, 32001, 8192), "x spans")
+
+
+@pytest.mark.parametrize("hidden", [1 << 31, (1 << 32) - 8, (1 << 32) - 7, (1 << 32) - 1])
+@pytest.mark.parametrize("rows", [16, 600])
+def test_hidden_sizes_past_31_bits(rows, hidden):
+    """Rounded up to whole 16-byte pieces the largest of them wrap to 0."""
+    refused(ce(rows=rows, hidden=hidden), "size")
+    refused(distill(head={"rows": rows, "hidden": hidden}), "size")
