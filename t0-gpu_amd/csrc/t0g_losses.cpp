@@ -25,6 +25,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <exception>
+#include <mutex>
 #include <vector>
 
 #include "t0g.h"
@@ -707,25 +709,39 @@ int run_loss(t0g_device *dev, const Problem &p) {
     return ok();
 }
 
+// No exception leaves a C entry: a vocabulary in very many pieces has a long list of them.
+template <class F>
+int guarded(F f) {
+    try {
+        return f();
+    } catch (const std::exception &e) {
+        return fail(T0G_ERR_OUT_OF_MEMORY, "host: %s", e.what());
+    }
+}
+
 int loss_call(t0g_device *dev, const t0g_linear_ce_desc *d, const t0g_linear_distill_desc *t) {
-    if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
-    if (!d) return fail(T0G_ERR_INVALID_ARG, "desc is NULL");
-    Problem p;
-    int rc = check_problem(d, t, &p);
-    if (rc) return rc;
-    std::lock_guard<std::mutex> lk(device_mutex(dev));
-    return run_loss(dev, p);
+    return guarded([&] {
+        if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
+        if (!d) return fail(T0G_ERR_INVALID_ARG, "desc is NULL");
+        Problem p;
+        int rc = check_problem(d, t, &p);
+        if (rc) return rc;
+        std::lock_guard<std::mutex> lk(device_mutex(dev));
+        return run_loss(dev, p);
+    });
 }
 
 int loss_scratch(const t0g_linear_ce_desc *d, const t0g_linear_distill_desc *t, size_t *bytes) {
-    if (!d || !bytes) return fail(T0G_ERR_INVALID_ARG, "NULL argument");
-    *bytes = 0;
-    Problem p;
-    Plan pl;
-    int rc = check_problem(d, t, &p);
-    if (rc || (rc = make_loss_plan(p, &pl))) return rc;
-    *bytes = pl.bytes;
-    return ok();
+    return guarded([&] {
+        if (!d || !bytes) return fail(T0G_ERR_INVALID_ARG, "NULL argument");
+        *bytes = 0;
+        Problem p;
+        Plan pl;
+        int rc = check_problem(d, t, &p);
+        if (rc || (rc = make_loss_plan(p, &pl))) return rc;
+        *bytes = pl.bytes;
+        return ok();
+    });
 }
 
 }  // namespace

@@ -1,5 +1,9 @@
 """Host side of the losses of a projection onto a vocabulary: what a call refuses, with the
 status and before anything runs, and the scratch that it asks for.  No GPU needed."""
+import os
+import subprocess
+import sys
+
 import pytest
 
 import t0g
@@ -135,3 +139,23 @@ def test_hidden_sizes_past_31_bits(rows, hidden):
     """Rounded up to whole 16-byte pieces the largest of them wrap to 0."""
     refused(ce(rows=rows, hidden=hidden), "size")
     refused(distill(head={"rows": rows, "hidden": hidden}), "size")
+
+
+def test_no_exception_leaves_a_call():
+    """A vocabulary in 2^28 pieces, whose list does not fit the memory that the process is given."""
+    script = """
+import resource, sys
+sys.path.insert(0, sys.argv[1])
+import t0g
+d = t0g.linear_ce_desc(1 << 56, 1 << 58, 1 << 20, 1 << 50, 1, (1 << 31) - 1, 64, max_piece=8)
+with open("/proc/self/statm") as f:
+    size = int(f.read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (size + (256 << 20), size + (256 << 20)))
+try:
+    t0g.linear_loss_scratch_size(d)
+except t0g.T0gError as e:
+    print("code", e.code)
+"""
+    package = os.path.dirname(os.path.abspath(t0g.__file__))
+    r = subprocess.run([sys.executable, "-c", script, package], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.split() == ["code", str(t0g.ERR_OUT_OF_MEMORY)], (r.returncode, r.stdout, r.stderr)
