@@ -518,7 +518,12 @@ T0G_API int t0g_matmul_kernel_name(uint32_t op, uint32_t m, uint32_t k, uint32_t
  * (and 256 tokens at least if w is NN).
  *
  * Products, statistics and losses are f32 on bf16 operands.  The logits' gradient
- * is rounded to bf16 once, as an operand of the products that give dx and dw.
+ * is rounded to bf16, as an operand of the products that give dx and dw, also where these
+ * are f32; up to 128 rows what that rounding leaves is multiplied too.  Above, where a
+ * call has several million logits, the probabilities it is made from are cut to 10
+ * significant bits (0.7 2^-9 at most, 0 on average; with a teacher's temperature T below 1
+ * beside labels 1 / T times that).  dx and dw are then within 0.0024 of the exact ones
+ * (root mean square; bf16 outputs within 0.0017 up to 128 rows).
  * Results do not depend on what ran before: no atomics, sums in a fixed order.
  * Calls are asynchronous on the device stream; the scratch (a piece of G, 2 GiB
  * at most or what max_piece leaves of it, f32 partial sums of dx if there are several
@@ -541,7 +546,8 @@ typedef struct t0g_linear_ce_desc {
     uint32_t transpose;             /* T0G_NT or T0G_NN: how w is stored               */
     uint32_t label_type;            /* t0g_index_type                                  */
     uint32_t dx_dtype, dw_dtype;    /* t0g_dtype                                       */
-    uint32_t max_piece;             /* tokens per piece of the vocabulary, at most; 0 = by size */
+    uint32_t max_piece;             /* tokens per piece of the vocabulary, at most, down to a multiple of 8
+                                     * (of 256 where the softmax is in the GEMM); below 8 it is 8; 0 = by size */
     float loss_scale;
     float logit_scale;              /* > 0                                             */
 } t0g_linear_ce_desc;
@@ -566,9 +572,10 @@ T0G_API int t0g_linear_distill_scratch_size(const t0g_linear_distill_desc *desc,
 /* How the losses run: T0G_LOSS_FORM_AUTO (0, the default) by size; T0G_LOSS_FORM_ROWS (1) with
  * a piece's f32 logits in the scratch and kernels over its rows; T0G_LOSS_FORM_FUSED (2)
  * with the softmax in the logits GEMM's epilogue wherever the operands allow it.  The
- * forms differ in the order of f32 sums and, with gradients of up to 128 rows, in G's
- * rounding (by rows its remainder goes through the products too).  Process-wide, for
- * later calls: for tests and measurements. */
+ * forms differ in the order of f32 sums and, with gradients, in G's rounding: by rows its
+ * remainder goes through the products too up to 128 rows, fused the last piece's
+ * probabilities are cut to 10 bits first.  Process-wide, for later calls: for tests and measurements, not while other threads make or size losses,
+ * whose scratch it changes. */
 #define T0G_LOSS_FORM_AUTO 0u
 #define T0G_LOSS_FORM_ROWS 1u
 #define T0G_LOSS_FORM_FUSED 2u

@@ -55,15 +55,19 @@ constexpr uint32_t kFusedRows = 128;
 constexpr uint64_t kFusedLogits = 5ull << 20, kFusedGradLogits = 8ull << 20;
 // Teacher's entries of a row in a block of T0G_LOSS_BLOCK columns, on average, up to which
 // the fused form is taken: its epilogue takes a row's entries one after another (147 of 280
-// tokens, 2985 rows of width 768: 313 us fused, 71 by rows).
+// tokens, 2985 rows of width 768: 313 us fused, 71 by rows).  Few entries on average may still crowd
+// in few blocks: all of a row's in its first ones, against spread evenly, 4096 rows of 131072 tokens,
+// width 2048, 128 entries 5.79 ms either way; 2048 rows of 32000, 64 entries 785 us against 768; 2048 rows of
+// 131072, width 1024, 1024 entries 2.30 ms against 2.07.
 constexpr uint64_t kFusedEntries = 8;
 // Rows up to which G goes into the products as two bf16, the rounded value and what the
 // rounding left: few rows' roundings do not average out (one row's dx has the label's
 // whole, up to 2^-8), and what bounds their products is the weight's bytes.
 constexpr uint32_t kPairRows = 128;
 // Rows from which an unaligned weight is copied, and what a copied piece takes at most.  Without
-// and with the copy, width 1023: loss alone over 50001 tokens 200 rows 97 / 97 us, 300 rows 120 /
-// 130, 777 rows 255 / 188; with gradients over 20001 tokens 300 rows 146 / 158, 777 rows 271 / 243.
+// and with the copy, width 1023: loss alone over 50001 tokens 300 rows 128 / 112 us, 512 rows 174 /
+// 116, 777 rows 243 / 167; with gradients over 20001 tokens 300 rows 140 / 166, 512 rows 187 / 184,
+// 777 rows 271 / 249.
 constexpr uint32_t kCopyRows = 512;
 constexpr uint64_t kCopyBytes = 512ull << 20;
 // Temperatures T at which the kept exponentials of the labels' softmax give the teacher's as well, to the
