@@ -75,7 +75,13 @@ typedef enum t0g_epilogue_op {
     T0G_OP_CLAMP = 8       /* x = min(max(x, clamp_min), clamp_max)                 */
 } t0g_epilogue_op;
 
-typedef enum t0g_dtype { T0G_F32 = 0, T0G_BF16 = 1 } t0g_dtype;
+/* The 8-bit types are those of the calls that name them (t0g_fp8_*, t0g_rms_norm). */
+typedef enum t0g_dtype {
+    T0G_F32 = 0,
+    T0G_BF16 = 1,
+    T0G_E4M3 = 2,   /* OCP e4m3: largest 448, NaN, no infinities */
+    T0G_E5M2 = 3    /* OCP e5m2: largest 57344                   */
+} t0g_dtype;
 
 /* GemmConfig (src/t0/gemm_gen.rs:56-84), also carrying a TileGemm
  * (src/t0/tile_ir.rs:85-117; wg_size = TileGemm::wg_size() = tile_m).  Same
@@ -580,6 +586,147 @@ T0G_API int t0g_linear_distill_scratch_size(const t0g_linear_distill_desc *desc,
 #define T0G_LOSS_FORM_ROWS 1u
 #define T0G_LOSS_FORM_FUSED 2u
 T0G_API int t0g_set_loss_form(uint32_t form);
+
+/* ---- the feed-forward layer: norm, 8-bit values and products, gated projections ---- *
+ * What stands around and inside a language model's feed-forward layer besides the plain
+ * GEMMs.  No reference counterpart as single calls: the reference has a norm kernel
+ * (src/t0/rmsnorm_kernels.rs) and runs the gate's activation as an epilogue
+ * (src/t0/tile_ir.rs:41-62); it has no 8-bit types.
+ *
+ * All calls are asynchronous on the device stream.  Arrays need the alignment of their
+ * elements only; leading dimensions are in elements, 0 = packed.  Sums, statistics and
+ * scales are f32, results do not depend on what ran before (no atomics, sums in a fixed
+ * order).  Outputs must not overlap inputs or each other, but for the in-place forms that
+ * a call names.  Scratch (where a ..._scratch_size call exists) belongs to the handle, grows
+ * on a shape's first call and cannot grow under stream capture: the call is refused there
+ * unless the same call ran before.  (Of a captured call's scratch: t0g_device_set_stream.)
+ *
+ * 8-bit values have an f32 scale for each block of 128 along a row (T0G_BLOCK_ROW) or of
+ * 128 rows by 128 columns (T0G_BLOCK_TILE; blocks at the end may be smaller):
+ *   scale = max(largest magnitude in the block, 2^-100) / 448 (e5m2: 57344)
+ *   q = value / scale, rounded to nearest even
+ * A NaN or an infinity makes all of its block's values NaN.  Scales are stored by blocks of
+ * columns: scales[column / 128][row], or [column / 128][row / 128]. */
+#define T0G_BLOCK_ROW 0u
+#define T0G_BLOCK_TILE 1u
+
+/* Root-mean-square norm with the residual's addition:
+ *   s = x + residual,  y = s (mean s^2 + eps)^-1/2 (weight + weight_offset)
+ * sum receives s rounded to its type; y and q are formed from the unrounded s, q (e4m3 or
+ * e5m2, blocks of 1 x 128) from the unrounded y.  sum may be x or residual itself (same
+ * address, leading dimension and type size), y may be x. */
+#define T0G_NORM_MAX 16384u   /* hidden size, at most */
+typedef struct t0g_rms_norm_desc {
+    uint64_t x;                  /* x_dtype [rows][ldx]                          */
+    uint64_t residual;           /* residual_dtype [rows][ldr], or 0             */
+    uint64_t weight;             /* weight_dtype [hidden], or 0: ones, no offset */
+    uint64_t sum;                /* out: sum_dtype [rows][ldsum], or 0           */
+    uint64_t y;                  /* out: y_dtype [rows][ldy], or 0               */
+    uint64_t q;                  /* out: q_dtype [rows][ldq], or 0               */
+    uint64_t scales;             /* out: f32 [ceil(hidden / 128)][ldsc], with q  */
+    uint32_t rows, hidden;
+    uint32_t ldx, ldr, ldsum, ldy, ldq, ldsc;
+    uint32_t x_dtype, residual_dtype, weight_dtype, sum_dtype, y_dtype;   /* T0G_F32 or T0G_BF16 */
+    uint32_t q_dtype;            /* T0G_E4M3 or T0G_E5M2                         */
+    float eps;                   /* >= 0                                         */
+    float weight_offset;
+} t0g_rms_norm_desc;
+T0G_API int t0g_rms_norm(t0g_device *dev, const t0g_rms_norm_desc *desc);
+
+/* Its gradients, for x = the sum that the forward call gave out:
+ *   n = x (mean x^2 + eps)^-1/2,  g = dy (weight + weight_offset)
+ *   dx = (mean x^2 + eps)^-1/2 (g - n mean(g n)) + dsum,  dweight = sum over the rows of dy n
+ * dx is the gradient of x and of the residual alike; dsum, what reaches the sum past the
+ * norm.  dx and dw: each only if asked for.  dx may be dy, x or dsum itself. */
+typedef struct t0g_rms_norm_backward_desc {
+    uint64_t dy;                 /* dy_dtype [rows][lddy]                        */
+    uint64_t x;                  /* x_dtype [rows][ldx]                          */
+    uint64_t weight;             /* weight_dtype [hidden], or 0                  */
+    uint64_t dsum;               /* dsum_dtype [rows][ldds], or 0                */
+    uint64_t dx;                 /* out: dx_dtype [rows][lddx], or 0             */
+    uint64_t dw;                 /* out: dw_dtype [hidden], or 0                 */
+    uint32_t rows, hidden;
+    uint32_t lddy, ldx, ldds, lddx;
+    uint32_t dy_dtype, x_dtype, weight_dtype, dsum_dtype, dx_dtype, dw_dtype;
+    float eps;
+    float weight_offset;
+} t0g_rms_norm_backward_desc;
+T0G_API int t0g_rms_norm_backward(t0g_device *dev, const t0g_rms_norm_backward_desc *desc);
+T0G_API int t0g_rms_norm_backward_scratch_size(const t0g_rms_norm_backward_desc *desc, size_t *bytes);
+
+/* x in 8 bits, and its transpose, whose blocks run along x's columns: T0G_BLOCK_ROW gives qt a
+ * scale for each 128 rows of a column, T0G_BLOCK_TILE the same scales as q.  q and qt: at
+ * least one of them.  t0g_fp8_gemm's operands for Y = X W^T and its gradients: X and dY by
+ * rows, W by tiles; dX takes W's transpose (by tiles), dW those of dY and X (by rows). */
+typedef struct t0g_fp8_quantize_desc {
+    uint64_t x;                  /* x_dtype [rows][ldx]                          */
+    uint64_t q;                  /* out: q_dtype [rows][ldq], or 0               */
+    uint64_t scales;             /* out: f32 [ceil(cols / 128)][ldsc], with q    */
+    uint64_t qt;                 /* out: q_dtype [cols][ldqt], or 0              */
+    uint64_t scales_t;           /* out: f32 [ceil(rows / 128)][ldsct], with qt  */
+    uint32_t rows, cols;
+    uint32_t ldx, ldq, ldsc, ldqt, ldsct;
+    uint32_t x_dtype;            /* T0G_F32 or T0G_BF16                          */
+    uint32_t q_dtype;            /* T0G_E4M3 or T0G_E5M2                         */
+    uint32_t block;              /* T0G_BLOCK_ROW or T0G_BLOCK_TILE              */
+} t0g_fp8_quantize_desc;
+T0G_API int t0g_fp8_quantize(t0g_device *dev, const t0g_fp8_quantize_desc *desc);
+
+/* C = A B^T of 8-bit values: the sum over blocks of K of a_scale b_scale times the sum of the
+ * block's products.  With out_dtype T0G_F32 these are exact and summed in f32.  With T0G_BF16
+ * they are the 8-bit matrix unit's: of each 8 neighbouring products it cuts what is below 2^-13
+ * of the largest one's power of two (in all about 2^-14 of the result, of bf16's 2^-9). */
+typedef struct t0g_fp8_gemm_desc {
+    uint64_t a;                  /* a_dtype [m][lda]                             */
+    uint64_t a_scales;           /* f32 [ceil(k / 128)][ldas >= m]               */
+    uint64_t b;                  /* b_dtype [n][ldb]                             */
+    uint64_t b_scales;           /* f32 [ceil(k / 128)][ldbs >= n, or its blocks] */
+    uint64_t c;                  /* out: out_dtype [m][ldc]                      */
+    uint32_t m, n, k;
+    uint32_t lda, ldb, ldc, ldas, ldbs;
+    uint32_t a_dtype, b_dtype;   /* T0G_E4M3 or T0G_E5M2                         */
+    uint32_t b_block;            /* T0G_BLOCK_ROW or T0G_BLOCK_TILE              */
+    uint32_t out_dtype;          /* T0G_F32 or T0G_BF16                          */
+} t0g_fp8_gemm_desc;
+T0G_API int t0g_fp8_gemm(t0g_device *dev, const t0g_fp8_gemm_desc *desc);
+T0G_API int t0g_fp8_gemm_scratch_size(const t0g_fp8_gemm_desc *desc, size_t *bytes);
+
+/* A gated pair of projections in one kernel: g = x Wg^T, u = x Wu^T, h = act(g) u, with act one
+ * of T0G_OP_SILU, T0G_OP_GELU (x sigmoid(1.702 x), as in the GEMMs' epilogues) and
+ * T0G_OP_RELU.  gate and up receive g and u in bf16 for the backward call, if asked for. */
+typedef struct t0g_gated_linear_desc {
+    uint64_t x;                  /* bf16 [rows][ldx]                             */
+    uint64_t wg, wu;             /* bf16, NT: [features][ldw], NN: [hidden][ldw] */
+    uint64_t h;                  /* out: h_dtype [rows][ldh]                     */
+    uint64_t gate, up;           /* out: bf16 [rows][ldg], or 0                  */
+    uint32_t rows, features, hidden;
+    uint32_t ldx, ldw, ldh, ldg;
+    uint32_t transpose;          /* T0G_NT or T0G_NN: how the weights are stored */
+    uint32_t activation;         /* t0g_epilogue_op                              */
+    uint32_t h_dtype;            /* T0G_F32 or T0G_BF16                          */
+} t0g_gated_linear_desc;
+T0G_API int t0g_gated_linear(t0g_device *dev, const t0g_gated_linear_desc *desc);
+T0G_API int t0g_gated_linear_scratch_size(const t0g_gated_linear_desc *desc, size_t *bytes);
+
+/* Its gradients: dg = dh u act'(g), du = dh act(g) (rounded to bf16, as operands),
+ *   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
+ * dx, dwg, dwu: each only if asked for.  gate and up: what the forward call kept, both or
+ * neither; without them g and u are computed again, not rounded. */
+typedef struct t0g_gated_linear_backward_desc {
+    uint64_t dh;                 /* dh_dtype [rows][lddh]                        */
+    uint64_t x, wg, wu;          /* as in the forward call                       */
+    uint64_t gate, up;           /* bf16 [rows][ldg], or 0                       */
+    uint64_t dx;                 /* out: dx_dtype [rows][lddx], or 0             */
+    uint64_t dwg, dwu;           /* out: dw_dtype, laid out as wg with lddw, or 0 */
+    uint32_t rows, features, hidden;
+    uint32_t lddh, ldx, ldw, ldg, lddx, lddw;
+    uint32_t transpose;
+    uint32_t activation;
+    uint32_t dh_dtype, dx_dtype, dw_dtype;   /* T0G_F32 or T0G_BF16              */
+    uint32_t reserved;           /* 0                                            */
+} t0g_gated_linear_backward_desc;
+T0G_API int t0g_gated_linear_backward(t0g_device *dev, const t0g_gated_linear_backward_desc *desc);
+T0G_API int t0g_gated_linear_backward_scratch_size(const t0g_gated_linear_backward_desc *desc, size_t *bytes);
 
 /* ---- GEMM autotuner and its on-disk cache ----------------------------------- *
  * GemmTuner (src/t0/auto_gemm.rs:28-417): benchmark the model's best candidate

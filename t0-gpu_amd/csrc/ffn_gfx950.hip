@@ -1,0 +1,61 @@
+// Operators of a model's feed-forward layer for MI355X (gfx950): its norm, values in 8 bits with
+// block scales, their product, and the gated pair of projections with its gradient.
+#define T0G_TILES_ONLY
+#include "gemm_gfx950.hip"
+#include "ffn_rows.h"
+#include "ffn_tile.h"
+
+#define NORM(NT, CH, KEEP) \
+    extern "C" __global__ void __launch_bounds__(NT) t0g_ffn_norm_##NT##x##CH(T0gNormArgs p) { t0g::rms_norm<NT, CH, KEEP>(p); }
+NORM(64, 1, true)
+NORM(256, 1, true)
+NORM(256, 2, true)
+NORM(512, 2, true)
+NORM(1024, 2, true)
+#define NORM_GRAD(NT, CH, KEEP)                                                                 \
+    extern "C" __global__ void __launch_bounds__(NT) t0g_ffn_norm_grad_##NT##x##CH(T0gNormGradArgs p) { \
+        t0g::rms_norm_grad<NT, CH, KEEP>(p);                                                    \
+    }
+NORM_GRAD(64, 1, true)
+NORM_GRAD(256, 1, true)
+NORM_GRAD(256, 2, true)
+NORM_GRAD(512, 2, true)
+NORM_GRAD(1024, 2, false)
+extern "C" __global__ void __launch_bounds__(256) t0g_ffn_column_sum(T0gColSumArgs p) { t0g::column_sum(p); }
+extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_rows(T0gQuantArgs p) { t0g::quantize_rows(p); }
+extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_tile(T0gQuantArgs p) { t0g::quantize_tile(p); }
+extern "C" __global__ void __launch_bounds__(256) t0g_ffn_gated_grad(T0gGatedGradArgs p) { t0g::gated_grad(p); }
+extern "C" __global__ void __launch_bounds__(256) t0g_ffn_pad_rows(T0gPadArgs p) { t0g::pad_rows(p); }
+extern "C" __global__ void __launch_bounds__(256) t0g_ffn_add_planes(T0gAddArgs p) { t0g::add_planes(p); }
+
+// Symbols: t0g_ffn_f8_<tile>_<type of A><type of B>_<blocks of B>_<output type>.
+#define F8_KERNEL(NAME, BM, BN, WM, WN, TYPES, FA, FB, BLOCK, B_TILE, OUT, WIDE)                                                   \
+    extern "C" __global__ void __launch_bounds__(64 * WM * WN) t0g_ffn_f8_##NAME##_##TYPES##_##BLOCK##_##OUT(T0gTileArgs p) { \
+        t0g::f8_tile<BM, BN, WM, WN, FA, FB, B_TILE, WIDE>(p);                                                                \
+    }
+#define F8_TYPES(NAME, BM, BN, WM, WN, TYPES, FA, FB)                        \
+    F8_KERNEL(NAME, BM, BN, WM, WN, TYPES, FA, FB, tile, true, bf16, false)  \
+    F8_KERNEL(NAME, BM, BN, WM, WN, TYPES, FA, FB, tile, true, f32, true)    \
+    F8_KERNEL(NAME, BM, BN, WM, WN, TYPES, FA, FB, row, false, bf16, false)  \
+    F8_KERNEL(NAME, BM, BN, WM, WN, TYPES, FA, FB, row, false, f32, true)
+#define F8_TILES(NAME, BM, BN, WM, WN)             \
+    F8_TYPES(NAME, BM, BN, WM, WN, e4e4, 0, 0)     \
+    F8_TYPES(NAME, BM, BN, WM, WN, e4e5, 0, 1)     \
+    F8_TYPES(NAME, BM, BN, WM, WN, e5e4, 1, 0)     \
+    F8_TYPES(NAME, BM, BN, WM, WN, e5e5, 1, 1)
+F8_TILES(128x128, 128, 128, 2, 2)
+
+#define GATED(NAME, BM, BN, WM, WN)                                                                            \
+    extern "C" __global__ void __launch_bounds__(64 * WM * WN) t0g_ffn_gated_##NAME##_nt(T0gTileArgs p) {      \
+        t0g::gated_tile<BM, BN, WM, WN, false, false>(p);                                                      \
+    }                                                                                                          \
+    extern "C" __global__ void __launch_bounds__(64 * WM * WN) t0g_ffn_gated_##NAME##_nn(T0gTileArgs p) {      \
+        t0g::gated_tile<BM, BN, WM, WN, true, false>(p);                                                       \
+    }                                                                                                          \
+    extern "C" __global__ void __launch_bounds__(64 * WM * WN) t0g_ffn_gated_##NAME##_nt_grad(T0gTileArgs p) { \
+        t0g::gated_tile<BM, BN, WM, WN, false, true>(p);                                                       \
+    }                                                                                                          \
+    extern "C" __global__ void __launch_bounds__(64 * WM * WN) t0g_ffn_gated_##NAME##_nn_grad(T0gTileArgs p) { \
+        t0g::gated_tile<BM, BN, WM, WN, true, true>(p);                                                        \
+    }
+GATED(128x64, 128, 64, 2, 2)

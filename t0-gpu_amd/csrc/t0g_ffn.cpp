@@ -1,0 +1,807 @@
+// The feed-forward layer's calls: argument checks, kernel choice, scratch and launches.  The
+// kernels are in ffn_gfx950.hip; the gated pair's gradients are products of the library's own GEMMs.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <exception>
+#include <mutex>
+#include <string>
+#include <vector>
+
+#include "t0g.h"
+#include "t0g_internal.h"
+#include "t0g_kernel_args.h"
+
+namespace t0g {
+
+namespace {
+
+// Limits of the kernels' 32-bit offsets within a tile of 256 rows: bytes of a row, and rows and
+// columns of an array.
+constexpr uint64_t kMaxRowBytes = (1ull << 31) / 256 - 128;
+constexpr uint32_t kMaxRows = 0x7FFFFFFFu;
+constexpr uint32_t kMaxGridY = 65535;
+
+uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+bool is_float(uint32_t t) { return t <= T0G_BF16; }
+bool is_f8(uint32_t t) { return t == T0G_E4M3 || t == T0G_E5M2; }
+uint32_t size_of(uint32_t t) { return t == T0G_F32 ? 4 : t == T0G_BF16 ? 2 : 1; }
+uint32_t blocks_of(uint32_t n) { return (n + T0G_SCALE_BLOCK - 1) / T0G_SCALE_BLOCK; }
+
+// A call's arrays: their leading dimensions, alignment, and that no output meets another array.
+class Arrays {
+  public:
+    int rc = T0G_OK;
+    void in(const char *name, uint64_t a, uint64_t rows, uint64_t cols, uint32_t *ld, uint32_t type) {
+        add(name, a, rows, cols, ld, type, false);
+    }
+    void out(const char *name, uint64_t a, uint64_t rows, uint64_t cols, uint32_t *ld, uint32_t type) {
+        add(name, a, rows, cols, ld, type, true);
+    }
+    // `output` may be `input` itself: every value is read before it is written, by the same thread.
+    void in_place(const char *output, const char *input) { allowed_.push_back({output, input}); }
+    int check() {
+        if (rc) return rc;
+        for (size_t i = 0; i < list_.size(); ++i)
+            for (size_t j = 0; j < list_.size(); ++j) {
+                const Array &o = list_[i], &a = list_[j];
+                if (!o.output || i == j || (a.output && j < i) || o.begin >= a.end || a.begin >= o.end) continue;
+                if (side_by_side(o, a) || side_by_side(a, o)) continue;
+                const bool same = o.begin == a.begin && o.ld == a.ld && o.size == a.size;
+                bool ok = false;
+                for (const auto &p : allowed_) ok = ok || (same && p.output == std::string(o.name) && p.input == std::string(a.name));
+                if (!ok) return fail(T0G_ERR_INVALID_ARG, "%s overlaps %s", o.name, a.name);
+            }
+        return T0G_OK;
+    }
+
+  private:
+    struct Array {
+        const char *name;
+        uint64_t begin, end, row;   // row: bytes of its values
+        uint32_t ld, size;
+        bool output;
+    };
+    struct Pair {
+        const char *output, *input;
+    };
+    // Columns of one tensor: rows equally far apart, b's values in the gaps of a's.
+    static bool side_by_side(const Array &a, const Array &b) {
+        const uint64_t pitch = (uint64_t)a.ld * a.size;
+        if (pitch != (uint64_t)b.ld * b.size || b.begin < a.begin) return false;
+        const uint64_t at = (b.begin - a.begin) % pitch;
+        return at >= a.row && at + b.row <= pitch;
+    }
+    std::vector<Array> list_;
+    std::vector<Pair> allowed_;
+
+    void add(const char *name, uint64_t a, uint64_t rows, uint64_t cols, uint32_t *ld, uint32_t type, bool output) {
+        const uint32_t size = size_of(type);
+        if (rc) return;
+        if (*ld == 0) *ld = (uint32_t)cols;
+        if (*ld < cols) {
+            rc = fail(T0G_ERR_INVALID_ARG, "leading dimension of %s: %u < %llu", name, *ld, (unsigned long long)cols);
+            return;
+        }
+        if (!a) return;
+        if (a % size) {
+            rc = fail(T0G_ERR_INVALID_ARG, "%s is not aligned to its elements of %u bytes", name, size);
+            return;
+        }
+        const uint64_t extent = rows && cols ? ((rows - 1) * *ld + cols) * size : 0;
+        if (extent > UINT64_MAX - a) {
+            rc = fail(T0G_ERR_INVALID_ARG, "%s ends past the address space", name);
+            return;
+        }
+        if (extent) list_.push_back(Array{name, a, a + extent, cols * size, *ld, size, output});
+    }
+};
+
+int check_float(const char *name, uint32_t t) {
+    return is_float(t) ? T0G_OK : fail(T0G_ERR_INVALID_ARG, "bad %s %u: f32 or bf16", name, t);
+}
+int check_f8(const char *name, uint32_t t) {
+    return is_f8(t) ? T0G_OK : fail(T0G_ERR_INVALID_ARG, "bad %s %u: e4m3 or e5m2", name, t);
+}
+
+// No exception leaves a C entry.
+template <class F>
+int guarded(F f) {
+    try {
+        return f();
+    } catch (const std::exception &e) {
+        return fail(T0G_ERR_OUT_OF_MEMORY, "host: %s", e.what());
+    }
+}
+
+uint32_t groups_for(uint64_t items, uint32_t per_group, uint32_t most) {
+    return (uint32_t)std::min<uint64_t>((items + per_group - 1) / per_group, most);
+}
+
+// ---- the norm ---------------------------------------------------------------------------
+int check_norm_sizes(uint32_t rows, uint32_t hidden, float eps, float offset) {
+    if (hidden == 0 || hidden > T0G_NORM_MAX || rows > kMaxRows)
+        return fail(T0G_ERR_INVALID_ARG, "bad size: %u rows, hidden %u (1 to %u)", rows, hidden, T0G_NORM_MAX);
+    if (!isfinite(eps) || eps < 0.0f) return fail(T0G_ERR_INVALID_ARG, "eps %g", (double)eps);
+    if (!isfinite(offset)) return fail(T0G_ERR_INVALID_ARG, "weight_offset %g", (double)offset);
+    return T0G_OK;
+}
+
+int check_norm(t0g_rms_norm_desc *d) {
+    int rc;
+    if ((rc = check_norm_sizes(d->rows, d->hidden, d->eps, d->weight_offset)) || (rc = check_float("x_dtype", d->x_dtype)) ||
+        (rc = check_float("residual_dtype", d->residual_dtype)) || (rc = check_float("weight_dtype", d->weight_dtype)) ||
+        (rc = check_float("sum_dtype", d->sum_dtype)) || (rc = check_float("y_dtype", d->y_dtype)) ||
+        (rc = check_f8("q_dtype", d->q_dtype)))
+        return rc;
+    if (!d->y && !d->q && !d->sum) return fail(T0G_ERR_INVALID_ARG, "no output: y, q or sum");
+    if (!d->q != !d->scales) return fail(T0G_ERR_INVALID_ARG, "q and scales go together");
+    if (d->rows && !d->x) return fail(T0G_ERR_INVALID_ARG, "NULL x");
+    uint32_t packed = d->hidden;
+    Arrays a;
+    a.in("x", d->x, d->rows, d->hidden, &d->ldx, d->x_dtype);
+    a.in("residual", d->residual, d->rows, d->hidden, &d->ldr, d->residual_dtype);
+    a.in("weight", d->weight, 1, d->hidden, &packed, d->weight_dtype);
+    a.out("sum", d->sum, d->rows, d->hidden, &d->ldsum, d->sum_dtype);
+    a.out("y", d->y, d->rows, d->hidden, &d->ldy, d->y_dtype);
+    a.out("q", d->q, d->rows, d->hidden, &d->ldq, d->q_dtype);
+    a.out("scales", d->scales, blocks_of(d->hidden), d->rows, &d->ldsc, T0G_F32);
+    a.in_place("sum", "x");
+    a.in_place("sum", "residual");
+    a.in_place("y", "x");
+    return a.check();
+}
+
+// Threads of a row and pieces of 8 values of a thread.
+struct RowShape {
+    const char *suffix;
+    uint32_t threads;
+};
+RowShape row_shape(uint32_t hidden) {
+    if (hidden <= 512) return {"64x1", 64};
+    if (hidden <= 2048) return {"256x1", 256};
+    if (hidden <= 4096) return {"256x2", 256};
+    if (hidden <= 8192) return {"512x2", 512};
+    return {"1024x2", 1024};
+}
+
+int norm_call(t0g_device *dev, const t0g_rms_norm_desc *desc) {
+    if (!desc) return fail(T0G_ERR_INVALID_ARG, "desc is NULL");
+    t0g_rms_norm_desc d = *desc;
+    int rc = check_norm(&d);
+    if (rc) return rc;
+    if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
+    std::lock_guard<std::mutex> lk(device_mutex(dev));
+    uint64_t scratch;
+    if ((rc = ffn_begin(dev, 0, &scratch)) || d.rows == 0) return rc;
+    T0gNormArgs a;
+    memset(&a, 0, sizeof a);
+    a.x = d.x;
+    a.residual = d.residual;
+    a.weight = d.weight;
+    a.sum = d.sum;
+    a.y = d.y;
+    a.q = d.q;
+    a.scales = d.scales;
+    a.rows = d.rows;
+    a.hidden = d.hidden;
+    a.ldx = d.ldx;
+    a.ldr = d.ldr;
+    a.ldsum = d.ldsum;
+    a.ldy = d.ldy;
+    a.ldq = d.ldq;
+    a.ldsc = d.ldsc;
+    a.eps = d.eps;
+    a.weight_offset = d.weight_offset;
+    a.flags = (d.x_dtype == T0G_F32 ? T0G_ROWS_X_F32 : 0) | (d.residual_dtype == T0G_F32 ? T0G_ROWS_R_F32 : 0) |
+              (d.weight_dtype == T0G_F32 ? T0G_ROWS_W_F32 : 0) | (d.sum_dtype == T0G_F32 ? T0G_ROWS_OUT_F32 : 0) |
+              (d.y_dtype == T0G_F32 ? T0G_ROWS_Y_F32 : 0) | (d.q_dtype == T0G_E5M2 ? T0G_ROWS_E5M2 : 0);
+    const RowShape s = row_shape(d.hidden);
+    return ffn_launch(dev, (std::string("t0g_ffn_norm_") + s.suffix).c_str(), std::min(d.rows, 1u << 20), 1, s.threads, &a, sizeof a);
+}
+
+int check_norm_grad(t0g_rms_norm_backward_desc *d) {
+    int rc;
+    if ((rc = check_norm_sizes(d->rows, d->hidden, d->eps, d->weight_offset)) || (rc = check_float("dy_dtype", d->dy_dtype)) ||
+        (rc = check_float("x_dtype", d->x_dtype)) || (rc = check_float("weight_dtype", d->weight_dtype)) ||
+        (rc = check_float("dsum_dtype", d->dsum_dtype)) || (rc = check_float("dx_dtype", d->dx_dtype)) ||
+        (rc = check_float("dw_dtype", d->dw_dtype)))
+        return rc;
+    if (!d->dx && !d->dw) return fail(T0G_ERR_INVALID_ARG, "no output: dx or dw");
+    if (d->rows && (!d->x || !d->dy)) return fail(T0G_ERR_INVALID_ARG, "NULL x or dy");
+    uint32_t packed = d->hidden;
+    Arrays a;
+    a.in("dy", d->dy, d->rows, d->hidden, &d->lddy, d->dy_dtype);
+    a.in("x", d->x, d->rows, d->hidden, &d->ldx, d->x_dtype);
+    a.in("weight", d->weight, 1, d->hidden, &packed, d->weight_dtype);
+    a.in("dsum", d->dsum, d->rows, d->hidden, &d->ldds, d->dsum_dtype);
+    a.out("dx", d->dx, d->rows, d->hidden, &d->lddx, d->dx_dtype);
+    a.out("dw", d->dw, 1, d->hidden, &packed, d->dw_dtype);
+    a.in_place("dx", "dy");
+    a.in_place("dx", "x");
+    a.in_place("dx", "dsum");
+    return a.check();
+}
+
+// Workgroups of the gradient kernel, each with a row of partial sums of dw.
+uint32_t norm_grad_groups(const t0g_rms_norm_backward_desc &d) { return std::min(d.rows, 512u); }
+uint32_t norm_grad_ld(const t0g_rms_norm_backward_desc &d) { return (uint32_t)round_up(d.hidden, 8); }
+size_t norm_grad_scratch(const t0g_rms_norm_backward_desc &d) {
+    return d.dw ? (size_t)norm_grad_groups(d) * norm_grad_ld(d) * 4 : 0;
+}
+
+int norm_grad_call(t0g_device *dev, const t0g_rms_norm_backward_desc *desc) {
+    if (!desc) return fail(T0G_ERR_INVALID_ARG, "desc is NULL");
+    t0g_rms_norm_backward_desc d = *desc;
+    int rc = check_norm_grad(&d);
+    if (rc) return rc;
+    if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
+    std::lock_guard<std::mutex> lk(device_mutex(dev));
+    uint64_t scratch;
+    if ((rc = ffn_begin(dev, norm_grad_scratch(d), &scratch))) return rc;
+    const uint32_t groups = norm_grad_groups(d);
+    if (d.rows) {
+        T0gNormGradArgs a;
+        memset(&a, 0, sizeof a);
+        a.dy = d.dy;
+        a.x = d.x;
+        a.weight = d.weight;
+        a.dsum = d.dsum;
+        a.dx = d.dx;
+        a.part = d.dw ? scratch : 0;
+        a.rows = d.rows;
+        a.hidden = d.hidden;
+        a.lddy = d.lddy;
+        a.ldx = d.ldx;
+        a.ldds = d.ldds;
+        a.lddx = d.lddx;
+        a.ldpart = norm_grad_ld(d);
+        a.eps = d.eps;
+        a.weight_offset = d.weight_offset;
+        a.flags = (d.dy_dtype == T0G_F32 ? T0G_ROWS_Y_F32 : 0) | (d.x_dtype == T0G_F32 ? T0G_ROWS_X_F32 : 0) |
+                  (d.weight_dtype == T0G_F32 ? T0G_ROWS_W_F32 : 0) | (d.dsum_dtype == T0G_F32 ? T0G_ROWS_R_F32 : 0) |
+                  (d.dx_dtype == T0G_F32 ? T0G_ROWS_OUT_F32 : 0);
+        const RowShape s = row_shape(d.hidden);
+        if ((rc = ffn_launch(dev, (std::string("t0g_ffn_norm_grad_") + s.suffix).c_str(), groups, 1, s.threads, &a, sizeof a))) return rc;
+    }
+    if (!d.dw) return ok();
+    T0gColSumArgs s;
+    memset(&s, 0, sizeof s);
+    s.part = scratch;
+    s.out = d.dw;
+    s.n = groups;   // of no rows: zeros
+    s.cols = d.hidden;
+    s.ldp = norm_grad_ld(d);
+    s.out_bf16 = d.dw_dtype == T0G_BF16;
+    return ffn_launch(dev, "t0g_ffn_column_sum", (d.hidden + 31) / 32, 1, 256, &s, sizeof s);
+}
+
+// ---- 8-bit values -----------------------------------------------------------------------
+int check_quantize(t0g_fp8_quantize_desc *d) {
+    int rc;
+    if ((rc = check_float("x_dtype", d->x_dtype)) || (rc = check_f8("q_dtype", d->q_dtype))) return rc;
+    if (d->block > T0G_BLOCK_TILE) return fail(T0G_ERR_INVALID_ARG, "bad block %u", d->block);
+    if (d->cols == 0 || d->cols > (1u << 30) || d->rows > (1u << 30))
+        return fail(T0G_ERR_INVALID_ARG, "bad size: %u rows, %u columns", d->rows, d->cols);
+    if (!d->q && !d->qt) return fail(T0G_ERR_INVALID_ARG, "no output: q or qt");
+    if (!d->q != !d->scales || !d->qt != !d->scales_t) return fail(T0G_ERR_INVALID_ARG, "8-bit values and scales go together");
+    if (d->rows && !d->x) return fail(T0G_ERR_INVALID_ARG, "NULL x");
+    const bool tile = d->block == T0G_BLOCK_TILE;
+    Arrays a;
+    a.in("x", d->x, d->rows, d->cols, &d->ldx, d->x_dtype);
+    a.out("q", d->q, d->rows, d->cols, &d->ldq, d->q_dtype);
+    a.out("scales", d->scales, blocks_of(d->cols), tile ? blocks_of(d->rows) : d->rows, &d->ldsc, T0G_F32);
+    a.out("qt", d->qt, d->cols, d->rows, &d->ldqt, d->q_dtype);
+    a.out("scales_t", d->scales_t, blocks_of(d->rows), tile ? blocks_of(d->cols) : d->cols, &d->ldsct, T0G_F32);
+    return a.check();
+}
+
+int quantize_call(t0g_device *dev, const t0g_fp8_quantize_desc *desc) {
+    if (!desc) return fail(T0G_ERR_INVALID_ARG, "desc is NULL");
+    t0g_fp8_quantize_desc d = *desc;
+    int rc = check_quantize(&d);
+    if (rc) return rc;
+    if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
+    std::lock_guard<std::mutex> lk(device_mutex(dev));
+    uint64_t scratch;
+    if ((rc = ffn_begin(dev, 0, &scratch)) || d.rows == 0) return rc;
+    T0gQuantArgs a;
+    memset(&a, 0, sizeof a);
+    a.x = d.x;
+    a.q = d.q;
+    a.scales = d.scales;
+    a.qt = d.qt;
+    a.scales_t = d.scales_t;
+    a.rows = d.rows;
+    a.cols = d.cols;
+    a.ldx = d.ldx;
+    a.ldq = d.ldq;
+    a.ldsc = d.ldsc;
+    a.ldqt = d.ldqt;
+    a.ldsct = d.ldsct;
+    a.flags = (d.x_dtype == T0G_F32 ? T0G_ROWS_X_F32 : 0) | (d.q_dtype == T0G_E5M2 ? T0G_ROWS_E5M2 : 0) |
+              (d.block == T0G_BLOCK_TILE ? T0G_ROWS_TILE : 0);
+    if (d.qt || d.block == T0G_BLOCK_TILE)
+        return ffn_launch(dev, "t0g_ffn_quantize_tile", blocks_of(d.cols), std::min(blocks_of(d.rows), kMaxGridY), 256, &a, sizeof a);
+    const uint32_t pieces = blocks_of(d.cols) * 16;
+    a.row_shift = 4;
+    while (a.row_shift < 8 && (1u << a.row_shift) < pieces) ++a.row_shift;
+    const uint32_t gx = (pieces + (1u << a.row_shift) - 1) >> a.row_shift, rows = 4 * (256u >> a.row_shift);
+    return ffn_launch(dev, "t0g_ffn_quantize_rows", gx, groups_for(d.rows, rows, kMaxGridY), 256, &a, sizeof a);
+}
+
+// ---- operands of the tile kernels -------------------------------------------------------
+// Rows of whole, aligned 16-byte pieces whose offsets in a tile fit 32 bits; others are copied to the scratch.
+struct Operand {
+    uint64_t addr = 0;
+    uint32_t rows = 0, cols = 0, ld = 0, size = 1;
+    bool copied = false;
+    uint64_t at = 0;   // in the scratch
+    uint32_t ldc = 0;
+    void set(uint64_t a, uint32_t r, uint32_t c, uint32_t l, uint32_t s) {
+        addr = a;
+        rows = r;
+        cols = c;
+        ld = l;
+        size = s;
+        copied = a % 16 || (uint64_t)l * s % 16 || (uint64_t)c * s % 16 || (uint64_t)l * s > kMaxRowBytes;
+        ldc = (uint32_t)(round_up((uint64_t)c * s, 128) / s);
+    }
+    uint64_t bytes() const { return copied ? (uint64_t)rows * ldc * size : 0; }
+    uint64_t address(uint64_t base) const { return copied ? base + at : addr; }
+    uint32_t pitch() const { return copied ? ldc : ld; }
+};
+
+uint64_t take(uint64_t *at, uint64_t bytes) {
+    const uint64_t a = *at;
+    *at += round_up(bytes, 256);
+    return a;
+}
+
+int run_pad(t0g_device *dev, const Operand &o, uint64_t base) {
+    if (!o.copied) return T0G_OK;
+    T0gPadArgs p;
+    memset(&p, 0, sizeof p);
+    p.src = o.addr;
+    p.dst = base + o.at;
+    p.rows = o.rows;
+    p.cols = o.cols;
+    p.lds = o.ld;
+    p.ldd = o.ldc;
+    p.size = o.size;
+    return ffn_launch(dev, "t0g_ffn_pad_rows", groups_for((uint64_t)o.rows * o.ldc * o.size / 8, 256, 1u << 16), 1, 256, &p, sizeof p);
+}
+
+int set_tiles(T0gTileArgs *a, uint32_t bm, uint32_t bn) {
+    const uint64_t tm = ((uint64_t)a->m + bm - 1) / bm, tn = ((uint64_t)a->n + bn - 1) / bn;
+    if (tm * tn >= (1u << 22)) return fail(T0G_ERR_INVALID_ARG, "bad size: %llu x %llu tiles", (unsigned long long)tm, (unsigned long long)tn);
+    a->tiles_m = (uint32_t)tm;
+    a->tiles_n = (uint32_t)tn;
+    a->group_m = 8;
+    return T0G_OK;
+}
+
+// ---- the 8-bit product ------------------------------------------------------------------
+int check_fp8_gemm(t0g_fp8_gemm_desc *d) {
+    int rc;
+    if ((rc = check_f8("a_dtype", d->a_dtype)) || (rc = check_f8("b_dtype", d->b_dtype)) || (rc = check_float("out_dtype", d->out_dtype)))
+        return rc;
+    if (d->b_block > T0G_BLOCK_TILE) return fail(T0G_ERR_INVALID_ARG, "bad b_block %u", d->b_block);
+    if (d->k == 0 || d->k > kMaxRowBytes || d->m > kMaxRows || d->n > kMaxRows)
+        return fail(T0G_ERR_INVALID_ARG, "bad size: m %u, n %u, k %u", d->m, d->n, d->k);
+    if (d->m && d->n && (!d->a || !d->b || !d->c || !d->a_scales || !d->b_scales)) return fail(T0G_ERR_INVALID_ARG, "NULL operand");
+    Arrays a;
+    a.in("a", d->a, d->m, d->k, &d->lda, d->a_dtype);
+    a.in("b", d->b, d->n, d->k, &d->ldb, d->b_dtype);
+    a.in("a_scales", d->a_scales, blocks_of(d->k), d->m, &d->ldas, T0G_F32);
+    a.in("b_scales", d->b_scales, blocks_of(d->k), d->b_block == T0G_BLOCK_TILE ? blocks_of(d->n) : d->n, &d->ldbs, T0G_F32);
+    a.out("c", d->c, d->m, d->n, &d->ldc, d->out_dtype);
+    return a.check();
+}
+
+struct Fp8Plan {
+    Operand a, b;
+    uint64_t bytes = 0;
+};
+void plan_fp8(const t0g_fp8_gemm_desc &d, Fp8Plan *p) {
+    p->a.set(d.a, d.m, d.k, d.lda, 1);
+    p->b.set(d.b, d.n, d.k, d.ldb, 1);
+    p->a.at = take(&p->bytes, p->a.bytes());
+    p->b.at = take(&p->bytes, p->b.bytes());
+}
+
+int fp8_gemm_call(t0g_device *dev, const t0g_fp8_gemm_desc *desc) {
+    if (!desc) return fail(T0G_ERR_INVALID_ARG, "desc is NULL");
+    t0g_fp8_gemm_desc d = *desc;
+    int rc = check_fp8_gemm(&d);
+    if (rc) return rc;
+    Fp8Plan pl;
+    plan_fp8(d, &pl);
+    T0gTileArgs t;
+    memset(&t, 0, sizeof t);
+    t.m = d.m;
+    t.n = d.n;
+    t.k = d.k;
+    if ((rc = set_tiles(&t, 128, 128))) return rc;
+    if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
+    std::lock_guard<std::mutex> lk(device_mutex(dev));
+    uint64_t base;
+    if ((rc = ffn_begin(dev, pl.bytes, &base)) || d.m == 0 || d.n == 0) return rc;
+    if ((rc = run_pad(dev, pl.a, base)) || (rc = run_pad(dev, pl.b, base))) return rc;
+    t.a = pl.a.address(base);
+    t.b = pl.b.address(base);
+    t.lda = pl.a.pitch();
+    t.ldb = pl.b.pitch();
+    t.as = d.a_scales;
+    t.bs = d.b_scales;
+    t.ldas = d.ldas;
+    t.ldbs = d.ldbs;
+    t.c = d.c;
+    t.ldc = d.ldc;
+    const std::string symbol = std::string("t0g_ffn_f8_128x128_") + (d.a_dtype == T0G_E4M3 ? "e4" : "e5") +
+                               (d.b_dtype == T0G_E4M3 ? "e4" : "e5") + (d.b_block == T0G_BLOCK_TILE ? "_tile" : "_row") +
+                               (d.out_dtype == T0G_F32 ? "_f32" : "_bf16");
+    return ffn_launch(dev, symbol.c_str(), t.tiles_m * t.tiles_n, 1, 256, &t, sizeof t);
+}
+
+// ---- gated projections ------------------------------------------------------------------
+int activation_code(uint32_t op, uint32_t *act) {
+    switch (op) {
+        case T0G_OP_SILU: *act = T0G_ACT_SILU; return T0G_OK;
+        case T0G_OP_GELU: *act = T0G_ACT_GELU; return T0G_OK;
+        case T0G_OP_RELU: *act = T0G_ACT_RELU; return T0G_OK;
+        default: return fail(T0G_ERR_INVALID_ARG, "activation %u: silu, gelu or relu", op);
+    }
+}
+
+int check_gated_sizes(uint32_t rows, uint32_t features, uint32_t hidden, uint32_t transpose) {
+    if (transpose > T0G_NN) return fail(T0G_ERR_INVALID_ARG, "transpose %u: the weights are NT or NN", transpose);
+    if (features == 0 || hidden == 0 || hidden > kMaxRowBytes / 2 || features > kMaxRowBytes / 2 || rows > kMaxRows)
+        return fail(T0G_ERR_INVALID_ARG, "bad size: %u rows, %u features, hidden %u", rows, features, hidden);
+    return T0G_OK;
+}
+
+int check_gated(t0g_gated_linear_desc *d, uint32_t *act) {
+    int rc;
+    if ((rc = check_gated_sizes(d->rows, d->features, d->hidden, d->transpose)) || (rc = activation_code(d->activation, act)) ||
+        (rc = check_float("h_dtype", d->h_dtype)))
+        return rc;
+    if (d->rows && (!d->x || !d->wg || !d->wu || !d->h)) return fail(T0G_ERR_INVALID_ARG, "NULL operand");
+    const bool nt = d->transpose == T0G_NT;
+    const uint32_t wr = nt ? d->features : d->hidden, wc = nt ? d->hidden : d->features;
+    Arrays a;
+    a.in("x", d->x, d->rows, d->hidden, &d->ldx, T0G_BF16);
+    a.in("wg", d->wg, wr, wc, &d->ldw, T0G_BF16);
+    a.in("wu", d->wu, wr, wc, &d->ldw, T0G_BF16);
+    a.out("h", d->h, d->rows, d->features, &d->ldh, d->h_dtype);
+    a.out("gate", d->gate, d->rows, d->features, &d->ldg, T0G_BF16);
+    a.out("up", d->up, d->rows, d->features, &d->ldg, T0G_BF16);
+    return a.check();
+}
+
+// The gated tile kernels' operands.
+struct GatedPlan {
+    Operand x, wg, wu;
+    void set(uint64_t xa, uint64_t g, uint64_t u, uint32_t rows, uint32_t features, uint32_t hidden, uint32_t ldx, uint32_t ldw,
+             uint32_t transpose, uint64_t *at) {
+        const bool nt = transpose == T0G_NT;
+        x.set(xa, rows, hidden, ldx, 2);
+        wg.set(g, nt ? features : hidden, nt ? hidden : features, ldw, 2);
+        wu.set(u, nt ? features : hidden, nt ? hidden : features, ldw, 2);
+        if (wg.copied || wu.copied) wg.copied = wu.copied = true;   // one leading dimension for both
+        for (Operand *o : {&x, &wg, &wu}) o->at = take(at, o->bytes());
+    }
+    int pad(t0g_device *dev, uint64_t base) const {
+        int rc;
+        if ((rc = run_pad(dev, x, base)) || (rc = run_pad(dev, wg, base))) return rc;
+        return run_pad(dev, wu, base);
+    }
+};
+
+int run_gated_tile(t0g_device *dev, T0gTileArgs *t, const GatedPlan &pl, uint64_t base, uint32_t transpose, const char *kind) {
+    t->a = pl.x.address(base);
+    t->b = pl.wg.address(base);
+    t->b2 = pl.wu.address(base);
+    t->lda = pl.x.pitch();
+    t->ldb = pl.wg.pitch();
+    int rc = set_tiles(t, 128, 64);
+    if (rc) return rc;
+    const std::string symbol = std::string("t0g_ffn_gated_128x64") + (transpose == T0G_NT ? "_nt" : "_nn") + kind;
+    return ffn_launch(dev, symbol.c_str(), t->tiles_m * t->tiles_n, 1, 256, t, sizeof *t);
+}
+
+int gated_plan(const t0g_gated_linear_desc &d, GatedPlan *pl, uint64_t *bytes) {
+    *bytes = 0;
+    pl->set(d.x, d.wg, d.wu, d.rows, d.features, d.hidden, d.ldx, d.ldw, d.transpose, bytes);
+    return T0G_OK;
+}
+
+int gated_call(t0g_device *dev, const t0g_gated_linear_desc *desc) {
+    if (!desc) return fail(T0G_ERR_INVALID_ARG, "desc is NULL");
+    t0g_gated_linear_desc d = *desc;
+    uint32_t act;
+    int rc = check_gated(&d, &act);
+    if (rc) return rc;
+    GatedPlan pl;
+    uint64_t bytes, base;
+    if ((rc = gated_plan(d, &pl, &bytes))) return rc;
+    if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
+    std::lock_guard<std::mutex> lk(device_mutex(dev));
+    if ((rc = ffn_begin(dev, bytes, &base)) || d.rows == 0) return rc;
+    T0gTileArgs t;
+    memset(&t, 0, sizeof t);
+    t.c = d.h;
+    t.ldc = d.ldh;
+    t.gate = d.gate;
+    t.up = d.up;
+    t.ldg = d.ldg;
+    t.m = d.rows;
+    t.n = d.features;
+    t.k = d.hidden;
+    t.act = act;
+    t.flags = d.h_dtype == T0G_F32 ? T0G_TILE_OUT_F32 : 0;
+    if ((rc = pl.pad(dev, base))) return rc;
+    return run_gated_tile(dev, &t, pl, base, d.transpose, "");
+}
+
+int check_gated_grad(t0g_gated_linear_backward_desc *d, uint32_t *act) {
+    int rc;
+    if ((rc = check_gated_sizes(d->rows, d->features, d->hidden, d->transpose)) || (rc = activation_code(d->activation, act)) ||
+        (rc = check_float("dh_dtype", d->dh_dtype)) || (rc = check_float("dx_dtype", d->dx_dtype)) ||
+        (rc = check_float("dw_dtype", d->dw_dtype)))
+        return rc;
+    if (d->reserved) return fail(T0G_ERR_INVALID_ARG, "reserved must be 0");
+    if (!d->dx && !d->dwg && !d->dwu) return fail(T0G_ERR_INVALID_ARG, "no output: dx, dwg or dwu");
+    if (!d->gate != !d->up) return fail(T0G_ERR_INVALID_ARG, "gate and up go together");
+    if (d->rows && (!d->dh || !d->x || !d->wg || !d->wu)) return fail(T0G_ERR_INVALID_ARG, "NULL operand");
+    const bool nt = d->transpose == T0G_NT;
+    const uint32_t wr = nt ? d->features : d->hidden, wc = nt ? d->hidden : d->features;
+    Arrays a;
+    a.in("dh", d->dh, d->rows, d->features, &d->lddh, d->dh_dtype);
+    a.in("x", d->x, d->rows, d->hidden, &d->ldx, T0G_BF16);
+    a.in("wg", d->wg, wr, wc, &d->ldw, T0G_BF16);
+    a.in("wu", d->wu, wr, wc, &d->ldw, T0G_BF16);
+    a.in("gate", d->gate, d->rows, d->features, &d->ldg, T0G_BF16);
+    a.in("up", d->up, d->rows, d->features, &d->ldg, T0G_BF16);
+    a.out("dx", d->dx, d->rows, d->hidden, &d->lddx, d->dx_dtype);
+    a.out("dwg", d->dwg, wr, wc, &d->lddw, d->dw_dtype);
+    a.out("dwu", d->dwu, wr, wc, &d->lddw, d->dw_dtype);
+    return a.check();
+}
+
+// The gradients' products on D = [dg | du], [rows][2 features rounded up to 8 each].
+struct GatedGradPlan {
+    GatedPlan tiles;                 // without the kept products
+    std::vector<t0g_gemm_desc> dx, dw;   // addresses in the scratch are offsets from its start
+    bool planes = false;             // dx in two products, added up
+    uint32_t half = 0, ldd = 0, ldp = 0;
+    uint64_t d = 0, p0 = 0, p1 = 0, ws = 0, ws_bytes = 0, bytes = 0;
+};
+
+t0g_gemm_desc product(uint64_t a, uint64_t b, uint64_t c, uint32_t m, uint32_t n, uint32_t k, uint32_t lda, uint32_t ldb,
+                      uint32_t ldc, uint32_t transpose, uint32_t dtype) {
+    t0g_gemm_desc g;
+    memset(&g, 0, sizeof g);
+    g.a = a;
+    g.b = b;
+    g.c = c;
+    g.m = m;
+    g.n = n;
+    g.k = k;
+    g.lda = lda;
+    g.ldb = ldb;
+    g.ldc = ldc;
+    g.transpose = transpose;
+    g.out_dtype = dtype;
+    return g;
+}
+
+// The plan for a scratch at `base` (0: sizes only; the GEMMs' choice does not depend on it but for its alignment).
+int plan_gated_grad(const t0g_gated_linear_backward_desc &d, uint64_t base, GatedGradPlan *pl) {
+    const bool nt = d.transpose == T0G_NT;
+    const uint32_t f = d.features, es = size_of(d.dw_dtype);
+    uint64_t at = 0;
+    if (!d.gate) pl->tiles.set(d.x, d.wg, d.wu, d.rows, f, d.hidden, d.ldx, d.ldw, d.transpose, &at);
+    pl->half = (uint32_t)round_up(f, 8);
+    pl->ldd = 2 * pl->half;
+    pl->d = take(&at, (uint64_t)d.rows * pl->ldd * 2);
+    const uint64_t dg = base + pl->d, du = dg + (uint64_t)pl->half * 2;
+    const bool whole = pl->half == f;
+    const uint64_t step = nt ? (uint64_t)f * d.ldw : f;
+    const bool w_stacked = whole && d.wu == d.wg + step * 2 && (nt || d.ldw >= 2 * f);
+    if (d.dx) {
+        const uint32_t tr = nt ? T0G_NN : T0G_NT;
+        if (w_stacked) {
+            pl->dx.push_back(product(dg, d.wg, d.dx, d.rows, d.hidden, 2 * f, pl->ldd, d.ldw, d.lddx, tr, d.dx_dtype));
+        } else {
+            pl->planes = true;
+            pl->ldp = (uint32_t)round_up(d.hidden, 4);
+            const uint64_t plane = (uint64_t)d.rows * pl->ldp * 4;
+            pl->p0 = take(&at, plane);
+            pl->p1 = take(&at, plane);
+            pl->dx.push_back(product(dg, d.wg, base + pl->p0, d.rows, d.hidden, f, pl->ldd, d.ldw, pl->ldp, tr, T0G_F32));
+            pl->dx.push_back(product(du, d.wu, base + pl->p1, d.rows, d.hidden, f, pl->ldd, d.ldw, pl->ldp, tr, T0G_F32));
+        }
+    }
+    auto dw = [&](uint64_t from, uint64_t to, uint32_t features) {
+        pl->dw.push_back(nt ? product(from, d.x, to, features, d.hidden, d.rows, pl->ldd, d.ldx, d.lddw, T0G_TN, d.dw_dtype)
+                            : product(d.x, from, to, d.hidden, features, d.rows, d.ldx, pl->ldd, d.lddw, T0G_TN, d.dw_dtype));
+    };
+    const uint64_t out_step = nt ? (uint64_t)f * d.lddw : f;
+    if (whole && d.dwg && d.dwu == d.dwg + out_step * es && (nt || d.lddw >= 2 * f)) {
+        dw(dg, d.dwg, 2 * f);
+    } else {
+        if (d.dwg) dw(dg, d.dwg, f);
+        if (d.dwu) dw(du, d.dwu, f);
+    }
+    if (d.rows)
+        for (const auto *list : {&pl->dx, &pl->dw})
+            for (const t0g_gemm_desc &g : *list) {
+                size_t bytes = 0;
+                int rc = losses_gemm_workspace(&g, false, &bytes);
+                if (rc) return rc;
+                pl->ws_bytes = std::max<uint64_t>(pl->ws_bytes, bytes);
+            }
+    pl->ws = take(&at, pl->ws_bytes);
+    pl->bytes = at;
+    return T0G_OK;
+}
+
+int gated_grad_call(t0g_device *dev, const t0g_gated_linear_backward_desc *desc) {
+    if (!desc) return fail(T0G_ERR_INVALID_ARG, "desc is NULL");
+    t0g_gated_linear_backward_desc d = *desc;
+    uint32_t act;
+    int rc = check_gated_grad(&d, &act);
+    if (rc) return rc;
+    uint64_t base = 0;
+    GatedGradPlan sizes, pl;
+    if ((rc = plan_gated_grad(d, 0, &sizes))) return rc;
+    if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
+    std::lock_guard<std::mutex> lk(device_mutex(dev));
+    if ((rc = ffn_begin(dev, sizes.bytes, &base)) || (rc = plan_gated_grad(d, base, &pl))) return rc;
+    if (d.rows && d.gate) {
+        T0gGatedGradArgs g;
+        memset(&g, 0, sizeof g);
+        g.dh = d.dh;
+        g.gate = d.gate;
+        g.up = d.up;
+        g.c = base + pl.d;
+        g.rows = d.rows;
+        g.features = d.features;
+        g.lddh = d.lddh;
+        g.ldg = d.ldg;
+        g.ldc = pl.ldd;
+        g.up_off = pl.half;
+        g.flags = d.dh_dtype == T0G_F32 ? T0G_TILE_DH_F32 : 0;
+        g.act = act;
+        const uint64_t pieces = (uint64_t)d.rows * ((d.features + 7) / 8);
+        if ((rc = ffn_launch(dev, "t0g_ffn_gated_grad", groups_for(pieces, 256, 1u << 16), 1, 256, &g, sizeof g))) return rc;
+    } else if (d.rows) {
+        T0gTileArgs t;
+        memset(&t, 0, sizeof t);
+        t.c = base + pl.d;
+        t.ldc = pl.ldd;
+        t.up_off = pl.half;
+        t.dh = d.dh;
+        t.lddh = d.lddh;
+        t.m = d.rows;
+        t.n = d.features;
+        t.k = d.hidden;
+        t.act = act;
+        t.flags = d.dh_dtype == T0G_F32 ? T0G_TILE_DH_F32 : 0;
+        if ((rc = pl.tiles.pad(dev, base)) || (rc = run_gated_tile(dev, &t, pl.tiles, base, d.transpose, "_grad"))) return rc;
+    }
+    auto run = [&](t0g_gemm_desc g) {
+        g.workspace = base + pl.ws;
+        g.workspace_bytes = pl.ws_bytes;
+        return losses_gemm(dev, &g, false);
+    };
+    if (d.rows) {
+        for (const t0g_gemm_desc &g : pl.dx)
+            if ((rc = run(g))) return rc;
+        if (pl.planes) {
+            T0gAddArgs a;
+            memset(&a, 0, sizeof a);
+            a.p0 = base + pl.p0;
+            a.p1 = base + pl.p1;
+            a.out = d.dx;
+            a.rows = d.rows;
+            a.cols = d.hidden;
+            a.ldp = pl.ldp;
+            a.ldo = d.lddx;
+            a.out_bf16 = d.dx_dtype == T0G_BF16;
+            if ((rc = ffn_launch(dev, "t0g_ffn_add_planes", groups_for((uint64_t)d.rows * (pl.ldp / 4), 256, 1u << 16), 1, 256, &a, sizeof a)))
+                return rc;
+        }
+    }
+    for (const t0g_gemm_desc &g : pl.dw)   // over no rows: zeros
+        if ((rc = run(g))) return rc;
+    return ok();
+}
+
+}  // namespace
+}  // namespace t0g
+
+extern "C" {
+
+int t0g_rms_norm(t0g_device *dev, const t0g_rms_norm_desc *desc) {
+    return t0g::guarded([&] { return t0g::norm_call(dev, desc); });
+}
+
+int t0g_rms_norm_backward(t0g_device *dev, const t0g_rms_norm_backward_desc *desc) {
+    return t0g::guarded([&] { return t0g::norm_grad_call(dev, desc); });
+}
+
+int t0g_rms_norm_backward_scratch_size(const t0g_rms_norm_backward_desc *desc, size_t *bytes) {
+    return t0g::guarded([&] {
+        if (!desc || !bytes) return t0g::fail(T0G_ERR_INVALID_ARG, "NULL argument");
+        *bytes = 0;
+        t0g_rms_norm_backward_desc d = *desc;
+        int rc = t0g::check_norm_grad(&d);
+        if (rc) return rc;
+        *bytes = t0g::norm_grad_scratch(d);
+        return t0g::ok();
+    });
+}
+
+int t0g_fp8_quantize(t0g_device *dev, const t0g_fp8_quantize_desc *desc) {
+    return t0g::guarded([&] { return t0g::quantize_call(dev, desc); });
+}
+
+int t0g_fp8_gemm(t0g_device *dev, const t0g_fp8_gemm_desc *desc) {
+    return t0g::guarded([&] { return t0g::fp8_gemm_call(dev, desc); });
+}
+
+int t0g_fp8_gemm_scratch_size(const t0g_fp8_gemm_desc *desc, size_t *bytes) {
+    return t0g::guarded([&] {
+        if (!desc || !bytes) return t0g::fail(T0G_ERR_INVALID_ARG, "NULL argument");
+        *bytes = 0;
+        t0g_fp8_gemm_desc d = *desc;
+        int rc = t0g::check_fp8_gemm(&d);
+        if (rc) return rc;
+        t0g::Fp8Plan pl;
+        t0g::plan_fp8(d, &pl);
+        *bytes = pl.bytes;
+        return t0g::ok();
+    });
+}
+
+int t0g_gated_linear(t0g_device *dev, const t0g_gated_linear_desc *desc) {
+    return t0g::guarded([&] { return t0g::gated_call(dev, desc); });
+}
+
+int t0g_gated_linear_scratch_size(const t0g_gated_linear_desc *desc, size_t *bytes) {
+    return t0g::guarded([&] {
+        if (!desc || !bytes) return t0g::fail(T0G_ERR_INVALID_ARG, "NULL argument");
+        *bytes = 0;
+        t0g_gated_linear_desc d = *desc;
+        uint32_t act;
+        t0g::GatedPlan pl;
+        uint64_t n;
+        int rc = t0g::check_gated(&d, &act);
+        if (rc || (rc = t0g::gated_plan(d, &pl, &n))) return rc;
+        *bytes = n;
+        return t0g::ok();
+    });
+}
+
+int t0g_gated_linear_backward(t0g_device *dev, const t0g_gated_linear_backward_desc *desc) {
+    return t0g::guarded([&] { return t0g::gated_grad_call(dev, desc); });
+}
+
+int t0g_gated_linear_backward_scratch_size(const t0g_gated_linear_backward_desc *desc, size_t *bytes) {
+    return t0g::guarded([&] {
+        if (!desc || !bytes) return t0g::fail(T0G_ERR_INVALID_ARG, "NULL argument");
+        *bytes = 0;
+        t0g_gated_linear_backward_desc d = *desc;
+        uint32_t act;
+        t0g::GatedGradPlan pl;
+        int rc = t0g::check_gated_grad(&d, &act);
+        if (rc || (rc = t0g::plan_gated_grad(d, 0, &pl))) return rc;
+        *bytes = pl.bytes;
+        return t0g::ok();
+    });
+}
+
+}  // extern "C"

@@ -86,6 +86,10 @@ int losses_begin(t0g_device *dev, size_t bytes, uint64_t *scratch);
 // Launch kernel `symbol` of the losses' code object on the device stream.
 int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, void *args, size_t args_size,
                   uint32_t threads = 256);
+// The same for the feed-forward layer's calls (t0g_ffn.cpp), whose scratch is the losses'.
+int ffn_begin(t0g_device *dev, size_t bytes, uint64_t *scratch);
+int ffn_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, uint32_t threads, void *args,
+               size_t args_size);
 // Workspace t0g_gemm may use for d (host only), and the GEMM itself.  padded: the operands' rows
 // hold whole 16-byte pieces, zeros past the sizes, which then need not be multiples of 8.
 int losses_gemm_workspace(const t0g_gemm_desc *d, bool padded, size_t *bytes);

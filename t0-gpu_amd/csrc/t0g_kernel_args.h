@@ -267,4 +267,93 @@ typedef struct T0gLossOuterArgs {
 #define T0G_EPI_OP_NEG 7u       /* x = -x                                          */
 #define T0G_EPI_OP_CLAMP 8u     /* x = min(max(x, clamp_lo), clamp_hi)             */
 
+/* ---- the feed-forward layer's operators (t0g_ffn_gfx950.hsaco) ---------------------- */
+#define T0G_SCALE_BLOCK 128u     /* values along a row that share a scale                */
+
+/* Root-mean-square norm of s = x + residual and its output in 16, 32 or 8 bits. */
+typedef struct T0gNormArgs {
+    uint64_t x, residual, weight;      /* residual, weight: 0 = none                     */
+    uint64_t sum, y, q, scales;        /* 0 = not wanted                                 */
+    uint32_t rows, hidden;
+    uint32_t ldx, ldr, ldsum, ldy, ldq, ldsc;
+    uint32_t flags;                    /* T0G_ROWS_*                                     */
+    float eps, weight_offset;
+    uint32_t reserved;
+} T0gNormArgs;
+#define T0G_ROWS_X_F32 1u
+#define T0G_ROWS_R_F32 2u        /* residual (norm), dsum (its gradient)                 */
+#define T0G_ROWS_W_F32 4u
+#define T0G_ROWS_OUT_F32 8u      /* sum, dx                                              */
+#define T0G_ROWS_Y_F32 16u       /* y, dy                                                */
+#define T0G_ROWS_E5M2 32u        /* q is e5m2, else e4m3                                 */
+#define T0G_ROWS_TILE 64u        /* a scale for each 128 x 128 values, else 1 x 128      */
+
+/* Its gradients.  part: f32 [workgroups][ldpart], each workgroup's sum of dw over its rows. */
+typedef struct T0gNormGradArgs {
+    uint64_t dy, x, weight, dsum, dx, part;
+    uint32_t rows, hidden;
+    uint32_t lddy, ldx, ldds, lddx, ldpart;
+    uint32_t flags;
+    float eps, weight_offset;
+    uint32_t reserved[2];
+} T0gNormGradArgs;
+
+/* out[c] = sum of n rows of part[.][ldp], in their order. */
+typedef struct T0gColSumArgs {
+    uint64_t part, out;
+    uint32_t n, cols, ldp, out_bf16;
+} T0gColSumArgs;
+
+/* Values in 8 bits with their scales, and (qt) the transposed matrix with its own. */
+typedef struct T0gQuantArgs {
+    uint64_t x, q, scales, qt, scales_t;
+    uint32_t rows, cols;
+    uint32_t ldx, ldq, ldsc, ldqt, ldsct;
+    uint32_t flags;
+    uint32_t row_shift;      /* 1 x 128 without qt: log2 of a row's threads              */
+    uint32_t reserved;
+} T0gQuantArgs;
+
+/* A product's tile kernels: C = A B^T of 8-bit values with scales, or a gated pair of bf16
+ * products with the same A.  Operands' rows are whole 16-byte pieces. */
+typedef struct T0gTileArgs {
+    uint64_t a, b, b2;       /* [m][lda]; [n][ldb] or [k][ldb]; b2: the second product's */
+    uint64_t as, bs;         /* f32 scales, [blocks of k][ldas], [blocks of k][ldbs]     */
+    uint64_t c;              /* [m][ldc]                                                 */
+    uint64_t gate, up;       /* gated: bf16 [m][ldg], the two products; 0 = not wanted   */
+    uint64_t dh;             /* gated, gradient: [m][lddh]; c is then [dgate | dup]      */
+    uint32_t m, n, k;
+    uint32_t lda, ldb, ldc, ldas, ldbs, ldg, lddh;
+    uint32_t tiles_m, tiles_n, group_m;
+    uint32_t flags;          /* T0G_TILE_*                                               */
+    uint32_t act;            /* T0G_ACT_*                                                */
+    uint32_t up_off;         /* gated, gradient: column of dup in c                      */
+} T0gTileArgs;
+#define T0G_TILE_OUT_F32 1u      /* c is f32, else bf16                                  */
+#define T0G_TILE_B_TILE 2u       /* a scale of B for each 128 x 128, else 1 x 128        */
+#define T0G_TILE_DH_F32 4u
+#define T0G_ACT_SILU 0u
+#define T0G_ACT_GELU 1u          /* x sigmoid(1.702 x)                                   */
+#define T0G_ACT_RELU 2u
+
+/* dgate and dup from the kept products: c is [rows][dgate | dup], bf16. */
+typedef struct T0gGatedGradArgs {
+    uint64_t dh, gate, up, c;
+    uint32_t rows, features;
+    uint32_t lddh, ldg, ldc;
+    uint32_t flags, act, up_off;
+} T0gGatedGradArgs;
+
+/* Rows of `cols` values into rows of ldd, zeros from cols on.  size: bytes of a value, 1 or 2. */
+typedef struct T0gPadArgs {
+    uint64_t src, dst;
+    uint32_t rows, cols, lds, ldd, size, reserved;
+} T0gPadArgs;
+
+/* out = p0 + p1, f32 planes of rows of ldp values. */
+typedef struct T0gAddArgs {
+    uint64_t p0, p1, out;
+    uint32_t rows, cols, ldp, ldo, out_bf16, reserved;
+} T0gAddArgs;
+
 #endif

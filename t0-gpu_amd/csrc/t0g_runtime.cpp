@@ -61,6 +61,16 @@ __asm__(".section .rodata.t0g_hsaco_loss,\"a\",@progbits\n"
         ".byte 0\n"
         ".previous\n");
 extern "C" const unsigned char t0g_hsaco_loss_begin[];
+// The feed-forward layer's (T0G_HSACO_FFN_FILE), loaded by its first call.
+__asm__(".section .rodata.t0g_hsaco_ffn,\"a\",@progbits\n"
+        ".p2align 12\n"
+        ".hidden t0g_hsaco_ffn_begin\n"
+        ".globl t0g_hsaco_ffn_begin\n"
+        "t0g_hsaco_ffn_begin:\n"
+        ".incbin \"" T0G_HSACO_FFN_FILE "\"\n"
+        ".byte 0\n"
+        ".previous\n");
+extern "C" const unsigned char t0g_hsaco_ffn_begin[];
 
 namespace t0g {
 
@@ -90,7 +100,9 @@ struct t0g_device {
     hipModule_t module_tl = nullptr;   // the timeline build of the same kernels (loaded on first use)
     hipModule_t module_loss = nullptr;   // the losses' kernels (loaded on first use)
     std::unordered_map<std::string, hipFunction_t> fns_loss;
-    uint64_t loss = 0;         // scratch of the losses
+    hipModule_t module_ffn = nullptr;    // the feed-forward layer's kernels (loaded on first use)
+    std::unordered_map<std::string, hipFunction_t> fns_ffn;
+    uint64_t loss = 0;         // scratch of the losses and of the feed-forward layer's calls
     size_t loss_bytes = 0;
     std::mutex mu;
     bool poisoned = false;
@@ -958,6 +970,7 @@ int t0g_device_close(t0g_device *dev) {
     if (dev->module) (void)hipModuleUnload(dev->module);
     if (dev->module_tl) (void)hipModuleUnload(dev->module_tl);
     if (dev->module_loss) (void)hipModuleUnload(dev->module_loss);
+    if (dev->module_ffn) (void)hipModuleUnload(dev->module_ffn);
     if (dev->order_event) (void)hipEventDestroy(dev->order_event);
     if (dev->own_stream) (void)hipStreamDestroy(dev->own_stream);
     delete dev;
@@ -1784,22 +1797,24 @@ static bool capturing(t0g_device *dev) {
     return T0G_HIP(hipStreamIsCapturing(dev->stream, &st)) != hipSuccess || st != hipStreamCaptureStatusNone;
 }
 
-// ---- for the losses (t0g_losses.cpp), with dev->mu held ---------------------------
+// ---- for the losses (t0g_losses.cpp) and the feed-forward layer (t0g_ffn.cpp), with dev->mu held
 std::mutex &device_mutex(t0g_device *dev) { return dev->mu; }
 
-int losses_begin(t0g_device *dev, size_t bytes, uint64_t *scratch) {
+// The code object `image` loaded as *module and a scratch of `bytes` there; `what` names them in errors.
+static int kernels_begin(t0g_device *dev, hipModule_t *module, const void *image, const char *what, size_t bytes,
+                         uint64_t *scratch) {
     int rc = check_usable(dev);
     if (rc) return rc;
-    if (!dev->module_loss || !dev->sk_sync || dev->loss_bytes < bytes) {
+    if (!*module || !dev->sk_sync || dev->loss_bytes < bytes) {
         if (capturing(dev))
             return fail(T0G_ERR_INVALID_ARG,
-                        "a loss under stream capture needs %zu bytes of scratch and the handle holds %zu: run the same "
+                        "%s under stream capture needs %zu bytes of scratch and the handle holds %zu: run the same "
                         "call once before the capture",
-                        bytes, dev->loss_bytes);
+                        what, bytes, dev->loss_bytes);
         hipError_t e;
-        if (!dev->module_loss && (e = T0G_HIP(module_load(&dev->module_loss, t0g_hsaco_loss_begin))) != hipSuccess) {
-            dev->module_loss = nullptr;
-            return hip_fail(e, "hipModuleLoadData(losses code object)");
+        if (!*module && (e = T0G_HIP(module_load(module, image))) != hipSuccess) {
+            *module = nullptr;
+            return hip_fail(e, "hipModuleLoadData(code object)");
         }
         if ((rc = ensure_sk_sync(dev))) return rc;
         if (dev->loss_bytes < bytes) {
@@ -1807,29 +1822,48 @@ int losses_begin(t0g_device *dev, size_t bytes, uint64_t *scratch) {
                 e = drop_scratch(dev, dev->loss);
                 dev->loss = 0;
                 dev->loss_bytes = 0;
-                if (e != hipSuccess) return poison(dev, hip_fail(e, "hipFree(loss scratch)"));
+                if (e != hipSuccess) return poison(dev, hip_fail(e, "hipFree(scratch)"));
             }
             void *p = nullptr;
-            if ((e = T0G_HIP(dev_malloc(&p, bytes))) != hipSuccess) return hip_fail(e, "hipMalloc(loss scratch)");
+            if ((e = T0G_HIP(dev_malloc(&p, bytes))) != hipSuccess) return hip_fail(e, "hipMalloc(scratch)");
             dev->loss = (uint64_t)p;
             dev->loss_bytes = bytes;
         }
     }
-    give_scratch(dev, dev->loss);
+    if (dev->loss) give_scratch(dev, dev->loss);
     *scratch = dev->loss;
     return T0G_OK;
 }
 
-int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, void *args, size_t args_size,
-                  uint32_t threads) {
-    auto it = dev->fns_loss.find(symbol);
-    if (it == dev->fns_loss.end()) {
+static int kernels_launch(t0g_device *dev, hipModule_t module, std::unordered_map<std::string, hipFunction_t> &fns,
+                          const char *symbol, uint32_t grid_x, uint32_t grid_y, uint32_t threads, void *args,
+                          size_t args_size) {
+    auto it = fns.find(symbol);
+    if (it == fns.end()) {
         hipFunction_t f = nullptr;
-        hipError_t e = T0G_HIP(hipModuleGetFunction(&f, dev->module_loss, symbol));
+        hipError_t e = T0G_HIP(hipModuleGetFunction(&f, module, symbol));
         if (e != hipSuccess) return hip_fail(e, symbol);
-        it = dev->fns_loss.emplace(symbol, f).first;
+        it = fns.emplace(symbol, f).first;
     }
     return launch(dev, it->second, grid_x, grid_y, 1, threads, args, args_size);
+}
+
+int losses_begin(t0g_device *dev, size_t bytes, uint64_t *scratch) {
+    return kernels_begin(dev, &dev->module_loss, t0g_hsaco_loss_begin, "a loss", bytes, scratch);
+}
+
+int losses_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, void *args, size_t args_size,
+                  uint32_t threads) {
+    return kernels_launch(dev, dev->module_loss, dev->fns_loss, symbol, grid_x, grid_y, threads, args, args_size);
+}
+
+int ffn_begin(t0g_device *dev, size_t bytes, uint64_t *scratch) {
+    return kernels_begin(dev, &dev->module_ffn, t0g_hsaco_ffn_begin, "a call", bytes, scratch);
+}
+
+int ffn_launch(t0g_device *dev, const char *symbol, uint32_t grid_x, uint32_t grid_y, uint32_t threads, void *args,
+               size_t args_size) {
+    return kernels_launch(dev, dev->module_ffn, dev->fns_ffn, symbol, grid_x, grid_y, threads, args, args_size);
 }
 
 int losses_gemm_workspace(const t0g_gemm_desc *d, bool padded, size_t *bytes) {

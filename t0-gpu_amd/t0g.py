@@ -39,7 +39,9 @@ ERR_OUT_OF_MEMORY = 7
 NT, NN, TN, TT = 0, 1, 2, 3
 LAYOUTS = {"NT": NT, "NN": NN, "TN": TN, "TT": TT}
 EPI_STORE_F32, EPI_BIAS_ADD, EPI_BIAS_ADD_RELU = 0, 1, 2
-F32, BF16 = 0, 1
+F32, BF16, E4M3, E5M2 = range(4)   # the 8-bit types: fp8_* and rms_norm
+BLOCK_ROW, BLOCK_TILE = 0, 1       # a scale for each 1 x 128 or 128 x 128 8-bit values
+NORM_MAX = 16384                   # rms_norm's hidden size, at most
 I32, I64 = 0, 1
 LOSS_FORM_AUTO, LOSS_FORM_ROWS, LOSS_FORM_FUSED = 0, 1, 2
 (MATMUL_FORWARD, MATMUL_BACKWARD_DATA, MATMUL_BACKWARD_WEIGHT, MATMUL_FORWARD_CACHED, MATMUL_BACKWARD_DATA_CACHED,
@@ -163,6 +165,33 @@ class LinearDistillDesc(ctypes.Structure):
         [(f, ctypes.c_uint32) for f in ("top_k", "ldt", "teacher_dtype", "token_type")] +
         [("temperature", ctypes.c_float), ("label_weight", ctypes.c_float), ("distill_weight", ctypes.c_float),
          ("reserved", ctypes.c_uint32)])
+
+
+def _struct(name, *parts):
+    """A ctypes structure of (type, "field field ...") parts."""
+    return type(name, (ctypes.Structure,), {"_fields_": [(f, t) for t, names in parts for f in names.split()]})
+
+
+RmsNormDesc = _struct(
+    "RmsNormDesc", (ctypes.c_uint64, "x residual weight sum y q scales"),
+    (ctypes.c_uint32, "rows hidden ldx ldr ldsum ldy ldq ldsc x_dtype residual_dtype weight_dtype sum_dtype y_dtype q_dtype"),
+    (ctypes.c_float, "eps weight_offset"))
+RmsNormBackwardDesc = _struct(
+    "RmsNormBackwardDesc", (ctypes.c_uint64, "dy x weight dsum dx dw"),
+    (ctypes.c_uint32, "rows hidden lddy ldx ldds lddx dy_dtype x_dtype weight_dtype dsum_dtype dx_dtype dw_dtype"),
+    (ctypes.c_float, "eps weight_offset"))
+Fp8QuantizeDesc = _struct(
+    "Fp8QuantizeDesc", (ctypes.c_uint64, "x q scales qt scales_t"),
+    (ctypes.c_uint32, "rows cols ldx ldq ldsc ldqt ldsct x_dtype q_dtype block"))
+Fp8GemmDesc = _struct(
+    "Fp8GemmDesc", (ctypes.c_uint64, "a a_scales b b_scales c"),
+    (ctypes.c_uint32, "m n k lda ldb ldc ldas ldbs a_dtype b_dtype b_block out_dtype"))
+GatedLinearDesc = _struct(
+    "GatedLinearDesc", (ctypes.c_uint64, "x wg wu h gate up"),
+    (ctypes.c_uint32, "rows features hidden ldx ldw ldh ldg transpose activation h_dtype"))
+GatedLinearBackwardDesc = _struct(
+    "GatedLinearBackwardDesc", (ctypes.c_uint64, "dh x wg wu gate up dx dwg dwu"),
+    (ctypes.c_uint32, "rows features hidden lddh ldx ldw ldg lddx lddw transpose activation dh_dtype dx_dtype dw_dtype reserved"))
 
 
 class KernelMeta(ctypes.Structure):
@@ -297,6 +326,13 @@ _sig("t0g_gemm_compile", ctypes.c_int, ctypes.POINTER(GemmDesc), ctypes.POINTER(
 _sig("t0g_linear_cross_entropy", ctypes.c_int, _p, ctypes.POINTER(LinearCeDesc))
 _sig("t0g_linear_distill", ctypes.c_int, _p, ctypes.POINTER(LinearDistillDesc))
 _sig("t0g_set_loss_form", ctypes.c_int, _u32)
+for _name, _desc, _scratch in (("rms_norm", RmsNormDesc, False), ("rms_norm_backward", RmsNormBackwardDesc, True),
+                               ("fp8_quantize", Fp8QuantizeDesc, False), ("fp8_gemm", Fp8GemmDesc, True),
+                               ("gated_linear", GatedLinearDesc, True),
+                               ("gated_linear_backward", GatedLinearBackwardDesc, True)):
+    _sig("t0g_" + _name, ctypes.c_int, _p, ctypes.POINTER(_desc))
+    if _scratch:
+        _sig("t0g_" + _name + "_scratch_size", ctypes.c_int, ctypes.POINTER(_desc), ctypes.POINTER(ctypes.c_size_t))
 _sig("t0g_linear_cross_entropy_scratch_size", ctypes.c_int, ctypes.POINTER(LinearCeDesc),
      ctypes.POINTER(ctypes.c_size_t))
 _sig("t0g_linear_distill_scratch_size", ctypes.c_int, ctypes.POINTER(LinearDistillDesc),
@@ -562,6 +598,84 @@ def linear_loss_scratch_size(desc):
     ce = isinstance(desc, LinearCeDesc)
     f = _lib.t0g_linear_cross_entropy_scratch_size if ce else _lib.t0g_linear_distill_scratch_size
     _check(f(ctypes.byref(desc), ctypes.byref(n)))
+    return n.value
+
+
+def _filled(cls, **fields):
+    d = cls()
+    for name, value in fields.items():
+        setattr(d, name, value)
+    return d
+
+
+def _layout(transpose):
+    return LAYOUTS[transpose] if isinstance(transpose, str) else transpose
+
+
+def rms_norm_desc(x, weight, rows, hidden, eps=1e-6, residual=0, sum=0, y=0, q=0, scales=0, weight_offset=0.0,
+                  ldx=0, ldr=0, ldsum=0, ldy=0, ldq=0, ldsc=0, x_dtype=BF16, residual_dtype=BF16, weight_dtype=BF16,
+                  sum_dtype=BF16, y_dtype=BF16, q_dtype=E4M3):
+    """Root-mean-square norm of x + residual ([rows][hidden]): the sum, the norm in 16 or 32 bits (y), and in 8 bits
+    (q) with the scales [blocks of 128 columns][rows].  residual, weight and the outputs: 0 = none."""
+    return _filled(RmsNormDesc, x=x, residual=residual, weight=weight, sum=sum, y=y, q=q, scales=scales, rows=rows,
+                   hidden=hidden, ldx=ldx, ldr=ldr, ldsum=ldsum, ldy=ldy, ldq=ldq, ldsc=ldsc, x_dtype=x_dtype,
+                   residual_dtype=residual_dtype, weight_dtype=weight_dtype, sum_dtype=sum_dtype, y_dtype=y_dtype,
+                   q_dtype=q_dtype, eps=eps, weight_offset=weight_offset)
+
+
+def rms_norm_backward_desc(dy, x, weight, rows, hidden, eps=1e-6, dsum=0, dx=0, dw=0, weight_offset=0.0, lddy=0, ldx=0,
+                           ldds=0, lddx=0, dy_dtype=BF16, x_dtype=BF16, weight_dtype=BF16, dsum_dtype=BF16, dx_dtype=BF16,
+                           dw_dtype=F32):
+    """Gradients of the norm, x being the sum that the forward call gave out; dsum: the gradient that reaches the
+    sum past the norm, or 0.  dx, dw: 0 = not wanted."""
+    return _filled(RmsNormBackwardDesc, dy=dy, x=x, weight=weight, dsum=dsum, dx=dx, dw=dw, rows=rows, hidden=hidden,
+                   lddy=lddy, ldx=ldx, ldds=ldds, lddx=lddx, dy_dtype=dy_dtype, x_dtype=x_dtype, weight_dtype=weight_dtype,
+                   dsum_dtype=dsum_dtype, dx_dtype=dx_dtype, dw_dtype=dw_dtype, eps=eps, weight_offset=weight_offset)
+
+
+def fp8_quantize_desc(x, q, scales, rows, cols, qt=0, scales_t=0, ldx=0, ldq=0, ldsc=0, ldqt=0, ldsct=0, x_dtype=BF16,
+                      q_dtype=E4M3, block=BLOCK_ROW):
+    """x [rows][cols] in 8 bits with a scale for each 1 x 128 (BLOCK_ROW: scales [blocks of columns][rows]) or 128 x 128
+    values (BLOCK_TILE: [blocks of columns][blocks of rows]), and its transpose (qt, scales_t), or one of them."""
+    return _filled(Fp8QuantizeDesc, x=x, q=q, scales=scales, qt=qt, scales_t=scales_t, rows=rows, cols=cols, ldx=ldx,
+                   ldq=ldq, ldsc=ldsc, ldqt=ldqt, ldsct=ldsct, x_dtype=x_dtype, q_dtype=q_dtype, block=block)
+
+
+def fp8_gemm_desc(a, a_scales, b, b_scales, c, m, n, k, lda=0, ldb=0, ldc=0, ldas=0, ldbs=0, a_dtype=E4M3, b_dtype=E4M3,
+                  b_block=BLOCK_TILE, out_dtype=BF16):
+    """C [m][n] = A B^T of 8-bit A [m][k] (a scale for each 1 x 128) and B [n][k] (b_block)."""
+    return _filled(Fp8GemmDesc, a=a, a_scales=a_scales, b=b, b_scales=b_scales, c=c, m=m, n=n, k=k, lda=lda, ldb=ldb,
+                   ldc=ldc, ldas=ldas, ldbs=ldbs, a_dtype=a_dtype, b_dtype=b_dtype, b_block=b_block, out_dtype=out_dtype)
+
+
+def gated_linear_desc(x, wg, wu, h, rows, features, hidden, transpose=NT, activation="silu", gate=0, up=0, ldx=0, ldw=0,
+                      ldh=0, ldg=0, h_dtype=BF16):
+    """h [rows][features] = act(x Wg^T) * (x Wu^T) for weights of [features][hidden] (NT) or [hidden][features] (NN);
+    gate, up: where to keep both products for the backward call, or 0."""
+    return _filled(GatedLinearDesc, x=x, wg=wg, wu=wu, h=h, gate=gate, up=up, rows=rows, features=features, hidden=hidden,
+                   ldx=ldx, ldw=ldw, ldh=ldh, ldg=ldg, transpose=_layout(transpose),
+                   activation=EPILOGUE_OPS.get(activation, activation), h_dtype=h_dtype)
+
+
+def gated_linear_backward_desc(dh, x, wg, wu, rows, features, hidden, transpose=NT, activation="silu", gate=0, up=0, dx=0,
+                               dwg=0, dwu=0, lddh=0, ldx=0, ldw=0, ldg=0, lddx=0, lddw=0, dh_dtype=BF16, dx_dtype=BF16,
+                               dw_dtype=BF16):
+    """Gradients of gated_linear; gate, up: what its call kept, or 0 (they are computed again).  dx, dwg, dwu: 0 = not
+    wanted."""
+    return _filled(GatedLinearBackwardDesc, dh=dh, x=x, wg=wg, wu=wu, gate=gate, up=up, dx=dx, dwg=dwg, dwu=dwu, rows=rows,
+                   features=features, hidden=hidden, lddh=lddh, ldx=ldx, ldw=ldw, ldg=ldg, lddx=lddx, lddw=lddw,
+                   transpose=_layout(transpose), activation=EPILOGUE_OPS.get(activation, activation), dh_dtype=dh_dtype,
+                   dx_dtype=dx_dtype, dw_dtype=dw_dtype)
+
+
+_FFN_SCRATCH = {RmsNormBackwardDesc: "rms_norm_backward", Fp8GemmDesc: "fp8_gemm", GatedLinearDesc: "gated_linear",
+                GatedLinearBackwardDesc: "gated_linear_backward"}
+
+
+def ffn_scratch_size(desc):
+    """Bytes of the handle's scratch that rms_norm_backward, fp8_gemm, gated_linear or gated_linear_backward takes."""
+    n = ctypes.c_size_t()
+    _check(getattr(_lib, f"t0g_{_FFN_SCRATCH[type(desc)]}_scratch_size")(ctypes.byref(desc), ctypes.byref(n)))
     return n.value
 
 
@@ -863,6 +977,25 @@ class GpuRuntime:
     def linear_distill(self, desc):
         """Enqueue a linear_distill_desc on the device stream (asynchronous)."""
         _check(_lib.t0g_linear_distill(self.handle, ctypes.byref(desc)))
+
+    def rms_norm(self, desc):
+        """Enqueue a rms_norm_desc on the device stream (asynchronous, as the calls below)."""
+        _check(_lib.t0g_rms_norm(self.handle, ctypes.byref(desc)))
+
+    def rms_norm_backward(self, desc):
+        _check(_lib.t0g_rms_norm_backward(self.handle, ctypes.byref(desc)))
+
+    def fp8_quantize(self, desc):
+        _check(_lib.t0g_fp8_quantize(self.handle, ctypes.byref(desc)))
+
+    def fp8_gemm(self, desc):
+        _check(_lib.t0g_fp8_gemm(self.handle, ctypes.byref(desc)))
+
+    def gated_linear(self, desc):
+        _check(_lib.t0g_gated_linear(self.handle, ctypes.byref(desc)))
+
+    def gated_linear_backward(self, desc):
+        _check(_lib.t0g_gated_linear_backward(self.handle, ctypes.byref(desc)))
 
     # Ignis bf16_matmul caller path (src/ignis/ops/bf16_matmul.rs) on f32 device tensors
     def f32_to_bf16(self, src, dst, n):
