@@ -4,6 +4,7 @@
 #include "gemm_gfx950.hip"
 #include "ffn_rows.h"
 #include "ffn_tile.h"
+#include "ffn_skinny.h"
 
 #define NORM(NT, CH, KEEP) \
     extern "C" __global__ void __launch_bounds__(NT) t0g_ffn_norm_##NT##x##CH(T0gNormArgs p) { t0g::rms_norm<NT, CH, KEEP>(p); }
@@ -44,6 +45,23 @@ extern "C" __global__ void __launch_bounds__(256) t0g_ffn_add_planes(T0gAddArgs 
     F8_TYPES(NAME, BM, BN, WM, WN, e5e4, 1, 0)     \
     F8_TYPES(NAME, BM, BN, WM, WN, e5e5, 1, 1)
 F8_TILES(128x128, 128, 128, 2, 2)
+
+#define F8_SKINNY(MT, TYPES, FA, FB)                                                                              \
+    extern "C" __global__ void __launch_bounds__(512) t0g_ffn_f8_skinny##MT##_##TYPES##_tile(T0gTileArgs p) {      \
+        t0g::f8_skinny<8, MT, FA, FB, true>(p);                                                                    \
+    }                                                                                                              \
+    extern "C" __global__ void __launch_bounds__(512) t0g_ffn_f8_skinny##MT##_##TYPES##_row(T0gTileArgs p) {       \
+        t0g::f8_skinny<8, MT, FA, FB, false>(p);                                                                   \
+    }
+#define F8_SKINNIES(MT)          \
+    F8_SKINNY(MT, e4e4, 0, 0)    \
+    F8_SKINNY(MT, e4e5, 0, 1)    \
+    F8_SKINNY(MT, e5e4, 1, 0)    \
+    F8_SKINNY(MT, e5e5, 1, 1)
+F8_SKINNIES(1)
+F8_SKINNIES(2)
+extern "C" __global__ void __launch_bounds__(512) t0g_ffn_gated_skinny1(T0gTileArgs p) { t0g::gated_skinny<8, 1>(p); }
+extern "C" __global__ void __launch_bounds__(512) t0g_ffn_gated_skinny2(T0gTileArgs p) { t0g::gated_skinny<8, 2>(p); }
 
 #define GATED(NAME, BM, BN, WM, WN)                                                                            \
     extern "C" __global__ void __launch_bounds__(64 * WM * WN) t0g_ffn_gated_##NAME##_nt(T0gTileArgs p) {      \

@@ -303,6 +303,28 @@ __device__ __forceinline__ void f8_tile(const T0gTileArgs& p) {
 // g = x Wg^T and u = x Wu^T of the same columns in one wave: a tile has BN columns of each, and
 // h = act(g) u is formed in registers.  GRAD: instead, with dh, dgate = dh u act'(g) and
 // dup = dh act(g), from products that were not kept.
+template <bool GRAD>
+__device__ __forceinline__ void gated_out(const T0gTileArgs& p, uint32_t row, uint32_t col, f32x4_t g, f32x4_t u) {
+    const uint32_t n = left4(p.n, col);
+    f32x4_t a, d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float act, slope;
+        activation(p.act, g[e], act, slope);
+        a[e] = act;
+        d[e] = slope;
+    }
+    if constexpr (GRAD) {
+        const f32x4_t dh = load4(p.dh, (uint64_t)row * p.lddh + col, n, p.flags & T0G_TILE_DH_F32);
+        store4(p.c, (uint64_t)row * p.ldc + col, n, false, dh * u * d);
+        store4(p.c, (uint64_t)row * p.ldc + p.up_off + col, n, false, dh * a);
+    } else {
+        store4(p.c, (uint64_t)row * p.ldc + col, n, p.flags & T0G_TILE_OUT_F32, a * u);
+        if (p.gate) store4(p.gate, (uint64_t)row * p.ldg + col, n, false, g);
+        if (p.up) store4(p.up, (uint64_t)row * p.ldg + col, n, false, u);
+    }
+}
+
 template <int BM, int BN, int WM, int WN, bool NC, bool GRAD>
 __device__ __forceinline__ void gated_tile(const T0gTileArgs& p) {
     constexpr int W = WM * WN, TM = BM / WM, TN = BN / WN, SM = TM / 16, SN = TN / 16;
@@ -377,26 +399,7 @@ __device__ __forceinline__ void gated_tile(const T0gTileArgs& p) {
         const uint32_t row = m0 + wm * TM + 16 * i + l16;
         if (row < p.m)
 #pragma unroll
-            for (int j = 0; j < SN; ++j) {
-                const uint32_t col = n0 + wn * TN + 16 * j + 4 * q, n = left4(p.n, col);
-                f32x4_t a, d;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float act, slope;
-                    activation(p.act, g[i][j][e], act, slope);
-                    a[e] = act;
-                    d[e] = slope;
-                }
-                if constexpr (GRAD) {
-                    const f32x4_t dh = load4(p.dh, (uint64_t)row * p.lddh + col, n, p.flags & T0G_TILE_DH_F32);
-                    store4(p.c, (uint64_t)row * p.ldc + col, n, false, dh * u[i][j] * d);
-                    store4(p.c, (uint64_t)row * p.ldc + p.up_off + col, n, false, dh * a);
-                } else {
-                    store4(p.c, (uint64_t)row * p.ldc + col, n, p.flags & T0G_TILE_OUT_F32, a * u[i][j]);
-                    if (p.gate) store4(p.gate, (uint64_t)row * p.ldg + col, n, false, g[i][j]);
-                    if (p.up) store4(p.up, (uint64_t)row * p.ldg + col, n, false, u[i][j]);
-                }
-            }
+            for (int j = 0; j < SN; ++j) gated_out<GRAD>(p, row, n0 + wn * TN + 16 * j + 4 * q, g[i][j], u[i][j]);
     }
 }
 

@@ -382,6 +382,11 @@ int set_tiles(T0gTileArgs *a, uint32_t bm, uint32_t bn) {
     return T0G_OK;
 }
 
+// Workgroups of a product of few rows.
+int skinny_groups(uint32_t n) {
+    return n >= (1u << 26) ? fail(T0G_ERR_INVALID_ARG, "bad size: %u columns", n) : T0G_OK;
+}
+
 // ---- the 8-bit product ------------------------------------------------------------------
 int check_fp8_gemm(t0g_fp8_gemm_desc *d) {
     int rc;
@@ -400,11 +405,17 @@ int check_fp8_gemm(t0g_fp8_gemm_desc *d) {
     return a.check();
 }
 
+// Rows up to which a product is bound by reading B, which then goes straight to registers.
+constexpr uint32_t kSkinnyRows = 32;
+
 struct Fp8Plan {
+    bool skinny = false;
     Operand a, b;
     uint64_t bytes = 0;
 };
 void plan_fp8(const t0g_fp8_gemm_desc &d, Fp8Plan *p) {
+    p->skinny = d.m <= kSkinnyRows;
+    if (p->skinny) return;
     p->a.set(d.a, d.m, d.k, d.lda, 1);
     p->b.set(d.b, d.n, d.k, d.ldb, 1);
     p->a.at = take(&p->bytes, p->a.bytes());
@@ -423,25 +434,30 @@ int fp8_gemm_call(t0g_device *dev, const t0g_fp8_gemm_desc *desc) {
     t.m = d.m;
     t.n = d.n;
     t.k = d.k;
-    if ((rc = set_tiles(&t, 128, 128))) return rc;
+    if ((rc = pl.skinny ? skinny_groups(d.n) : set_tiles(&t, 128, 128))) return rc;
     if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
     std::lock_guard<std::mutex> lk(device_mutex(dev));
     uint64_t base;
     if ((rc = ffn_begin(dev, pl.bytes, &base)) || d.m == 0 || d.n == 0) return rc;
     if ((rc = run_pad(dev, pl.a, base)) || (rc = run_pad(dev, pl.b, base))) return rc;
-    t.a = pl.a.address(base);
-    t.b = pl.b.address(base);
-    t.lda = pl.a.pitch();
-    t.ldb = pl.b.pitch();
+    t.a = pl.skinny ? d.a : pl.a.address(base);
+    t.b = pl.skinny ? d.b : pl.b.address(base);
+    t.lda = pl.skinny ? d.lda : pl.a.pitch();
+    t.ldb = pl.skinny ? d.ldb : pl.b.pitch();
     t.as = d.a_scales;
     t.bs = d.b_scales;
     t.ldas = d.ldas;
     t.ldbs = d.ldbs;
     t.c = d.c;
     t.ldc = d.ldc;
-    const std::string symbol = std::string("t0g_ffn_f8_128x128_") + (d.a_dtype == T0G_E4M3 ? "e4" : "e5") +
-                               (d.b_dtype == T0G_E4M3 ? "e4" : "e5") + (d.b_block == T0G_BLOCK_TILE ? "_tile" : "_row") +
-                               (d.out_dtype == T0G_F32 ? "_f32" : "_bf16");
+    const std::string types = std::string(d.a_dtype == T0G_E4M3 ? "e4" : "e5") + (d.b_dtype == T0G_E4M3 ? "e4" : "e5") +
+                              (d.b_block == T0G_BLOCK_TILE ? "_tile" : "_row");
+    if (pl.skinny) {
+        t.flags = d.out_dtype == T0G_F32 ? T0G_TILE_OUT_F32 : 0;
+        const std::string symbol = std::string("t0g_ffn_f8_skinny") + (d.m <= 16 ? "1_" : "2_") + types;
+        return ffn_launch(dev, symbol.c_str(), (d.n + 15) / 16, 1, 512, &t, sizeof t);
+    }
+    const std::string symbol = "t0g_ffn_f8_128x128_" + types + (d.out_dtype == T0G_F32 ? "_f32" : "_bf16");
     return ffn_launch(dev, symbol.c_str(), t.tiles_m * t.tiles_n, 1, 256, &t, sizeof t);
 }
 
@@ -482,6 +498,7 @@ int check_gated(t0g_gated_linear_desc *d, uint32_t *act) {
 
 // The gated tile kernels' operands.
 struct GatedPlan {
+    bool skinny = false;
     Operand x, wg, wu;
     void set(uint64_t xa, uint64_t g, uint64_t u, uint32_t rows, uint32_t features, uint32_t hidden, uint32_t ldx, uint32_t ldw,
              uint32_t transpose, uint64_t *at) {
@@ -513,6 +530,8 @@ int run_gated_tile(t0g_device *dev, T0gTileArgs *t, const GatedPlan &pl, uint64_
 
 int gated_plan(const t0g_gated_linear_desc &d, GatedPlan *pl, uint64_t *bytes) {
     *bytes = 0;
+    pl->skinny = d.transpose == T0G_NT && d.rows <= kSkinnyRows;
+    if (pl->skinny) return T0G_OK;
     pl->set(d.x, d.wg, d.wu, d.rows, d.features, d.hidden, d.ldx, d.ldw, d.transpose, bytes);
     return T0G_OK;
 }
@@ -541,6 +560,15 @@ int gated_call(t0g_device *dev, const t0g_gated_linear_desc *desc) {
     t.k = d.hidden;
     t.act = act;
     t.flags = d.h_dtype == T0G_F32 ? T0G_TILE_OUT_F32 : 0;
+    if (pl.skinny) {
+        t.a = d.x;
+        t.b = d.wg;
+        t.b2 = d.wu;
+        t.lda = d.ldx;
+        t.ldb = d.ldw;
+        return ffn_launch(dev, d.rows <= 16 ? "t0g_ffn_gated_skinny1" : "t0g_ffn_gated_skinny2", (d.features + 15) / 16, 1, 512, &t,
+                          sizeof t);
+    }
     if ((rc = pl.pad(dev, base))) return rc;
     return run_gated_tile(dev, &t, pl, base, d.transpose, "");
 }
