@@ -5,6 +5,7 @@
 #include "ffn_rows.h"
 #include "ffn_tile.h"
 #include "ffn_skinny.h"
+#include "ffn_big.h"
 
 #define NORM(NT, CH, KEEP) \
     extern "C" __global__ void __launch_bounds__(NT) t0g_ffn_norm_##NT##x##CH(T0gNormArgs p) { t0g::rms_norm<NT, CH, KEEP>(p); }
@@ -46,6 +47,17 @@ extern "C" __global__ void __launch_bounds__(256) t0g_ffn_add_planes(T0gAddArgs 
     F8_TYPES(NAME, BM, BN, WM, WN, e5e5, 1, 1)
 F8_TILES(128x128, 128, 128, 2, 2)
 
+#define F8_BIG(TYPES, FA, FB)                                                                                   \
+    extern "C" __global__ void __launch_bounds__(512) t0g_ffn_f8_256x256_##TYPES##_tile_bf16(T0gTileArgs p) {   \
+        t0g::f8_big<FA, FB, true>(p);                                                                           \
+    }                                                                                                           \
+    extern "C" __global__ void __launch_bounds__(512) t0g_ffn_f8_256x256_##TYPES##_row_bf16(T0gTileArgs p) {    \
+        t0g::f8_big<FA, FB, false>(p);                                                                          \
+    }
+F8_BIG(e4e4, 0, 0)
+F8_BIG(e4e5, 0, 1)
+F8_BIG(e5e4, 1, 0)
+F8_BIG(e5e5, 1, 1)
 #define F8_SKINNY(MT, TYPES, FA, FB)                                                                              \
     extern "C" __global__ void __launch_bounds__(512) t0g_ffn_f8_skinny##MT##_##TYPES##_tile(T0gTileArgs p) {      \
         t0g::f8_skinny<8, MT, FA, FB, true>(p);                                                                    \

@@ -108,6 +108,7 @@ __device__ __forceinline__ void f8_skinny(const T0gTileArgs& p) {
     for (; blk + (U - 1) * W < full; blk += U * W) {
 #pragma unroll
         for (int u = 0; u < U; ++u) load(u, blk + u * W, false);
+        __builtin_amdgcn_sched_barrier(0);   // all of them on their way before the first is waited for
 #pragma unroll
         for (int u = 0; u < U; ++u) multiply(u);
     }
@@ -155,6 +156,7 @@ __device__ __forceinline__ void gated_skinny(const T0gTileArgs& p) {
     for (; blk + (U - 1) * W < full; blk += U * W) {
 #pragma unroll
         for (int u = 0; u < U; ++u) load(u, blk + u * W, false);
+        __builtin_amdgcn_sched_barrier(0);   // all of them on their way before the first is waited for
 #pragma unroll
         for (int u = 0; u < U; ++u) multiply(u);
     }

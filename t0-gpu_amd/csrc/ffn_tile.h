@@ -56,11 +56,14 @@ struct RowsK {
         frag = (wrow + l16) * 128 + ((q ^ ((l16 >> 1) & 7u)) << 4);
     }
     // Stage at byte k0 of K, kb bytes in all.
+    __device__ __forceinline__ u32x4_t rsrc(uint32_t k0) const { return rsrc_words_wide(base, bytes, k0); }
+    __device__ __forceinline__ void issue_one(int i, u32x4_t r, uint32_t lds, uint32_t k0, uint32_t kb, uint32_t wave) const {
+        dma16(r, k0 + kcol < kb ? off + i * step : kOob, lds + (i * W + wave) * 1024);
+    }
     __device__ __forceinline__ void issue(uint32_t lds, uint32_t k0, uint32_t kb, uint32_t wave) const {
-        const u32x4_t r = rsrc_words_wide(base, bytes, k0);
-        const bool ok = k0 + kcol < kb;
+        const u32x4_t r = rsrc(k0);
 #pragma unroll
-        for (int i = 0; i < kInstr; ++i) dma16(r, ok ? off + i * step : kOob, lds + (i * W + wave) * 1024);
+        for (int i = 0; i < kInstr; ++i) issue_one(i, r, lds, k0, kb, wave);
     }
     // Chunks q and 4 + q of 16 rows: K values in an order of their own, the same for both operands.
     template <int HALF>

@@ -434,7 +434,8 @@ int fp8_gemm_call(t0g_device *dev, const t0g_fp8_gemm_desc *desc) {
     t.m = d.m;
     t.n = d.n;
     t.k = d.k;
-    if ((rc = pl.skinny ? skinny_groups(d.n) : set_tiles(&t, 128, 128))) return rc;
+    const bool big = d.out_dtype == T0G_BF16 && ((uint64_t)d.m + 255) / 256 * (((uint64_t)d.n + 255) / 256) >= kNumCUs;
+    if ((rc = pl.skinny ? skinny_groups(d.n) : big ? set_tiles(&t, 256, 256) : set_tiles(&t, 128, 128))) return rc;
     if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
     std::lock_guard<std::mutex> lk(device_mutex(dev));
     uint64_t base;
@@ -457,8 +458,8 @@ int fp8_gemm_call(t0g_device *dev, const t0g_fp8_gemm_desc *desc) {
         const std::string symbol = std::string("t0g_ffn_f8_skinny") + (d.m <= 16 ? "1_" : "2_") + types;
         return ffn_launch(dev, symbol.c_str(), (d.n + 15) / 16, 1, 512, &t, sizeof t);
     }
-    const std::string symbol = "t0g_ffn_f8_128x128_" + types + (d.out_dtype == T0G_F32 ? "_f32" : "_bf16");
-    return ffn_launch(dev, symbol.c_str(), t.tiles_m * t.tiles_n, 1, 256, &t, sizeof t);
+    const std::string symbol = (big ? "t0g_ffn_f8_256x256_" : "t0g_ffn_f8_128x128_") + types + (d.out_dtype == T0G_F32 ? "_f32" : "_bf16");
+    return ffn_launch(dev, symbol.c_str(), t.tiles_m * t.tiles_n, 1, big ? 512 : 256, &t, sizeof t);
 }
 
 // ---- gated projections ------------------------------------------------------------------

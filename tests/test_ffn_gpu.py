@@ -371,6 +371,13 @@ def test_f8_gemm(rt, m, n, k, block, at, bt, out):
     f8_gemm(rt, m, n, k, at, bt, block, out)
 
 
+@pytest.mark.parametrize("m,n,k", [(4096, 4096, 128), (3900, 4200, 1200), (4100, 8000, 400), (8200, 2500, 1040)])
+@pytest.mark.parametrize("block", ["row", "tile"])
+@pytest.mark.parametrize("at,bt,out", [(E4, E4, BF16), (E5, E4, BF16), (E4, E5, F32)])
+def test_f8_gemm_many_tiles(rt, m, n, k, block, at, bt, out):
+    f8_gemm(rt, m, n, k, at, bt, block, out)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 77, 300), (3, 640, 512), (16, 129, 1000), (40, 130, 256), (70, 400, 784), (300, 290, 640)])
 @pytest.mark.parametrize("block", ["row", "tile"])
 @pytest.mark.parametrize("pad,offset", [(3, 1), (16, 16), (1, 0), (128, 4)])
