@@ -32,7 +32,8 @@ extern "C" __global__ void __launch_bounds__(256) t0g_ffn_add_planes(T0gAddArgs 
 
 // Symbols: t0g_ffn_f8_<tile>_<type of A><type of B>_<blocks of B>_<output type>.
 #define F8_KERNEL(NAME, BM, BN, WM, WN, TYPES, FA, FB, BLOCK, B_TILE, OUT, WIDE)                                                   \
-    extern "C" __global__ void __launch_bounds__(64 * WM * WN) t0g_ffn_f8_##NAME##_##TYPES##_##BLOCK##_##OUT(T0gTileArgs p) { \
+    extern "C" __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2)))                     \
+        t0g_ffn_f8_##NAME##_##TYPES##_##BLOCK##_##OUT(T0gTileArgs p) {                                                        \
         t0g::f8_tile<BM, BN, WM, WN, FA, FB, B_TILE, WIDE>(p);                                                                \
     }
 #define F8_TYPES(NAME, BM, BN, WM, WN, TYPES, FA, FB)                        \

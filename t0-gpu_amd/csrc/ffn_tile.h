@@ -248,44 +248,74 @@ __device__ __forceinline__ void f8_tile(const T0gTileArgs& p) {
         barrier_no_fence();
         const uint32_t nxt = lds0 + (cur == lds0 ? STAGE : 0u);
         if (s + 1 < nst) issue(s + 1, nxt);
-        i32x8_t fb[WIDE ? 1 : SN];
-        i32x4_t wb[WIDE ? SN : 1][4];
-        f32x4_t sbv[SN];
-#pragma unroll
-        for (int j = 0; j < SN; ++j) {
-            if constexpr (WIDE)
-                widen<FB>(lb.template read<0>(cur + A, j), lb.template read<1>(cur + A, j), wb[j]);
-            else
-                fb[j] = join(lb.template read<0>(cur + A, j), lb.template read<1>(cur + A, j));
-            if constexpr (!B_TILE)
-                sbv[j] = *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(
-                    (uintptr_t)(cur + AB + BM * 4 + (wn * TN + 16 * j + 4 * q) * 4));
-        }
+        f32x4_t sbv[B_TILE ? 1 : SN];
+        float f[SM];
 #pragma unroll
         for (int i = 0; i < SM; ++i) {
-            i32x8_t fa;
-            i32x4_t wa[4];
-            if constexpr (WIDE)
-                widen<FA>(la.template read<0>(cur, i), la.template read<1>(cur, i), wa);
-            else
-                fa = join(la.template read<0>(cur, i), la.template read<1>(cur, i));
-            float sa = *reinterpret_cast<const __attribute__((address_space(3))) float*>((uintptr_t)(cur + AB + (wm * TM + 16 * i + l16) * 4));
-            if constexpr (B_TILE) sa *= sb;
+            f[i] = reinterpret_cast<const __attribute__((address_space(3))) float*>((uintptr_t)(cur + AB + (wm * TM + l16) * 4))[16 * i];
+            if constexpr (B_TILE) f[i] *= sb;
+        }
+        if constexpr (!B_TILE)
 #pragma unroll
-            for (int j = 0; j < SN; ++j) {
-                f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (WIDE)
+            for (int j = 0; j < SN; ++j)
+                sbv[j] = reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(
+                    (uintptr_t)(cur + AB + (BM + wn * TN + 4 * q) * 4))[4 * j];
+        auto add = [&](int i, int j, int e, const f32x4_t& v) {
+            acc[i][j][e] = __builtin_fmaf(B_TILE ? v[e] : v[e] * sbv[B_TILE ? 0 : j][e], f[i], acc[i][j][e]);
+        };
+        // The order of the instructions is pinned, the vector instructions on a result some matrix instructions
+        // behind it: the compiler's own puts them right behind, where the wave waits for it.
+        if constexpr (WIDE) {
+            i32x4_t wb[SN][4], wa[2][4], lo = la.template read<0>(cur, 0), hi = la.template read<1>(cur, 0);
+            f32x4_t v[2][SN];
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) v = mfma_bf16(wb[j][h], wa[h], v);
-                else
-                    v = mfma_f8<FB, FA>(fb[j], fa, v);
+            for (int j = 0; j < SN; ++j) widen<FB>(lb.template read<0>(cur + A, j), lb.template read<1>(cur + A, j), wb[j]);
+            widen<FA>(lo, hi, wa[0]);
+            // beside a row's 4 SN matrix instructions: the additions of the row before, and the conversion of the next
+            static_assert(SN == 4, "16 additions of 4 values beside 16 matrix instructions");
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (B_TILE)
-                        acc[i][j][e] = __builtin_fmaf(v[e], sa, acc[i][j][e]);
-                    else
-                        acc[i][j][e] = __builtin_fmaf(v[e] * sbv[j][e], sa, acc[i][j][e]);
+            for (int i = 0; i < SM; ++i) {
+                if (i + 1 < SM) {
+                    lo = la.template read<0>(cur, i + 1);
+                    hi = la.template read<1>(cur, i + 1);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < 4 * SN; ++t) {
+                    const int h = t / SN, j = t % SN;
+                    v[i & 1][j] = mfma_bf16(wb[j][h], wa[i & 1][h], h ? v[i & 1][j] : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+                    if (i > 0) add(i - 1, t / 4, t % 4, v[(i - 1) & 1][t / 4]);
+                    if (i + 1 < SM && t >= 6 && t % 3 == 0) {
+                        const int g = (t - 6) / 3;
+                        wa[(i + 1) & 1][g] = g == 0   ? wide8<FA>(lo[0], lo[1])
+                                             : g == 1 ? wide8<FA>(lo[2], lo[3])
+                                             : g == 2 ? wide8<FA>(hi[0], hi[1])
+                                                      : wide8<FA>(hi[2], hi[3]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 4 * SN; ++t) add(SM - 1, t / 4, t % 4, v[(SM - 1) & 1][t / 4]);
+        } else {
+            constexpr int kBehind = 3, T = SM * SN;
+            i32x8_t fb[SN], fa[2];
+            f32x4_t v[kBehind + 1];
+            auto read_a = [&](int i) { fa[i & 1] = join(la.template read<0>(cur, i), la.template read<1>(cur, i)); };
+            read_a(0);
+#pragma unroll
+            for (int j = 0; j < SN; ++j) fb[j] = join(lb.template read<0>(cur + A, j), lb.template read<1>(cur + A, j));
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < T + kBehind; ++t) {
+                if (t < T) {
+                    v[t % (kBehind + 1)] = mfma_f8<FB, FA>(fb[t % SN], fa[t / SN & 1], f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+                    if (t % SN == 0 && t / SN + 1 < SM) read_a(t / SN + 1);
+                }
+                if (t >= kBehind)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) add((t - kBehind) / SN, (t - kBehind) % SN, e, v[(t - kBehind) % (kBehind + 1)]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         cur = nxt;
