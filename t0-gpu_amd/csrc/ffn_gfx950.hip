@@ -6,6 +6,7 @@
 #include "ffn_tile.h"
 #include "ffn_skinny.h"
 #include "ffn_big.h"
+#include "ffn_gated.h"
 
 #define NORM(NT, CH, KEEP) \
     extern "C" __global__ void __launch_bounds__(NT) t0g_ffn_norm_##NT##x##CH(T0gNormArgs p) { t0g::rms_norm<NT, CH, KEEP>(p); }
@@ -90,3 +91,9 @@ extern "C" __global__ void __launch_bounds__(512) t0g_ffn_gated_skinny2(T0gTileA
         t0g::gated_tile<BM, BN, WM, WN, true, true>(p);                                                        \
     }
 GATED(128x64, 128, 64, 2, 2)
+extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) t0g_ffn_gated_256x128_nt(T0gTileArgs p) {
+    t0g::gated_big<false>(p);
+}
+extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) t0g_ffn_gated_256x128_nn(T0gTileArgs p) {
+    t0g::gated_big<true>(p);
+}

@@ -39,42 +39,6 @@ __device__ __forceinline__ uint32_t pack_e(float lo, float hi) {
     return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi) << 2, __builtin_bit_cast(uint32_t, lo) << 2, 0x07060302u);
 }
 
-// One 16-row band of a wave's sub-tiles, packed in 16 bits (w[j]: the lane's 4 rows of
-// column 16 j + c), through LDS to 16-byte stores of whole lines, as store_tile_bf16_tr
-// does.  `c`: address of the wave tile's first element, rows ldc apart.
-template <int SN>
-__device__ __forceinline__ void store_band16(const uint64_t (&w)[SN], uint64_t c, uint32_t ldc, int i, uint32_t lane,
-                                             uint32_t lds) {
-    typedef short v4s __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) v4s lds_v4s;
-    typedef __attribute__((address_space(3))) uint64_t lds_u64;
-    const uint32_t reg = lds + (uint32_t)(i & 1) * (SN * 16 * 32);
-    const uint32_t l16 = lane & 15u, q = lane >> 4, r = (lane >> 2) & 3u, s = lane & 3u;
-#pragma unroll
-    for (int j = 0; j < SN; ++j) *reinterpret_cast<lds_u64*>((uintptr_t)(reg + bf16_stage_off(16u * j + l16, q))) = w[j];
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    const uint32_t rcol = 16u * q + 8u * (s & 1u) + r, rpc = s >> 1;
-    const uint32_t srow = 4u * ((l16 >> 2) >> 1) + s, scol = 16u * q + 8u * ((l16 >> 2) & 1u);
-    const uint64_t cb = c + ((uint64_t)srow * ldc + scol) * 2u;
-#pragma unroll
-    for (int u = 0; u < SN / 4; ++u)
-#pragma unroll
-        for (int pp = 0; pp < 2; ++pp) {
-            const uint32_t c0 = 64u * u + rcol, piece = 2u * pp + rpc;
-            const v4s lo =
-                __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)(reg + bf16_stage_off(c0, piece)));
-            const v4s hi =
-                __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)(reg + bf16_stage_off(c0 + 4u, piece)));
-            u32x4_t v;
-            v[0] = __builtin_bit_cast(uint32_t, __builtin_shufflevector(lo, lo, 0, 1));
-            v[1] = __builtin_bit_cast(uint32_t, __builtin_shufflevector(lo, lo, 2, 3));
-            v[2] = __builtin_bit_cast(uint32_t, __builtin_shufflevector(hi, hi, 0, 1));
-            v[3] = __builtin_bit_cast(uint32_t, __builtin_shufflevector(hi, hi, 2, 3));
-            const uint64_t addr = cb + ((uint64_t)(16u * i + 8u * pp) * ldc + 64u * u) * 2u;
-            __builtin_nontemporal_store(v, reinterpret_cast<__attribute__((address_space(1))) u32x4_t*>((uintptr_t)addr));
-        }
-}
-
 // The raw logits of the entries (sorted tokens of each row) in a wave's 128 x 128 tile.
 // Lane l looks after rows l and 64 + l.  Which entries a row has there, and its first two
 // tokens, are loaded two bands of statistics ahead of their use, which covers the

@@ -517,15 +517,25 @@ struct GatedPlan {
     }
 };
 
+// Whether the 256x256 tile takes a gated pair: enough tiles for all CUs, and 32-bit offsets in the operands.
+bool gated_big(const T0gTileArgs &t, bool nt) {
+    const uint64_t tiles = ((uint64_t)t.m + 255) / 256 * (((uint64_t)t.n + 127) / 128);
+    const uint64_t most = 1ull << 30, wspan = ((uint64_t)(nt ? t.n + 256 : t.k + 64)) * t.ldb;
+    const uint64_t apart = t.b < t.b2 ? t.b2 - t.b : t.b - t.b2;
+    return tiles >= kNumCUs && (t.m + 256ull) * t.lda < most && wspan < most && t.lda >= 64 &&
+           (nt ? t.ldb >= 64 : t.ldb >= 256 && apart + wspan * 2 < (1ull << 31) - 4096);   // offsets out of range stay so less 3 KB
+}
+
 int run_gated_tile(t0g_device *dev, T0gTileArgs *t, const GatedPlan &pl, uint64_t base, uint32_t transpose, const char *kind) {
     t->a = pl.x.address(base);
     t->b = pl.wg.address(base);
     t->b2 = pl.wu.address(base);
     t->lda = pl.x.pitch();
     t->ldb = pl.wg.pitch();
-    int rc = set_tiles(t, 128, 64);
+    const bool nt = transpose == T0G_NT, big = !*kind && gated_big(*t, nt);
+    int rc = big ? set_tiles(t, 256, 128) : set_tiles(t, 128, 64);
     if (rc) return rc;
-    const std::string symbol = std::string("t0g_ffn_gated_128x64") + (transpose == T0G_NT ? "_nt" : "_nn") + kind;
+    const std::string symbol = std::string(big ? "t0g_ffn_gated_256x128" : "t0g_ffn_gated_128x64") + (nt ? "_nt" : "_nn") + kind;
     return ffn_launch(dev, symbol.c_str(), t->tiles_m * t->tiles_n, 1, 256, t, sizeof *t);
 }
 

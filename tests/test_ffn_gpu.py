@@ -521,6 +521,16 @@ def test_gated(rt, rows, f, hidden, layout, act, out, pad, offset, apart):
     c.free()
 
 
+@pytest.mark.parametrize("rows,f,hidden", [(2048, 4096, 64), (2000, 4200, 200), (4100, 2050, 330), (300, 16400, 77)])
+@pytest.mark.parametrize("layout", ["NT", "NN"])
+@pytest.mark.parametrize("act,out,keep,pad,offset,apart", [("silu", BF16, True, 0, 0, False), ("gelu", F32, False, 8, 8, True),
+                                                           ("silu", BF16, False, 3, 1, False)])
+def test_gated_many_tiles(rt, rows, f, hidden, layout, act, out, keep, pad, offset, apart):
+    c = Gated(rt, rows, f, hidden, layout, act, pad, offset, apart)
+    c.forward(keep, out)
+    c.free()
+
+
 @pytest.mark.parametrize("rows,f,hidden", [(1, 1, 1), (1, 64, 64), (3, 65, 72), (16, 63, 200), (17, 128, 77), (64, 72, 512), (130, 264, 136),
                                            (300, 520, 264), (520, 301, 129)])
 @pytest.mark.parametrize("layout", ["NT", "NN"])
