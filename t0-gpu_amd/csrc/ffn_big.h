@@ -30,17 +30,16 @@ __device__ __forceinline__ void f8_big(const T0gTileArgs& p) {
         for (int j = 0; j < SN; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     // A stage past the end brings zeros and reads no memory.  Scales, 64 a request: waves 0 to 3 bring A's, 4 to 7 B's.
     const bool mine = wave < 4;
-    const uint64_t sbase = mine ? p.as + (uint64_t)m0 * 4 : p.bs + (uint64_t)n0 * 4, sld = (uint64_t)(mine ? p.ldas : p.ldbs) * 4;
-    const uint64_t sbytes = (uint64_t)(mine ? p.m - m0 : B_TILE ? 0u : p.n - n0) * 4;
-    const uint32_t soff = (64 * (wave & 3u) + lane) * 4;
+    const uint32_t at64 = 64 * (wave & 3u) + lane;   // a scale for each 128 columns is spread to the columns
+    const uint64_t sbase = mine ? p.as : p.bs, sld = (uint64_t)(mine ? p.ldas : p.ldbs) * 4;
+    const uint64_t sbytes = (uint64_t)(mine ? p.m : B_TILE ? (p.n + 127) / 128 : p.n) * 4;
+    const uint32_t soff = (mine ? m0 + at64 : B_TILE ? (n0 + at64) / 128 : n0 + at64) * 4;
     auto issue_scales = [&](uint32_t s, uint32_t lds) {
         const u32x4_t r = rsrc_words_wide(sbase, (s < nst ? sbytes : 0u) + (uint64_t)s * sld, (uint64_t)s * sld);
         dma4(r, soff, lds + AB + 256 * wave);
     };
     typedef const __attribute__((address_space(3))) f32x4_t lds_f32x4;
     typedef const __attribute__((address_space(3))) float lds_f32;
-    const uint32_t bcol = min((n0 + wn * TN) / 128, (p.n - 1) / 128);
-    auto scale_b = [&](uint32_t s) { return B_TILE ? *at<const float>(p.bs, (uint64_t)min(s, nst - 1) * p.ldbs + bcol) : 0.0f; };
     i32x8_t fb[SN], fa[3];
     f32x4_t sbv[B_TILE ? 1 : SN];
     float sa[3];
@@ -63,7 +62,6 @@ __device__ __forceinline__ void f8_big(const T0gTileArgs& p) {
 #pragma unroll
     for (int j = 0; j < SN; ++j) read_b(lds0, j);
     uint32_t cur = lds0;
-    float sb = scale_b(0);
     // Matrix instruction t and, beside it, the vector instructions on the result of t - kBehind and a read for
     // a row of sub-tiles to come, pinned in this order: the compiler's own puts each result's use right
     // behind it, where the wave waits for it.  The last two rows of sub-tiles go column by column, so that
@@ -75,8 +73,9 @@ __device__ __forceinline__ void f8_big(const T0gTileArgs& p) {
     static_assert(2 * OpA::kInstr <= 2 * SN && 2 * OpB::kInstr < kLast, "a stage's requests fit");
     for (uint32_t s = 0; s < nst; ++s) {
         const uint32_t nxt = lds0 + (cur == lds0 ? STAGE : 0u);
-        const float sbc = sb;
-        sb = scale_b(s + 1);
+        // (through LDS: a load of the compiler's would be waited for together with all DMA before it)
+        float sbc = 0.0f;
+        if constexpr (B_TILE) sbc = *reinterpret_cast<lds_f32*>((uintptr_t)(cur + AB + (BM + wn * TN) * 4));
 #pragma unroll
         for (int j = 0; j < SN; ++j) read_sb(cur, j);
         const u32x4_t rb = lb.rsrc((s + 1) * 128), ra = la.rsrc((s + 2) * 128);
@@ -123,6 +122,7 @@ __device__ __forceinline__ void f8_big(const T0gTileArgs& p) {
         }
         cur = nxt;
     }
+    T0G_WAIT_VMCNT(0);   // stages past the end: the LDS is the next workgroup's
 #pragma unroll
     for (int i = 0; i < SM; ++i) {
         const uint32_t row = m0 + wm * TM + 16 * i + l16;

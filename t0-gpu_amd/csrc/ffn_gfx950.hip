@@ -29,25 +29,27 @@ extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_rows(T0gQuant
 extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_tile(T0gQuantArgs p) { t0g::quantize_tile(p); }
 extern "C" __global__ void __launch_bounds__(256) t0g_ffn_gated_grad(T0gGatedGradArgs p) { t0g::gated_grad(p); }
 extern "C" __global__ void __launch_bounds__(256) t0g_ffn_pad_rows(T0gPadArgs p) { t0g::pad_rows(p); }
+extern "C" __global__ void __launch_bounds__(256) t0g_ffn_join_slices(T0gJoinArgs p) { t0g::join_slices(p); }
 extern "C" __global__ void __launch_bounds__(256) t0g_ffn_add_planes(T0gAddArgs p) { t0g::add_planes(p); }
 
 // Symbols: t0g_ffn_f8_<tile>_<type of A><type of B>_<blocks of B>_<output type>.
-#define F8_KERNEL(NAME, BM, BN, WM, WN, TYPES, FA, FB, BLOCK, B_TILE, OUT, WIDE)                                                   \
+#define F8_KERNEL(NAME, BM, BN, WM, WN, NS, TYPES, FA, FB, BLOCK, B_TILE, OUT, WIDE)                                                   \
     extern "C" __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2)))                     \
         t0g_ffn_f8_##NAME##_##TYPES##_##BLOCK##_##OUT(T0gTileArgs p) {                                                        \
-        t0g::f8_tile<BM, BN, WM, WN, FA, FB, B_TILE, WIDE>(p);                                                                \
+        t0g::f8_tile<BM, BN, WM, WN, NS, FA, FB, B_TILE, WIDE>(p);                                                               \
     }
-#define F8_TYPES(NAME, BM, BN, WM, WN, TYPES, FA, FB)                        \
-    F8_KERNEL(NAME, BM, BN, WM, WN, TYPES, FA, FB, tile, true, bf16, false)  \
-    F8_KERNEL(NAME, BM, BN, WM, WN, TYPES, FA, FB, tile, true, f32, true)    \
-    F8_KERNEL(NAME, BM, BN, WM, WN, TYPES, FA, FB, row, false, bf16, false)  \
-    F8_KERNEL(NAME, BM, BN, WM, WN, TYPES, FA, FB, row, false, f32, true)
-#define F8_TILES(NAME, BM, BN, WM, WN)             \
-    F8_TYPES(NAME, BM, BN, WM, WN, e4e4, 0, 0)     \
-    F8_TYPES(NAME, BM, BN, WM, WN, e4e5, 0, 1)     \
-    F8_TYPES(NAME, BM, BN, WM, WN, e5e4, 1, 0)     \
-    F8_TYPES(NAME, BM, BN, WM, WN, e5e5, 1, 1)
-F8_TILES(128x128, 128, 128, 2, 2)
+#define F8_TYPES(NAME, BM, BN, WM, WN, NS, TYPES, FA, FB)                        \
+    F8_KERNEL(NAME, BM, BN, WM, WN, NS, TYPES, FA, FB, tile, true, bf16, false)  \
+    F8_KERNEL(NAME, BM, BN, WM, WN, NS, TYPES, FA, FB, tile, true, f32, true)    \
+    F8_KERNEL(NAME, BM, BN, WM, WN, NS, TYPES, FA, FB, row, false, bf16, false)  \
+    F8_KERNEL(NAME, BM, BN, WM, WN, NS, TYPES, FA, FB, row, false, f32, true)
+#define F8_TILES(NAME, BM, BN, WM, WN, NS)             \
+    F8_TYPES(NAME, BM, BN, WM, WN, NS, e4e4, 0, 0)     \
+    F8_TYPES(NAME, BM, BN, WM, WN, NS, e4e5, 0, 1)     \
+    F8_TYPES(NAME, BM, BN, WM, WN, NS, e5e4, 1, 0)     \
+    F8_TYPES(NAME, BM, BN, WM, WN, NS, e5e5, 1, 1)
+F8_TILES(128x128, 128, 128, 2, 2, 2)
+F8_TILES(64x128, 64, 128, 2, 2, 3)
 
 #define F8_BIG(TYPES, FA, FB)                                                                                   \
     extern "C" __global__ void __launch_bounds__(512) t0g_ffn_f8_256x256_##TYPES##_tile_bf16(T0gTileArgs p) {   \
@@ -77,20 +79,21 @@ F8_SKINNIES(2)
 extern "C" __global__ void __launch_bounds__(512) t0g_ffn_gated_skinny1(T0gTileArgs p) { t0g::gated_skinny<8, 1>(p); }
 extern "C" __global__ void __launch_bounds__(512) t0g_ffn_gated_skinny2(T0gTileArgs p) { t0g::gated_skinny<8, 2>(p); }
 
-#define GATED(NAME, BM, BN, WM, WN)                                                                            \
+#define GATED(NAME, BM, BN, WM, WN, NS)                                                                            \
     extern "C" __global__ void __launch_bounds__(64 * WM * WN) t0g_ffn_gated_##NAME##_nt(T0gTileArgs p) {      \
-        t0g::gated_tile<BM, BN, WM, WN, false, false>(p);                                                      \
+        t0g::gated_tile<BM, BN, WM, WN, NS, false, false>(p);                                                      \
     }                                                                                                          \
     extern "C" __global__ void __launch_bounds__(64 * WM * WN) t0g_ffn_gated_##NAME##_nn(T0gTileArgs p) {      \
-        t0g::gated_tile<BM, BN, WM, WN, true, false>(p);                                                       \
+        t0g::gated_tile<BM, BN, WM, WN, NS, true, false>(p);                                                       \
     }                                                                                                          \
     extern "C" __global__ void __launch_bounds__(64 * WM * WN) t0g_ffn_gated_##NAME##_nt_grad(T0gTileArgs p) { \
-        t0g::gated_tile<BM, BN, WM, WN, false, true>(p);                                                       \
+        t0g::gated_tile<BM, BN, WM, WN, NS, false, true>(p);                                                       \
     }                                                                                                          \
     extern "C" __global__ void __launch_bounds__(64 * WM * WN) t0g_ffn_gated_##NAME##_nn_grad(T0gTileArgs p) { \
-        t0g::gated_tile<BM, BN, WM, WN, true, true>(p);                                                        \
+        t0g::gated_tile<BM, BN, WM, WN, NS, true, true>(p);                                                        \
     }
-GATED(128x64, 128, 64, 2, 2)
+GATED(128x64, 128, 64, 2, 2, 2)
+GATED(64x64, 64, 64, 2, 2, 3)
 extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) t0g_ffn_gated_256x128_nt(T0gTileArgs p) {
     t0g::gated_big<false>(p);
 }

@@ -531,23 +531,23 @@ __device__ __forceinline__ void gated_grad(const T0gGatedGradArgs& p) {
     }
 }
 
+// A wave a row, 16 bytes a lane; rows may start anywhere.
 __device__ __forceinline__ void pad_rows(const T0gPadArgs& p) {
-    const uint32_t step = 8 / p.size, per_row = p.ldd / step;   // pieces of 8 bytes
-    const uint64_t pieces = (uint64_t)p.rows * per_row;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t row = i / per_row;
-        const uint32_t c = (uint32_t)(i - row * per_row) * step;
-        const uint64_t from = p.src + (row * p.lds + c) * p.size;
-        const uint32_t n = c < p.cols ? min(p.cols - c, step) * p.size : 0u;   // bytes
-        u32x2_t w = {0u, 0u};
-        if (n == 8) {
-            w = *at<const u32x2_any>(from);
-        } else {
+    typedef u32x4_t u32x4_byte __attribute__((aligned(1)));
+    const auto& o = p.a[blockIdx.y];
+    for (uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6); row < o.rows; row += gridDim.x * 4) {
+        const uint64_t from = o.src + row * o.lds, to = o.dst + row * o.ldd;
+        for (uint32_t c = 16 * (threadIdx.x & 63u); c < o.ldd; c += 1024) {
+            u32x4_t w = {0u, 0u, 0u, 0u};
+            if (c + 16 <= o.bytes) {
+                w = *at<const u32x4_byte>(from + c);
+            } else {
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e)
-                if (e < n) w[e / 4] |= (uint32_t)*at<const uint8_t>(from, e) << (8 * (e & 3));
+                for (uint32_t e = 0; e < 16; ++e)
+                    if (c + e < o.bytes) w[e / 4] |= (uint32_t)*at<const uint8_t>(from + c, e) << (8 * (e & 3));
+            }
+            *at<u32x4_t>(to + c) = w;
         }
-        *at<u32x2_t>(p.dst + i * 8) = w;
     }
 }
 

@@ -1,6 +1,6 @@
 // Tile kernels of the feed-forward layer's products: C = A B^T of 8-bit values with block
 // scales, and the gated pair of bf16 products.  Both stage 128 bytes of K of every row (128
-// values of 8 bits, 64 of bf16) in LDS by DMA, two stages in turn, and multiply 16x16
+// values of 8 bits, 64 of bf16) in LDS by DMA, NS stages in turn, and multiply 16x16
 // sub-tiles with the operands swapped: the matrix unit's rows are C's columns, so lane
 // (q, c) of a sub-tile holds columns 4 q .. 4 q + 3 of row c of C, neighbours in memory, and
 // a row's scale is one register.
@@ -199,14 +199,15 @@ __device__ __forceinline__ uint32_t left4(uint32_t n, uint32_t c) { return c < n
 // values and on ones spread over 8 binades), far below bf16's own rounding but not below f32's.  So
 // results in f32 (WIDE) come from bf16 matrix instructions, at half the rate, on the values converted in
 // registers: their products and sums are exact to f32's rounding (1e-8).
-template <int BM, int BN, int WM, int WN, int FA, int FB, bool B_TILE, bool WIDE>
+template <int BM, int BN, int WM, int WN, int NS, int FA, int FB, bool B_TILE, bool WIDE>
 __device__ __forceinline__ void f8_tile(const T0gTileArgs& p) {
     constexpr int W = WM * WN, TM = BM / WM, TN = BN / WN, SM = TM / 16, SN = TN / 16;
     static_assert(!B_TILE || 128 % TN == 0, "one scale of B for a wave's columns");
     using OpA = RowsK<BM, W>;
     using OpB = RowsK<BN, W>;
-    constexpr uint32_t A = OpA::kBytes, AB = A + OpB::kBytes, SCALES = (BM + BN) * 4, STAGE = AB + SCALES;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
+    constexpr uint32_t A = OpA::kBytes, AB = A + OpB::kBytes, STAGE = AB + W * 256;
+    static_assert(W * 64 == BM + BN || (W * 64 > BM + BN && W % 2 == 0), "a wave brings 64 scales");
+    __shared__ __attribute__((aligned(1024))) char smem[NS * STAGE];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t wm = wave / WN, wn = wave % WN, l16 = lane & 15u, q = lane >> 4;
     uint32_t tm, tn;
@@ -218,42 +219,47 @@ __device__ __forceinline__ void f8_tile(const T0gTileArgs& p) {
     la.init(p.a, m0, p.m, p.lda, kb, wave, lane, wm * TM);
     lb.init(p.b, n0, p.n, p.ldb, kb, wave, lane, wn * TN);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem));
-    const uint32_t nst = (p.k + 127) / 128;
+    const uint32_t first = blockIdx.y * p.split_stages, end = min(first + p.split_stages, (p.k + 127) / 128);
     f32x4_t acc[SM][SN];
 #pragma unroll
     for (int i = 0; i < SM; ++i)
 #pragma unroll
         for (int j = 0; j < SN; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
+    // Scales, 64 a request: the first BM / 64 waves bring A's, the next BN / 64 B's.  A stage past the end brings zeros.
+    const bool mine = wave < BM / 64;
+    const uint32_t part = mine ? wave : wave - BM / 64;
+    const uint32_t col = n0 + 64 * part + lane;   // with a scale for each 128 columns they are spread to the columns
+    const uint64_t sbase = mine ? p.as : p.bs, sld = (uint64_t)(mine ? p.ldas : p.ldbs) * 4;
+    const uint64_t sbytes = (uint64_t)(mine ? p.m : wave >= (BM + BN) / 64 ? 0u : B_TILE ? (p.n + 127) / 128 : p.n) * 4;
+    const uint32_t soff = (mine ? m0 + 64 * part + lane : B_TILE ? col / 128 : col) * 4;
     auto issue = [&](uint32_t s, uint32_t lds) {
         la.issue(lds, s * 128, kb, wave);
         lb.issue(lds + A, s * 128, kb, wave);
-        // the scales of the tile's rows, 64 a request
-        const u32x4_t ra = rsrc_words_wide(p.as + (uint64_t)m0 * 4, ((uint64_t)s * p.ldas + (p.m - m0)) * 4, (uint64_t)s * p.ldas * 4);
-        if constexpr (BM / 64 <= W) {
-            if (wave < BM / 64) dma4(ra, (64 * wave + lane) * 4, lds + AB + 256 * wave);
-        }
-        if constexpr (!B_TILE) {
-            const u32x4_t rb = rsrc_words_wide(p.bs + (uint64_t)n0 * 4, ((uint64_t)s * p.ldbs + (p.n - n0)) * 4, (uint64_t)s * p.ldbs * 4);
-            if (wave < BN / 64) dma4(rb, (64 * wave + lane) * 4, lds + AB + BM * 4 + 256 * wave);
-        }
+        const u32x4_t r = rsrc_words_wide(sbase, (s < end ? sbytes : 0u) + s * sld, s * sld);
+        dma4(r, soff, lds + AB + 256 * wave);
     };
-    static_assert(BM / 64 <= W && BN / 64 <= W, "one request of scales for a wave");
-    if (nst) issue(0, lds0);
-    uint32_t cur = lds0;
-    for (uint32_t s = 0; s < nst; ++s) {
-        float sb = 0.0f;
-        if constexpr (B_TILE) sb = *at<const float>(p.bs, (uint64_t)s * p.ldbs + min((n0 + wn * TN) / 128, (p.n - 1) / 128));
-        __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0): the stage is there; lgkmcnt(0): the one before is read
+    constexpr int kVmem = OpA::kInstr + OpB::kInstr + 1;
+    for (int s = 0; s < NS - 1; ++s) issue(first + s, lds0 + s * STAGE);
+    uint32_t cur = lds0, fill = lds0 + (NS - 1) * STAGE;
+    for (uint32_t s = first; s < end; ++s) {
+        // this stage is there (NS - 2 later ones may be on their way), and the one before is read
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        T0G_WAIT_VMCNT(kVmem * (NS - 2));
         barrier_no_fence();
-        const uint32_t nxt = lds0 + (cur == lds0 ? STAGE : 0u);
-        if (s + 1 < nst) issue(s + 1, nxt);
+        issue(s + NS - 1, fill);
+        fill = fill + STAGE == lds0 + NS * STAGE ? lds0 : fill + STAGE;
+        const uint32_t nxt = cur + STAGE == lds0 + NS * STAGE ? lds0 : cur + STAGE;
         f32x4_t sbv[B_TILE ? 1 : SN];
         float f[SM];
 #pragma unroll
         for (int i = 0; i < SM; ++i) {
             f[i] = reinterpret_cast<const __attribute__((address_space(3))) float*>((uintptr_t)(cur + AB + (wm * TM + l16) * 4))[16 * i];
-            if constexpr (B_TILE) f[i] *= sb;
+        }
+        if constexpr (B_TILE) {
+            const float sb = *reinterpret_cast<const __attribute__((address_space(3))) float*>((uintptr_t)(cur + AB + (BM + wn * TN) * 4));
+#pragma unroll
+            for (int i = 0; i < SM; ++i) f[i] *= sb;
         }
         if constexpr (!B_TILE)
 #pragma unroll
@@ -320,6 +326,10 @@ __device__ __forceinline__ void f8_tile(const T0gTileArgs& p) {
         }
         cur = nxt;
     }
+    T0G_WAIT_VMCNT(0);   // stages past the end
+    // a slice of K: f32 into its plane
+    const uint64_t to = p.planes ? p.planes + (uint64_t)blockIdx.y * p.m * p.ldp * 4 : p.c;
+    const uint32_t ld = p.planes ? p.ldp : p.ldc;
 #pragma unroll
     for (int i = 0; i < SM; ++i) {
         const uint32_t row = m0 + wm * TM + 16 * i + l16;
@@ -327,7 +337,7 @@ __device__ __forceinline__ void f8_tile(const T0gTileArgs& p) {
 #pragma unroll
             for (int j = 0; j < SN; ++j) {
                 const uint32_t col = n0 + wn * TN + 16 * j + 4 * q;
-                store4(p.c, (uint64_t)row * p.ldc + col, left4(p.n, col), WIDE, acc[i][j]);
+                store4(to, (uint64_t)row * ld + col, left4(p.n, col), WIDE || p.planes, acc[i][j]);
             }
     }
 }
@@ -358,13 +368,13 @@ __device__ __forceinline__ void gated_out(const T0gTileArgs& p, uint32_t row, ui
     }
 }
 
-template <int BM, int BN, int WM, int WN, bool NC, bool GRAD>
+template <int BM, int BN, int WM, int WN, int NS, bool NC, bool GRAD>
 __device__ __forceinline__ void gated_tile(const T0gTileArgs& p) {
     constexpr int W = WM * WN, TM = BM / WM, TN = BN / WN, SM = TM / 16, SN = TN / 16;
     using OpA = RowsK<BM, W>;
     using OpB = typename std::conditional<NC, RowsN<BN, W>, RowsK<BN, W>>::type;
     constexpr uint32_t A = OpA::kBytes, B = OpB::kBytes, STAGE = A + 2 * B;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
+    __shared__ __attribute__((aligned(1024))) char smem[NS * STAGE];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t wm = wave / WN, wn = wave % WN, l16 = lane & 15u, q = lane >> 4;
     uint32_t tm, tn;
@@ -382,13 +392,13 @@ __device__ __forceinline__ void gated_tile(const T0gTileArgs& p) {
         lu.init(p.b2, n0, p.n, (uint64_t)p.ldb * 2, kb, wave, lane, wn * TN);
     }
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem));
-    const uint32_t nst = (p.k + 63) / 64;
+    const uint32_t first = blockIdx.y * p.split_stages, end = min(first + p.split_stages, (p.k + 63) / 64);
     f32x4_t g[SM][SN], u[SM][SN];
 #pragma unroll
     for (int i = 0; i < SM; ++i)
 #pragma unroll
         for (int j = 0; j < SN; ++j) g[i][j] = u[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    auto issue = [&](uint32_t s, uint32_t lds) {
+    auto issue = [&](uint32_t s, uint32_t lds) {   // past the end: zeros
         la.issue(lds, s * 128, kb, wave);
         if constexpr (NC) {
             lg.issue(lds + A, s * 64, p.k, wave, lane);
@@ -398,13 +408,17 @@ __device__ __forceinline__ void gated_tile(const T0gTileArgs& p) {
             lu.issue(lds + A + B, s * 128, kb, wave);
         }
     };
-    issue(0, lds0);
-    uint32_t cur = lds0;
-    for (uint32_t s = 0; s < nst; ++s) {
-        __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0): the stage is there; lgkmcnt(0): the one before is read
+    constexpr int kVmem = OpA::kInstr + 2 * OpB::kInstr;
+    for (int s = 0; s < NS - 1; ++s) issue(first + s, lds0 + s * STAGE);
+    uint32_t cur = lds0, fill = lds0 + (NS - 1) * STAGE;
+    for (uint32_t s = first; s < end; ++s) {
+        // this stage is there (NS - 2 later ones may be on their way), and the one before is read
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        T0G_WAIT_VMCNT(kVmem * (NS - 2));
         barrier_no_fence();
-        const uint32_t nxt = lds0 + (cur == lds0 ? STAGE : 0u);
-        if (s + 1 < nst) issue(s + 1, nxt);
+        issue(s + NS - 1, fill);
+        fill = fill + STAGE == lds0 + NS * STAGE ? lds0 : fill + STAGE;
+        const uint32_t nxt = cur + STAGE == lds0 + NS * STAGE ? lds0 : cur + STAGE;
         auto half = [&](auto h) {
             constexpr int H = h.value;
             i32x4_t fg[SN], fu[SN];
@@ -427,12 +441,49 @@ __device__ __forceinline__ void gated_tile(const T0gTileArgs& p) {
         half(std::integral_constant<int, 1>{});
         cur = nxt;
     }
+    T0G_WAIT_VMCNT(0);   // stages past the end
 #pragma unroll
     for (int i = 0; i < SM; ++i) {
         const uint32_t row = m0 + wm * TM + 16 * i + l16;
         if (row < p.m)
 #pragma unroll
-            for (int j = 0; j < SN; ++j) gated_out<GRAD>(p, row, n0 + wn * TN + 16 * j + 4 * q, g[i][j], u[i][j]);
+            for (int j = 0; j < SN; ++j) {
+                const uint32_t col = n0 + wn * TN + 16 * j + 4 * q;
+                if (p.planes) {   // a slice of K
+                    const uint64_t to = p.planes + 2 * (uint64_t)blockIdx.y * p.m * p.ldp * 4;
+                    store4(to, (uint64_t)row * p.ldp + col, left4(p.n, col), true, g[i][j]);
+                    store4(to + (uint64_t)p.m * p.ldp * 4, (uint64_t)row * p.ldp + col, left4(p.n, col), true, u[i][j]);
+                } else {
+                    gated_out<GRAD>(p, row, col, g[i][j], u[i][j]);
+                }
+            }
+    }
+}
+
+// The slices of K in their order, 4 columns a thread.
+__device__ __forceinline__ void join_slices(const T0gJoinArgs& a) {
+    const T0gTileArgs& p = a.t;
+    const uint32_t per_row = p.ldp / 4;
+    const uint64_t plane = (uint64_t)p.m * p.ldp * 4;
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < p.m * per_row; i += gridDim.x * 256) {   // below 2^31: the host's
+        const uint32_t row = i / per_row, col = 4 * (i - row * per_row);
+        const uint64_t at_ = p.planes + (uint64_t)i * 16;
+        f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f}, u = v;
+        if (col >= p.n) continue;
+        for (uint32_t s = 0; s < a.slices; ++s) {
+            if (a.gated) {
+                v += *at<const f32x4_t>(at_ + 2 * s * plane);
+                u += *at<const f32x4_t>(at_ + (2 * s + 1) * plane);
+            } else {
+                v += *at<const f32x4_t>(at_ + s * plane);
+            }
+        }
+        if (a.gated == 2)
+            gated_out<true>(p, row, col, v, u);
+        else if (a.gated)
+            gated_out<false>(p, row, col, v, u);
+        else
+            store4(p.c, (uint64_t)row * p.ldc + col, left4(p.n, col), p.flags & T0G_TILE_OUT_F32, v);
     }
 }
 

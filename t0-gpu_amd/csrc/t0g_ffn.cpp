@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <exception>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -359,18 +360,51 @@ uint64_t take(uint64_t *at, uint64_t bytes) {
     return a;
 }
 
-int run_pad(t0g_device *dev, const Operand &o, uint64_t base) {
-    if (!o.copied) return T0G_OK;
+// Copies those of up to three operands that need it, in one launch.
+int run_pad(t0g_device *dev, std::initializer_list<const Operand *> list, uint64_t base) {
     T0gPadArgs p;
     memset(&p, 0, sizeof p);
-    p.src = o.addr;
-    p.dst = base + o.at;
-    p.rows = o.rows;
-    p.cols = o.cols;
-    p.lds = o.ld;
-    p.ldd = o.ldc;
-    p.size = o.size;
-    return ffn_launch(dev, "t0g_ffn_pad_rows", groups_for((uint64_t)o.rows * o.ldc * o.size / 8, 256, 1u << 16), 1, 256, &p, sizeof p);
+    uint32_t n = 0, rows = 0;
+    for (const Operand *o : list) {
+        if (!o->copied || o->rows == 0) continue;
+        auto &a = p.a[n++];
+        a.src = o->addr;
+        a.dst = base + o->at;
+        a.lds = (uint64_t)o->ld * o->size;
+        a.ldd = (uint64_t)o->ldc * o->size;
+        a.rows = o->rows;
+        a.bytes = o->cols * o->size;
+        rows = std::max(rows, o->rows);
+    }
+    return n ? ffn_launch(dev, "t0g_ffn_pad_rows", groups_for(rows, 4, 1u << 16), n, 256, &p, sizeof p) : (int)T0G_OK;
+}
+
+// The K of a product of few tiles goes to several workgroups, in slices of at least kLeastStages stages, until kFill
+// workgroups are there; their sums go to f32 planes.
+constexpr uint32_t kFill = 2 * kNumCUs, kLeastStages = 4;
+struct Slices {
+    uint32_t n = 1, stages = 0, ldp = 0;
+    uint64_t at = 0, bytes = 0;
+    void set(uint64_t tiles, uint32_t k_stages, uint32_t m, uint32_t n_, uint32_t products) {
+        stages = k_stages;
+        if (tiles == 0 || tiles > kFill / 2) return;
+        const uint32_t want = (uint32_t)std::min<uint64_t>(kFill / tiles, k_stages / kLeastStages);
+        if (want < 2) return;
+        stages = (k_stages + want - 1) / want;
+        n = (k_stages + stages - 1) / stages;
+        ldp = (uint32_t)round_up(n_, 4);
+        bytes = (uint64_t)n * products * m * ldp * 4;
+    }
+};
+uint64_t tiles_of(uint32_t m, uint32_t n, uint32_t bm, uint32_t bn) { return ((uint64_t)m + bm - 1) / bm * (((uint64_t)n + bn - 1) / bn); }
+
+int run_join(t0g_device *dev, const T0gTileArgs &t, const Slices &s, uint32_t gated) {
+    T0gJoinArgs j;
+    memset(&j, 0, sizeof j);
+    j.t = t;
+    j.slices = s.n;
+    j.gated = gated;
+    return ffn_launch(dev, "t0g_ffn_join_slices", groups_for((uint64_t)t.m * (s.ldp / 4), 256, 1u << 16), 1, 256, &j, sizeof j);
 }
 
 int set_tiles(T0gTileArgs *a, uint32_t bm, uint32_t bn) {
@@ -408,18 +442,25 @@ int check_fp8_gemm(t0g_fp8_gemm_desc *d) {
 // Rows up to which a product is bound by reading B, which then goes straight to registers.
 constexpr uint32_t kSkinnyRows = 32;
 
+enum class Fp8Tile { Skinny, Small, Middle, Big };
 struct Fp8Plan {
-    bool skinny = false;
+    Fp8Tile tile = Fp8Tile::Skinny;
     Operand a, b;
+    Slices slices;
     uint64_t bytes = 0;
 };
 void plan_fp8(const t0g_fp8_gemm_desc &d, Fp8Plan *p) {
-    p->skinny = d.m <= kSkinnyRows;
-    if (p->skinny) return;
+    if (d.m <= kSkinnyRows) return;
+    if (d.out_dtype == T0G_BF16 && tiles_of(d.m, d.n, 256, 256) >= kNumCUs)
+        p->tile = Fp8Tile::Big;
+    else
+        p->tile = tiles_of(d.m, d.n, 128, 128) >= 2 * kNumCUs ? Fp8Tile::Middle : Fp8Tile::Small;
     p->a.set(d.a, d.m, d.k, d.lda, 1);
     p->b.set(d.b, d.n, d.k, d.ldb, 1);
     p->a.at = take(&p->bytes, p->a.bytes());
     p->b.at = take(&p->bytes, p->b.bytes());
+    p->slices.set(p->tile == Fp8Tile::Small ? tiles_of(d.m, d.n, 64, 128) : 0, blocks_of(d.k), d.m, d.n, 1);
+    p->slices.at = take(&p->bytes, p->slices.bytes);
 }
 
 int fp8_gemm_call(t0g_device *dev, const t0g_fp8_gemm_desc *desc) {
@@ -434,32 +475,41 @@ int fp8_gemm_call(t0g_device *dev, const t0g_fp8_gemm_desc *desc) {
     t.m = d.m;
     t.n = d.n;
     t.k = d.k;
-    const bool big = d.out_dtype == T0G_BF16 && ((uint64_t)d.m + 255) / 256 * (((uint64_t)d.n + 255) / 256) >= kNumCUs;
-    if ((rc = pl.skinny ? skinny_groups(d.n) : big ? set_tiles(&t, 256, 256) : set_tiles(&t, 128, 128))) return rc;
+    const bool skinny = pl.tile == Fp8Tile::Skinny, big = pl.tile == Fp8Tile::Big, small = pl.tile == Fp8Tile::Small;
+    if ((rc = skinny ? skinny_groups(d.n) : big ? set_tiles(&t, 256, 256) : set_tiles(&t, small ? 64 : 128, 128))) return rc;
     if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
     std::lock_guard<std::mutex> lk(device_mutex(dev));
     uint64_t base;
     if ((rc = ffn_begin(dev, pl.bytes, &base)) || d.m == 0 || d.n == 0) return rc;
-    if ((rc = run_pad(dev, pl.a, base)) || (rc = run_pad(dev, pl.b, base))) return rc;
-    t.a = pl.skinny ? d.a : pl.a.address(base);
-    t.b = pl.skinny ? d.b : pl.b.address(base);
-    t.lda = pl.skinny ? d.lda : pl.a.pitch();
-    t.ldb = pl.skinny ? d.ldb : pl.b.pitch();
     t.as = d.a_scales;
     t.bs = d.b_scales;
     t.ldas = d.ldas;
     t.ldbs = d.ldbs;
     t.c = d.c;
     t.ldc = d.ldc;
+    t.flags = d.out_dtype == T0G_F32 ? T0G_TILE_OUT_F32 : 0;
     const std::string types = std::string(d.a_dtype == T0G_E4M3 ? "e4" : "e5") + (d.b_dtype == T0G_E4M3 ? "e4" : "e5") +
                               (d.b_block == T0G_BLOCK_TILE ? "_tile" : "_row");
-    if (pl.skinny) {
-        t.flags = d.out_dtype == T0G_F32 ? T0G_TILE_OUT_F32 : 0;
+    if (skinny) {
+        t.a = d.a;
+        t.b = d.b;
+        t.lda = d.lda;
+        t.ldb = d.ldb;
         const std::string symbol = std::string("t0g_ffn_f8_skinny") + (d.m <= 16 ? "1_" : "2_") + types;
         return ffn_launch(dev, symbol.c_str(), (d.n + 15) / 16, 1, 512, &t, sizeof t);
     }
-    const std::string symbol = (big ? "t0g_ffn_f8_256x256_" : "t0g_ffn_f8_128x128_") + types + (d.out_dtype == T0G_F32 ? "_f32" : "_bf16");
-    return ffn_launch(dev, symbol.c_str(), t.tiles_m * t.tiles_n, 1, big ? 512 : 256, &t, sizeof t);
+    if ((rc = run_pad(dev, {&pl.a, &pl.b}, base))) return rc;
+    t.a = pl.a.address(base);
+    t.b = pl.b.address(base);
+    t.lda = pl.a.pitch();
+    t.ldb = pl.b.pitch();
+    t.split_stages = pl.slices.stages;
+    t.planes = pl.slices.n > 1 ? base + pl.slices.at : 0;
+    t.ldp = pl.slices.ldp;
+    const std::string symbol = (big ? "t0g_ffn_f8_256x256_" : small ? "t0g_ffn_f8_64x128_" : "t0g_ffn_f8_128x128_") + types +
+                               (d.out_dtype == T0G_F32 ? "_f32" : "_bf16");
+    if ((rc = ffn_launch(dev, symbol.c_str(), t.tiles_m * t.tiles_n, pl.slices.n, big ? 512 : 256, &t, sizeof t))) return rc;
+    return pl.slices.n > 1 ? run_join(dev, t, pl.slices, 0) : (int)T0G_OK;
 }
 
 // ---- gated projections ------------------------------------------------------------------
@@ -498,52 +548,59 @@ int check_gated(t0g_gated_linear_desc *d, uint32_t *act) {
 }
 
 // The gated tile kernels' operands.
+enum class GatedTile { Skinny, Small, Middle, Big };
 struct GatedPlan {
-    bool skinny = false;
+    GatedTile tile = GatedTile::Skinny;
     Operand x, wg, wu;
+    Slices slices;
+    // grad: the kernels that give dgate and dup, which the 256x256 tile and the few rows' kernel do not.
     void set(uint64_t xa, uint64_t g, uint64_t u, uint32_t rows, uint32_t features, uint32_t hidden, uint32_t ldx, uint32_t ldw,
-             uint32_t transpose, uint64_t *at) {
+             uint32_t transpose, bool grad, uint64_t *at) {
         const bool nt = transpose == T0G_NT;
+        if (nt && rows <= kSkinnyRows && !grad) return;
         x.set(xa, rows, hidden, ldx, 2);
         wg.set(g, nt ? features : hidden, nt ? hidden : features, ldw, 2);
         wu.set(u, nt ? features : hidden, nt ? hidden : features, ldw, 2);
         if (wg.copied || wu.copied) wg.copied = wu.copied = true;   // one leading dimension for both
         for (Operand *o : {&x, &wg, &wu}) o->at = take(at, o->bytes());
+        if (!grad && big(rows, features, hidden, nt))
+            tile = GatedTile::Big;
+        else
+            tile = tiles_of(rows, features, 128, 64) >= 2 * kNumCUs ? GatedTile::Middle : GatedTile::Small;
+        slices.set(tile == GatedTile::Small ? tiles_of(rows, features, 64, 64) : 0, (hidden + 63) / 64, rows, features, 2);
+        slices.at = take(at, slices.bytes);
     }
-    int pad(t0g_device *dev, uint64_t base) const {
-        int rc;
-        if ((rc = run_pad(dev, x, base)) || (rc = run_pad(dev, wg, base))) return rc;
-        return run_pad(dev, wu, base);
+    // Whether the 256x256 tile takes it: enough tiles for all CUs, and 32-bit offsets in the operands.
+    bool big(uint32_t rows, uint32_t features, uint32_t hidden, bool nt) const {
+        const uint64_t most = 1ull << 30, ldb = wg.pitch(), wspan = (nt ? features + 256ull : hidden + 64ull) * ldb;
+        const uint64_t g = wg.address(0), u = wu.address(0), apart = g < u ? u - g : g - u;   // as far apart in the scratch
+        return tiles_of(rows, features, 256, 128) >= kNumCUs && (rows + 256ull) * x.pitch() < most && wspan < most && x.pitch() >= 64 &&
+               (nt ? ldb >= 64 : ldb >= 256 && apart + wspan * 2 < (1ull << 31) - 4096);   // offsets out of range stay so less 3 KB
     }
 };
 
-// Whether the 256x256 tile takes a gated pair: enough tiles for all CUs, and 32-bit offsets in the operands.
-bool gated_big(const T0gTileArgs &t, bool nt) {
-    const uint64_t tiles = ((uint64_t)t.m + 255) / 256 * (((uint64_t)t.n + 127) / 128);
-    const uint64_t most = 1ull << 30, wspan = ((uint64_t)(nt ? t.n + 256 : t.k + 64)) * t.ldb;
-    const uint64_t apart = t.b < t.b2 ? t.b2 - t.b : t.b - t.b2;
-    return tiles >= kNumCUs && (t.m + 256ull) * t.lda < most && wspan < most && t.lda >= 64 &&
-           (nt ? t.ldb >= 64 : t.ldb >= 256 && apart + wspan * 2 < (1ull << 31) - 4096);   // offsets out of range stay so less 3 KB
-}
-
-int run_gated_tile(t0g_device *dev, T0gTileArgs *t, const GatedPlan &pl, uint64_t base, uint32_t transpose, const char *kind) {
+// kind: 1 the forward call's outputs, 2 its gradient's.
+int run_gated_tile(t0g_device *dev, T0gTileArgs *t, const GatedPlan &pl, uint64_t base, uint32_t transpose, uint32_t kind) {
     t->a = pl.x.address(base);
     t->b = pl.wg.address(base);
     t->b2 = pl.wu.address(base);
     t->lda = pl.x.pitch();
     t->ldb = pl.wg.pitch();
-    const bool nt = transpose == T0G_NT, big = !*kind && gated_big(*t, nt);
-    int rc = big ? set_tiles(t, 256, 128) : set_tiles(t, 128, 64);
-    if (rc) return rc;
-    const std::string symbol = std::string(big ? "t0g_ffn_gated_256x128" : "t0g_ffn_gated_128x64") + (nt ? "_nt" : "_nn") + kind;
-    return ffn_launch(dev, symbol.c_str(), t->tiles_m * t->tiles_n, 1, 256, t, sizeof *t);
+    t->split_stages = pl.slices.stages;
+    t->planes = pl.slices.n > 1 ? base + pl.slices.at : 0;
+    t->ldp = pl.slices.ldp;
+    const bool nt = transpose == T0G_NT, big = pl.tile == GatedTile::Big, small = pl.tile == GatedTile::Small;
+    int rc = big ? set_tiles(t, 256, 128) : set_tiles(t, small ? 64 : 128, 64);
+    if (rc || (rc = run_pad(dev, {&pl.x, &pl.wg, &pl.wu}, base))) return rc;
+    const std::string symbol = std::string(big ? "t0g_ffn_gated_256x128" : small ? "t0g_ffn_gated_64x64" : "t0g_ffn_gated_128x64") +
+                               (nt ? "_nt" : "_nn") + (kind == 2 ? "_grad" : "");
+    if ((rc = ffn_launch(dev, symbol.c_str(), t->tiles_m * t->tiles_n, pl.slices.n, 256, t, sizeof *t))) return rc;
+    return pl.slices.n > 1 ? run_join(dev, *t, pl.slices, kind) : (int)T0G_OK;
 }
 
 int gated_plan(const t0g_gated_linear_desc &d, GatedPlan *pl, uint64_t *bytes) {
     *bytes = 0;
-    pl->skinny = d.transpose == T0G_NT && d.rows <= kSkinnyRows;
-    if (pl->skinny) return T0G_OK;
-    pl->set(d.x, d.wg, d.wu, d.rows, d.features, d.hidden, d.ldx, d.ldw, d.transpose, bytes);
+    pl->set(d.x, d.wg, d.wu, d.rows, d.features, d.hidden, d.ldx, d.ldw, d.transpose, false, bytes);
     return T0G_OK;
 }
 
@@ -571,7 +628,7 @@ int gated_call(t0g_device *dev, const t0g_gated_linear_desc *desc) {
     t.k = d.hidden;
     t.act = act;
     t.flags = d.h_dtype == T0G_F32 ? T0G_TILE_OUT_F32 : 0;
-    if (pl.skinny) {
+    if (pl.tile == GatedTile::Skinny) {
         t.a = d.x;
         t.b = d.wg;
         t.b2 = d.wu;
@@ -580,8 +637,7 @@ int gated_call(t0g_device *dev, const t0g_gated_linear_desc *desc) {
         return ffn_launch(dev, d.rows <= 16 ? "t0g_ffn_gated_skinny1" : "t0g_ffn_gated_skinny2", (d.features + 15) / 16, 1, 512, &t,
                           sizeof t);
     }
-    if ((rc = pl.pad(dev, base))) return rc;
-    return run_gated_tile(dev, &t, pl, base, d.transpose, "");
+    return run_gated_tile(dev, &t, pl, base, d.transpose, 1);
 }
 
 int check_gated_grad(t0g_gated_linear_backward_desc *d, uint32_t *act) {
@@ -641,7 +697,7 @@ int plan_gated_grad(const t0g_gated_linear_backward_desc &d, uint64_t base, Gate
     const bool nt = d.transpose == T0G_NT;
     const uint32_t f = d.features, es = size_of(d.dw_dtype);
     uint64_t at = 0;
-    if (!d.gate) pl->tiles.set(d.x, d.wg, d.wu, d.rows, f, d.hidden, d.ldx, d.ldw, d.transpose, &at);
+    if (!d.gate) pl->tiles.set(d.x, d.wg, d.wu, d.rows, f, d.hidden, d.ldx, d.ldw, d.transpose, true, &at);
     pl->half = (uint32_t)round_up(f, 8);
     pl->ldd = 2 * pl->half;
     pl->d = take(&at, (uint64_t)d.rows * pl->ldd * 2);
@@ -729,7 +785,7 @@ int gated_grad_call(t0g_device *dev, const t0g_gated_linear_backward_desc *desc)
         t.k = d.hidden;
         t.act = act;
         t.flags = d.dh_dtype == T0G_F32 ? T0G_TILE_DH_F32 : 0;
-        if ((rc = pl.tiles.pad(dev, base)) || (rc = run_gated_tile(dev, &t, pl.tiles, base, d.transpose, "_grad"))) return rc;
+        if ((rc = run_gated_tile(dev, &t, pl.tiles, base, d.transpose, 2))) return rc;
     }
     auto run = [&](t0g_gemm_desc g) {
         g.workspace = base + pl.ws;

@@ -328,6 +328,10 @@ typedef struct T0gTileArgs {
     uint32_t flags;          /* T0G_TILE_*                                               */
     uint32_t act;            /* T0G_ACT_*                                                */
     uint32_t up_off;         /* gated, gradient: column of dup in c                      */
+    uint32_t split_stages;   /* 128-byte stages of K of a workgroup of a K slice (grid y) */
+    uint32_t reserved;
+    uint64_t planes;         /* more than one slice: f32 [slice][products][m][ldp], else 0 */
+    uint32_t ldp, reserved2; /* multiple of 4                                            */
 } T0gTileArgs;
 #define T0G_TILE_OUT_F32 1u      /* c is f32, else bf16                                  */
 #define T0G_TILE_B_TILE 2u       /* a scale of B for each 128 x 128, else 1 x 128        */
@@ -344,11 +348,22 @@ typedef struct T0gGatedGradArgs {
     uint32_t flags, act, up_off;
 } T0gGatedGradArgs;
 
-/* Rows of `cols` values into rows of ldd, zeros from cols on.  size: bytes of a value, 1 or 2. */
+/* Up to three arrays' rows into rows of whole 16-byte pieces, zeros past their values; all in bytes.
+ * rows 0: none.  grid y: the array. */
 typedef struct T0gPadArgs {
-    uint64_t src, dst;
-    uint32_t rows, cols, lds, ldd, size, reserved;
+    struct {
+        uint64_t src, dst, lds, ldd;
+        uint32_t rows, bytes;
+    } a[3];
 } T0gPadArgs;
+
+/* The slices of K added up in their order, and what follows: c, or the gated pair's outputs.  t: the tile
+ * kernel's arguments. */
+typedef struct T0gJoinArgs {
+    T0gTileArgs t;
+    uint32_t slices;
+    uint32_t gated;          /* 0: one product; 1: h, gate and up; 2: dgate and dup      */
+} T0gJoinArgs;
 
 /* out = p0 + p1, f32 planes of rows of ldp values. */
 typedef struct T0gAddArgs {
