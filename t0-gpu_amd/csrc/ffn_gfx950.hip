@@ -8,23 +8,36 @@
 #include "ffn_big.h"
 #include "ffn_gated.h"
 
-#define NORM(NT, CH, KEEP) \
-    extern "C" __global__ void __launch_bounds__(NT) t0g_ffn_norm_##NT##x##CH(T0gNormArgs p) { t0g::rms_norm<NT, CH, KEEP>(p); }
-NORM(64, 1, true)
-NORM(256, 1, true)
-NORM(256, 2, true)
-NORM(512, 2, true)
-NORM(1024, 2, true)
-#define NORM_GRAD(NT, CH, KEEP)                                                                 \
-    extern "C" __global__ void __launch_bounds__(NT) t0g_ffn_norm_grad_##NT##x##CH(T0gNormGradArgs p) { \
-        t0g::rms_norm_grad<NT, CH, KEEP>(p);                                                    \
+// Symbols: t0g_ffn_norm[_grad]_<threads of a row>x<pieces of a thread>[_fast].
+#define NORM(NT, CH, R, SUFFIX, FAST)                                                                      \
+    extern "C" __global__ void __launch_bounds__(NT * R) t0g_ffn_norm_##NT##x##CH##SUFFIX(T0gNormArgs p) { \
+        t0g::rms_norm<NT, CH, R, FAST>(p);                                                                 \
     }
-NORM_GRAD(64, 1, true)
-NORM_GRAD(256, 1, true)
-NORM_GRAD(256, 2, true)
-NORM_GRAD(512, 2, true)
-NORM_GRAD(1024, 2, false)
-extern "C" __global__ void __launch_bounds__(256) t0g_ffn_column_sum(T0gColSumArgs p) { t0g::column_sum(p); }
+NORM(64, 1, 4, , false)
+NORM(256, 1, 1, , false)
+NORM(256, 2, 1, , false)
+NORM(512, 2, 1, , false)
+NORM(1024, 2, 1, , false)
+NORM(64, 1, 4, _fast, true)
+NORM(256, 1, 1, _fast, true)
+NORM(256, 2, 1, _fast, true)
+NORM(512, 2, 1, _fast, true)
+NORM(1024, 2, 1, _fast, true)
+#define NORM_GRAD(NT, CH, R, SUFFIX, FAST, KEEP, PRE)                                                              \
+    extern "C" __global__ void __launch_bounds__(NT * R) t0g_ffn_norm_grad_##NT##x##CH##SUFFIX(T0gNormGradArgs p) { \
+        t0g::rms_norm_grad<NT, CH, R, FAST, KEEP, PRE>(p);                                                         \
+    }
+NORM_GRAD(64, 1, 4, , false, true, false)
+NORM_GRAD(256, 1, 1, , false, true, false)
+NORM_GRAD(256, 2, 1, , false, true, false)
+NORM_GRAD(512, 2, 1, , false, true, false)
+NORM_GRAD(1024, 2, 1, , false, false, false)
+NORM_GRAD(64, 1, 4, _fast, true, true, true)
+NORM_GRAD(256, 1, 1, _fast, true, true, true)
+NORM_GRAD(256, 2, 1, _fast, true, true, true)
+NORM_GRAD(512, 2, 1, _fast, true, true, true)
+NORM_GRAD(1024, 2, 1, _fast, true, true, false)
+extern "C" __global__ void __launch_bounds__(1024) t0g_ffn_column_sum(T0gColSumArgs p) { t0g::column_sum(p); }
 extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_rows(T0gQuantArgs p) { t0g::quantize_rows(p); }
 extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_tile(T0gQuantArgs p) { t0g::quantize_tile(p); }
 extern "C" __global__ void __launch_bounds__(256) t0g_ffn_gated_grad(T0gGatedGradArgs p) { t0g::gated_grad(p); }

@@ -170,70 +170,64 @@ __device__ __forceinline__ void store_f8x8(uint64_t addr, uint32_t n, u32x2_t w)
     }
 }
 
-// Valid values of the piece of 8 at column c of a row of `cols`.
-__device__ __forceinline__ uint32_t left8(uint32_t cols, uint32_t c) { return c < cols ? min(cols - c, 8u) : 0u; }
+// Valid values of the piece of 8 at column c of a row of `cols`; FAST: of whole pieces.
+template <bool FAST = false>
+__device__ __forceinline__ uint32_t left8(uint32_t cols, uint32_t c) {
+    return c < cols ? (FAST ? 8u : min(cols - c, 8u)) : 0u;
+}
 
 // ---- the norm --------------------------------------------------------------------------
-// y = s rho (w + offset), rho = (mean s^2 + eps)^-1/2, s = x + residual.  A workgroup takes a
-// row, NT threads with CH pieces of 8 each, and (KEEP) keeps it in registers between the sum of
-// squares and the output: memory is read and written once.  Long rows are read again, from the caches.
-template <int NT, int CH, bool KEEP>
+// y = s rho (w + offset), rho = (mean s^2 + eps)^-1/2, s = x + residual.  NT threads take a row, with CH pieces
+// of 8 each, and keep it in registers between the sum of squares and the output: memory is read and
+// written once.  Rows of one wave go R to a workgroup.  FAST: bf16 inputs of whole pieces of 8, which need
+// half the registers: 8192x4096 with the residual into e4m3 in 43 us that way, 53 with types and ends
+// looked at in the kernel.
+template <int NT, int CH, int R, bool FAST>
 __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
     constexpr int W = NT / 64;
+    static_assert(R == 1 || NT == 64, "several rows: a wave each");
     __shared__ float t[2][W];
-    const bool xf = p.flags & T0G_ROWS_X_F32, rf = p.flags & T0G_ROWS_R_F32, wf = p.flags & T0G_ROWS_W_F32,
+    const bool xf = !FAST && p.flags & T0G_ROWS_X_F32, rf = !FAST && p.flags & T0G_ROWS_R_F32, wf = !FAST && p.flags & T0G_ROWS_W_F32,
                e5m2 = p.flags & T0G_ROWS_E5M2;
+    const uint32_t first = threadIdx.x % NT, step = gridDim.x * R;
     uint32_t turn = 0;
-    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-        Raw8 x[KEEP ? CH : 1], r[KEEP ? CH : 1], w[KEEP ? CH : 1];
-        auto load = [&](int i, bool weight, Raw8& xi, Raw8& ri, Raw8& wi) {
-            const uint32_t c = 8 * (i * NT + threadIdx.x), n = left8(p.hidden, c);
-            xi = load8(p.x, (uint64_t)row * p.ldx + c, n, xf);
-            if (p.residual) ri = load8(p.residual, (uint64_t)row * p.ldr + c, n, rf);
-            if (p.weight && weight) wi = load8(p.weight, c, n, wf);
+    for (uint32_t row = blockIdx.x * R + threadIdx.x / NT; row < p.rows; row += step, turn ^= 1) {
+        Raw8 x[CH], r[CH], w[CH];
+        auto load = [&](int i) {
+            const uint32_t c = 8 * (i * NT + first), n = left8<FAST>(p.hidden, c);
+            x[i] = load8(p.x, (uint64_t)row * p.ldx + c, n, xf);
+            if (p.residual) r[i] = load8(p.residual, (uint64_t)row * p.ldr + c, n, rf);
+            if (p.weight) w[i] = load8(p.weight, c, n, wf);
         };
-        auto add = [&](int i, float (&s)[8]) {
-            values8(x[KEEP ? i : 0], xf, s);
-            if (p.residual) {
-                float d[8];
-                values8(r[KEEP ? i : 0], rf, d);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s[e] += d[e];
-            }
-        };
-        if constexpr (KEEP)
-#pragma unroll
-            for (int i = 0; i < CH; ++i) load(i, true, x[i], r[i], w[i]);
-        float s[KEEP ? CH : 1][8], sum[1] = {0.0f};
+        for (int i = 0; i < CH; ++i) load(i);
+        float s[CH][8], sum[1] = {0.0f};
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            if constexpr (!KEEP) load(i, false, x[0], r[0], w[0]);
-            const int k = KEEP ? i : 0;
-            add(i, s[k]);
+            values8(x[i], xf, s[i]);
+            if (p.residual) {
+                float d[8];
+                values8(r[i], rf, d);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum[0] = __builtin_fmaf(s[k][e], s[k][e], sum[0]);
-            if constexpr (!KEEP) __builtin_amdgcn_sched_barrier(0);
+                for (int e = 0; e < 8; ++e) s[i][e] += d[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[0] = __builtin_fmaf(s[i][e], s[i][e], sum[0]);
         }
         block_sum<W>(sum, t[turn]);
         const float rho = 1.0f / __builtin_sqrtf(sum[0] / (float)p.hidden + p.eps);
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            const uint32_t c = 8 * (i * NT + threadIdx.x), n = left8(p.hidden, c);
-            const int k = KEEP ? i : 0;
-            if constexpr (!KEEP) {
-                __builtin_amdgcn_sched_barrier(0);
-                load(i, true, x[0], r[0], w[0]);
-                add(i, s[0]);
-            }
-            if (p.sum) store8(p.sum, (uint64_t)row * p.ldsum + c, n, p.flags & T0G_ROWS_OUT_F32, s[k]);
+            const uint32_t c = 8 * (i * NT + first), n = left8<FAST>(p.hidden, c);
+            if (p.sum) store8(p.sum, (uint64_t)row * p.ldsum + c, n, p.flags & T0G_ROWS_OUT_F32, s[i]);
             float v[8];
             if (p.weight) {
-                values8(w[k], wf, v);
+                values8(w[i], wf, v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = s[k][e] * rho * (v[e] + p.weight_offset);
+                for (int e = 0; e < 8; ++e) v[e] = s[i][e] * rho * (v[e] + p.weight_offset);
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = s[k][e] * rho;
+                for (int e = 0; e < 8; ++e) v[e] = s[i][e] * rho;
             }
             if (p.y) store8(p.y, (uint64_t)row * p.ldy + c, n, p.flags & T0G_ROWS_Y_F32, v);
             if (p.q) {
@@ -249,20 +243,23 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
 }
 
 // With n = s rho and g = dy (w + offset):  ds = rho (g - n mean(g n)) + dsum,  dw = sum over rows of dy n.
-// mean(g n) = rho mean(g s), so one pass over the row gives both sums.  A workgroup takes every
-// gridDim.x-th row and adds up its part of dw in registers, in the order of its rows.  KEEP: the row stays in
-// registers between the sums and ds; else it is read again, from the caches.
-template <int NT, int CH, bool KEEP>
+// mean(g n) = rho mean(g s), so one pass over the row gives both sums.  NT threads take a row, R rows a workgroup,
+// which goes on to every gridDim.x-th of them.  Each thread adds up its part of dw in registers, in the order of
+// its rows.  FAST: bf16 inputs of whole pieces of 8.  PRE: the next row's are on their way while this one's
+// sums are formed.  KEEP: the row stays in registers between the sums and ds; else it is read again, from the caches.
+template <int NT, int CH, int R, bool FAST, bool KEEP, bool PRE>
 __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
     constexpr int W = NT / 64;
+    static_assert(R == 1 || (NT == 64 && CH == 1), "several rows: a wave each");
     __shared__ float t[2][2 * W];
-    const bool yf = p.flags & T0G_ROWS_Y_F32, xf = p.flags & T0G_ROWS_X_F32, wf = p.flags & T0G_ROWS_W_F32,
-               sf = p.flags & T0G_ROWS_R_F32;
+    const bool yf = !FAST && p.flags & T0G_ROWS_Y_F32, xf = !FAST && p.flags & T0G_ROWS_X_F32, wf = !FAST && p.flags & T0G_ROWS_W_F32,
+               sf = !FAST && p.flags & T0G_ROWS_R_F32;
+    const uint32_t first = threadIdx.x % NT;
     float dw[CH][8];
     Raw8 w[KEEP ? CH : 1];
     auto load_weight = [&](int i) {
-        const uint32_t c = 8 * (i * NT + threadIdx.x);
-        if (p.weight) w[KEEP ? i : 0] = load8(p.weight, c, left8(p.hidden, c), wf);
+        const uint32_t c = 8 * (i * NT + first);
+        if (p.weight) w[KEEP ? i : 0] = load8(p.weight, c, left8<FAST>(p.hidden, c), wf);
     };
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
@@ -280,24 +277,33 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
             for (int e = 0; e < 8; ++e) v[e] = 1.0f;
         }
     };
-    uint32_t turn = 0;
-    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-        Raw8 y[KEEP ? CH : 1], x[KEEP ? CH : 1], d[KEEP ? CH : 1];
-        auto load = [&](int i, Raw8& yi, Raw8& xi, Raw8& di) {
-            const uint32_t c = 8 * (i * NT + threadIdx.x), n = left8(p.hidden, c);
-            yi = load8(p.dy, (uint64_t)row * p.lddy + c, n, yf);
-            xi = load8(p.x, (uint64_t)row * p.ldx + c, n, xf);
-            if (p.dsum && p.dx) di = load8(p.dsum, (uint64_t)row * p.ldds + c, n, sf);
-        };
-        if constexpr (KEEP)
+    constexpr int K = KEEP ? CH : 1;
+    Raw8 y[K], x[K], d[K];
+    auto load = [&](uint32_t row, int i, Raw8& yi, Raw8& xi, Raw8& di) {
+        const uint32_t c = 8 * (i * NT + first), n = row < p.rows ? left8<FAST>(p.hidden, c) : 0u;
+        yi = load8(p.dy, (uint64_t)row * p.lddy + c, n, yf);
+        xi = load8(p.x, (uint64_t)row * p.ldx + c, n, xf);
+        if (p.dsum && p.dx) di = load8(p.dsum, (uint64_t)row * p.ldds + c, n, sf);
+    };
+    uint32_t turn = 0, row = blockIdx.x * R + threadIdx.x / NT;
+    const uint32_t step = gridDim.x * R;
+    if constexpr (PRE)
 #pragma unroll
-            for (int i = 0; i < CH; ++i) load(i, y[i], x[i], d[i]);
+        for (int i = 0; i < CH; ++i) load(row, i, y[i], x[i], d[i]);
+    for (; row < p.rows; row += step, turn ^= 1) {
+        Raw8 y2[K], x2[K], d2[K];
+        if constexpr (PRE)   // row + step below 2^32: both are below 2^31
+#pragma unroll
+            for (int i = 0; i < CH; ++i) load(row + step, i, y2[i], x2[i], d2[i]);
+        else if constexpr (KEEP)
+#pragma unroll
+            for (int i = 0; i < CH; ++i) load(row, i, y[i], x[i], d[i]);
         float sums[2] = {0.0f, 0.0f};   // of s^2 and g s
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             if constexpr (!KEEP) {
                 __builtin_amdgcn_sched_barrier(0);
-                load(i, y[0], x[0], d[0]);
+                load(row, i, y[0], x[0], d[0]);
                 load_weight(i);
             }
             float a[8], s[8], g[8];
@@ -317,7 +323,7 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
         for (int i = 0; i < CH; ++i) {
             if constexpr (!KEEP) {
                 __builtin_amdgcn_sched_barrier(0);
-                load(i, y[0], x[0], d[0]);
+                load(row, i, y[0], x[0], d[0]);
                 load_weight(i);
             }
             float a[8], s[8], g[8];
@@ -328,7 +334,7 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dw[i][e] = __builtin_fmaf(a[e], s[e] * rho, dw[i][e]);
             if (p.dx) {
-                const uint32_t c = 8 * (i * NT + threadIdx.x);
+                const uint32_t c = 8 * (i * NT + first);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) g[e] = rho * (a[e] * g[e] - back * s[e]);
                 if (p.dsum) {
@@ -336,30 +342,56 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) g[e] += a[e];
                 }
-                store8(p.dx, (uint64_t)row * p.lddx + c, left8(p.hidden, c), p.flags & T0G_ROWS_OUT_F32, g);
+                store8(p.dx, (uint64_t)row * p.lddx + c, left8<FAST>(p.hidden, c), p.flags & T0G_ROWS_OUT_F32, g);
             }
         }
-    }
-    if (p.part)
+        if constexpr (PRE)
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const uint32_t c = 8 * (i * NT + threadIdx.x);
-            store8(p.part, (uint64_t)blockIdx.x * p.ldpart + c, left8(p.hidden, c), true, dw[i]);
-        }
+            for (int i = 0; i < CH; ++i) {
+                y[i] = y2[i];
+                x[i] = x2[i];
+                d[i] = d2[i];
+            }
+    }
+    if (!p.part) return;
+    if constexpr (R > 1) {   // the workgroup's rows' parts, in their order
+        __shared__ float parts[R][64][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) parts[threadIdx.x / NT][first][e] = dw[0][e];
+        __syncthreads();
+        if (threadIdx.x >= NT) return;
+#pragma unroll
+        for (int r = 1; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dw[0][e] += parts[r][first][e];
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const uint32_t c = 8 * (i * NT + first);
+        store8(p.part, (uint64_t)blockIdx.x * p.ldpart + c, left8<FAST>(p.hidden, c), true, dw[i]);
+    }
 }
 
-// A workgroup adds up 32 columns: thread (r, g) = (tid / 8, tid % 8) every 32nd row of 4 of them, and the
-// 32 sums of a column are then added in order.
+// A workgroup adds up 32 columns: thread (r, g) = (tid / 8, tid % 8) every 128th row of 4 of them, then 16 threads
+// 8 of these sums each, and one their 16, always in the same order.
 __device__ __forceinline__ void column_sum(const T0gColSumArgs& p) {
-    __shared__ f32x4_t part[32][8];
+    __shared__ f32x4_t part[128][8];
     const uint32_t g = threadIdx.x & 7u, r = threadIdx.x >> 3, c = 32 * blockIdx.x + 4 * g;
     f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (c < p.cols)   // rows of ldp values, a multiple of 8
-        for (uint32_t i = r; i < p.n; i += 32) v += *at<const f32x4_t>(p.part + ((uint64_t)i * p.ldp + c) * 4);
+#pragma unroll 4
+        for (uint32_t i = r; i < p.n; i += 128) v += *at<const f32x4_t>(p.part + ((uint64_t)i * p.ldp + c) * 4);
     part[r][g] = v;
     __syncthreads();
+    if (r < 16) {
+#pragma unroll
+        for (uint32_t i = 1; i < 8; ++i) v += part[r + 16 * i][g];
+        part[r][g] = v;
+    }
+    __syncthreads();
     if (r != 0) return;
-    for (uint32_t i = 1; i < 32; ++i) v += part[i][g];
+#pragma unroll
+    for (uint32_t i = 1; i < 16; ++i) v += part[i][g];
 #pragma unroll
     for (uint32_t e = 0; e < 4; ++e)
         if (c + e < p.cols) {
@@ -531,6 +563,17 @@ __device__ __forceinline__ void gated_grad(const T0gGatedGradArgs& p) {
     }
 }
 
+// Bytes [c, c + 16) of a row that ends at `end` > c, zeros past it; all loads are in the row, none waits for another.
+__device__ __forceinline__ u32x4_t tail16(uint64_t row, uint32_t c, uint32_t end) {
+    uint8_t b[16];
+#pragma unroll
+    for (uint32_t e = 0; e < 16; ++e) b[e] = *at<const uint8_t>(row, min(c + e, end - 1));
+    u32x4_t w = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (uint32_t e = 0; e < 16; ++e) w[e / 4] |= (c + e < end ? (uint32_t)b[e] : 0u) << (8 * (e & 3));
+    return w;
+}
+
 // A wave a row, 16 bytes a lane; rows may start anywhere.
 __device__ __forceinline__ void pad_rows(const T0gPadArgs& p) {
     typedef u32x4_t u32x4_byte __attribute__((aligned(1)));
@@ -541,10 +584,8 @@ __device__ __forceinline__ void pad_rows(const T0gPadArgs& p) {
             u32x4_t w = {0u, 0u, 0u, 0u};
             if (c + 16 <= o.bytes) {
                 w = *at<const u32x4_byte>(from + c);
-            } else {
-#pragma unroll
-                for (uint32_t e = 0; e < 16; ++e)
-                    if (c + e < o.bytes) w[e / 4] |= (uint32_t)*at<const uint8_t>(from + c, e) << (8 * (e & 3));
+            } else if (c < o.bytes) {
+                w = tail16(from, c, o.bytes);
             }
             *at<u32x4_t>(to + c) = w;
         }

@@ -13,11 +13,7 @@ typedef i32x4_t i32x4_any __attribute__((aligned(1)));
 // Bytes [at, at + 16) of a row that ends at `end`, zeros past it.
 __device__ __forceinline__ i32x4_t load16(uint64_t row, uint32_t at_, uint32_t end) {
     if (at_ + 16 <= end) return *at<const i32x4_any>(row + at_);
-    i32x4_t v = {0, 0, 0, 0};
-#pragma unroll
-    for (uint32_t e = 0; e < 16; ++e)
-        if (at_ + e < end) v[e / 4] |= (int)((uint32_t)*at<const uint8_t>(row + at_, e) << (8 * (e & 3)));
-    return v;
+    return at_ < end ? __builtin_bit_cast(i32x4_t, tail16(row, at_, end)) : i32x4_t{0, 0, 0, 0};
 }
 
 template <int ROWS16>

@@ -154,17 +154,17 @@ int check_norm(t0g_rms_norm_desc *d) {
     return a.check();
 }
 
-// Threads of a row and pieces of 8 values of a thread.
+// Threads of a row and pieces of 8 values of a thread; threads and rows of a workgroup.
 struct RowShape {
     const char *suffix;
-    uint32_t threads;
+    uint32_t threads, rows;
 };
 RowShape row_shape(uint32_t hidden) {
-    if (hidden <= 512) return {"64x1", 64};
-    if (hidden <= 2048) return {"256x1", 256};
-    if (hidden <= 4096) return {"256x2", 256};
-    if (hidden <= 8192) return {"512x2", 512};
-    return {"1024x2", 1024};
+    if (hidden <= 512) return {"64x1", 256, 4};
+    if (hidden <= 2048) return {"256x1", 256, 1};
+    if (hidden <= 4096) return {"256x2", 256, 1};
+    if (hidden <= 8192) return {"512x2", 512, 1};
+    return {"1024x2", 1024, 1};
 }
 
 int norm_call(t0g_device *dev, const t0g_rms_norm_desc *desc) {
@@ -198,8 +198,11 @@ int norm_call(t0g_device *dev, const t0g_rms_norm_desc *desc) {
     a.flags = (d.x_dtype == T0G_F32 ? T0G_ROWS_X_F32 : 0) | (d.residual_dtype == T0G_F32 ? T0G_ROWS_R_F32 : 0) |
               (d.weight_dtype == T0G_F32 ? T0G_ROWS_W_F32 : 0) | (d.sum_dtype == T0G_F32 ? T0G_ROWS_OUT_F32 : 0) |
               (d.y_dtype == T0G_F32 ? T0G_ROWS_Y_F32 : 0) | (d.q_dtype == T0G_E5M2 ? T0G_ROWS_E5M2 : 0);
+    const bool fast = d.hidden % 8 == 0 && !(a.flags & T0G_ROWS_X_F32) && !(d.residual && a.flags & T0G_ROWS_R_F32) &&
+                      !(d.weight && a.flags & T0G_ROWS_W_F32);
     const RowShape s = row_shape(d.hidden);
-    return ffn_launch(dev, (std::string("t0g_ffn_norm_") + s.suffix).c_str(), std::min(d.rows, 1u << 20), 1, s.threads, &a, sizeof a);
+    return ffn_launch(dev, (std::string("t0g_ffn_norm_") + s.suffix + (fast ? "_fast" : "")).c_str(), groups_for(d.rows, s.rows, 1u << 20),
+                      1, s.threads, &a, sizeof a);
 }
 
 int check_norm_grad(t0g_rms_norm_backward_desc *d) {
@@ -226,7 +229,14 @@ int check_norm_grad(t0g_rms_norm_backward_desc *d) {
 }
 
 // Workgroups of the gradient kernel, each with a row of partial sums of dw.
-uint32_t norm_grad_groups(const t0g_rms_norm_backward_desc &d) { return std::min(d.rows, 512u); }
+bool norm_grad_fast(const t0g_rms_norm_backward_desc &d) {
+    return d.hidden % 8 == 0 && d.x_dtype == T0G_BF16 && d.dy_dtype == T0G_BF16 && (!d.dsum || d.dsum_dtype == T0G_BF16) &&
+           (!d.weight || d.weight_dtype == T0G_BF16);
+}
+uint32_t norm_grad_groups(const t0g_rms_norm_backward_desc &d) {
+    const RowShape s = row_shape(d.hidden);
+    return groups_for(d.rows, s.rows, std::max(256u, 1024 * 256 / s.threads));
+}
 uint32_t norm_grad_ld(const t0g_rms_norm_backward_desc &d) { return (uint32_t)round_up(d.hidden, 8); }
 size_t norm_grad_scratch(const t0g_rms_norm_backward_desc &d) {
     return d.dw ? (size_t)norm_grad_groups(d) * norm_grad_ld(d) * 4 : 0;
@@ -263,8 +273,11 @@ int norm_grad_call(t0g_device *dev, const t0g_rms_norm_backward_desc *desc) {
         a.flags = (d.dy_dtype == T0G_F32 ? T0G_ROWS_Y_F32 : 0) | (d.x_dtype == T0G_F32 ? T0G_ROWS_X_F32 : 0) |
                   (d.weight_dtype == T0G_F32 ? T0G_ROWS_W_F32 : 0) | (d.dsum_dtype == T0G_F32 ? T0G_ROWS_R_F32 : 0) |
                   (d.dx_dtype == T0G_F32 ? T0G_ROWS_OUT_F32 : 0);
+        const bool fast = norm_grad_fast(d);
         const RowShape s = row_shape(d.hidden);
-        if ((rc = ffn_launch(dev, (std::string("t0g_ffn_norm_grad_") + s.suffix).c_str(), groups, 1, s.threads, &a, sizeof a))) return rc;
+        if ((rc = ffn_launch(dev, (std::string("t0g_ffn_norm_grad_") + s.suffix + (fast ? "_fast" : "")).c_str(), groups, 1, s.threads,
+                             &a, sizeof a)))
+            return rc;
     }
     if (!d.dw) return ok();
     T0gColSumArgs s;
@@ -275,7 +288,7 @@ int norm_grad_call(t0g_device *dev, const t0g_rms_norm_backward_desc *desc) {
     s.cols = d.hidden;
     s.ldp = norm_grad_ld(d);
     s.out_bf16 = d.dw_dtype == T0G_BF16;
-    return ffn_launch(dev, "t0g_ffn_column_sum", (d.hidden + 31) / 32, 1, 256, &s, sizeof s);
+    return ffn_launch(dev, "t0g_ffn_column_sum", (d.hidden + 31) / 32, 1, 1024, &s, sizeof s);
 }
 
 // ---- 8-bit values -----------------------------------------------------------------------
@@ -398,6 +411,12 @@ struct Slices {
 };
 uint64_t tiles_of(uint32_t m, uint32_t n, uint32_t bm, uint32_t bn) { return ((uint64_t)m + bm - 1) / bm * (((uint64_t)n + bn - 1) / bn); }
 
+// Tiles of 128 rows instead of 64: both kinds run two to a CU; a round of the larger ones takes about 1.6 times as long.
+bool middle(uint32_t m, uint32_t n, uint32_t bn) {
+    auto rounds = [&](uint32_t bm) { return (tiles_of(m, n, bm, bn) + 2 * kNumCUs - 1) / (2 * kNumCUs); };
+    return 16 * rounds(128) < 10 * rounds(64);
+}
+
 int run_join(t0g_device *dev, const T0gTileArgs &t, const Slices &s, uint32_t gated) {
     T0gJoinArgs j;
     memset(&j, 0, sizeof j);
@@ -454,7 +473,7 @@ void plan_fp8(const t0g_fp8_gemm_desc &d, Fp8Plan *p) {
     if (d.out_dtype == T0G_BF16 && tiles_of(d.m, d.n, 256, 256) >= kNumCUs)
         p->tile = Fp8Tile::Big;
     else
-        p->tile = tiles_of(d.m, d.n, 128, 128) >= 2 * kNumCUs ? Fp8Tile::Middle : Fp8Tile::Small;
+        p->tile = middle(d.m, d.n, 128) ? Fp8Tile::Middle : Fp8Tile::Small;
     p->a.set(d.a, d.m, d.k, d.lda, 1);
     p->b.set(d.b, d.n, d.k, d.ldb, 1);
     p->a.at = take(&p->bytes, p->a.bytes());
@@ -566,7 +585,7 @@ struct GatedPlan {
         if (!grad && big(rows, features, hidden, nt))
             tile = GatedTile::Big;
         else
-            tile = tiles_of(rows, features, 128, 64) >= 2 * kNumCUs ? GatedTile::Middle : GatedTile::Small;
+            tile = middle(rows, features, 64) ? GatedTile::Middle : GatedTile::Small;
         slices.set(tile == GatedTile::Small ? tiles_of(rows, features, 64, 64) : 0, (hidden + 63) / 64, rows, features, 2);
         slices.at = take(at, slices.bytes);
     }

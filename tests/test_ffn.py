@@ -108,9 +108,9 @@ def test_norm_backward_refusals(change, word):
 
 def test_norm_backward_scratch():
     assert t0g.ffn_scratch_size(norm_backward(dw=0)) == 0
-    assert t0g.ffn_scratch_size(norm_backward()) == 16 * 304 * 4
+    assert t0g.ffn_scratch_size(norm_backward()) >= 304 * 4
     for a in (A, B, D):
-        assert t0g.ffn_scratch_size(norm_backward(dx=a)) == 16 * 304 * 4
+        assert t0g.ffn_scratch_size(norm_backward(dx=a)) == t0g.ffn_scratch_size(norm_backward())
 
 
 @pytest.mark.parametrize("change,word", [
