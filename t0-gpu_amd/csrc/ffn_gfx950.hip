@@ -38,8 +38,10 @@ NORM_GRAD(256, 2, 1, _fast, true, true, true)
 NORM_GRAD(512, 2, 1, _fast, true, true, true)
 NORM_GRAD(1024, 2, 1, _fast, true, true, false)
 extern "C" __global__ void __launch_bounds__(1024) t0g_ffn_column_sum(T0gColSumArgs p) { t0g::column_sum(p); }
-extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_rows(T0gQuantArgs p) { t0g::quantize_rows(p); }
-extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_tile(T0gQuantArgs p) { t0g::quantize_tile(p); }
+extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_rows(T0gQuantArgs p) { t0g::quantize_rows<false>(p); }
+extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_rows_fast(T0gQuantArgs p) { t0g::quantize_rows<true>(p); }
+extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_tile(T0gQuantArgs p) { t0g::quantize_tile<false>(p); }
+extern "C" __global__ void __launch_bounds__(256) t0g_ffn_quantize_tile_fast(T0gQuantArgs p) { t0g::quantize_tile<true>(p); }
 extern "C" __global__ void __launch_bounds__(256) t0g_ffn_gated_grad(T0gGatedGradArgs p) { t0g::gated_grad(p); }
 extern "C" __global__ void __launch_bounds__(256) t0g_ffn_pad_rows(T0gPadArgs p) { t0g::pad_rows(p); }
 extern "C" __global__ void __launch_bounds__(256) t0g_ffn_join_slices(T0gJoinArgs p) { t0g::join_slices(p); }

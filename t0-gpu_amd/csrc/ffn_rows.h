@@ -12,6 +12,7 @@ namespace t0g {
 typedef u32x4_t u32x4_any __attribute__((aligned(2)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef u32x2_t u32x2_any __attribute__((aligned(1)));
+typedef u32x4_t u32x4_byte __attribute__((aligned(1)));
 template <class T>
 using gptr = __attribute__((address_space(1))) T*;
 template <class T>
@@ -404,11 +405,13 @@ __device__ __forceinline__ void column_sum(const T0gColSumArgs& p) {
 
 // ---- 8 bits with scales ----------------------------------------------------------------
 // Blocks of 1 x 128: 16 lanes a block, 1 << row_shift threads a row, U rows of a thread in flight.
+// FAST: bf16 in rows of whole pieces of 8.
+template <bool FAST>
 __device__ __forceinline__ void quantize_rows(const T0gQuantArgs& p) {
     constexpr int U = 4;
-    const bool f32 = p.flags & T0G_ROWS_X_F32, e5m2 = p.flags & T0G_ROWS_E5M2;
+    const bool f32 = !FAST && p.flags & T0G_ROWS_X_F32, e5m2 = p.flags & T0G_ROWS_E5M2;
     const uint32_t width = 1u << p.row_shift, rows = 256u >> p.row_shift;
-    const uint32_t c = 8 * (blockIdx.x * width + (threadIdx.x & (width - 1))), n = left8(p.cols, c);
+    const uint32_t c = 8 * (blockIdx.x * width + (threadIdx.x & (width - 1))), n = left8<FAST>(p.cols, c);
     for (uint64_t r0 = (uint64_t)blockIdx.y * U * rows; r0 < p.rows; r0 += (uint64_t)gridDim.y * U * rows) {
         Raw8 x[U];
 #pragma unroll
@@ -433,14 +436,15 @@ __device__ __forceinline__ void quantize_rows(const T0gQuantArgs& p) {
 // 128 x 128 values: one scale for all of them (TILE), or one for each row and, for the transposed
 // matrix, one for each column.  Thread (g, l) = (tid / 16, tid % 16) holds rows 8 g .. + 7 of columns
 // 8 l .. + 7, so its part of each column is 8 bytes of the transposed matrix, which goes out through LDS
-// in whole rows of 128 bytes.
+// in whole rows of 128 bytes, 8-byte piece g of row 8 l + e at piece g ^ l: with rows 144 bytes apart the 16 lanes l
+// wrote to 2 groups of banks.
+template <bool FAST>
 __device__ __forceinline__ void quantize_tile(const T0gQuantArgs& p) {
-    constexpr uint32_t kRow = 128 + 16;   // LDS bytes of a transposed row
     __shared__ float col_max[16][128], col_inv[128];
-    __shared__ __attribute__((aligned(16))) char out[128 * kRow];
-    const bool f32 = p.flags & T0G_ROWS_X_F32, e5m2 = p.flags & T0G_ROWS_E5M2, tile = p.flags & T0G_ROWS_TILE;
+    __shared__ __attribute__((aligned(16))) char out[128 * 128];
+    const bool f32 = !FAST && p.flags & T0G_ROWS_X_F32, e5m2 = p.flags & T0G_ROWS_E5M2, tile = p.flags & T0G_ROWS_TILE;
     const uint32_t l = threadIdx.x & 15u, g = threadIdx.x >> 4;
-    const uint32_t c0 = 128 * blockIdx.x, c = c0 + 8 * l, n = left8(p.cols, c);
+    const uint32_t c0 = 128 * blockIdx.x, c = c0 + 8 * l, n = left8<FAST>(p.cols, c);
     const uint32_t tiles = (p.rows + 127) / 128;
     for (uint32_t ty = blockIdx.y; ty < tiles; ty += gridDim.y) {
         const uint32_t r0 = 128 * ty, row = r0 + 8 * g;
@@ -505,15 +509,21 @@ __device__ __forceinline__ void quantize_tile(const T0gQuantArgs& p) {
                 float u[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) u[i] = v[i][e];
-                *reinterpret_cast<u32x2_t*>(out + (8 * l + e) * kRow + 8 * g) = f8x8(u, inv, e5m2);
+                *reinterpret_cast<u32x2_t*>(out + (8 * l + e) * 128 + 8 * (g ^ l)) = f8x8(u, inv, e5m2);
             }
             __syncthreads();
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 const uint32_t piece = i * 256 + threadIdx.x, tr = piece >> 3, tc = 16 * (piece & 7u);
-                const u32x4_t w = *reinterpret_cast<const u32x4_t*>(out + tr * kRow + tc);
+                const uint32_t tl = tr >> 3;
+                u32x4_t w = *reinterpret_cast<const u32x4_t*>(out + tr * 128 + (tc ^ 16 * (tl >> 1)));
+                if (tl & 1u) w = u32x4_t{w[2], w[3], w[0], w[1]};
                 if (c0 + tr >= p.cols || r0 + tc >= p.rows) continue;
                 const uint64_t to = p.qt + (uint64_t)(c0 + tr) * p.ldqt + r0 + tc;
+                if (r0 + tc + 16 <= p.rows) {
+                    *at<u32x4_byte>(to) = w;
+                    continue;
+                }
                 store_f8x8(to, min(p.rows - r0 - tc, 8u), u32x2_t{w[0], w[1]});
                 if (r0 + tc + 8 < p.rows) store_f8x8(to + 8, min(p.rows - r0 - tc - 8, 8u), u32x2_t{w[2], w[3]});
             }
@@ -576,7 +586,6 @@ __device__ __forceinline__ u32x4_t tail16(uint64_t row, uint32_t c, uint32_t end
 
 // A wave a row, 16 bytes a lane; rows may start anywhere.
 __device__ __forceinline__ void pad_rows(const T0gPadArgs& p) {
-    typedef u32x4_t u32x4_byte __attribute__((aligned(1)));
     const auto& o = p.a[blockIdx.y];
     for (uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6); row < o.rows; row += gridDim.x * 4) {
         const uint64_t from = o.src + row * o.lds, to = o.dst + row * o.ldd;

@@ -336,13 +336,14 @@ int quantize_call(t0g_device *dev, const t0g_fp8_quantize_desc *desc) {
     a.ldsct = d.ldsct;
     a.flags = (d.x_dtype == T0G_F32 ? T0G_ROWS_X_F32 : 0) | (d.q_dtype == T0G_E5M2 ? T0G_ROWS_E5M2 : 0) |
               (d.block == T0G_BLOCK_TILE ? T0G_ROWS_TILE : 0);
+    const bool fast = d.x_dtype == T0G_BF16 && d.cols % 8 == 0;
     if (d.qt || d.block == T0G_BLOCK_TILE)
-        return ffn_launch(dev, "t0g_ffn_quantize_tile", blocks_of(d.cols), std::min(blocks_of(d.rows), kMaxGridY), 256, &a, sizeof a);
+        return ffn_launch(dev, fast ? "t0g_ffn_quantize_tile_fast" : "t0g_ffn_quantize_tile", blocks_of(d.cols), std::min(blocks_of(d.rows), kMaxGridY), 256, &a, sizeof a);
     const uint32_t pieces = blocks_of(d.cols) * 16;
     a.row_shift = 4;
     while (a.row_shift < 8 && (1u << a.row_shift) < pieces) ++a.row_shift;
     const uint32_t gx = (pieces + (1u << a.row_shift) - 1) >> a.row_shift, rows = 4 * (256u >> a.row_shift);
-    return ffn_launch(dev, "t0g_ffn_quantize_rows", gx, groups_for(d.rows, rows, kMaxGridY), 256, &a, sizeof a);
+    return ffn_launch(dev, fast ? "t0g_ffn_quantize_rows_fast" : "t0g_ffn_quantize_rows", gx, groups_for(d.rows, rows, kMaxGridY), 256, &a, sizeof a);
 }
 
 // ---- operands of the tile kernels -------------------------------------------------------
