@@ -447,7 +447,8 @@ int check_fp8_gemm(t0g_fp8_gemm_desc *d) {
     if ((rc = check_f8("a_dtype", d->a_dtype)) || (rc = check_f8("b_dtype", d->b_dtype)) || (rc = check_float("out_dtype", d->out_dtype)))
         return rc;
     if (d->b_block > T0G_BLOCK_TILE) return fail(T0G_ERR_INVALID_ARG, "bad b_block %u", d->b_block);
-    if (d->k == 0 || d->k > kMaxRowBytes || d->m > kMaxRows || d->n > kMaxRows)
+    // offsets into a row of scales are 32 bits
+    if (d->k == 0 || d->k > kMaxRowBytes || d->m > (1u << 28) || d->n > (1u << 28))
         return fail(T0G_ERR_INVALID_ARG, "bad size: m %u, n %u, k %u", d->m, d->n, d->k);
     if (d->m && d->n && (!d->a || !d->b || !d->c || !d->a_scales || !d->b_scales)) return fail(T0G_ERR_INVALID_ARG, "NULL operand");
     Arrays a;

@@ -579,6 +579,41 @@ def test_gated_backward_against_differences(rt):
             assert abs(slope - got[name].reshape(-1)[i]) <= 0.02 * got[name].abs().max(), (name, i)
 
 
+def test_rows_far_apart(rt):
+    """Rows 2.4 GB apart, the third beyond 2^32 bytes: norms, 8-bit values, and products of few and of more rows."""
+    ld, rows, k = 1_200_000_003, 3, 300
+    big = rt.alloc((2 * ld + 64 * 512) * 2)
+    try:
+        g = torch.Generator().manual_seed(1)
+        x, w = data(g, rows, k), data(g, 1, k)[0]
+        for r in range(rows):
+            rt.write(big + 2 * r * ld, raw(x[r].clone()))
+        b = Bufs(rt)
+        (wa, _), (ya, _), (dya, _) = b.inp(w, True), b.out("y", x.shape, F32), b.inp(data(g, rows, k))
+        (qa, _), (ca, _), (ta, _), (tc, _) = (b.out("q", x.shape, E4), b.out("scales", (3, rows), F32), b.out("qt", (k, rows), E4),
+                                              b.out("scales_t", (1, k), F32))
+        rt.rms_norm(t0g.rms_norm_desc(big, wa, rows, k, y=ya, y_dtype=t0g.F32, ldx=ld))
+        rt.fp8_quantize(t0g.fp8_quantize_desc(big, qa, ca, rows, k, qt=ta, scales_t=tc, ldx=ld))
+        got = b.read()
+        y = norm_of(x, None, w, 0.0, 1e-6)[2]
+        near(got["y"], y, (U + NORM_REL) * y.abs(), "y")
+        check_f8(got["q"], got["scales"], x.double(), E4, what="q")
+        check_f8(got["qt"], got["scales_t"], x.double().t(), E4, what="qt")
+        # the same memory as B's rows, bytes apart the same
+        for m in (2, 40):
+            (a, sa), (q, sq) = f8_operand(g, m, k, E4, False), f8_operand(g, rows, k, E4, False)
+            for r in range(rows):
+                rt.write(big + 2 * r * ld, raw(q[r].clone()))
+            b = Bufs(rt)
+            (aa, _), (sa_, _), (sq_, _), (ca, _) = b.inp(a), b.inp(sa), b.inp(sq), b.out("c", (m, rows), F32)
+            rt.fp8_gemm(t0g.fp8_gemm_desc(aa, sa_, big, sq_, ca, m, rows, k, ldb=2 * ld, b_block=t0g.BLOCK_ROW, out_dtype=t0g.F32))
+            av, bv = a.double() * spread(sa.double(), a.shape), q.double() * spread(sq.double(), q.shape)
+            near(b.read()["c"], av @ bv.t(), 2 * (128 + 3 + 70) * U * (av.abs() @ bv.abs().t()) + U * (av @ bv.t()).abs(), f"{m} rows")
+    finally:
+        rt.wait_idle()
+        rt.free(big)
+
+
 def test_empty_calls(rt):
     """No rows, or no columns of the product: nothing is written, and NULL arrays are no error."""
     rt.rms_norm(t0g.rms_norm_desc(0, 0, 0, 64, y=4096))
