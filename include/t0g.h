@@ -604,7 +604,8 @@ T0G_API int t0g_set_loss_form(uint32_t form);
  * 8-bit values have an f32 scale for each block of 128 along a row (T0G_BLOCK_ROW) or of
  * 128 rows by 128 columns (T0G_BLOCK_TILE; blocks at the end may be smaller):
  *   scale = max(largest magnitude in the block, 2^-100) / 448 (e5m2: 57344)
- *   q = value / scale, rounded to nearest even
+ *   q = value / scale, rounded to nearest even (by the inverse: a quotient within 2^-22 of a
+ *       border between two roundings may go either way)
  * A NaN or an infinity makes all of its block's values NaN.  Scales are stored by blocks of
  * columns: scales[column / 128][row], or [column / 128][row / 128]. */
 #define T0G_BLOCK_ROW 0u
@@ -675,7 +676,8 @@ T0G_API int t0g_fp8_quantize(t0g_device *dev, const t0g_fp8_quantize_desc *desc)
 /* C = A B^T of 8-bit values: the sum over blocks of K of a_scale b_scale times the sum of the
  * block's products.  With out_dtype T0G_F32 these are exact and summed in f32.  With T0G_BF16
  * they are the 8-bit matrix unit's: of each 8 neighbouring products it cuts what is below 2^-13
- * of the largest one's power of two (in all about 2^-14 of the result, of bf16's 2^-9). */
+ * of the largest one's power of two (in all about 2^-14 of the result, of bf16's 2^-9), but for
+ * up to 32 rows, which are as with T0G_F32.  k up to 8388480, m and n up to 2^28. */
 typedef struct t0g_fp8_gemm_desc {
     uint64_t a;                  /* a_dtype [m][lda]                             */
     uint64_t a_scales;           /* f32 [ceil(k / 128)][ldas >= m]               */
@@ -693,7 +695,8 @@ T0G_API int t0g_fp8_gemm_scratch_size(const t0g_fp8_gemm_desc *desc, size_t *byt
 
 /* A gated pair of projections in one kernel: g = x Wg^T, u = x Wu^T, h = act(g) u, with act one
  * of T0G_OP_SILU, T0G_OP_GELU (x sigmoid(1.702 x), as in the GEMMs' epilogues) and
- * T0G_OP_RELU.  gate and up receive g and u in bf16 for the backward call, if asked for. */
+ * T0G_OP_RELU.  gate and up receive g and u in bf16 for the backward call, if asked for.
+ * hidden and features up to 4194240. */
 typedef struct t0g_gated_linear_desc {
     uint64_t x;                  /* bf16 [rows][ldx]                             */
     uint64_t wg, wu;             /* bf16, NT: [features][ldw], NN: [hidden][ldw] */

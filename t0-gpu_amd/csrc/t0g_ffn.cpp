@@ -154,7 +154,9 @@ int check_norm(t0g_rms_norm_desc *d) {
     return a.check();
 }
 
-// Threads of a row and pieces of 8 values of a thread; threads and rows of a workgroup.
+// Threads of a row and pieces of 8 values of a thread; threads and rows of a workgroup.  Up to 512 values a wave has
+// the row to itself (gradients of 12527x205: 27 us; one row to a workgroup 105); two pieces a thread up to 8192
+// leave registers for several workgroups on a CU.
 struct RowShape {
     const char *suffix;
     uint32_t threads, rows;
@@ -393,8 +395,9 @@ int run_pad(t0g_device *dev, std::initializer_list<const Operand *> list, uint64
     return n ? ffn_launch(dev, "t0g_ffn_pad_rows", groups_for(rows, 4, 1u << 16), n, 256, &p, sizeof p) : (int)T0G_OK;
 }
 
-// The K of a product of few tiles goes to several workgroups, in slices of at least kLeastStages stages, until kFill
-// workgroups are there; their sums go to f32 planes.
+// The K of a product of few tiles goes to several workgroups, in slices of at least kLeastStages stages (a slice's
+// first loads take about as long as two stages), until kFill workgroups, two for each CU, are there; their sums go
+// to f32 planes.  (64 rows of 11008x4096 in 8 bits 18 us, 64 of 4096x11008 into f32 22.)
 constexpr uint32_t kFill = 2 * kNumCUs, kLeastStages = 4;
 struct Slices {
     uint32_t n = 1, stages = 0, ldp = 0;
@@ -412,7 +415,9 @@ struct Slices {
 };
 uint64_t tiles_of(uint32_t m, uint32_t n, uint32_t bm, uint32_t bn) { return ((uint64_t)m + bm - 1) / bm * (((uint64_t)n + bn - 1) / bn); }
 
-// Tiles of 128 rows instead of 64: both kinds run two to a CU; a round of the larger ones takes about 1.6 times as long.
+// Tiles of 128 rows instead of 64: both kinds run two to a CU; a round of the larger ones takes about 1.6 times as
+// long (gated 1000x2731x1023, 688 tiles in two rounds or 344 in one: 28 us or 25; 8 bits 777x5001x1023, 520 or 280:
+// 22 either way).
 bool middle(uint32_t m, uint32_t n, uint32_t bn) {
     auto rounds = [&](uint32_t bm) { return (tiles_of(m, n, bm, bn) + 2 * kNumCUs - 1) / (2 * kNumCUs); };
     return 16 * rounds(128) < 10 * rounds(64);
@@ -460,7 +465,9 @@ int check_fp8_gemm(t0g_fp8_gemm_desc *d) {
     return a.check();
 }
 
-// Rows up to which a product is bound by reading B, which then goes straight to registers.
+// Rows up to which a product is bound by reading B, which then goes straight to registers.  11008x4096 in 8 bits:
+// one row 10 us (64-row tiles, two LDS stages: 40), 24 rows 17, where the tiles take 18 for 64; gated, one row
+// 35 (62), 24 rows 47 (64 rows 53).
 constexpr uint32_t kSkinnyRows = 32;
 
 enum class Fp8Tile { Skinny, Small, Middle, Big };
@@ -472,6 +479,7 @@ struct Fp8Plan {
 };
 void plan_fp8(const t0g_fp8_gemm_desc &d, Fp8Plan *p) {
     if (d.m <= kSkinnyRows) return;
+    // 8192x8192x8192: 460 us in 256x256 tiles, 709 in 128x128
     if (d.out_dtype == T0G_BF16 && tiles_of(d.m, d.n, 256, 256) >= kNumCUs)
         p->tile = Fp8Tile::Big;
     else
@@ -591,7 +599,8 @@ struct GatedPlan {
         slices.set(tile == GatedTile::Small ? tiles_of(rows, features, 64, 64) : 0, (hidden + 63) / 64, rows, features, 2);
         slices.at = take(at, slices.bytes);
     }
-    // Whether the 256x256 tile takes it: enough tiles for all CUs, and 32-bit offsets in the operands.
+    // Whether the 256x256 tile takes it: enough tiles for all CUs, and 32-bit offsets in the operands.  2048x11008x4096
+    // and its gradients: 962 us so, 1025 in 128x64 tiles.
     bool big(uint32_t rows, uint32_t features, uint32_t hidden, bool nt) const {
         const uint64_t most = 1ull << 30, ldb = wg.pitch(), wspan = (nt ? features + 256ull : hidden + 64ull) * ldb;
         const uint64_t g = wg.address(0), u = wu.address(0), apart = g < u ? u - g : g - u;   // as far apart in the scratch

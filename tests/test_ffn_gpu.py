@@ -142,7 +142,7 @@ def norm_of(x, r, w, offset, eps):
 
 
 @pytest.mark.parametrize("rows,hidden", [(1, 1), (3, 7), (2, 64), (5, 127), (4, 128), (3, 129), (2, 512), (3, 513), (2, 1000),
-                                         (3, 2048), (2, 2049), (300, 1023), (2, 4096), (3, 4097), (2, 8192), (2, 8193), (2, 16383),
+                                         (3, 2048), (2, 2049), (2, 3001), (2, 3000), (2, 12001), (2, 12000), (300, 1023), (2, 4096), (3, 4097), (2, 8192), (2, 8193), (2, 16383),
                                          (1, 16384)])
 @pytest.mark.parametrize("xt,rt_,wt,yt", [(BF16, BF16, BF16, BF16), (F32, F32, F32, F32), (BF16, F32, F32, BF16), (F32, None, None, F32)])
 @pytest.mark.parametrize("pad,offset", [(0, 0), (3, 1)])
@@ -206,8 +206,8 @@ def test_norm_of_zeros_infinities_and_nan(rt):
     assert bool(torch.isnan(stands[1, :128]).all() and torch.isnan(stands[2]).all())
 
 
-@pytest.mark.parametrize("rows,hidden", [(1, 1), (2, 5), (3, 64), (1, 129), (4, 512), (700, 300), (1500, 2047), (3, 4096), (3, 4100),
-                                         (5, 8192), (2, 8195), (515, 16384)])
+@pytest.mark.parametrize("rows,hidden", [(1, 1), (2, 5), (3, 64), (1, 129), (4, 512), (700, 300), (1500, 2047), (3, 3001), (3, 3000), (3, 4096), (3, 4100),
+                                         (2, 12001), (2, 12000), (5, 8192), (2, 8195), (515, 16384)])
 @pytest.mark.parametrize("xt,yt,wt,st", [(BF16, BF16, BF16, BF16), (F32, F32, F32, F32), (F32, BF16, None, None), (BF16, F32, F32, F32)])
 @pytest.mark.parametrize("pad,offset", [(0, 0), (5, 1)])
 def test_norm_backward(rt, rows, hidden, xt, yt, wt, st, pad, offset):
