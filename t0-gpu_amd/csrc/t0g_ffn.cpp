@@ -441,19 +441,14 @@ int set_tiles(T0gTileArgs *a, uint32_t bm, uint32_t bn) {
     return T0G_OK;
 }
 
-// Workgroups of a product of few rows.
-int skinny_groups(uint32_t n) {
-    return n >= (1u << 26) ? fail(T0G_ERR_INVALID_ARG, "bad size: %u columns", n) : T0G_OK;
-}
-
 // ---- the 8-bit product ------------------------------------------------------------------
 int check_fp8_gemm(t0g_fp8_gemm_desc *d) {
     int rc;
     if ((rc = check_f8("a_dtype", d->a_dtype)) || (rc = check_f8("b_dtype", d->b_dtype)) || (rc = check_float("out_dtype", d->out_dtype)))
         return rc;
     if (d->b_block > T0G_BLOCK_TILE) return fail(T0G_ERR_INVALID_ARG, "bad b_block %u", d->b_block);
-    // offsets into a row of scales are 32 bits
-    if (d->k == 0 || d->k > kMaxRowBytes || d->m > (1u << 28) || d->n > (1u << 28))
+    // offsets into a row of scales are 32 bits, and so are a launch's threads
+    if (d->k == 0 || d->k > kMaxRowBytes || d->m > (1u << 28) || d->n > (1u << 26))
         return fail(T0G_ERR_INVALID_ARG, "bad size: m %u, n %u, k %u", d->m, d->n, d->k);
     if (d->m && d->n && (!d->a || !d->b || !d->c || !d->a_scales || !d->b_scales)) return fail(T0G_ERR_INVALID_ARG, "NULL operand");
     Arrays a;
@@ -505,7 +500,7 @@ int fp8_gemm_call(t0g_device *dev, const t0g_fp8_gemm_desc *desc) {
     t.n = d.n;
     t.k = d.k;
     const bool skinny = pl.tile == Fp8Tile::Skinny, big = pl.tile == Fp8Tile::Big, small = pl.tile == Fp8Tile::Small;
-    if ((rc = skinny ? skinny_groups(d.n) : big ? set_tiles(&t, 256, 256) : set_tiles(&t, small ? 64 : 128, 128))) return rc;
+    if (!skinny && (rc = big ? set_tiles(&t, 256, 256) : set_tiles(&t, small ? 64 : 128, 128))) return rc;
     if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
     std::lock_guard<std::mutex> lk(device_mutex(dev));
     uint64_t base;

@@ -125,7 +125,7 @@ def test_quantize_refusals(change, word):
 
 
 @pytest.mark.parametrize("change,word", [
-    ({"k": 0}, "size"), ({"k": 1 << 23}, "size"), ({"m": (1 << 28) + 1}, "size"), ({"n": (1 << 28) + 1}, "size"), ({"a_dtype": 1}, "a_dtype"),
+    ({"k": 0}, "size"), ({"k": 1 << 23}, "size"), ({"m": (1 << 28) + 1}, "size"), ({"n": (1 << 26) + 1}, "size"), ({"a_dtype": 1}, "a_dtype"),
     ({"b_dtype": 0}, "b_dtype"), ({"out_dtype": 2}, "out_dtype"), ({"b_block": 2}, "b_block"), ({"a": 0}, "NULL"), ({"b": 0}, "NULL"),
     ({"c": 0}, "NULL"), ({"a_scales": 0}, "NULL"), ({"b_scales": 0}, "NULL"), ({"lda": 299}, "a"), ({"ldb": 299}, "b"), ({"ldc": 255}, "c"),
     ({"ldas": 15}, "a_scales"), ({"ldbs": 1}, "b_scales"), ({"b_block": 0, "ldbs": 255}, "b_scales"), ({"c": E + 1}, "aligned"),
