@@ -604,8 +604,8 @@ T0G_API int t0g_set_loss_form(uint32_t form);
  * 8-bit values have an f32 scale for each block of 128 along a row (T0G_BLOCK_ROW) or of
  * 128 rows by 128 columns (T0G_BLOCK_TILE; blocks at the end may be smaller):
  *   scale = max(largest magnitude in the block, 2^-100) / 448 (e5m2: 57344)
- *   q = value / scale, rounded to nearest even (by the inverse: a quotient within 2^-22 of a
- *       border between two roundings may go either way)
+ *   q = value / scale, rounded to nearest even; the quotient, of the block's largest magnitude and
+ *       not of the rounded scale, goes through one f32 rounding on the way
  * A NaN or an infinity makes all of its block's values NaN.  Scales are stored by blocks of
  * columns: scales[column / 128][row], or [column / 128][row / 128]. */
 #define T0G_BLOCK_ROW 0u

@@ -127,18 +127,24 @@ __device__ __forceinline__ void store8(uint64_t base, uint64_t i, uint32_t n, bo
 // ---- 8 bits ----------------------------------------------------------------------------
 // A block's scale is max(largest magnitude, 2^-100) / the type's largest value: 0.5 units of
 // its 4 or 3 bits is then all that a value loses, and a block of zeros has a scale too.
-// Values are multiplied by the quotient's inverse, which is within 2 units of 2^-24 of the
-// division and so moves only values that close to a border between two roundings.  With a
-// NaN or an infinity among them all of a block's values come out as NaN.
+// A value is multiplied by the quotient's inverse in two parts, inv + rest, which is within 2^-45 of it, and the
+// product rounded once to f32.  Quotients on a border between two roundings are common among bf16 values: with the
+// inverse in one part 3e-4 of normal values went to the wrong side.  Such a quotient has few bits, so that
+// it comes out as it is and goes to the even neighbour; the others of bf16 values are 2^-14 of themselves away
+// from a border or more.  With a NaN or an infinity among them all of a block's values come out as NaN.
 constexpr float kLeastAmax = 7.888609052210118e-31f;   // 2^-100
 __device__ __forceinline__ float f8_most(bool e5m2) { return e5m2 ? 57344.0f : 448.0f; }
 struct BlockScale {
-    float scale, inv;
+    float scale, inv, rest;
 };
 __device__ __forceinline__ BlockScale block_scale(float amax, bool e5m2) {
     const float most = f8_most(e5m2);
     amax = max_(amax, kLeastAmax);
-    return BlockScale{amax / most, most / amax};
+    float inv = most / amax, r = __builtin_fmaf(-inv, amax, most);
+    // rounded down, so that rest is not negative and zeros keep their sign
+    inv = r < 0.0f ? __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, inv) - 1u) : inv;
+    r = __builtin_fmaf(-inv, amax, most);
+    return BlockScale{amax / most, inv, r > 0.0f ? r * (e5m2 ? 1.0f / 57344.0f : 1.0f / 448.0f) * inv : 0.0f};
 }
 __device__ __forceinline__ float amax8(const float (&v)[8]) {
     float m = __builtin_fabsf(v[0]);
@@ -157,9 +163,11 @@ __device__ __forceinline__ uint32_t f8x4(float a, float b, float c, float d, boo
     }
     return (uint32_t)w;
 }
-__device__ __forceinline__ u32x2_t f8x8(const float (&v)[8], float inv, bool e5m2) {
-    return u32x2_t{f8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv, e5m2),
-                   f8x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv, e5m2)};
+__device__ __forceinline__ u32x2_t f8x8(const float (&v)[8], float inv, float rest, bool e5m2) {
+    float t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = __builtin_fmaf(v[e], inv, v[e] * rest);
+    return u32x2_t{f8x4(t[0], t[1], t[2], t[3], e5m2), f8x4(t[4], t[5], t[6], t[7], e5m2)};
 }
 __device__ __forceinline__ void store_f8x8(uint64_t addr, uint32_t n, u32x2_t w) {
     if (n >= 8) {
@@ -236,7 +244,7 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) v[e] = e < n ? v[e] : 0.0f;
                 const BlockScale b = block_scale(row16_max(amax8(v)), e5m2);
-                store_f8x8(p.q + (uint64_t)row * p.ldq + c, n, f8x8(v, b.inv, e5m2));
+                store_f8x8(p.q + (uint64_t)row * p.ldq + c, n, f8x8(v, b.inv, b.rest, e5m2));
                 if ((threadIdx.x & 15u) == 0 && n) *at<float>(p.scales, (uint64_t)(c / T0G_SCALE_BLOCK) * p.ldsc + row) = b.scale;
             }
         }
@@ -426,7 +434,7 @@ __device__ __forceinline__ void quantize_rows(const T0gQuantArgs& p) {
             values8(x[u], f32, v);
             const BlockScale b = block_scale(row16_max(amax8(v)), e5m2);
             if (row < p.rows && n) {
-                store_f8x8(p.q + row * p.ldq + c, n, f8x8(v, b.inv, e5m2));
+                store_f8x8(p.q + row * p.ldq + c, n, f8x8(v, b.inv, b.rest, e5m2));
                 if ((threadIdx.x & 15u) == 0) *at<float>(p.scales, (uint64_t)(c / T0G_SCALE_BLOCK) * p.ldsc + row) = b.scale;
             }
         }
@@ -440,7 +448,7 @@ __device__ __forceinline__ void quantize_rows(const T0gQuantArgs& p) {
 // wrote to 2 groups of banks.
 template <bool FAST>
 __device__ __forceinline__ void quantize_tile(const T0gQuantArgs& p) {
-    __shared__ float col_max[16][128], col_inv[128];
+    __shared__ float col_max[16][128], col_inv[128], col_rest[128];
     __shared__ __attribute__((aligned(16))) char out[128 * 128];
     const bool f32 = !FAST && p.flags & T0G_ROWS_X_F32, e5m2 = p.flags & T0G_ROWS_E5M2, tile = p.flags & T0G_ROWS_TILE;
     const uint32_t l = threadIdx.x & 15u, g = threadIdx.x >> 4;
@@ -464,7 +472,7 @@ __device__ __forceinline__ void quantize_tile(const T0gQuantArgs& p) {
 #pragma unroll
             for (int i = 1; i < 8; ++i) cm[e] = max_(cm[e], __builtin_fabsf(v[i][e]));
         }
-        BlockScale whole = {0.0f, 0.0f};
+        BlockScale whole = {0.0f, 0.0f, 0.0f};
         if (tile) {
             float m = top[0];
 #pragma unroll
@@ -484,7 +492,7 @@ __device__ __forceinline__ void quantize_tile(const T0gQuantArgs& p) {
             for (uint32_t i = 0; i < 8; ++i) {
                 const BlockScale b = tile ? whole : block_scale(top[i], e5m2);
                 if (row + i < p.rows && n) {
-                    store_f8x8(p.q + (uint64_t)(row + i) * p.ldq + c, n, f8x8(v[i], b.inv, e5m2));
+                    store_f8x8(p.q + (uint64_t)(row + i) * p.ldq + c, n, f8x8(v[i], b.inv, b.rest, e5m2));
                     if (!tile && l == 0) *at<float>(p.scales, (uint64_t)blockIdx.x * p.ldsc + row + i) = b.scale;
                 }
             }
@@ -499,17 +507,18 @@ __device__ __forceinline__ void quantize_tile(const T0gQuantArgs& p) {
                     for (int i = 1; i < 16; ++i) m = max_(m, col_max[i][threadIdx.x]);
                     const BlockScale b = block_scale(m, e5m2);
                     col_inv[threadIdx.x] = b.inv;
+                    col_rest[threadIdx.x] = b.rest;
                     if (c0 + threadIdx.x < p.cols) *at<float>(p.scales_t, (uint64_t)ty * p.ldsct + c0 + threadIdx.x) = b.scale;
                 }
                 __syncthreads();
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float inv = tile ? whole.inv : col_inv[8 * l + e];
+                const float inv = tile ? whole.inv : col_inv[8 * l + e], rest = tile ? whole.rest : col_rest[8 * l + e];
                 float u[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) u[i] = v[i][e];
-                *reinterpret_cast<u32x2_t*>(out + (8 * l + e) * 128 + 8 * (g ^ l)) = f8x8(u, inv, e5m2);
+                *reinterpret_cast<u32x2_t*>(out + (8 * l + e) * 128 + 8 * (g ^ l)) = f8x8(u, inv, rest, e5m2);
             }
             __syncthreads();
 #pragma unroll
