@@ -185,6 +185,14 @@ __device__ __forceinline__ uint32_t left8(uint32_t cols, uint32_t c) {
     return c < cols ? (FAST ? 8u : min(cols - c, 8u)) : 0u;
 }
 
+// n as a new value to the compiler, which otherwise forms the lane masks of all comparisons with it before the
+// loop over the rows and runs out of scalar registers.
+template <bool FAST>
+__device__ __forceinline__ uint32_t anew(uint32_t n) {
+    if constexpr (!FAST) asm volatile("" : "+v"(n));
+    return n;
+}
+
 // ---- the norm --------------------------------------------------------------------------
 // y = s rho (w + offset), rho = (mean s^2 + eps)^-1/2, s = x + residual.  NT threads take a row, with CH pieces
 // of 8 each, and keep it in registers between the sum of squares and the output: memory is read and
@@ -203,7 +211,7 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
     for (uint32_t row = blockIdx.x * R + threadIdx.x / NT; row < p.rows; row += step, turn ^= 1) {
         Raw8 x[CH], r[CH], w[CH];
         auto load = [&](int i) {
-            const uint32_t c = 8 * (i * NT + first), n = left8<FAST>(p.hidden, c);
+            const uint32_t c = 8 * (i * NT + first), n = anew<FAST>(left8<FAST>(p.hidden, c));
             x[i] = load8(p.x, (uint64_t)row * p.ldx + c, n, xf);
             if (p.residual) r[i] = load8(p.residual, (uint64_t)row * p.ldr + c, n, rf);
             if (p.weight) w[i] = load8(p.weight, c, n, wf);
@@ -227,7 +235,7 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
         const float rho = 1.0f / __builtin_sqrtf(sum[0] / (float)p.hidden + p.eps);
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            const uint32_t c = 8 * (i * NT + first), n = left8<FAST>(p.hidden, c);
+            const uint32_t c = 8 * (i * NT + first), n = anew<FAST>(left8<FAST>(p.hidden, c));
             if (p.sum) store8(p.sum, (uint64_t)row * p.ldsum + c, n, p.flags & T0G_ROWS_OUT_F32, s[i]);
             float v[8];
             if (p.weight) {
@@ -268,7 +276,7 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
     Raw8 w[KEEP ? CH : 1];
     auto load_weight = [&](int i) {
         const uint32_t c = 8 * (i * NT + first);
-        if (p.weight) w[KEEP ? i : 0] = load8(p.weight, c, left8<FAST>(p.hidden, c), wf);
+        if (p.weight) w[KEEP ? i : 0] = load8(p.weight, c, anew<FAST>(left8<FAST>(p.hidden, c)), wf);
     };
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
@@ -289,7 +297,7 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
     constexpr int K = KEEP ? CH : 1;
     Raw8 y[K], x[K], d[K];
     auto load = [&](uint32_t row, int i, Raw8& yi, Raw8& xi, Raw8& di) {
-        const uint32_t c = 8 * (i * NT + first), n = row < p.rows ? left8<FAST>(p.hidden, c) : 0u;
+        const uint32_t c = 8 * (i * NT + first), n = anew<FAST>(row < p.rows ? left8<FAST>(p.hidden, c) : 0u);
         yi = load8(p.dy, (uint64_t)row * p.lddy + c, n, yf);
         xi = load8(p.x, (uint64_t)row * p.ldx + c, n, xf);
         if (p.dsum && p.dx) di = load8(p.dsum, (uint64_t)row * p.ldds + c, n, sf);
@@ -351,7 +359,7 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) g[e] += a[e];
                 }
-                store8(p.dx, (uint64_t)row * p.lddx + c, left8<FAST>(p.hidden, c), p.flags & T0G_ROWS_OUT_F32, g);
+                store8(p.dx, (uint64_t)row * p.lddx + c, anew<FAST>(left8<FAST>(p.hidden, c)), p.flags & T0G_ROWS_OUT_F32, g);
             }
         }
         if constexpr (PRE)
