@@ -614,7 +614,8 @@ T0G_API int t0g_set_loss_form(uint32_t form);
 /* Root-mean-square norm with the residual's addition:
  *   s = x + residual,  y = s (mean s^2 + eps)^-1/2 (weight + weight_offset)
  * sum receives s rounded to its type; y and q are formed from the unrounded s, q (e4m3 or
- * e5m2, blocks of 1 x 128) from the unrounded y.  sum may be x or residual itself (same
+ * e5m2, blocks of 1 x 128) from the unrounded y.  s may be of any magnitude: its squares are
+ * scaled where f32 does not hold their sum.  sum may be x or residual itself (same
  * address, leading dimension and type size), y may be x. */
 #define T0G_NORM_MAX 16384u   /* hidden size, at most */
 typedef struct t0g_rms_norm_desc {
@@ -638,7 +639,8 @@ T0G_API int t0g_rms_norm(t0g_device *dev, const t0g_rms_norm_desc *desc);
  *   n = x (mean x^2 + eps)^-1/2,  g = dy (weight + weight_offset)
  *   dx = (mean x^2 + eps)^-1/2 (g - n mean(g n)) + dsum,  dweight = sum over the rows of dy n
  * dx is the gradient of x and of the residual alike; dsum, what reaches the sum past the
- * norm.  dx and dw: each only if asked for.  dx may be dy, x or dsum itself. */
+ * norm.  x may be of any magnitude, g up to 2^64.  dx and dw: each only if asked for.  dx may be
+ * dy, x or dsum itself. */
 typedef struct t0g_rms_norm_backward_desc {
     uint64_t dy;                 /* dy_dtype [rows][lddy]                        */
     uint64_t x;                  /* x_dtype [rows][ldx]                          */

@@ -194,6 +194,31 @@ __device__ __forceinline__ uint32_t anew(uint32_t n) {
 }
 
 // ---- the norm --------------------------------------------------------------------------
+// What a row's values are multiplied by for their sum of squares: 1, or a power of two where f32 does not hold the sum
+// (16384 squares of values up to 2^128, or eps is so small that squares it would lose count), and then they are added up
+// again.  The same in all threads of the row.
+__device__ __forceinline__ float range_scale(float sum, float eps) {
+    const float k = sum > 0x1p96f ? 0x1p-80f : sum < 0x1p-90f && eps < 0x1p-60f ? 0x1p90f : 1.0f;
+    return __builtin_bit_cast(float, uniform_u32(__builtin_bit_cast(uint32_t, k)));
+}
+// rho = mean^-1/2 as a power of two times a value from 1 to 2, so that s * scale is about 1 in a row of any magnitude.
+// mean: of the squares times k^2.
+struct Rate {
+    float scale, rest;
+};
+__device__ __forceinline__ Rate rate_of(float mean, float k) {
+    const float rho = 1.0f / __builtin_sqrtf(mean);
+    const uint32_t w = __builtin_bit_cast(uint32_t, rho);
+    Rate r = {__builtin_bit_cast(float, w & 0x7F800000u), rho == rho ? __builtin_bit_cast(float, (w & 0x007FFFFFu) | 0x3F800000u) : rho};
+    if (k > 1.0f) {   // scale stays below 2^128
+        const float most = __builtin_fminf(r.scale, 0x1p127f / k);
+        r.rest *= r.scale / most;
+        r.scale = most;
+    }
+    r.scale *= k;
+    return r;
+}
+
 // y = s rho (w + offset), rho = (mean s^2 + eps)^-1/2, s = x + residual.  NT threads take a row, with CH pieces
 // of 8 each, and keep it in registers between the sum of squares and the output: memory is read and
 // written once.  Rows of one wave go R to a workgroup.  FAST: bf16 inputs of whole pieces of 8, which need
@@ -232,7 +257,17 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
             for (int e = 0; e < 8; ++e) sum[0] = __builtin_fmaf(s[i][e], s[i][e], sum[0]);
         }
         block_sum<W>(sum, t[turn]);
-        const float rho = 1.0f / __builtin_sqrtf(sum[0] / (float)p.hidden + p.eps);
+        const float k = range_scale(sum[0], p.eps);
+        if (k != 1.0f) {
+            sum[0] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[0] = __builtin_fmaf(s[i][e] * k, s[i][e] * k, sum[0]);
+            turn ^= 1;
+            block_sum<W>(sum, t[turn]);
+        }
+        const Rate rho = rate_of(sum[0] / (float)p.hidden + p.eps * k * k, k);
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const uint32_t c = 8 * (i * NT + first), n = anew<FAST>(left8<FAST>(p.hidden, c));
@@ -241,10 +276,10 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
             if (p.weight) {
                 values8(w[i], wf, v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = s[i][e] * rho * (v[e] + p.weight_offset);
+                for (int e = 0; e < 8; ++e) v[e] = s[i][e] * rho.scale * rho.rest * (v[e] + p.weight_offset);
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = s[i][e] * rho;
+                for (int e = 0; e < 8; ++e) v[e] = s[i][e] * rho.scale * rho.rest;
             }
             if (p.y) store8(p.y, (uint64_t)row * p.ldy + c, n, p.flags & T0G_ROWS_Y_F32, v);
             if (p.q) {
@@ -315,27 +350,36 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
         else if constexpr (KEEP)
 #pragma unroll
             for (int i = 0; i < CH; ++i) load(row, i, y[i], x[i], d[i]);
-        float sums[2] = {0.0f, 0.0f};   // of s^2 and g s
+        float sums[2] = {0.0f, 0.0f};   // of (s k)^2 and g s k
+        auto add_up = [&](float k) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            if constexpr (!KEEP) {
-                __builtin_amdgcn_sched_barrier(0);
-                load(row, i, y[0], x[0], d[0]);
-                load_weight(i);
-            }
-            float a[8], s[8], g[8];
-            values8(y[KEEP ? i : 0], yf, a);
-            values8(x[KEEP ? i : 0], xf, s);
-            weight(i, g);
+            for (int i = 0; i < CH; ++i) {
+                if constexpr (!KEEP) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    load(row, i, y[0], x[0], d[0]);
+                    load_weight(i);
+                }
+                float a[8], s[8], g[8];
+                values8(y[KEEP ? i : 0], yf, a);
+                values8(x[KEEP ? i : 0], xf, s);
+                weight(i, g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                sums[0] = __builtin_fmaf(s[e], s[e], sums[0]);
-                sums[1] = __builtin_fmaf(a[e] * g[e], s[e], sums[1]);
+                for (int e = 0; e < 8; ++e) {
+                    sums[0] = __builtin_fmaf(s[e] * k, s[e] * k, sums[0]);
+                    sums[1] = __builtin_fmaf(a[e] * g[e], s[e] * k, sums[1]);
+                }
             }
+            block_sum<W>(sums, t[turn]);
+        };
+        add_up(1.0f);
+        const float k = range_scale(sums[0], p.eps);
+        if (k != 1.0f) {
+            sums[0] = sums[1] = 0.0f;
+            turn ^= 1;
+            add_up(k);
         }
-        block_sum<W>(sums, t[turn]);
-        const float rho = 1.0f / __builtin_sqrtf(sums[0] / (float)p.hidden + p.eps);
-        const float back = rho * rho * (sums[1] / (float)p.hidden);   // rho mean(g n)
+        const Rate rho = rate_of(sums[0] / (float)p.hidden + p.eps * k * k, k);
+        const float back = rho.rest * rho.rest * (rho.scale / k * (sums[1] / (float)p.hidden));   // n mean(g n) = back s scale
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             if constexpr (!KEEP) {
@@ -349,11 +393,11 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
             weight(i, g);
             if (p.part)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) dw[i][e] = __builtin_fmaf(a[e], s[e] * rho, dw[i][e]);
+                for (int e = 0; e < 8; ++e) dw[i][e] = __builtin_fmaf(a[e], s[e] * rho.scale * rho.rest, dw[i][e]);
             if (p.dx) {
                 const uint32_t c = 8 * (i * NT + first);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] = rho * (a[e] * g[e] - back * s[e]);
+                for (int e = 0; e < 8; ++e) g[e] = rho.rest * (a[e] * g[e] - back * (s[e] * rho.scale)) * rho.scale;
                 if (p.dsum) {
                     values8(d[KEEP ? i : 0], sf, a);
 #pragma unroll
