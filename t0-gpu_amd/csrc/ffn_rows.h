@@ -137,14 +137,16 @@ __device__ __forceinline__ float f8_most(bool e5m2) { return e5m2 ? 57344.0f : 4
 struct BlockScale {
     float scale, inv, rest;
 };
-__device__ __forceinline__ BlockScale block_scale(float amax, bool e5m2) {
-    const float most = f8_most(e5m2);
-    amax = max_(amax, kLeastAmax);
+// `factor`: from 1 to 2, that all of the block's values (and amax) are yet to be multiplied by.  It is no part of the
+// quotients, which so have no rounding of it, but where the least scale takes over.
+__device__ __forceinline__ BlockScale block_scale(float amax, bool e5m2, float factor = 1.0f) {
+    const float most = f8_most(e5m2), top = amax * factor;
+    amax = top < kLeastAmax ? kLeastAmax / factor : amax;
     float inv = most / amax, r = __builtin_fmaf(-inv, amax, most);
     // rounded down, so that rest is not negative and zeros keep their sign
     inv = r < 0.0f ? __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, inv) - 1u) : inv;
     r = __builtin_fmaf(-inv, amax, most);
-    return BlockScale{amax / most, inv, r > 0.0f ? r * (e5m2 ? 1.0f / 57344.0f : 1.0f / 448.0f) * inv : 0.0f};
+    return BlockScale{max_(top, kLeastAmax) / most, inv, r > 0.0f ? r * (e5m2 ? 1.0f / 57344.0f : 1.0f / 448.0f) * inv : 0.0f};
 }
 __device__ __forceinline__ float amax8(const float (&v)[8]) {
     float m = __builtin_fabsf(v[0]);
@@ -272,21 +274,28 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
         for (int i = 0; i < CH; ++i) {
             const uint32_t c = 8 * (i * NT + first), n = anew<FAST>(left8<FAST>(p.hidden, c));
             if (p.sum) store8(p.sum, (uint64_t)row * p.ldsum + c, n, p.flags & T0G_ROWS_OUT_F32, s[i]);
-            float v[8];
+            float v[8], g[8];   // y = v rho.rest
             if (p.weight) {
-                values8(w[i], wf, v);
+                values8(w[i], wf, g);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = s[i][e] * rho.scale * rho.rest * (v[e] + p.weight_offset);
+                for (int e = 0; e < 8; ++e) g[e] += p.weight_offset;
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = s[i][e] * rho.scale * rho.rest;
+                for (int e = 0; e < 8; ++e) g[e] = 1.0f;
             }
-            if (p.y) store8(p.y, (uint64_t)row * p.ldy + c, n, p.flags & T0G_ROWS_Y_F32, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = s[i][e] * rho.scale;
+            if (p.y) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = v[e] * rho.rest * g[e];
+                store8(p.y, (uint64_t)row * p.ldy + c, n, p.flags & T0G_ROWS_Y_F32, y);
+            }
             if (p.q) {
                 // a row's last piece holds zeros past its values, for any rho but an infinite one
 #pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) v[e] = e < n ? v[e] : 0.0f;
-                const BlockScale b = block_scale(row16_max(amax8(v)), e5m2);
+                for (uint32_t e = 0; e < 8; ++e) v[e] = e < n ? v[e] * g[e] : 0.0f;
+                const BlockScale b = block_scale(row16_max(amax8(v)), e5m2, rho.rest);
                 store_f8x8(p.q + (uint64_t)row * p.ldq + c, n, f8x8(v, b.inv, b.rest, e5m2));
                 if ((threadIdx.x & 15u) == 0 && n) *at<float>(p.scales, (uint64_t)(c / T0G_SCALE_BLOCK) * p.ldsc + row) = b.scale;
             }

@@ -61,3 +61,26 @@ def test_quantize_on_borders(rt, rows, cols, block, qt, xt):   # noqa: F811
             if name in got:
                 wrong = bits(got[name]) != bits(want)
                 assert not bool(wrong.any()), f"{name}: {int(wrong.sum())} of {want.numel()} values"
+
+
+@pytest.mark.parametrize("hidden", [384, 1000, 4096, 8200])
+@pytest.mark.parametrize("qt", [E4, E5])
+@pytest.mark.parametrize("wt,woff", [(None, 0.0), (BF16, 0.0), (F32, 0.0), (F32, 1.0)])
+def test_norm_on_borders(rt, hidden, qt, wt, woff):   # noqa: F811
+    """The norm's factor leaves the quotients, which are x (w + offset) most / amax: of 16 significant bits above and below (w + offset:
+    of 8, in f32 as well), so that one that is on no border is 2^-22 of itself away and f32's rounding does not matter."""
+    g = torch.Generator().manual_seed(hidden)
+    rows = 300
+    x = data(g, rows, hidden, BF16, 2.0)
+    w = (1 + 0.1 * data(g, 1, hidden, F32)[0]).to(BF16) if wt else None
+    if woff:
+        w = (w.float() - woff).to(BF16)
+        w = torch.where((w.float() + woff).to(BF16).float() == w.float() + woff, w, torch.zeros_like(w))
+    b = Bufs(rt)
+    (xa, _), (wa, _) = b.inp(x), b.inp(w.to(wt) if wt else None, True)
+    (qa, _), (ca, _) = b.out("q", x.shape, qt), b.out("scales", (blocks(hidden), rows), F32)
+    rt.rms_norm(t0g.rms_norm_desc(xa, wa, rows, hidden, q=qa, scales=ca, weight_offset=woff, weight_dtype=TYPES[wt or BF16], q_dtype=TYPES[qt]))
+    u = quotients(x.double() * ((w.double() + woff) if wt else 1.0), qt)
+    assert int(on_border(u, qt).sum()) >= 3
+    wrong = bits(b.read()["q"]) != bits(u.float().to(qt))
+    assert not bool(wrong.any()), f"{int(wrong.sum())} of {u.numel()} values"
