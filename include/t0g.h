@@ -698,7 +698,8 @@ T0G_API int t0g_fp8_gemm_scratch_size(const t0g_fp8_gemm_desc *desc, size_t *byt
 
 /* A gated pair of projections in one kernel: g = x Wg^T, u = x Wu^T, h = act(g) u, with act one
  * of T0G_OP_SILU, T0G_OP_GELU (x sigmoid(1.702 x), as in the GEMMs' epilogues) and
- * T0G_OP_RELU.  gate and up receive g and u in bf16 for the backward call, if asked for.
+ * T0G_OP_RELU.  A NaN in g is one in act(g) and act'(g); of an infinite g relu is max(g, 0), the
+ * others what the formula gives.  gate and up receive g and u in bf16 for the backward call, if asked for.
  * hidden and features up to 4194240. */
 typedef struct t0g_gated_linear_desc {
     uint64_t x;                  /* bf16 [rows][ldx]                             */

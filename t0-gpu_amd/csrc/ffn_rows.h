@@ -604,11 +604,12 @@ __device__ __forceinline__ void quantize_tile(const T0gQuantArgs& p) {
 
 // ---- around the products ---------------------------------------------------------------
 // a = act(g) and its derivative.  The exponential and the reciprocal are the hardware's, each
-// within 2^-22, as in the GEMMs' epilogues.
+// within 2^-22, as in the GEMMs' epilogues.  A NaN passes on, into the derivative too; infinities go through the
+// formula: relu gives 0 or infinity, the others NaN for -infinity and for the derivatives.
 __device__ __forceinline__ void activation(uint32_t act, float g, float& a, float& slope) {
     if (act == T0G_ACT_RELU) {
-        a = g > 0.0f ? g : g * 0.0f;   // NaN passes on
-        slope = g > 0.0f ? 1.0f : 0.0f;
+        a = g < 0.0f ? 0.0f : g;
+        slope = g > 0.0f ? 1.0f : g == g ? 0.0f : g;
         return;
     }
     const float k = act == T0G_ACT_GELU ? 1.702f : 1.0f;
