@@ -615,7 +615,7 @@ __device__ __forceinline__ void activation(uint32_t act, float g, float& a, floa
     const float k = act == T0G_ACT_GELU ? 1.702f : 1.0f;
     const float sig = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * k * g));
     a = g * sig;
-    slope = __builtin_fmaf(k * a, 1.0f - sig, sig);
+    slope = __builtin_fmaf(a, k * (1.0f - sig), sig);   // k a first would leave f32's range
 }
 
 // From the kept products: dgate = dh up act'(gate), dup = dh act(gate).

@@ -1,4 +1,4 @@
-"""Gates that are infinite or not a number: the gated projections and their gradients against the
+"""Gates that are infinite, not a number, or near the largest f32: the gated projections and their gradients against the
 formulas in 64 bits, in which the same elements are infinite or not a number.
 
 A gate is infinite where x and Wg multiply to more than f32 holds (2^120 by +-2^10, u untouched by a zero in Wu), and not a number in a feature
@@ -91,7 +91,7 @@ def test_backward_of_kept_gates(rt, rows, f, hidden, layout, act):   # noqa: F81
     c.x[:, 0] = 1.0
     g, u = (torch.randn(rows, f, generator=torch.Generator().manual_seed(s)).to(BF16) for s in (1, 2))
     c.wg.nan_to_num_(0.25)
-    g[1, 5], g[2, 6], g[3, 7] = INF, -INF, NAN
+    g[1, 5], g[2, 6], g[3, 7], g[4, 8], g[5, 9] = INF, -INF, NAN, 3.0e38, -3.0e38
     b = c.b = Bufs(rt)
     lay = (lambda w: w) if layout == "NT" else (lambda w: w.t().contiguous())
     (xa, _), (wga, _), (wua, _), (da, _), (ga, _), (ua, _) = (b.inp(t) for t in (c.x, lay(c.wg), lay(c.wu), c.dh, g, u))
