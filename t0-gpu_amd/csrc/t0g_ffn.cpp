@@ -432,13 +432,20 @@ int run_join(t0g_device *dev, const T0gTileArgs &t, const Slices &s, uint32_t ga
     return ffn_launch(dev, "t0g_ffn_join_slices", groups_for((uint64_t)t.m * (s.ldp / 4), 256, 1u << 16), 1, 256, &j, sizeof j);
 }
 
-int set_tiles(T0gTileArgs *a, uint32_t bm, uint32_t bn) {
-    const uint64_t tm = ((uint64_t)a->m + bm - 1) / bm, tn = ((uint64_t)a->n + bn - 1) / bn;
-    if (tm * tn >= (1u << 22)) return fail(T0G_ERR_INVALID_ARG, "bad size: %llu x %llu tiles", (unsigned long long)tm, (unsigned long long)tn);
-    a->tiles_m = (uint32_t)tm;
-    a->tiles_n = (uint32_t)tn;
+// Rows and columns of a kernel's tile.
+struct Tile {
+    uint32_t m, n;
+};
+// A launch has fewer than 2^32 threads, 512 of a tile at most.
+int check_tiles(uint32_t m, uint32_t n, Tile tile) {
+    if (tiles_of(m, n, tile.m, tile.n) < (1u << 22)) return T0G_OK;
+    return fail(T0G_ERR_INVALID_ARG, "bad size: %u x %u in %llu tiles of %u x %u", m, n, (unsigned long long)tiles_of(m, n, tile.m, tile.n),
+                tile.m, tile.n);
+}
+void set_tiles(T0gTileArgs *a, Tile tile) {
+    a->tiles_m = (a->m - 1) / tile.m + 1;
+    a->tiles_n = (a->n - 1) / tile.n + 1;
     a->group_m = 8;
-    return T0G_OK;
 }
 
 // ---- the 8-bit product ------------------------------------------------------------------
@@ -471,20 +478,23 @@ struct Fp8Plan {
     Operand a, b;
     Slices slices;
     uint64_t bytes = 0;
+    Tile size() const { return tile == Fp8Tile::Big ? Tile{256, 256} : Tile{tile == Fp8Tile::Small ? 64u : 128u, 128}; }
 };
-void plan_fp8(const t0g_fp8_gemm_desc &d, Fp8Plan *p) {
-    if (d.m <= kSkinnyRows) return;
+int plan_fp8(const t0g_fp8_gemm_desc &d, Fp8Plan *p) {
+    if (d.m <= kSkinnyRows || d.n == 0) return T0G_OK;
     // 8192x8192x8192: 460 us in 256x256 tiles, 709 in 128x128
     if (d.out_dtype == T0G_BF16 && tiles_of(d.m, d.n, 256, 256) >= kNumCUs)
         p->tile = Fp8Tile::Big;
     else
         p->tile = middle(d.m, d.n, 128) ? Fp8Tile::Middle : Fp8Tile::Small;
+    if (int rc = check_tiles(d.m, d.n, p->size())) return rc;
     p->a.set(d.a, d.m, d.k, d.lda, 1);
     p->b.set(d.b, d.n, d.k, d.ldb, 1);
     p->a.at = take(&p->bytes, p->a.bytes());
     p->b.at = take(&p->bytes, p->b.bytes());
     p->slices.set(p->tile == Fp8Tile::Small ? tiles_of(d.m, d.n, 64, 128) : 0, blocks_of(d.k), d.m, d.n, 1);
     p->slices.at = take(&p->bytes, p->slices.bytes);
+    return T0G_OK;
 }
 
 int fp8_gemm_call(t0g_device *dev, const t0g_fp8_gemm_desc *desc) {
@@ -493,14 +503,13 @@ int fp8_gemm_call(t0g_device *dev, const t0g_fp8_gemm_desc *desc) {
     int rc = check_fp8_gemm(&d);
     if (rc) return rc;
     Fp8Plan pl;
-    plan_fp8(d, &pl);
+    if ((rc = plan_fp8(d, &pl))) return rc;
     T0gTileArgs t;
     memset(&t, 0, sizeof t);
     t.m = d.m;
     t.n = d.n;
     t.k = d.k;
     const bool skinny = pl.tile == Fp8Tile::Skinny, big = pl.tile == Fp8Tile::Big, small = pl.tile == Fp8Tile::Small;
-    if (!skinny && (rc = big ? set_tiles(&t, 256, 256) : set_tiles(&t, small ? 64 : 128, 128))) return rc;
     if (!dev) return fail(T0G_ERR_INVALID_ARG, "device is NULL");
     std::lock_guard<std::mutex> lk(device_mutex(dev));
     uint64_t base;
@@ -523,6 +532,7 @@ int fp8_gemm_call(t0g_device *dev, const t0g_fp8_gemm_desc *desc) {
         return ffn_launch(dev, symbol.c_str(), (d.n + 15) / 16, 1, 512, &t, sizeof t);
     }
     if ((rc = run_pad(dev, {&pl.a, &pl.b}, base))) return rc;
+    set_tiles(&t, pl.size());
     t.a = pl.a.address(base);
     t.b = pl.b.address(base);
     t.lda = pl.a.pitch();
@@ -577,11 +587,12 @@ struct GatedPlan {
     GatedTile tile = GatedTile::Skinny;
     Operand x, wg, wu;
     Slices slices;
+    Tile size() const { return tile == GatedTile::Big ? Tile{256, 128} : Tile{tile == GatedTile::Small ? 64u : 128u, 64}; }
     // grad: the kernels that give dgate and dup, which the 256x256 tile and the few rows' kernel do not.
-    void set(uint64_t xa, uint64_t g, uint64_t u, uint32_t rows, uint32_t features, uint32_t hidden, uint32_t ldx, uint32_t ldw,
+    int set(uint64_t xa, uint64_t g, uint64_t u, uint32_t rows, uint32_t features, uint32_t hidden, uint32_t ldx, uint32_t ldw,
              uint32_t transpose, bool grad, uint64_t *at) {
         const bool nt = transpose == T0G_NT;
-        if (nt && rows <= kSkinnyRows && !grad) return;
+        if ((nt && rows <= kSkinnyRows && !grad) || rows == 0) return T0G_OK;
         x.set(xa, rows, hidden, ldx, 2);
         wg.set(g, nt ? features : hidden, nt ? hidden : features, ldw, 2);
         wu.set(u, nt ? features : hidden, nt ? hidden : features, ldw, 2);
@@ -591,8 +602,10 @@ struct GatedPlan {
             tile = GatedTile::Big;
         else
             tile = middle(rows, features, 64) ? GatedTile::Middle : GatedTile::Small;
+        if (int rc = check_tiles(rows, features, size())) return rc;
         slices.set(tile == GatedTile::Small ? tiles_of(rows, features, 64, 64) : 0, (hidden + 63) / 64, rows, features, 2);
         slices.at = take(at, slices.bytes);
+        return T0G_OK;
     }
     // Whether the 256x256 tile takes it: enough tiles for all CUs, and 32-bit offsets in the operands.  2048x11008x4096
     // and its gradients: 962 us so, 1025 in 128x64 tiles.
@@ -615,8 +628,9 @@ int run_gated_tile(t0g_device *dev, T0gTileArgs *t, const GatedPlan &pl, uint64_
     t->planes = pl.slices.n > 1 ? base + pl.slices.at : 0;
     t->ldp = pl.slices.ldp;
     const bool nt = transpose == T0G_NT, big = pl.tile == GatedTile::Big, small = pl.tile == GatedTile::Small;
-    int rc = big ? set_tiles(t, 256, 128) : set_tiles(t, small ? 64 : 128, 64);
-    if (rc || (rc = run_pad(dev, {&pl.x, &pl.wg, &pl.wu}, base))) return rc;
+    set_tiles(t, pl.size());
+    int rc;
+    if ((rc = run_pad(dev, {&pl.x, &pl.wg, &pl.wu}, base))) return rc;
     const std::string symbol = std::string(big ? "t0g_ffn_gated_256x128" : small ? "t0g_ffn_gated_64x64" : "t0g_ffn_gated_128x64") +
                                (nt ? "_nt" : "_nn") + (kind == 2 ? "_grad" : "");
     if ((rc = ffn_launch(dev, symbol.c_str(), t->tiles_m * t->tiles_n, pl.slices.n, 256, t, sizeof *t))) return rc;
@@ -625,8 +639,7 @@ int run_gated_tile(t0g_device *dev, T0gTileArgs *t, const GatedPlan &pl, uint64_
 
 int gated_plan(const t0g_gated_linear_desc &d, GatedPlan *pl, uint64_t *bytes) {
     *bytes = 0;
-    pl->set(d.x, d.wg, d.wu, d.rows, d.features, d.hidden, d.ldx, d.ldw, d.transpose, false, bytes);
-    return T0G_OK;
+    return pl->set(d.x, d.wg, d.wu, d.rows, d.features, d.hidden, d.ldx, d.ldw, d.transpose, false, bytes);
 }
 
 int gated_call(t0g_device *dev, const t0g_gated_linear_desc *desc) {
@@ -722,7 +735,8 @@ int plan_gated_grad(const t0g_gated_linear_backward_desc &d, uint64_t base, Gate
     const bool nt = d.transpose == T0G_NT;
     const uint32_t f = d.features, es = size_of(d.dw_dtype);
     uint64_t at = 0;
-    if (!d.gate) pl->tiles.set(d.x, d.wg, d.wu, d.rows, f, d.hidden, d.ldx, d.ldw, d.transpose, true, &at);
+    if (!d.gate)
+        if (int rc = pl->tiles.set(d.x, d.wg, d.wu, d.rows, f, d.hidden, d.ldx, d.ldw, d.transpose, true, &at)) return rc;
     pl->half = (uint32_t)round_up(f, 8);
     pl->ldd = 2 * pl->half;
     pl->d = take(&at, (uint64_t)d.rows * pl->ldd * 2);
@@ -881,7 +895,7 @@ int t0g_fp8_gemm_scratch_size(const t0g_fp8_gemm_desc *desc, size_t *bytes) {
         int rc = t0g::check_fp8_gemm(&d);
         if (rc) return rc;
         t0g::Fp8Plan pl;
-        t0g::plan_fp8(d, &pl);
+        if ((rc = t0g::plan_fp8(d, &pl))) return rc;
         *bytes = pl.bytes;
         return t0g::ok();
     });
