@@ -703,13 +703,20 @@ int check_gated_grad(t0g_gated_linear_backward_desc *d, uint32_t *act) {
     return a.check();
 }
 
+// Products that add up to one output.
+struct Sum {
+    uint64_t out;
+    uint32_t rows, cols, ld, dtype;
+    std::vector<t0g_gemm_desc> terms;
+    uint64_t plane() const { return (uint64_t)rows * ldp() * 4; }
+    uint32_t ldp() const { return (uint32_t)round_up(cols, 4); }
+};
 // The gradients' products on D = [dg | du], [rows][2 features rounded up to 8 each].
 struct GatedGradPlan {
     GatedPlan tiles;                 // without the kept products
-    std::vector<t0g_gemm_desc> dx, dw;   // addresses in the scratch are offsets from its start
-    bool planes = false;             // dx in two products, added up
-    uint32_t half = 0, ldd = 0, ldp = 0;
-    uint64_t d = 0, p0 = 0, p1 = 0, ws = 0, ws_bytes = 0, bytes = 0;
+    std::vector<Sum> sums;           // addresses in the scratch are offsets from its start
+    uint32_t half = 0, ldd = 0;
+    uint64_t d = 0, p0 = 0, p1 = 0, ws = 0, ws_bytes = 0, bytes = 0;   // p0, p1: f32 planes of sums of several terms
 };
 
 t0g_gemm_desc product(uint64_t a, uint64_t b, uint64_t c, uint32_t m, uint32_t n, uint32_t k, uint32_t lda, uint32_t ldb,
@@ -730,8 +737,8 @@ t0g_gemm_desc product(uint64_t a, uint64_t b, uint64_t c, uint32_t m, uint32_t n
     return g;
 }
 
-// The plan for a scratch at `base` (0: sizes only; the GEMMs' choice does not depend on it but for its alignment).
-int plan_gated_grad(const t0g_gated_linear_backward_desc &d, uint64_t base, GatedGradPlan *pl) {
+// pieces: every operand below 2^30 elements, by fewer rows of it at a time.
+int plan_products(const t0g_gated_linear_backward_desc &d, uint64_t base, bool pieces, GatedGradPlan *pl) {
     const bool nt = d.transpose == T0G_NT;
     const uint32_t f = d.features, es = size_of(d.dw_dtype);
     uint64_t at = 0;
@@ -744,23 +751,50 @@ int plan_gated_grad(const t0g_gated_linear_backward_desc &d, uint64_t base, Gate
     const bool whole = pl->half == f;
     const uint64_t step = nt ? (uint64_t)f * d.ldw : f;
     const bool w_stacked = whole && d.wu == d.wg + step * 2 && (nt || d.ldw >= 2 * f);
+    // Rows of a piece.  One row alone may be followed by anything: its leading dimension is then its length.
+    auto fit = [&](uint32_t rows, uint32_t ld) {
+        const uint32_t most = ((1u << 30) - 1) / ld;
+        return pieces ? std::min(rows, most >= 64 ? most / 64 * 64 : std::max(1u, most)) : rows;
+    };
+    auto pitch = [&](uint32_t rows, uint32_t ld, uint32_t cols) { return pieces && rows == 1 ? cols : ld; };
     if (d.dx) {
-        const uint32_t tr = nt ? T0G_NN : T0G_NT;
-        if (w_stacked) {
-            pl->dx.push_back(product(dg, d.wg, d.dx, d.rows, d.hidden, 2 * f, pl->ldd, d.ldw, d.lddx, tr, d.dx_dtype));
-        } else {
-            pl->planes = true;
-            pl->ldp = (uint32_t)round_up(d.hidden, 4);
-            const uint64_t plane = (uint64_t)d.rows * pl->ldp * 4;
-            pl->p0 = take(&at, plane);
-            pl->p1 = take(&at, plane);
-            pl->dx.push_back(product(dg, d.wg, base + pl->p0, d.rows, d.hidden, f, pl->ldd, d.ldw, pl->ldp, tr, T0G_F32));
-            pl->dx.push_back(product(du, d.wu, base + pl->p1, d.rows, d.hidden, f, pl->ldd, d.ldw, pl->ldp, tr, T0G_F32));
-        }
+        struct Pair {
+            uint64_t d, w;
+            uint32_t k;
+        };
+        std::vector<Pair> pairs = {{dg, d.wg, w_stacked ? 2 * f : f}};
+        if (!w_stacked) pairs.push_back({du, d.wu, f});
+        const uint32_t rows = fit(d.rows, pl->ldd), cols = nt ? d.hidden : fit(d.hidden, d.ldw);
+        for (uint32_t r0 = 0; r0 < d.rows; r0 += rows)
+            for (uint32_t c0 = 0; c0 < d.hidden; c0 += cols) {
+                const uint32_t r = std::min(rows, d.rows - r0), c = std::min(cols, d.hidden - c0);
+                Sum s{d.dx + ((uint64_t)r0 * d.lddx + c0) * size_of(d.dx_dtype), r, c, d.lddx, d.dx_dtype, {}};
+                for (const Pair &p : pairs) {
+                    const uint32_t ks = nt ? fit(p.k, d.ldw) : p.k;
+                    for (uint32_t k0 = 0; k0 < p.k; k0 += ks) {
+                        const uint32_t k = std::min(ks, p.k - k0);
+                        const uint64_t from = p.d + ((uint64_t)r0 * pl->ldd + k0) * 2;
+                        s.terms.push_back(nt ? product(from, p.w + (uint64_t)k0 * d.ldw * 2, s.out, r, c, k, pl->ldd, pitch(k, d.ldw, c), d.lddx,
+                                                       T0G_NN, d.dx_dtype)
+                                             : product(from, p.w + (uint64_t)c0 * d.ldw * 2, s.out, r, c, k, pl->ldd, pitch(c, d.ldw, k), d.lddx,
+                                                       T0G_NT, d.dx_dtype));
+                    }
+                }
+                pl->sums.push_back(s);
+            }
     }
     auto dw = [&](uint64_t from, uint64_t to, uint32_t features) {
-        pl->dw.push_back(nt ? product(from, d.x, to, features, d.hidden, d.rows, pl->ldd, d.ldx, d.lddw, T0G_TN, d.dw_dtype)
-                            : product(d.x, from, to, d.hidden, features, d.rows, d.ldx, pl->ldd, d.lddw, T0G_TN, d.dw_dtype));
+        Sum s{to, nt ? features : d.hidden, nt ? d.hidden : features, d.lddw, d.dw_dtype, {}};
+        const uint32_t rows = std::min(fit(d.rows, pl->ldd), fit(d.rows, d.ldx));
+        uint32_t r0 = 0;
+        do {   // over no rows: one product, zeros
+            const uint32_t r = std::min(rows, d.rows - r0), ldx = pitch(r, d.ldx, d.hidden);
+            const uint64_t dr = from + (uint64_t)r0 * pl->ldd * 2, x = d.x + (uint64_t)r0 * d.ldx * 2;
+            s.terms.push_back(nt ? product(dr, x, to, features, d.hidden, r, pl->ldd, ldx, d.lddw, T0G_TN, d.dw_dtype)
+                                 : product(x, dr, to, d.hidden, features, r, ldx, pl->ldd, d.lddw, T0G_TN, d.dw_dtype));
+            r0 += r;
+        } while (r0 < d.rows);
+        pl->sums.push_back(s);
     };
     const uint64_t out_step = nt ? (uint64_t)f * d.lddw : f;
     if (whole && d.dwg && d.dwu == d.dwg + out_step * es && (nt || d.lddw >= 2 * f)) {
@@ -769,17 +803,39 @@ int plan_gated_grad(const t0g_gated_linear_backward_desc &d, uint64_t base, Gate
         if (d.dwg) dw(dg, d.dwg, f);
         if (d.dwu) dw(du, d.dwu, f);
     }
-    if (d.rows)
-        for (const auto *list : {&pl->dx, &pl->dw})
-            for (const t0g_gemm_desc &g : *list) {
-                size_t bytes = 0;
-                int rc = losses_gemm_workspace(&g, false, &bytes);
-                if (rc) return rc;
-                pl->ws_bytes = std::max<uint64_t>(pl->ws_bytes, bytes);
+    uint64_t plane = 0;
+    for (const Sum &s : pl->sums)
+        if (s.terms.size() > 1) plane = std::max(plane, s.plane());
+    pl->p0 = take(&at, plane);
+    pl->p1 = take(&at, plane);
+    for (Sum &s : pl->sums)
+        for (t0g_gemm_desc &g : s.terms) {
+            if (s.terms.size() > 1) {
+                g.c = base + (&g == &s.terms[0] ? pl->p0 : pl->p1);
+                g.ldc = s.ldp();
+                g.out_dtype = T0G_F32;
             }
+            if (!d.rows) continue;
+            size_t bytes = 0;
+            int rc = losses_gemm_workspace(&g, false, &bytes);
+            if (rc) return rc;
+            pl->ws_bytes = std::max<uint64_t>(pl->ws_bytes, bytes);
+        }
     pl->ws = take(&at, pl->ws_bytes);
     pl->bytes = at;
     return T0G_OK;
+}
+
+// The plan for a scratch at `base` (0: sizes only; the GEMMs' choice does not depend on it but for its alignment).  The GEMMs
+// take operands of whole 16-byte pieces at most sizes, and others (an odd number of features makes D one) below 2^31
+// elements: where they refuse the whole, it goes in pieces.
+int plan_gated_grad(const t0g_gated_linear_backward_desc &d, uint64_t base, GatedGradPlan *pl) {
+    int rc = plan_products(d, base, false, pl);
+    if (rc == T0G_ERR_INVALID_ARG) {
+        *pl = GatedGradPlan();
+        rc = plan_products(d, base, true, pl);
+    }
+    return rc;
 }
 
 int gated_grad_call(t0g_device *dev, const t0g_gated_linear_backward_desc *desc) {
@@ -831,26 +887,25 @@ int gated_grad_call(t0g_device *dev, const t0g_gated_linear_backward_desc *desc)
         g.workspace_bytes = pl.ws_bytes;
         return losses_gemm(dev, &g, false);
     };
-    if (d.rows) {
-        for (const t0g_gemm_desc &g : pl.dx)
-            if ((rc = run(g))) return rc;
-        if (pl.planes) {
+    for (const Sum &sum : pl.sums)
+        for (size_t i = 0; i < sum.terms.size(); ++i) {
+            if ((rc = run(sum.terms[i]))) return rc;
+            if (i == 0) continue;
+            // the first term's plane takes the others', and the last sum goes out
+            const bool last = i + 1 == sum.terms.size();
             T0gAddArgs a;
             memset(&a, 0, sizeof a);
             a.p0 = base + pl.p0;
             a.p1 = base + pl.p1;
-            a.out = d.dx;
-            a.rows = d.rows;
-            a.cols = d.hidden;
-            a.ldp = pl.ldp;
-            a.ldo = d.lddx;
-            a.out_bf16 = d.dx_dtype == T0G_BF16;
-            if ((rc = ffn_launch(dev, "t0g_ffn_add_planes", groups_for((uint64_t)d.rows * (pl.ldp / 4), 256, 1u << 16), 1, 256, &a, sizeof a)))
+            a.out = last ? sum.out : a.p0;
+            a.rows = sum.rows;
+            a.cols = sum.cols;
+            a.ldp = sum.ldp();
+            a.ldo = last ? sum.ld : a.ldp;
+            a.out_bf16 = last && sum.dtype == T0G_BF16;
+            if ((rc = ffn_launch(dev, "t0g_ffn_add_planes", groups_for((uint64_t)a.rows * (a.ldp / 4), 256, 1u << 16), 1, 256, &a, sizeof a)))
                 return rc;
         }
-    }
-    for (const t0g_gemm_desc &g : pl.dw)   // over no rows: zeros
-        if ((rc = run(g))) return rc;
     return ok();
 }
 

@@ -32,9 +32,13 @@ def taken(d):
     (gemm(1 << 20, 1 << 16, out_dtype=t0g.F32), gemm((1 << 20) - 128, 1 << 16, out_dtype=t0g.F32)),   # of 128 x 128
     (gated(1 << 22, 1 << 15), gated((1 << 22) - 256, 1 << 15)),                                       # of 256 x 128
     (gated(1 << 25, 1 << 10), gated((1 << 25) - 256, 1 << 9)),                                        # x past 2^30 elements: of 128 x 64
-    (gated_backward(1 << 20, 1 << 15), None),
+    (gated_backward(1 << 20, 1 << 15), gated_backward((1 << 20) - 128, 1 << 15)),
 ])
 def test_number_of_tiles(over, below):
     refused(over, "bad size")
-    if below:
-        taken(below)
+    taken(below)
+
+
+def test_backward_of_kept_products_has_no_tiles():
+    d = gated_backward(1 << 20, 1 << 15, gate=FAR[9], up=FAR[10])
+    taken(d)
