@@ -1830,8 +1830,8 @@ static int kernels_begin(t0g_device *dev, hipModule_t *module, const void *image
             dev->loss_bytes = bytes;
         }
     }
-    if (dev->loss) give_scratch(dev, dev->loss);
-    *scratch = dev->loss;
+    if (bytes) give_scratch(dev, dev->loss);   // a call without scratch holds no block in its graph
+    *scratch = bytes ? dev->loss : 0;
     return T0G_OK;
 }
 
