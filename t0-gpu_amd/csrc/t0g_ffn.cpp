@@ -737,6 +737,8 @@ t0g_gemm_desc product(uint64_t a, uint64_t b, uint64_t c, uint32_t m, uint32_t n
     return g;
 }
 
+// No card holds operands of more pieces: one is 1 GiB or more.
+constexpr uint64_t kMostPieces = 1u << 15;
 // pieces: every operand below 2^30 elements, by fewer rows of it at a time.
 int plan_products(const t0g_gated_linear_backward_desc &d, uint64_t base, bool pieces, GatedGradPlan *pl) {
     const bool nt = d.transpose == T0G_NT;
@@ -757,6 +759,10 @@ int plan_products(const t0g_gated_linear_backward_desc &d, uint64_t base, bool p
         return pieces ? std::min(rows, most >= 64 ? most / 64 * 64 : std::max(1u, most)) : rows;
     };
     auto pitch = [&](uint32_t rows, uint32_t ld, uint32_t cols) { return pieces && rows == 1 ? cols : ld; };
+    auto parts = [](uint64_t n, uint32_t step) { return n ? (n - 1) / step + 1 : 0; };
+    const uint64_t d_parts = parts(d.rows, fit(d.rows, pl->ldd)), w_rows = nt ? f : d.hidden;
+    if (d_parts * parts(w_rows, fit((uint32_t)w_rows, d.ldw)) > kMostPieces || parts(d.rows, fit(d.rows, d.ldx)) > kMostPieces)
+        return fail(T0G_ERR_INVALID_ARG, "bad size: %u rows, %u features, hidden %u with rows %u and %u apart", d.rows, f, d.hidden, d.ldx, d.ldw);
     if (d.dx) {
         struct Pair {
             uint64_t d, w;

@@ -86,3 +86,15 @@ def test_gated_scratch():
     assert t0g.ffn_scratch_size(gated(64, 512, 80, ldx=81)) == 64 * 256
     # 8 tiles, 64 stages of K in sixteen slices, two f32 planes each
     assert t0g.ffn_scratch_size(gated(64, 512, 4096)) == 16 * 2 * 64 * 512 * 4
+
+
+@pytest.mark.parametrize("layout", ["NT", "NN"])
+@pytest.mark.parametrize("kw", [dict(ldx=1 << 31), dict(ldw=1 << 31), dict(ldw=(1 << 32) - 1, ldx=(1 << 32) - 1)])
+def test_backward_of_operands_that_no_memory_holds(layout, kw):
+    """Refused before a product for each of their pieces is laid out."""
+    rows, f, hidden = 1 << 24, (1 << 20) + 1, (1 << 20) + 1
+    far = [i << 59 for i in range(1, 12)]
+    d = t0g.gated_linear_backward_desc(*far[:4], rows, f, hidden, transpose=layout, gate=far[9], up=far[10], dx=far[6], dwg=far[7], dwu=far[8], **kw)
+    refused(d, "bad size")
+    d.rows, d.features, d.hidden = 300, 45, 9
+    taken(d)
