@@ -334,7 +334,6 @@ typedef struct T0gTileArgs {
     uint32_t ldp, reserved2; /* multiple of 4                                            */
 } T0gTileArgs;
 #define T0G_TILE_OUT_F32 1u      /* c is f32, else bf16                                  */
-#define T0G_TILE_B_TILE 2u       /* a scale of B for each 128 x 128, else 1 x 128        */
 #define T0G_TILE_DH_F32 4u
 #define T0G_ACT_SILU 0u
 #define T0G_ACT_GELU 1u          /* x sigmoid(1.702 x)                                   */
