@@ -137,8 +137,8 @@ __device__ __forceinline__ float f8_most(bool e5m2) { return e5m2 ? 57344.0f : 4
 struct BlockScale {
     float scale, inv, rest;
 };
-// `factor`: from 1 to 2, that all of the block's values (and amax) are yet to be multiplied by.  It is no part of the
-// quotients, which so have no rounding of it, but where the least scale takes over.
+// `factor`: what all of the block's values (and amax) are yet to be multiplied by.  It is no part of the quotients,
+// which so have no rounding of it, but where the least scale takes over.
 __device__ __forceinline__ BlockScale block_scale(float amax, bool e5m2, float factor = 1.0f) {
     const float most = f8_most(e5m2), top = amax * factor;
     amax = top < kLeastAmax ? kLeastAmax / factor : amax;
@@ -189,38 +189,21 @@ __device__ __forceinline__ uint32_t left8(uint32_t cols, uint32_t c) {
 
 // n as a new value to the compiler, which otherwise forms the lane masks of all comparisons with it before the
 // loop over the rows and runs out of scalar registers.
-template <bool FAST>
+template <bool DO>
 __device__ __forceinline__ uint32_t anew(uint32_t n) {
-    if constexpr (!FAST) asm volatile("" : "+v"(n));
+    if constexpr (DO) asm volatile("" : "+v"(n));
     return n;
 }
 
 // ---- the norm --------------------------------------------------------------------------
-// What a row's values are multiplied by for their sum of squares: 1, or a power of two where f32 does not hold the sum
-// (16384 squares of values up to 2^128, or eps is so small that squares it would lose count), and then they are added up
-// again.  The same in all threads of the row.
+// What a row's values are multiplied by: 1, or a power of two where f32 does not hold the sum of their squares (16384
+// of values up to 2^128, or squares that it would lose and that count, with so small an eps).  They are then
+// added up again, and rho is theirs: s rho stays the same, and rho^2 and 1 / rho^2 are always f32's.  The same in all
+// threads of the row.
 __device__ __forceinline__ float range_scale(float sum, float eps) {
     const float k = sum > 0x1p96f ? 0x1p-80f : sum < 0x1p-90f && eps < 0x1p-60f ? 0x1p90f : 1.0f;
     return __builtin_bit_cast(float, uniform_u32(__builtin_bit_cast(uint32_t, k)));
 }
-// rho = mean^-1/2 as a power of two times a value from 1 to 2, so that s * scale is about 1 in a row of any magnitude.
-// mean: of the squares times k^2.
-struct Rate {
-    float scale, rest;
-};
-__device__ __forceinline__ Rate rate_of(float mean, float k) {
-    const float rho = 1.0f / __builtin_sqrtf(mean);
-    const uint32_t w = __builtin_bit_cast(uint32_t, rho);
-    Rate r = {__builtin_bit_cast(float, w & 0x7F800000u), rho == rho ? __builtin_bit_cast(float, (w & 0x007FFFFFu) | 0x3F800000u) : rho};
-    if (k > 1.0f) {   // scale stays below 2^128
-        const float most = __builtin_fminf(r.scale, 0x1p127f / k);
-        r.rest *= r.scale / most;
-        r.scale = most;
-    }
-    r.scale *= k;
-    return r;
-}
-
 // y = s rho (w + offset), rho = (mean s^2 + eps)^-1/2, s = x + residual.  NT threads take a row, with CH pieces
 // of 8 each, and keep it in registers between the sum of squares and the output: memory is read and
 // written once.  Rows of one wave go R to a workgroup.  FAST: bf16 inputs of whole pieces of 8, which need
@@ -238,7 +221,7 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
     for (uint32_t row = blockIdx.x * R + threadIdx.x / NT; row < p.rows; row += step, turn ^= 1) {
         Raw8 x[CH], r[CH], w[CH];
         auto load = [&](int i) {
-            const uint32_t c = 8 * (i * NT + first), n = anew<FAST>(left8<FAST>(p.hidden, c));
+            const uint32_t c = 8 * (i * NT + first), n = anew<!FAST && (CH > 1)>(left8<FAST>(p.hidden, c));
             x[i] = load8(p.x, (uint64_t)row * p.ldx + c, n, xf);
             if (p.residual) r[i] = load8(p.residual, (uint64_t)row * p.ldr + c, n, rf);
             if (p.weight) w[i] = load8(p.weight, c, n, wf);
@@ -258,23 +241,33 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[0] = __builtin_fmaf(s[i][e], s[i][e], sum[0]);
         }
+        if (p.sum)
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const uint32_t c = 8 * (i * NT + first);
+                store8(p.sum, (uint64_t)row * p.ldsum + c, anew<!FAST && (CH > 1)>(left8<FAST>(p.hidden, c)), p.flags & T0G_ROWS_OUT_F32, s[i]);
+            }
         block_sum<W>(sum, t[turn]);
-        const float k = range_scale(sum[0], p.eps);
+        float eps = p.eps;
+        const float k = range_scale(sum[0], eps);
         if (k != 1.0f) {
             sum[0] = 0.0f;
 #pragma unroll
             for (int i = 0; i < CH; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum[0] = __builtin_fmaf(s[i][e] * k, s[i][e] * k, sum[0]);
+                for (int e = 0; e < 8; ++e) {
+                    s[i][e] *= k;
+                    sum[0] = __builtin_fmaf(s[i][e], s[i][e], sum[0]);
+                }
+            eps = eps * k * k;
             turn ^= 1;
             block_sum<W>(sum, t[turn]);
         }
-        const Rate rho = rate_of(sum[0] / (float)p.hidden + p.eps * k * k, k);
+        const float rho = 1.0f / __builtin_sqrtf(sum[0] / (float)p.hidden + eps);
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            const uint32_t c = 8 * (i * NT + first), n = anew<FAST>(left8<FAST>(p.hidden, c));
-            if (p.sum) store8(p.sum, (uint64_t)row * p.ldsum + c, n, p.flags & T0G_ROWS_OUT_F32, s[i]);
-            float v[8], g[8];   // y = v rho.rest
+            const uint32_t c = 8 * (i * NT + first), n = anew<!FAST && (CH > 1)>(left8<FAST>(p.hidden, c));
+            float v[8], g[8];
             if (p.weight) {
                 values8(w[i], wf, g);
 #pragma unroll
@@ -283,19 +276,16 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) g[e] = 1.0f;
             }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = s[i][e] * rho.scale;
             if (p.y) {
-                float y[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = v[e] * rho.rest * g[e];
-                store8(p.y, (uint64_t)row * p.ldy + c, n, p.flags & T0G_ROWS_Y_F32, y);
+                for (int e = 0; e < 8; ++e) v[e] = s[i][e] * rho * g[e];
+                store8(p.y, (uint64_t)row * p.ldy + c, n, p.flags & T0G_ROWS_Y_F32, v);
             }
             if (p.q) {
                 // a row's last piece holds zeros past its values, for any rho but an infinite one
 #pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) v[e] = e < n ? v[e] * g[e] : 0.0f;
-                const BlockScale b = block_scale(row16_max(amax8(v)), e5m2, rho.rest);
+                for (uint32_t e = 0; e < 8; ++e) v[e] = e < n ? s[i][e] * g[e] : 0.0f;
+                const BlockScale b = block_scale(row16_max(amax8(v)), e5m2, rho);
                 store_f8x8(p.q + (uint64_t)row * p.ldq + c, n, f8x8(v, b.inv, b.rest, e5m2));
                 if ((threadIdx.x & 15u) == 0 && n) *at<float>(p.scales, (uint64_t)(c / T0G_SCALE_BLOCK) * p.ldsc + row) = b.scale;
             }
@@ -320,7 +310,7 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
     Raw8 w[KEEP ? CH : 1];
     auto load_weight = [&](int i) {
         const uint32_t c = 8 * (i * NT + first);
-        if (p.weight) w[KEEP ? i : 0] = load8(p.weight, c, anew<FAST>(left8<FAST>(p.hidden, c)), wf);
+        if (p.weight) w[KEEP ? i : 0] = load8(p.weight, c, anew<!FAST && (CH > 1)>(left8<FAST>(p.hidden, c)), wf);
     };
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
@@ -341,7 +331,7 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
     constexpr int K = KEEP ? CH : 1;
     Raw8 y[K], x[K], d[K];
     auto load = [&](uint32_t row, int i, Raw8& yi, Raw8& xi, Raw8& di) {
-        const uint32_t c = 8 * (i * NT + first), n = anew<FAST>(row < p.rows ? left8<FAST>(p.hidden, c) : 0u);
+        const uint32_t c = 8 * (i * NT + first), n = anew<!FAST && (CH > 1)>(row < p.rows ? left8<FAST>(p.hidden, c) : 0u);
         yi = load8(p.dy, (uint64_t)row * p.lddy + c, n, yf);
         xi = load8(p.x, (uint64_t)row * p.ldx + c, n, xf);
         if (p.dsum && p.dx) di = load8(p.dsum, (uint64_t)row * p.ldds + c, n, sf);
@@ -359,7 +349,7 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
         else if constexpr (KEEP)
 #pragma unroll
             for (int i = 0; i < CH; ++i) load(row, i, y[i], x[i], d[i]);
-        float sums[2] = {0.0f, 0.0f};   // of (s k)^2 and g s k
+        float sums[2] = {0.0f, 0.0f};   // of s^2 and g s
         auto add_up = [&](float k) {
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
@@ -374,9 +364,13 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
                 weight(i, g);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    sums[0] = __builtin_fmaf(s[e] * k, s[e] * k, sums[0]);
-                    sums[1] = __builtin_fmaf(a[e] * g[e], s[e] * k, sums[1]);
+                    s[e] *= k;
+                    sums[0] = __builtin_fmaf(s[e], s[e], sums[0]);
+                    sums[1] = __builtin_fmaf(a[e] * g[e], s[e], sums[1]);
                 }
+                if constexpr (FAST)
+                    if (k != 1.0f)   // a power of two: bf16 holds these too
+                        x[i].lo = u32x4_t{pack2(s[0], s[1]), pack2(s[2], s[3]), pack2(s[4], s[5]), pack2(s[6], s[7])};
             }
             block_sum<W>(sums, t[turn]);
         };
@@ -387,8 +381,8 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
             turn ^= 1;
             add_up(k);
         }
-        const Rate rho = rate_of(sums[0] / (float)p.hidden + p.eps * k * k, k);
-        const float back = rho.rest * rho.rest * (rho.scale / k * (sums[1] / (float)p.hidden));   // n mean(g n) = back s scale
+        const float rho = 1.0f / __builtin_sqrtf(sums[0] / (float)p.hidden + p.eps * k * k);
+        const float back = rho * rho * (sums[1] / (float)p.hidden);   // rho mean(g n)
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             if constexpr (!KEEP) {
@@ -400,19 +394,25 @@ __device__ __forceinline__ void rms_norm_grad(const T0gNormGradArgs& p) {
             values8(y[KEEP ? i : 0], yf, a);
             values8(x[KEEP ? i : 0], xf, s);
             weight(i, g);
+            if constexpr (!FAST)   // (under a branch, as below, this takes 20 registers more)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[e] *= k;
             if (p.part)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) dw[i][e] = __builtin_fmaf(a[e], s[e] * rho.scale * rho.rest, dw[i][e]);
+                for (int e = 0; e < 8; ++e) dw[i][e] = __builtin_fmaf(a[e], s[e] * rho, dw[i][e]);
             if (p.dx) {
                 const uint32_t c = 8 * (i * NT + first);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] = rho.rest * (a[e] * g[e] - back * (s[e] * rho.scale)) * rho.scale;
+                for (int e = 0; e < 8; ++e) g[e] = rho * (a[e] * g[e] - back * s[e]);
+                if (!FAST || k != 1.0f)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) g[e] *= k;
                 if (p.dsum) {
                     values8(d[KEEP ? i : 0], sf, a);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) g[e] += a[e];
                 }
-                store8(p.dx, (uint64_t)row * p.lddx + c, anew<FAST>(left8<FAST>(p.hidden, c)), p.flags & T0G_ROWS_OUT_F32, g);
+                store8(p.dx, (uint64_t)row * p.lddx + c, anew<!FAST && (CH > 1)>(left8<FAST>(p.hidden, c)), p.flags & T0G_ROWS_OUT_F32, g);
             }
         }
         if constexpr (PRE)
