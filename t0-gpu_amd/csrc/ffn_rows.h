@@ -207,7 +207,7 @@ __device__ __forceinline__ float range_scale(float sum, float eps) {
 // y = s rho (w + offset), rho = (mean s^2 + eps)^-1/2, s = x + residual.  NT threads take a row, with CH pieces
 // of 8 each, and keep it in registers between the sum of squares and the output: memory is read and
 // written once.  Rows of one wave go R to a workgroup.  FAST: bf16 inputs of whole pieces of 8, which need
-// half the registers: 8192x4096 with the residual into e4m3 in 43 us that way, 53 with types and ends
+// half the registers: 8192x4096 with the residual into e4m3 in 44 us that way, 53 with types and ends
 // looked at in the kernel.
 template <int NT, int CH, int R, bool FAST>
 __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
@@ -264,6 +264,10 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
             block_sum<W>(sum, t[turn]);
         }
         const float rho = 1.0f / __builtin_sqrtf(sum[0] / (float)p.hidden + eps);
+        // as a power of two, which rounds nothing and keeps s (w + offset) in range, times a value from 1 to 2
+        const uint32_t bits = __builtin_bit_cast(uint32_t, rho);
+        const float rho2 = __builtin_bit_cast(float, bits & 0x7F800000u);
+        const float rest = rho == rho ? __builtin_bit_cast(float, (bits & 0x007FFFFFu) | 0x3F800000u) : rho;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const uint32_t c = 8 * (i * NT + first), n = anew<!FAST && (CH > 1)>(left8<FAST>(p.hidden, c));
@@ -284,8 +288,8 @@ __device__ __forceinline__ void rms_norm(const T0gNormArgs& p) {
             if (p.q) {
                 // a row's last piece holds zeros past its values, for any rho but an infinite one
 #pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) v[e] = e < n ? s[i][e] * g[e] : 0.0f;
-                const BlockScale b = block_scale(row16_max(amax8(v)), e5m2, rho);
+                for (uint32_t e = 0; e < 8; ++e) v[e] = e < n ? s[i][e] * rho2 * g[e] : 0.0f;
+                const BlockScale b = block_scale(row16_max(amax8(v)), e5m2, rest);
                 store_f8x8(p.q + (uint64_t)row * p.ldq + c, n, f8x8(v, b.inv, b.rest, e5m2));
                 if ((threadIdx.x & 15u) == 0 && n) *at<float>(p.scales, (uint64_t)(c / T0G_SCALE_BLOCK) * p.ldsc + row) = b.scale;
             }

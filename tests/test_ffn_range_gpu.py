@@ -69,3 +69,19 @@ def test_norm_backward_of_any_magnitude(rt, rows, hidden, dtype, amp, each):   #
     near(got["dx"], want, U * want.abs() + 2 * NORM_REL * size + 2 * LEAST[F32], "dx")
     each = dy.double() * n
     near(got["dw"], each.sum(0, keepdim=True), (U + NORM_REL + (rows + 34) * U) * each.abs().sum(0, keepdim=True), "dw")
+
+
+@pytest.mark.parametrize("hidden", [300, 4096, 9001])
+@pytest.mark.parametrize("size,weight", [(1e-12, 1e-26), (1e-20, 1e-24), (1e13, 1e25), (1e30, 1e30), (1e-30, 1e36)])
+def test_norm_in_8_bits_of_weights_of_any_magnitude(rt, hidden, size, weight):   # noqa: F811
+    """x times the weight, without the norm's factor, is not f32's."""
+    g = torch.Generator().manual_seed(hidden)
+    x, w = rows_of(g, [size] * 3, hidden, F32), rows_of(g, [weight], hidden, F32)[0]
+    b = Bufs(rt)
+    (xa, _), (wa, _), (ya, _) = b.inp(x), b.inp(w, True), b.out("y", x.shape, F32)
+    (qa, _), (ca, _) = b.out("q", x.shape, E4), b.out("scales", (blocks(hidden), 3), F32)
+    f = t0g.F32
+    rt.rms_norm(t0g.rms_norm_desc(xa, wa, 3, hidden, eps=0.0, y=ya, q=qa, scales=ca, x_dtype=f, weight_dtype=f, y_dtype=f))
+    got, y = b.read(), norm_of(x, None, w, 0.0, 0.0)[2]
+    near(got["y"], y, (U + NORM_REL) * y.abs() + 2 * LEAST[F32], "y")
+    check_f8(got["q"], got["scales"], y, E4, slack=NORM_REL, what="q")
