@@ -482,7 +482,7 @@ struct Fp8Plan {
 };
 int plan_fp8(const t0g_fp8_gemm_desc &d, Fp8Plan *p) {
     if (d.m <= kSkinnyRows || d.n == 0) return T0G_OK;
-    // 8192x8192x8192: 460 us in 256x256 tiles, 709 in 128x128
+    // 8192x8192x8192: 474 to 486 us in 256x256 tiles, 709 in 128x128
     if (d.out_dtype == T0G_BF16 && tiles_of(d.m, d.n, 256, 256) >= kNumCUs)
         p->tile = Fp8Tile::Big;
     else
@@ -608,7 +608,7 @@ struct GatedPlan {
         return T0G_OK;
     }
     // Whether the 256x256 tile takes it: enough tiles for all CUs, and 32-bit offsets in the operands.  2048x11008x4096
-    // and its gradients: 962 us so, 1025 in 128x64 tiles.
+    // and its gradients: 944 to 985 us so, 1025 in 128x64 tiles.
     bool big(uint32_t rows, uint32_t features, uint32_t hidden, bool nt) const {
         const uint64_t most = 1ull << 30, ldb = wg.pitch(), wspan = (nt ? features + 256ull : hidden + 64ull) * ldb;
         const uint64_t g = wg.address(0), u = wu.address(0), apart = g < u ? u - g : g - u;   // as far apart in the scratch
