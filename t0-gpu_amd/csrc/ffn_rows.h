@@ -622,7 +622,8 @@ __device__ __forceinline__ void activation(uint32_t act, float g, float& a, floa
     slope = __builtin_fmaf(a, k * (1.0f - sig), sig);   // k a first would leave f32's range
 }
 
-// From the kept products: dgate = dh up act'(gate), dup = dh act(gate).
+// From the kept products: dgate = dh up act'(gate), dup = dh act(gate), in bf16 as the operands of the gradients' products:
+// in f32 these would leave the matrix units' bf16 rate, in two bf16 parts take twice as long.
 __device__ __forceinline__ void gated_grad(const T0gGatedGradArgs& p) {
     const uint32_t per_row = (p.features + 7) / 8;
     const uint64_t pieces = (uint64_t)p.rows * per_row;

@@ -154,3 +154,50 @@ def test_quantize_of_more_rows_than_a_launch_has(rt, rows, cols, want):   # noqa
     rt.fp8_quantize(d)
     got = b.read()
     check_f8(got["q"], got["scales"], x.double() if want == "q" else x.double().t(), E4, what=want)
+
+
+# ---- ends of rows -----------------------------------------------------------------------
+ENDS = [n + r for n in (504, 520, 2040, 2048, 4088, 4096, 8184, 8192, 16376) for r in range(1, 9)]
+
+
+@pytest.mark.parametrize("hidden", ENDS)
+@pytest.mark.parametrize("xt,rt_,wt,yt,pad,offset", [(BF16, BF16, BF16, BF16, 0, 0), (F32, F32, F32, F32, 3, 1)])
+def test_norm_at_every_end(rt, hidden, xt, rt_, wt, yt, pad, offset):   # noqa: F811
+    """Last pieces of every length, on both sides of each kernel's limit."""
+    base.test_norm(rt, 3, hidden, xt, rt_, wt, yt, pad, offset)
+
+
+@pytest.mark.parametrize("hidden", ENDS)
+@pytest.mark.parametrize("xt,yt,wt,st,pad,offset", [(BF16, BF16, BF16, BF16, 0, 0), (F32, BF16, F32, F32, 5, 1)])
+def test_norm_backward_at_every_end(rt, hidden, xt, yt, wt, st, pad, offset):   # noqa: F811
+    base.test_norm_backward(rt, 5, hidden, xt, yt, wt, st, pad, offset)
+
+
+@pytest.mark.parametrize("cols", [n + r for n in (120, 248, 2040) for r in range(1, 17)])
+@pytest.mark.parametrize("xt", [BF16, F32])
+@pytest.mark.parametrize("block", ["row", "tile"])
+def test_quantize_at_every_end(rt, cols, xt, block):   # noqa: F811
+    base.test_quantize(rt, 130 + cols % 16, cols, xt, E4, block, "q qt", 3, 1)
+
+
+@pytest.mark.parametrize("n", range(57, 74))
+@pytest.mark.parametrize("layout", ["NT", "NN"])
+def test_gated_at_every_end(rt, n, layout):   # noqa: F811
+    c = Gated(rt, n, n + 3, n + 7, layout, "silu", 3, 1, apart=True)
+    c.forward(True)
+    c.free()
+    Gated(rt, n, n + 3, n + 7, layout, "silu", 1, 0, apart=True).backward(n % 2 == 0)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 2048])
+@pytest.mark.parametrize("layout", ["NT", "NN"])
+def test_gated_of_one_weight(rt, rows, layout):   # noqa: F811
+    """Both projections by the same array."""
+    f, hidden = (4096, 64) if rows == 2048 else (72, 136)
+    c = Gated(rt, rows, f, hidden, layout, "silu", apart=True)
+    c.wu, c.ua, c.u, c.eu = c.wg, c.ga, c.g, c.eg
+    c.forward(True)
+    if rows != 2048:
+        c.backward(False)
+    else:
+        c.free()
